@@ -433,6 +433,150 @@ typedef struct rf_accum_leaf {
 RF_API rf_status rf_accumulate(const rf_accum_leaf* leaves, int32_t n_leaves, int32_t mode, int32_t n_acc,
                                void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Residual blocks with 8-bit saved activations (no reference counterpart).
+ *
+ * A checkpoint of an activation [rows, cols] is int8 codes [rows, pitch],
+ * pitch = 32 * ceil(cols / 32), zero past cols, and one exponent byte per 32
+ * columns [rows, pitch / 32].  With E the biased f32 exponent of a block's
+ * largest magnitude, e = max(E - 6, 1), the step is 2^(e - 127), a code is
+ * round-to-nearest-even(x / step) within +-127 and reads back as code * step.
+ * A block that holds an Inf or NaN has e = 255 and reads back as NaN.  Code
+ * buffers are 16-byte aligned.
+ *
+ * Activations are row-major with a row stride in elements (columns
+ * contiguous); outputs are dense.  Sums are held in f32 in a fixed order: the
+ * same inputs give the same bits.  Calls enqueue on `stream`, allocate
+ * nothing and never synchronise, so they may be captured into a graph;
+ * workspaces come from the caller.  rows = 0 is a call on nothing (sums over
+ * rows are zero). */
+
+/* x [rows, cols] of `dtype` into a checkpoint. */
+RF_API rf_status rf_checkpoint_store(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                                     int8_t* codes, uint8_t* exponents, void* stream);
+
+/* The values of a checkpoint, rounded to `dtype`, into out [rows, cols]. */
+RF_API rf_status rf_checkpoint_load(const int8_t* codes, const uint8_t* exponents, int64_t rows, int64_t cols,
+                                    int32_t dtype, void* out, void* stream);
+
+/* Activations of rf_gated: a(g) = g sigmoid(g); g Phi(g) with the normal
+ * distribution function; its tanh form. */
+#define RF_ACT_SILU 0
+#define RF_ACT_GELU 1
+#define RF_ACT_GELU_TANH 2
+
+/* h = a(gate) * up and its backward pass.  Every tensor is [rows, cols] of
+ * `dtype`. */
+typedef struct rf_gated {
+    int64_t rows, cols;
+    int32_t dtype;
+    int32_t activation;        /* RF_ACT_* */
+    const void* gate;          /* read by the backward pass unless gate_codes are given */
+    const void* up;
+    int64_t gate_stride, up_stride;
+    int8_t* gate_codes;        /* forward: written; backward: read; NULL: no checkpoint */
+    uint8_t* gate_exponents;
+    int8_t* up_codes;          /* with gate_codes, or NULL */
+    uint8_t* up_exponents;
+    void* h;                   /* forward: [rows, cols] dense */
+    int8_t* h_codes;           /* forward: a checkpoint of h too, or NULL */
+    uint8_t* h_exponents;
+    const void* dh;            /* backward */
+    int64_t dh_stride;
+    void* dgate;               /* backward outputs, row strides below */
+    void* dup;
+    int64_t dgate_stride, dup_stride;
+} rf_gated;
+
+RF_API rf_status rf_gated_forward(const rf_gated* args, void* stream);
+RF_API rf_status rf_gated_backward(const rf_gated* args, void* stream);
+
+/* rf_norm.post / next */
+#define RF_NORM_ABSENT 0 /* the part is not there */
+#define RF_NORM_NONE 1   /* post only: no normalisation, n = branch */
+#define RF_NORM_RMS 2    /* xhat = x / sqrt(mean(x^2) + eps) */
+#define RF_NORM_LAYER 3  /* xhat = (x - mean) / sqrt(mean((x - mean)^2) + eps) */
+
+/* The norms around a block.
+ *   post part: n = uhat * weight + bias, uhat the normalised branch,
+ *              hidden = residual_scale * residual + branch_scale * gate * n
+ *   next part: y = hhat * next_weight + next_bias, hhat the normalised hidden
+ * post absent: `hidden` is the input (the norm before a block).  The next
+ * part acts on hidden as it is stored.  rows / gates consecutive rows share
+ * a row of `gate` [gates, cols]; gates = 0: no gate.
+ * The backward pass reads the normalised rows from the codes where they are
+ * given and from branch / hidden otherwise, with the saved statistics:
+ *   t = dhidden + d(next norm)(dy),  dresidual = residual_scale * t,
+ *   dbranch = d(post norm)(branch_scale * gate * t); post absent: dresidual = t
+ *   is the gradient at hidden and residual_scale is not read. */
+typedef struct rf_norm {
+    int64_t rows, cols, gates;
+    int32_t dtype;             /* residual, hidden, dhidden, dresidual */
+    int32_t branch_dtype;      /* branch, y, dy, dbranch: dtype, or a 16-bit type beside f32 */
+    int32_t post, next;        /* RF_NORM_*; one of them at least is there */
+    float post_eps, next_eps, branch_scale, residual_scale;
+    const void* residual;
+    const void* branch;
+    void* hidden;              /* post: forward writes it (stride cols); post absent: the input */
+    int64_t residual_stride, branch_stride, hidden_stride;
+    const void* weight;        /* [cols] or NULL (ones) */
+    const void* bias;          /* [cols] or NULL (zeros) */
+    const void* gate;
+    const void* next_weight;
+    const void* next_bias;
+    int32_t weight_dtype, bias_dtype, gate_dtype, next_weight_dtype, next_bias_dtype;
+    int32_t reserved;          /* 0 */
+    void* y;                   /* [rows, cols] */
+    int8_t* branch_codes;      /* forward: written unless NULL; backward: read unless NULL */
+    uint8_t* branch_exponents;
+    int8_t* hidden_codes;
+    uint8_t* hidden_exponents;
+    int8_t* y_codes;           /* forward: a checkpoint of y too, or NULL */
+    uint8_t* y_exponents;
+    float* post_mean;          /* [rows] statistics: forward writes them unless NULL */
+    float* post_rstd;
+    float* next_mean;
+    float* next_rstd;
+    const void* dhidden;       /* backward; NULL: zero */
+    const void* dy;
+    int64_t dhidden_stride, dy_stride;
+    void* dresidual;           /* [rows, cols] */
+    void* dbranch;             /* [rows, cols] */
+    void* dweight;             /* gradients of the vectors, in their types; NULL: not wanted */
+    void* dbias;
+    void* dgate;               /* [gates, cols] */
+    void* dnext_weight;
+    void* dnext_bias;
+} rf_norm;
+
+RF_API rf_status rf_norm_forward(const rf_norm* args, void* stream);
+
+/* Bytes of device workspace (256-byte aligned) of rf_norm_backward on the
+ * current device. */
+RF_API rf_status rf_norm_backward_workspace(const rf_norm* args, int64_t* bytes);
+RF_API rf_status rf_norm_backward(const rf_norm* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A linear layer's weight gradient from its input's checkpoint:
+ *   out[n, k] = (accumulate ? out[n, k] : 0) + sum over rows t of dy[t, n] x[t, k]
+ * dy [rows, outs] of dy_dtype, x the checkpoint's values [rows, cols], out
+ * [outs, cols] dense of out_dtype.  Products are exact and sums f32 for every
+ * dy_dtype. */
+typedef struct rf_weight_grad {
+    int64_t rows, outs, cols;
+    int32_t dy_dtype, out_dtype;
+    const void* dy;
+    int64_t dy_stride;
+    const int8_t* codes;
+    const uint8_t* exponents;
+    void* out;
+    int32_t accumulate;
+    int32_t reserved; /* 0 */
+} rf_weight_grad;
+
+RF_API rf_status rf_linear_weight_grad_workspace(const rf_weight_grad* args, int64_t* bytes);
+RF_API rf_status rf_linear_weight_grad(const rf_weight_grad* args, void* workspace, int64_t workspace_bytes,
+                                       void* stream);
+
 /* Host-side: the 256 f32 values of a dynamic codebook (adam8.py:461-503). */
 RF_API rf_status rf_codebook(int32_t quantizer, float* out256);
 

@@ -42,10 +42,42 @@ from .utils import apply_updates, apply_updates_prefix
 
 __version__ = "0.1.0"
 
+# The residual-block operators (blocks.py) and their differentiable forms
+# (autograd.py) import torch; the names load on first use.
+_BLOCKS = (
+    "ActivationCheckpoint",
+    "PostnormGrads",
+    "PrenormGrads",
+    "checkpoint_activations",
+    "gated_activation",
+    "gated_activation_grad",
+    "linear_weight_grad",
+    "postnorm_residual",
+    "postnorm_residual_grad",
+    "prenorm",
+    "prenorm_grad",
+    "restore_activations",
+)
+
+
+def __getattr__(name):
+    import importlib
+
+    if name in _BLOCKS:
+        value = getattr(importlib.import_module(".blocks", __name__), name)
+    elif name in ("autograd", "blocks"):
+        value = importlib.import_module("." + name, __name__)
+    else:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    globals()[name] = value
+    return value
+
+
 __all__ = (
     "DYNAMIC_SIGNED_CODEBOOK_ID",
     "DYNAMIC_UNSIGNED_CODEBOOK_ID",
     "SYMMETRIC_INT8_CODEBOOK_ID",
+    "ActivationCheckpoint",
     "ApplyIfFiniteState",
     "EmptyState",
     "GlobalNormClipState",
@@ -56,6 +88,8 @@ __all__ = (
     "MultiSteps",
     "MultiStepsState",
     "MultiTransformState",
+    "PostnormGrads",
+    "PrenormGrads",
     "QuantizedBlocks",
     "ScaleByAdam8State",
     "ScaleByAdamState",
@@ -69,17 +103,27 @@ __all__ = (
     "apply_if_finite",
     "apply_updates",
     "apply_updates_prefix",
+    "autograd",
     "chain",
+    "checkpoint_activations",
     "clip_by_global_norm",
     "dequantize_blocks",
     "dequantize_state_tree",
     "estimate_quantized_moment_bytes",
+    "gated_activation",
+    "gated_activation_grad",
+    "linear_weight_grad",
     "masked",
     "multi_transform",
+    "postnorm_residual",
+    "postnorm_residual_grad",
+    "prenorm",
+    "prenorm_grad",
     "prng",
     "quantize_blocks",
     "quantize_state_tree",
     "quantized_nbytes",
+    "restore_activations",
     "scale_by_adam",
     "scale_by_adam8",
     "tree_state_nbytes",

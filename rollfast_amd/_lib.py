@@ -36,6 +36,8 @@ RF_LEAF_SCALE_BF16 = 8
 RF_LEAF_SCALE_F16 = 16
 RF_ACC_SUM, RF_ACC_MEAN, RF_ACC_ZERO = 0, 1, 2
 RF_NOALLOC_SCRATCH_BYTES = 8 << 20
+RF_ACT_SILU, RF_ACT_GELU, RF_ACT_GELU_TANH = 0, 1, 2
+RF_NORM_ABSENT, RF_NORM_NONE, RF_NORM_RMS, RF_NORM_LAYER = 0, 1, 2, 3
 
 _p = ctypes.c_void_p
 
@@ -148,6 +150,51 @@ class ApplyLeaf(ctypes.Structure):
     ]
 
 
+_i32, _i64, _f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+
+class Gated(ctypes.Structure):
+    _fields_ = [
+        *((n, _i64) for n in ("rows", "cols")),
+        *((n, _i32) for n in ("dtype", "activation")),
+        *((n, _p) for n in ("gate", "up")),
+        *((n, _i64) for n in ("gate_stride", "up_stride")),
+        *((n, _p) for n in ("gate_codes", "gate_exponents", "up_codes", "up_exponents", "h", "h_codes", "h_exponents",
+                            "dh")),
+        ("dh_stride", _i64),
+        *((n, _p) for n in ("dgate", "dup")),
+        *((n, _i64) for n in ("dgate_stride", "dup_stride")),
+    ]
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [
+        *((n, _i64) for n in ("rows", "cols", "gates")),
+        *((n, _i32) for n in ("dtype", "branch_dtype", "post", "next")),
+        *((n, _f32) for n in ("post_eps", "next_eps", "branch_scale", "residual_scale")),
+        *((n, _p) for n in ("residual", "branch", "hidden")),
+        *((n, _i64) for n in ("residual_stride", "branch_stride", "hidden_stride")),
+        *((n, _p) for n in ("weight", "bias", "gate", "next_weight", "next_bias")),
+        *((n, _i32) for n in ("weight_dtype", "bias_dtype", "gate_dtype", "next_weight_dtype", "next_bias_dtype",
+                              "reserved")),
+        *((n, _p) for n in ("y", "branch_codes", "branch_exponents", "hidden_codes", "hidden_exponents", "y_codes",
+                            "y_exponents", "post_mean", "post_rstd", "next_mean", "next_rstd", "dhidden", "dy")),
+        *((n, _i64) for n in ("dhidden_stride", "dy_stride")),
+        *((n, _p) for n in ("dresidual", "dbranch", "dweight", "dbias", "dgate", "dnext_weight", "dnext_bias")),
+    ]
+
+
+class WeightGrad(ctypes.Structure):
+    _fields_ = [
+        *((n, _i64) for n in ("rows", "outs", "cols")),
+        *((n, _i32) for n in ("dy_dtype", "out_dtype")),
+        ("dy", _p),
+        ("dy_stride", _i64),
+        *((n, _p) for n in ("codes", "exponents", "out")),
+        *((n, _i32) for n in ("accumulate", "reserved")),
+    ]
+
+
 assert ctypes.sizeof(Adam8Leaf) == 120
 assert ctypes.sizeof(Adam8Hparams) == 128
 assert ctypes.sizeof(Adam8Group) == 32
@@ -177,6 +224,15 @@ EXPORTS = (
     "rf_magma_scale",
     "rf_magma_apply_updates",
     "rf_accumulate",
+    "rf_checkpoint_store",
+    "rf_checkpoint_load",
+    "rf_gated_forward",
+    "rf_gated_backward",
+    "rf_norm_forward",
+    "rf_norm_backward_workspace",
+    "rf_norm_backward",
+    "rf_linear_weight_grad_workspace",
+    "rf_linear_weight_grad",
     "rf_codebook",
     "rf_host_table_codes",
     "rf_host_search_index",
@@ -226,6 +282,15 @@ def lib() -> ctypes.CDLL:
     L.rf_magma_scale.argtypes = [ctypes.POINTER(MagmaLeaf), i32, _p, _p, f32, f32, u32, u32, i32, f32, _p, _p]
     L.rf_magma_apply_updates.argtypes = [ctypes.POINTER(ApplyLeaf), i32, _p, f32, i32, u32, u32, _p]
     L.rf_accumulate.argtypes = [ctypes.POINTER(AccumLeaf), i32, i32, i32, _p]
+    L.rf_checkpoint_store.argtypes = [_p, i32, i64, i64, i64, _p, _p, _p]
+    L.rf_checkpoint_load.argtypes = [_p, _p, i64, i64, i32, _p, _p]
+    L.rf_gated_forward.argtypes = [ctypes.POINTER(Gated), _p]
+    L.rf_gated_backward.argtypes = [ctypes.POINTER(Gated), _p]
+    L.rf_norm_forward.argtypes = [ctypes.POINTER(Norm), _p]
+    L.rf_norm_backward_workspace.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(i64)]
+    L.rf_norm_backward.argtypes = [ctypes.POINTER(Norm), _p, i64, _p]
+    L.rf_linear_weight_grad_workspace.argtypes = [ctypes.POINTER(WeightGrad), ctypes.POINTER(i64)]
+    L.rf_linear_weight_grad.argtypes = [ctypes.POINTER(WeightGrad), _p, i64, _p]
     L.rf_codebook.argtypes = [i32, _p]
     L.rf_host_table_codes.argtypes = [i32, u32, i64, _p]
     L.rf_host_search_index.argtypes = [i32, u32, i64, _p]

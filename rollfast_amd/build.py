@@ -32,6 +32,13 @@ INST_SRC = os.path.join(CSRC, "rf_adam8_inst.hip")
 TILE_SRC = os.path.join(CSRC, "rf_tile_inst.hip")
 # One object per (apply, moment SR, exact) instance of the step kernels.
 VARIANTS = [(a, m, e) for a in (0, 1) for m in (0, 1) for e in (0, 1)]
+# The residual-block operators: host entries with the element-wise kernels,
+# the weight-gradient product, and the norm kernels, one object per (residual
+# type, branch type).
+BLOCK_SRC = os.path.join(CSRC, "rf_block_host.hip")
+WGRAD_SRC = os.path.join(CSRC, "rf_wgrad.hip")
+NORM_SRC = os.path.join(CSRC, "rf_norm_inst.hip")
+NORM_PAIRS = [(0, 0), (1, 1), (2, 2), (0, 1), (0, 2)]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -65,6 +72,12 @@ def _compile_jobs():
         obj = os.path.join(OBJ_DIR, f"rf_tile_a{a}_m{m}_e{e}.o")
         defs = [f"-DRFI_APPLY={a}", f"-DRFI_MSR={m}", f"-DRFI_EXACT={e}"]
         jobs.append(([HIPCC, *FLAGS, *inc, *defs, "-c", TILE_SRC, "-o", obj], obj))
+    for src, name in ((BLOCK_SRC, "rf_block_host.o"), (WGRAD_SRC, "rf_wgrad.o")):
+        obj = os.path.join(OBJ_DIR, name)
+        jobs.append(([HIPCC, *FLAGS, *inc, "-c", src, "-o", obj], obj))
+    for t, u in NORM_PAIRS:
+        obj = os.path.join(OBJ_DIR, f"rf_norm_t{t}_u{u}.o")
+        jobs.append(([HIPCC, *FLAGS, *inc, f"-DRFI_T={t}", f"-DRFI_U={u}", "-c", NORM_SRC, "-o", obj], obj))
     return jobs
 
 
@@ -97,8 +110,15 @@ def _sources_of(obj: str) -> list:
     """The source files an output is built from (headers included)."""
     inc = [os.path.join(REPO, "include", "rfadam8.h")]
     dev = [os.path.join(CSRC, name) for name in ("rf_device.h", "rf_tile.h", "rf_tables.h")]
+    blk = [os.path.join(CSRC, name) for name in ("rf_block.h", "rf_norm.h", "rf_norm_launch.h")]
     if obj.endswith("rf_host.o"):
         return [HOST_SRC, *dev, *inc]
+    if os.path.basename(obj) == "rf_block_host.o":
+        return [BLOCK_SRC, *blk, *inc]
+    if os.path.basename(obj) == "rf_wgrad.o":
+        return [WGRAD_SRC, *blk, *inc]
+    if os.path.basename(obj).startswith("rf_norm"):
+        return [NORM_SRC, *blk, *inc]
     if os.path.basename(obj).startswith("rf_tile"):
         return [TILE_SRC, *dev, *inc]
     if obj.endswith(".o"):
@@ -118,7 +138,7 @@ def build(verbose: bool = False, jobs: int | None = None, incremental: bool = Fa
     the path of the built ``.so``.  ``incremental``: recompile only the
     objects older than their sources."""
     os.makedirs(OBJ_DIR, exist_ok=True)
-    max_par = jobs or min(3 * len(VARIANTS) + 1, max(1, os.cpu_count() or 1))
+    max_par = jobs or min(len(_compile_jobs()), max(1, os.cpu_count() or 1))
     # the moment-SR objects compile longest: first, so that none runs alone at the end
     pending = sorted(_compile_jobs(), key=lambda job: ("_m1_" not in job[1], "tile" in job[1])) + [_pyhost_job()]
     if incremental:

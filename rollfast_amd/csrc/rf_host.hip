@@ -37,6 +37,42 @@ rf_status fail(rf_status code, const std::string& msg)
     } while (0)
 }  // namespace
 
+// The residual-block entries' errors and device properties (rf_block.h).
+namespace rf {
+rf_status report(rf_status code, const char* msg) noexcept
+{
+    try {
+        g_err = msg;
+    } catch (...) {  // no memory for the message
+        g_err.clear();
+    }
+    return code;
+}
+
+rf_status report_hip(hipError_t e, const char* what) noexcept
+{
+    try {
+        g_err = std::string(what) + ": " + hipGetErrorString(e);
+    } catch (...) {
+        g_err.clear();
+    }
+    return RF_ERR_HIP;
+}
+
+rf_status device_cus(int* out) noexcept
+{
+    static std::atomic<int> cus[64];  // by device; an entry is written once with the same value
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return report_hip(e, "hipGetDevice");
+    if (dev >= 0 && dev < 64 && (*out = cus[dev].load(std::memory_order_relaxed)) > 0) return RF_OK;
+    e = hipDeviceGetAttribute(out, hipDeviceAttributeMultiprocessorCount, dev);
+    if (e != hipSuccess) return report_hip(e, "hipDeviceGetAttribute");
+    if (dev >= 0 && dev < 64) cus[dev].store(*out, std::memory_order_relaxed);
+    return RF_OK;
+}
+}  // namespace rf
+
 // Instances of the step kernel (rf_adam8_inst.hip, one object per variant).
 namespace rf {
 adam_kernel_t rf_pick_adam8_a0_m0_e0(int dtype_combo, bool psr, bool nest);

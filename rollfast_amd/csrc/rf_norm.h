@@ -1,0 +1,731 @@
+// rf_norm.h -- the norms around a block: forward and backward kernels.
+//
+// Rows of up to 8192 columns stay in registers from their one load to their
+// last use (two chunks of eight columns per lane at most, 64 to 512 lanes a
+// row); wider rows are walked again by the lanes that loaded them (k_*_wide).
+// The parameter vectors' gradients are sums over rows: a workgroup adds its
+// own rows in registers and writes one partial row, k_norm_finish adds the
+// partial rows in their order.  No atomics: the same inputs give the same bits.
+//
+// The gradients of the gate, the weight and the bias of the post part come
+// from two column sums of a group of rows with a common gate,
+//   P = sum uhat t,  Q = sum t:
+//   dgate = s (w P + b Q),  dweight = s sum_groups gate P,  dbias = s sum_groups gate Q.
+//
+// The backward pass needs the row means of g2 xhat and of gn uhat, gn = h t
+// with h = s gate w and t = e - k0 - k1 xhat, e = dhidden + rstd2 g2,
+// k1 = rstd2 mean(g2 xhat), k0 = rstd2 mean(g2).  The second mean depends on
+// the first through t; written out,
+//   sum gn uhat = sum h e uhat - k0 sum h uhat - k1 sum h xhat uhat
+//   sum gn      = sum h e      - k0 sum h      - k1 sum h xhat
+// every sum is known after one walk of the row, so a row costs one exchange
+// between its waves instead of two.
+#pragma once
+
+#include "rf_block.h"
+
+namespace rfb {
+
+constexpr int MAX_WAVES = 8;  // waves of a row in the register kernels
+
+// How the rows of a backward pass are dealt out.
+struct NormPlan {
+    int32_t pieces;    // pieces of a group, each a workgroup (0: workgroups take whole groups)
+    int32_t workers;   // workgroups = partial rows
+    int32_t vectors;   // partial rows' vectors
+    int32_t i_p, i_q, i_w2, i_b2;  // their indices, -1 absent
+    int64_t group_rows;            // rows that share a gate
+    int64_t groups;
+};
+
+__device__ __forceinline__ int64_t part(int64_t n, int64_t i, int64_t of) { return n * i / of; }
+
+// Sums of NS values over the tpr lanes of a row.  `red` has two halves used
+// in turn, so one barrier a call is enough: a half is written again only
+// after the barrier of the call between.
+template <int NS> __device__ __forceinline__ void row_sums(float (&s)[NS], float (*red)[MAX_WAVES][8], int& half)
+{
+#pragma unroll
+    for (int k = 0; k < NS; ++k) s[k] = wave_sum(s[k]);
+    const int waves = blockDim.x / WAVE;
+    if (waves > 1) {
+        const int w = threadIdx.x / WAVE;
+        if ((threadIdx.x & (WAVE - 1)) == 0) {
+#pragma unroll
+            for (int k = 0; k < NS; ++k) red[half][w][k] = s[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+            float t = 0.0f;
+            for (int i = 0; i < waves; ++i) t += red[half][i][k];
+            s[k] = t;
+        }
+        half ^= 1;
+    }
+}
+
+template <typename T> __device__ __forceinline__ T* row_of(T* p, int64_t row, int64_t stride) { return p + row * stride; }
+
+// ------------------------------------------------------------- forward -----
+// blockDim (tpr, ny): tpr lanes a row; ny > 1 only where a wave holds a row.
+template <typename T, typename U, bool EXIT, bool NEXT, int NV>
+__global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
+{
+    __shared__ float red[2][MAX_WAVES][8];
+    int half = 0;
+    const int tid = threadIdx.x, tpr = blockDim.x;
+    const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
+    const float inv_cols = 1.0f / (float)cols;
+    const int64_t r0 = part(a.rows, blockIdx.x, gridDim.x), r1 = part(a.rows, blockIdx.x + 1, gridDim.x);
+    const int64_t group_rows = a.gates > 1 ? a.rows / a.gates : 0;
+    float A[NV][8], B[NV][8], w2[NV][8], b2[NV][8];
+    int64_t group = -1;
+    auto load_post = [&](int64_t g) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            float gt[8];
+            vector8(a.weight, a.weight_dtype, c, cols - c, 1.0f, A[j]);
+            vector8(a.bias, a.bias_dtype, c, cols - c, 0.0f, B[j]);
+            vector8(a.gate, a.gate_dtype, g * cols + c, cols - c, 1.0f, gt);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                A[j][k] *= a.branch_scale * gt[k];
+                B[j][k] *= a.branch_scale * gt[k];
+            }
+        }
+    };
+    if constexpr (EXIT) {
+        if (group_rows == 0) load_post(0);
+    }
+    if constexpr (NEXT) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            vector8(a.next_weight, a.next_weight_dtype, c, cols - c, 1.0f, w2[j]);
+            vector8(a.next_bias, a.next_bias_dtype, c, cols - c, 0.0f, b2[j]);
+        }
+    }
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += blockDim.y) {
+        Raw<T> rr[NV];
+        Raw<U> ur[EXIT ? NV : 1];
+        const T* rp = EXIT ? (const T*)a.residual + r * a.residual_stride : (const T*)a.hidden + r * a.hidden_stride;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            rr[j] = load8(rp + c, cols - c);
+            if constexpr (EXIT) ur[j] = load8((const U*)a.branch + r * a.branch_stride + c, cols - c);
+        }
+        if constexpr (EXIT) {
+            if (group_rows && r / group_rows != group) {
+                group = r / group_rows;
+                load_post(group);
+            }
+            float mean = 0.0f, rstd = 1.0f;
+            if (a.post == RF_NORM_LAYER) {
+                float s[1] = {0.0f};
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    float u[8];
+                    widen8(ur[j], u);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) s[0] += u[k];
+                }
+                row_sums(s, red, half);
+                mean = s[0] * inv_cols;
+            }
+            if (a.post != RF_NORM_NONE) {
+                float s[1] = {0.0f};
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
+                    float u[8];
+                    widen8(ur[j], u);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float d = k < left ? u[k] - mean : 0.0f;
+                        s[0] = fmaf(d, d, s[0]);
+                    }
+                }
+                row_sums(s, red, half);
+                rstd = 1.0f / sqrtf(s[0] * inv_cols + a.post_eps);
+                if (tid == 0) {
+                    if (a.post_rstd) a.post_rstd[r] = rstd;
+                    if (a.post_mean) a.post_mean[r] = mean;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                if (ch < nch) {
+                    float u[8], x[8], o[8];
+                    widen8(ur[j], u);
+                    widen8(rr[j], x);
+                    if (a.branch_codes) put_codes(a.branch_codes, a.branch_exponents, r, pitch, ch, encode8(u));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        o[k] = c + k < cols ? fmaf(a.residual_scale, x[k], fmaf((u[k] - mean) * rstd, A[j][k], B[j][k])) : 0.0f;
+                    rr[j] = narrow8<T>(o);
+                    put8((T*)a.hidden + r * cols + c, rr[j], cols - c);
+                }
+            }
+        }
+        if constexpr (NEXT) {
+            float mean = 0.0f;
+            if (a.next == RF_NORM_LAYER) {
+                float s[1] = {0.0f};
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    float v[8];
+                    widen8(rr[j], v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) s[0] += v[k];
+                }
+                row_sums(s, red, half);
+                mean = s[0] * inv_cols;
+            }
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
+                float v[8];
+                widen8(rr[j], v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float d = k < left ? v[k] - mean : 0.0f;
+                    s[0] = fmaf(d, d, s[0]);
+                }
+            }
+            row_sums(s, red, half);
+            const float rstd = 1.0f / sqrtf(s[0] * inv_cols + a.next_eps);
+            if (tid == 0) {
+                if (a.next_rstd) a.next_rstd[r] = rstd;
+                if (a.next_mean) a.next_mean[r] = mean;
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                if (ch < nch) {
+                    float v[8], y[8];
+                    widen8(rr[j], v);
+                    if (a.hidden_codes) put_codes(a.hidden_codes, a.hidden_exponents, r, pitch, ch, encode8(v));
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        y[k] = c + k < cols ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[j][k]) : 0.0f;
+                    const Raw<U> yr = narrow8<U>(y);
+                    put8((U*)a.y + r * cols + c, yr, cols - c);
+                    if (a.y_codes) {
+                        widen8(yr, y);
+                        put_codes(a.y_codes, a.y_exponents, r, pitch, ch, encode8(y));
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Rows wider than the register kernels take: the lanes walk their columns
+// again instead of keeping them.  A lane reads back only what it wrote itself.
+template <typename T, typename U, bool EXIT, bool NEXT>
+__global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
+{
+    __shared__ float red[2][MAX_WAVES][8];
+    int half = 0;
+    const int tid = threadIdx.x, tpr = blockDim.x;
+    const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
+    const float inv_cols = 1.0f / (float)cols;
+    // mean and 1 / sqrt(variance + eps) of the row at p
+    auto stats = [&](auto* p, int kind, float eps, float& mean, float& rstd) {
+        mean = 0.0f;
+        if (kind == RF_NORM_LAYER) {
+            float s[1] = {0.0f};
+            for (int64_t ch = tid; ch < nch; ch += tpr) {
+                float v[8];
+                widen8(load8(p + ch * CHUNK, cols - ch * CHUNK), v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[0] += v[k];
+            }
+            row_sums(s, red, half);
+            mean = s[0] * inv_cols;
+        }
+        float s[1] = {0.0f};
+        for (int64_t ch = tid; ch < nch; ch += tpr) {
+            const int64_t left = cols - ch * CHUNK;
+            float v[8];
+            widen8(load8(p + ch * CHUNK, left), v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float d = k < left ? v[k] - mean : 0.0f;
+                s[0] = fmaf(d, d, s[0]);
+            }
+        }
+        row_sums(s, red, half);
+        rstd = 1.0f / sqrtf(s[0] * inv_cols + eps);
+    };
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const int64_t g = a.gates > 1 ? r / (a.rows / a.gates) : 0;
+        T* hp = (T*)a.hidden + r * (EXIT ? cols : a.hidden_stride);
+        if constexpr (EXIT) {
+            const U* up = (const U*)a.branch + r * a.branch_stride;
+            const T* rp = (const T*)a.residual + r * a.residual_stride;
+            float mean = 0.0f, rstd = 1.0f;
+            if (a.post != RF_NORM_NONE) {
+                stats(up, a.post, a.post_eps, mean, rstd);
+                if (tid == 0) {
+                    if (a.post_rstd) a.post_rstd[r] = rstd;
+                    if (a.post_mean) a.post_mean[r] = mean;
+                }
+            }
+            for (int64_t ch = tid; ch < nch; ch += tpr) {
+                const int64_t c = ch * CHUNK, left = cols - c;
+                float u[8], x[8], w[8], b[8], gt[8], o[8];
+                widen8(load8(up + c, left), u);
+                widen8(load8(rp + c, left), x);
+                vector8(a.weight, a.weight_dtype, c, left, 1.0f, w);
+                vector8(a.bias, a.bias_dtype, c, left, 0.0f, b);
+                vector8(a.gate, a.gate_dtype, g * cols + c, left, 1.0f, gt);
+                if (a.branch_codes) put_codes(a.branch_codes, a.branch_exponents, r, pitch, ch, encode8(u));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float s = a.branch_scale * gt[k];
+                    o[k] = fmaf(a.residual_scale, x[k], fmaf((u[k] - mean) * rstd, w[k] * s, b[k] * s));
+                }
+                put8(hp + c, narrow8<T>(o), left);
+            }
+        }
+        if constexpr (NEXT) {
+            float mean, rstd;
+            stats(hp, a.next, a.next_eps, mean, rstd);
+            if (tid == 0) {
+                if (a.next_rstd) a.next_rstd[r] = rstd;
+                if (a.next_mean) a.next_mean[r] = mean;
+            }
+            for (int64_t ch = tid; ch < nch; ch += tpr) {
+                const int64_t c = ch * CHUNK, left = cols - c;
+                float v[8], w[8], b[8], y[8];
+                widen8(load8((const T*)hp + c, left), v);
+                vector8(a.next_weight, a.next_weight_dtype, c, left, 1.0f, w);
+                vector8(a.next_bias, a.next_bias_dtype, c, left, 0.0f, b);
+                if (a.hidden_codes) put_codes(a.hidden_codes, a.hidden_exponents, r, pitch, ch, encode8(v));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = k < left ? fmaf((v[k] - mean) * rstd, w[k], b[k]) : 0.0f;
+                const Raw<U> yr = narrow8<U>(y);
+                put8((U*)a.y + r * cols + c, yr, left);
+                if (a.y_codes) {
+                    widen8(yr, y);
+                    put_codes(a.y_codes, a.y_exponents, r, pitch, ch, encode8(y));
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ backward -----
+// The saved row of a norm: a checkpoint, or the tensor itself.
+template <typename T, bool SRC8> struct Saved {
+    Raw<T> t;
+    __device__ __forceinline__ void load(const T* p, int64_t stride, const int8_t*, const uint8_t*, int64_t r, int64_t,
+                                         int64_t ch, int64_t, int64_t cols)
+    {
+        t = load8(p + r * stride + ch * CHUNK, cols - ch * CHUNK);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const { widen8(t, v); }
+};
+template <typename T> struct Saved<T, true> {
+    Codes t;
+    __device__ __forceinline__ void load(const T*, int64_t, const int8_t* codes, const uint8_t* exps, int64_t r,
+                                         int64_t pitch, int64_t ch, int64_t nch, int64_t)
+    {
+        t = Codes{};
+        if (ch < nch) t = get_codes(codes, exps, r, pitch, ch);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const { decode8(t, v); }
+};
+
+// FULL: LayerNorm or a bias somewhere (the sums of g, t and their columns).
+template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, int NV>
+__global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const NormPlan plan, float* __restrict__ partial)
+{
+    __shared__ float red[2][MAX_WAVES][8];
+    extern __shared__ float cols_lds[];
+    int half = 0;
+    const int tid = threadIdx.x, tpr = blockDim.x, ty = threadIdx.y, ny = blockDim.y;
+    const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
+    const float inv_cols = 1.0f / (float)cols;
+    const bool post_layer = FULL && EXIT && a.post == RF_NORM_LAYER, next_layer = FULL && NEXT && a.next == RF_NORM_LAYER;
+    const bool post_norm = EXIT && a.post != RF_NORM_NONE;
+    const bool whole_groups = EXIT && plan.pieces == 0;
+    float P[EXIT ? NV : 1][8] = {}, Q[EXIT && FULL ? NV : 1][8] = {};
+    float W2[NEXT ? NV : 1][8] = {}, B2[NEXT && FULL ? NV : 1][8] = {};
+    float h[EXIT ? NV : 1][8], w2[NEXT ? NV : 1][8];
+    if constexpr (NEXT) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            vector8(a.next_weight, a.next_weight_dtype, c, cols - c, 1.0f, w2[j]);
+        }
+    }
+    // groups of this workgroup and the rows of each
+    const int64_t g0 = whole_groups ? part(plan.groups, blockIdx.x, gridDim.x) + ty
+                                    : blockIdx.x / max(plan.pieces, 1);
+    const int64_t g1 = whole_groups ? part(plan.groups, blockIdx.x + 1, gridDim.x) : g0 + 1;
+    // whole groups: the sums over groups, of this wave's or workgroup's columns
+    float* const sums_p = cols_lds + (int64_t)ty * (FULL ? 2 : 1) * pitch;
+    float* const sums_q = sums_p + pitch;
+    if (whole_groups) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t ch = tid + j * tpr;
+            if (ch < nch) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    sums_p[ch * CHUNK + k] = 0.0f;
+                    if (FULL) sums_q[ch * CHUNK + k] = 0.0f;
+                }
+            }
+        }
+    }
+    for (int64_t g = g0; g < g1; g += whole_groups ? ny : 1) {
+        int64_t r0 = g * plan.group_rows, r1 = r0 + plan.group_rows;
+        if (!whole_groups) {
+            const int64_t piece = blockIdx.x % max(plan.pieces, 1);
+            r1 = r0 + part(plan.group_rows, piece + 1, plan.pieces);
+            r0 += part(plan.group_rows, piece, plan.pieces) + ty;
+        }
+        if constexpr (EXIT) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                float gt[8];
+                vector8(a.weight, a.weight_dtype, c, cols - c, 1.0f, h[j]);
+                vector8(a.gate, a.gate_dtype, g * cols + c, cols - c, 1.0f, gt);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) h[j][k] = c + k < cols ? h[j][k] * a.branch_scale * gt[k] : 0.0f;
+            }
+        }
+        for (int64_t r = r0; r < r1; r += whole_groups ? 1 : ny) {
+            Raw<T> dhr[NV];
+            Raw<U> dyr[NEXT ? NV : 1];
+            Saved<U, SRC8> us[EXIT ? NV : 1];
+            Saved<T, SRC8> hs[NEXT ? NV : 1];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                dhr[j] = zero8<T>();
+                if (a.dhidden) dhr[j] = load8((const T*)a.dhidden + r * a.dhidden_stride + c, cols - c);
+                if constexpr (NEXT) {
+                    dyr[j] = load8((const U*)a.dy + r * a.dy_stride + c, cols - c);
+                    hs[j].load((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch,
+                               cols);
+                }
+                if constexpr (EXIT)
+                    us[j].load((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch,
+                               cols);
+            }
+            const float rstd1 = post_norm ? a.post_rstd[r] : 1.0f, mean1 = post_layer ? a.post_mean[r] : 0.0f;
+            const float rstd2 = NEXT ? a.next_rstd[r] : 0.0f, mean2 = next_layer ? a.next_mean[r] : 0.0f;
+            float e[NV][8], x[NEXT ? NV : 1][8], u[EXIT ? NV : 1][8];
+            // g2 xhat, h e uhat, h xhat uhat; FULL: g2, h uhat, h e, h, h xhat
+            float s[FULL ? 8 : 3] = {};
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
+                widen8(dhr[j], e[j]);
+                if constexpr (NEXT) {
+                    float dy[8];
+                    widen8(dyr[j], dy);
+                    hs[j].get(x[j]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        x[j][k] = k < left ? (x[j][k] - mean2) * rstd2 : 0.0f;
+                        const float g2 = dy[k] * w2[j][k];
+                        W2[j][k] = fmaf(dy[k], x[j][k], W2[j][k]);
+                        if constexpr (FULL) {
+                            B2[j][k] += dy[k];
+                            s[3] += k < left ? g2 : 0.0f;
+                        }
+                        s[0] = fmaf(g2, x[j][k], s[0]);
+                        e[j][k] = fmaf(rstd2, g2, e[j][k]);
+                    }
+                }
+                if constexpr (EXIT) {
+                    us[j].get(u[j]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        u[j][k] = k < left ? (u[j][k] - mean1) * rstd1 : 0.0f;
+                        const float hu = h[j][k] * u[j][k];
+                        s[1] = fmaf(e[j][k], hu, s[1]);
+                        if constexpr (NEXT) s[2] = fmaf(x[j][k], hu, s[2]);
+                        if constexpr (FULL) {
+                            s[4] += hu;
+                            s[5] = fmaf(h[j][k], e[j][k], s[5]);
+                            s[6] += h[j][k];
+                            if constexpr (NEXT) s[7] = fmaf(h[j][k], x[j][k], s[7]);
+                        }
+                    }
+                }
+            }
+            row_sums(s, red, half);
+            const float k1 = NEXT ? rstd2 * (s[0] * inv_cols) : 0.0f;
+            float k0 = 0.0f, m1 = s[1] - k1 * s[2], m0 = 0.0f;
+            if constexpr (FULL) {
+                k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
+                m1 -= k0 * s[4];
+                m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
+            }
+            m1 = post_norm ? m1 * inv_cols : 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                if (ch < nch) {
+                    float o[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if constexpr (NEXT) e[j][k] -= fmaf(k1, x[j][k], k0);
+                        o[k] = EXIT ? a.residual_scale * e[j][k] : e[j][k];
+                    }
+                    put8((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
+                    if constexpr (EXIT) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            P[j][k] = fmaf(u[j][k], e[j][k], P[j][k]);
+                            if constexpr (FULL) Q[j][k] += e[j][k];
+                            o[k] = rstd1 * (fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1);
+                        }
+                        put8((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
+                    }
+                }
+            }
+        }
+        if constexpr (EXIT) {
+            if (whole_groups) {  // this group is complete: its gate's gradient, and its share of the sums
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                    if (ch < nch) {
+                        float w[8], b[8], gt[8];
+                        vector8(a.weight, a.weight_dtype, c, cols - c, 1.0f, w);
+                        vector8(a.bias, a.bias_dtype, c, cols - c, 0.0f, b);
+                        vector8(a.gate, a.gate_dtype, g * cols + c, cols - c, 1.0f, gt);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float q = FULL ? Q[FULL ? j : 0][k] : 0.0f;
+                            if (a.dgate && c + k < cols)
+                                put_scalar(a.dgate, a.gate_dtype, g * cols + c + k,
+                                           a.branch_scale * fmaf(w[k], P[j][k], b[k] * q));
+                            sums_p[c + k] = fmaf(gt[k], P[j][k], sums_p[c + k]);
+                            P[j][k] = 0.0f;
+                            if constexpr (FULL) {
+                                sums_q[c + k] = fmaf(gt[k], q, sums_q[c + k]);
+                                Q[j][k] = 0.0f;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (EXIT) {
+        if (whole_groups) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr;
+                if (ch < nch) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        P[j][k] = sums_p[ch * CHUNK + k];
+                        if constexpr (FULL) Q[j][k] = sums_q[ch * CHUNK + k];
+                    }
+                }
+            }
+        }
+    }
+    // one partial row a workgroup: its waves' sums are added in their order
+    float* const out = partial + (int64_t)blockIdx.x * plan.vectors * cols;
+    auto finish = [&](auto& acc, int index) {
+        if (index < 0) return;
+        if (ny > 1) {
+            for (int k = 0; k < ny; ++k) {
+                __syncthreads();
+                if (ty == k) {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        const int64_t ch = tid + j * tpr;
+                        if (ch < nch) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                float* at = cols_lds + ch * CHUNK + i;
+                                acc[j][i] = k ? *at + acc[j][i] : acc[j][i];
+                                *at = acc[j][i];
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        if (ty == ny - 1) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                if (ch < nch) {
+                    Raw<float> v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v.a[i] = __float_as_uint(acc[j][i]);
+                        v.b[i] = __float_as_uint(acc[j][i + 4]);
+                    }
+                    put8(out + index * cols + c, v, cols - c);
+                }
+            }
+        }
+    };
+    if constexpr (EXIT) {
+        finish(P, plan.i_p);
+        if constexpr (FULL) finish(Q, plan.i_q);
+    }
+    if constexpr (NEXT) {
+        finish(W2, plan.i_w2);
+        if constexpr (FULL) finish(B2, plan.i_b2);
+    }
+}
+
+// Rows wider than the register kernels take.  A workgroup's column sums are
+// its own partial row in memory, each column added to by one lane.
+template <typename T, typename U, bool EXIT, bool NEXT, bool SRC8>
+__global__ __launch_bounds__(512) void k_norm_backward_wide(const rf_norm a, const NormPlan plan,
+                                                            float* __restrict__ partial)
+{
+    __shared__ float red[2][MAX_WAVES][8];
+    int half = 0;
+    const int tid = threadIdx.x, tpr = blockDim.x;
+    const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
+    const float inv_cols = 1.0f / (float)cols;
+    const bool post_layer = EXIT && a.post == RF_NORM_LAYER, next_layer = NEXT && a.next == RF_NORM_LAYER;
+    const bool post_norm = EXIT && a.post != RF_NORM_NONE;
+    const bool whole_groups = EXIT && plan.pieces == 0;
+    float* const mine = partial + (int64_t)blockIdx.x * plan.vectors * cols;
+    // whole groups: the sums of the current group, behind the partial rows
+    float* const group_sums = partial + ((int64_t)plan.workers * plan.vectors + 2 * (int64_t)blockIdx.x) * cols;
+    for (int64_t ch = tid; ch < nch; ch += tpr)
+        for (int64_t c = ch * CHUNK; c < min(cols, (ch + 1) * CHUNK); ++c) {
+            for (int v = 0; v < plan.vectors; ++v) mine[v * cols + c] = 0.0f;
+            if (whole_groups) group_sums[c] = group_sums[cols + c] = 0.0f;
+        }
+    const int64_t g0 = whole_groups ? part(plan.groups, blockIdx.x, gridDim.x) : blockIdx.x / max(plan.pieces, 1);
+    const int64_t g1 = whole_groups ? part(plan.groups, blockIdx.x + 1, gridDim.x) : g0 + 1;
+    float* const sum_p = whole_groups ? group_sums : mine + (int64_t)max(plan.i_p, 0) * cols;
+    float* const sum_q = whole_groups ? group_sums + cols : mine + (int64_t)max(plan.i_q, 0) * cols;
+    const bool want_q = whole_groups || plan.i_q >= 0;
+    for (int64_t g = g0; g < g1; ++g) {
+        int64_t r0 = g * plan.group_rows, r1 = r0 + plan.group_rows;
+        if (!whole_groups) {
+            const int64_t piece = blockIdx.x % max(plan.pieces, 1);
+            r1 = r0 + part(plan.group_rows, piece + 1, plan.pieces);
+            r0 += part(plan.group_rows, piece, plan.pieces);
+        }
+        for (int64_t r = r0; r < r1; ++r) {
+            const float rstd1 = post_norm ? a.post_rstd[r] : 1.0f, mean1 = post_layer ? a.post_mean[r] : 0.0f;
+            const float rstd2 = NEXT ? a.next_rstd[r] : 0.0f, mean2 = next_layer ? a.next_mean[r] : 0.0f;
+            // e = dhidden + rstd2 g2, xhat, uhat and h of a chunk
+            auto chunk = [&](int64_t ch, float (&e)[8], float (&x)[8], float (&u)[8], float (&h)[8], float (&dy)[8],
+                             float (&g2)[8]) {
+                const int64_t c = ch * CHUNK, left = cols - c;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[k] = x[k] = u[k] = h[k] = dy[k] = g2[k] = 0.0f;
+                if (a.dhidden) widen8(load8((const T*)a.dhidden + r * a.dhidden_stride + c, left), e);
+                if constexpr (NEXT) {
+                    float w[8];
+                    Saved<T, SRC8> hs;
+                    hs.load((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch, cols);
+                    hs.get(x);
+                    widen8(load8((const U*)a.dy + r * a.dy_stride + c, left), dy);
+                    vector8(a.next_weight, a.next_weight_dtype, c, left, 1.0f, w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        x[k] = k < left ? (x[k] - mean2) * rstd2 : 0.0f;
+                        g2[k] = dy[k] * w[k];
+                        e[k] = fmaf(rstd2, g2[k], e[k]);
+                    }
+                }
+                if constexpr (EXIT) {
+                    float gt[8];
+                    Saved<U, SRC8> us;
+                    us.load((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch, cols);
+                    us.get(u);
+                    vector8(a.weight, a.weight_dtype, c, left, 1.0f, h);
+                    vector8(a.gate, a.gate_dtype, g * cols + c, left, 1.0f, gt);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        u[k] = k < left ? (u[k] - mean1) * rstd1 : 0.0f;
+                        h[k] = k < left ? h[k] * a.branch_scale * gt[k] : 0.0f;
+                    }
+                }
+            };
+            float s[8] = {};
+            for (int64_t ch = tid; ch < nch; ch += tpr) {
+                float e[8], x[8], u[8], h[8], dy[8], g2[8];
+                chunk(ch, e, x, u, h, dy, g2);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float hu = h[k] * u[k];
+                    s[0] = fmaf(g2[k], x[k], s[0]);
+                    s[1] = fmaf(e[k], hu, s[1]);
+                    s[2] = fmaf(x[k], hu, s[2]);
+                    s[3] += ch * CHUNK + k < cols ? g2[k] : 0.0f;
+                    s[4] += hu;
+                    s[5] = fmaf(h[k], e[k], s[5]);
+                    s[6] += h[k];
+                    s[7] = fmaf(h[k], x[k], s[7]);
+                }
+            }
+            row_sums(s, red, half);
+            const float k1 = rstd2 * (s[0] * inv_cols), k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
+            const float m1 = post_norm ? (s[1] - k1 * s[2] - k0 * s[4]) * inv_cols : 0.0f;
+            const float m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
+            for (int64_t ch = tid; ch < nch; ch += tpr) {
+                const int64_t c = ch * CHUNK;
+                float e[8], x[8], u[8], h[8], dy[8], g2[8], o[8];
+                chunk(ch, e, x, u, h, dy, g2);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (NEXT) e[k] -= fmaf(k1, x[k], k0);
+                    o[k] = EXIT ? a.residual_scale * e[k] : e[k];
+                }
+                put8((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
+                for (int k = 0; k < 8 && c + k < cols; ++k) {
+                    if constexpr (NEXT) {
+                        if (plan.i_w2 >= 0) mine[plan.i_w2 * cols + c + k] += dy[k] * x[k];
+                        if (plan.i_b2 >= 0) mine[plan.i_b2 * cols + c + k] += dy[k];
+                    }
+                    if constexpr (EXIT) {
+                        if (plan.i_p >= 0) sum_p[c + k] += u[k] * e[k];
+                        if (want_q && plan.i_p >= 0) sum_q[c + k] += e[k];
+                    }
+                }
+                if constexpr (EXIT) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) o[k] = rstd1 * (fmaf(h[k], e[k], -m0) - u[k] * m1);
+                    put8((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
+                }
+            }
+        }
+        if constexpr (EXIT) {
+            if (whole_groups && plan.i_p >= 0) {
+                for (int64_t ch = tid; ch < nch; ch += tpr)
+                    for (int64_t c = ch * CHUNK; c < min(cols, (ch + 1) * CHUNK); ++c) {
+                        const float w = a.weight ? scalar_at(a.weight, a.weight_dtype, c) : 1.0f;
+                        const float b = a.bias ? scalar_at(a.bias, a.bias_dtype, c) : 0.0f;
+                        const float gt = scalar_at(a.gate, a.gate_dtype, g * cols + c);
+                        const float p = sum_p[c], q = sum_q[c];
+                        if (a.dgate) put_scalar(a.dgate, a.gate_dtype, g * cols + c, a.branch_scale * fmaf(w, p, b * q));
+                        mine[plan.i_p * cols + c] += gt * p;
+                        if (plan.i_q >= 0) mine[plan.i_q * cols + c] += gt * q;
+                        sum_p[c] = sum_q[c] = 0.0f;
+                    }
+            }
+        }
+    }
+}
+
+}  // namespace rfb

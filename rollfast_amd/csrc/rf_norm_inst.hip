@@ -1,0 +1,62 @@
+// rf_norm_inst.hip -- the norm kernels of one (residual type, branch type)
+// pair, RFI_T and RFI_U (RF_F32 / RF_BF16 / RF_F16); one object each.
+#include "rf_norm.h"
+#include "rf_norm_launch.h"
+
+namespace rfb {
+
+template <int DT> struct Elem;
+template <> struct Elem<RF_F32> { using type = float; };
+template <> struct Elem<RF_BF16> { using type = bf16; };
+template <> struct Elem<RF_F16> { using type = f16; };
+using T = Elem<RFI_T>::type;
+using U = Elem<RFI_U>::type;
+
+template <bool EXIT, bool NEXT> static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
+{
+    const dim3 grid((unsigned)s.workers), block(s.tpr, s.ny);
+    if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, 1><<<grid, block, 0, st>>>(a);
+    else if (s.nv == 2) k_norm_forward<T, U, EXIT, NEXT, 2><<<grid, block, 0, st>>>(a);
+    else k_norm_forward_wide<T, U, EXIT, NEXT><<<grid, block, 0, st>>>(a);
+}
+
+template <bool EXIT, bool NEXT, bool FULL, bool SRC8>
+static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
+{
+    const dim3 grid((unsigned)p.workers), block(s.tpr, s.ny);
+    if (s.nv == 1) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, 1><<<grid, block, s.lds, st>>>(a, p, partial);
+    else if (s.nv == 2) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, 2><<<grid, block, s.lds, st>>>(a, p, partial);
+    else k_norm_backward_wide<T, U, EXIT, NEXT, SRC8><<<grid, block, 0, st>>>(a, p, partial);
+}
+
+template <bool EXIT, bool NEXT>
+static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
+{
+    if (s.full) {
+        if (s.src8) backward<EXIT, NEXT, true, true>(a, s, p, partial, st);
+        else backward<EXIT, NEXT, true, false>(a, s, p, partial, st);
+    } else {
+        if (s.src8) backward<EXIT, NEXT, false, true>(a, s, p, partial, st);
+        else backward<EXIT, NEXT, false, false>(a, s, p, partial, st);
+    }
+}
+
+#define RFI_CAT2(a, b, c) a##b##_##c
+#define RFI_CAT(a, b, c) RFI_CAT2(a, b, c)
+
+void RFI_CAT(norm_forward_, RFI_T, RFI_U)(const rf_norm& a, const NormShape& s, hipStream_t st)
+{
+    if (a.post == RF_NORM_ABSENT) forward<false, true>(a, s, st);
+    else if (a.next == RF_NORM_ABSENT) forward<true, false>(a, s, st);
+    else forward<true, true>(a, s, st);
+}
+
+void RFI_CAT(norm_backward_, RFI_T, RFI_U)(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial,
+                                           hipStream_t st)
+{
+    if (a.post == RF_NORM_ABSENT) backward<false, true>(a, s, p, partial, st);
+    else if (a.next == RF_NORM_ABSENT) backward<true, false>(a, s, p, partial, st);
+    else backward<true, true>(a, s, p, partial, st);
+}
+
+}  // namespace rfb
