@@ -238,6 +238,8 @@ def linear_weight_grad(dy, checkpoint: ActivationCheckpoint, *, out=None, accumu
         raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {tuple(checkpoint.shape)}: their rows differ")
     v, stride = _rows(dy, "dy")
     outs = dy.shape[-1]
+    if stride >= 1 << 24:  # the kernel addresses a few rows by 32 bits
+        v, stride = v.contiguous(), outs
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
