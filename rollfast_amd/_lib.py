@@ -306,28 +306,49 @@ def lib() -> ctypes.CDLL:
 
 
 _pyhost = None
+_pyblocks = None
+
+
+def _host_module(name: str):
+    import importlib.util
+    import sysconfig
+
+    path = os.path.join(os.path.dirname(LIB_PATH), name + sysconfig.get_config_var("EXT_SUFFIX"))
+    if not os.path.exists(path):
+        raise LibraryMissing(f"{path} is not built; run `python -m rollfast_amd.build` first")
+    spec = importlib.util.spec_from_file_location("rollfast_amd._lib." + name, path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
 
 
 def pyhost():
     """The native host fast-path module ``_rfhost`` (built with the library
     by ``rollfast_amd.build``); raises if it is not built."""
     global _pyhost
-    if _pyhost is not None:
-        return _pyhost
-    import importlib.util
-    import sysconfig
+    if _pyhost is None:
+        from ._base import MaskedNode
 
-    from ._base import MaskedNode
+        mod = _host_module("_rfhost")
+        mod.set_masked_node_type(MaskedNode)
+        _pyhost = mod
+    return _pyhost
 
-    path = os.path.join(os.path.dirname(LIB_PATH), "_rfhost" + sysconfig.get_config_var("EXT_SUFFIX"))
-    if not os.path.exists(path):
-        raise LibraryMissing(f"{path} is not built; run `python -m rollfast_amd.build` first")
-    spec = importlib.util.spec_from_file_location("rollfast_amd._lib._rfhost", path)
-    mod = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(mod)
-    mod.set_masked_node_type(MaskedNode)
-    _pyhost = mod
-    return mod
+
+def pyblocks():
+    """The native host module ``_rfblocks`` of the residual-block operators
+    (built with the library by ``rollfast_amd.build``)."""
+    global _pyblocks
+    if _pyblocks is None:
+        import torch
+
+        L = lib()
+        mod = _host_module("_rfblocks")
+        names = [n for n in EXPORTS if n.startswith(("rf_checkpoint_", "rf_gated_", "rf_norm_", "rf_linear_"))]
+        mod.set_entries({n: ctypes.cast(getattr(L, n), _p).value for n in (*names, "rf_last_error")},
+                        torch._C._cuda_getCurrentRawStream, torch.nn.Parameter)
+        _pyblocks = mod
+    return _pyblocks
 
 
 def check(status: int, what: str) -> None:

@@ -30,19 +30,24 @@ def _stash(ctx, saved):
     """Moves saved's tensors to save_for_backward (which also notices a write
     to one of them before the backward pass)."""
     ctx.set_materialize_grads(False)  # no zeros for the checkpoint's buffers
-    names = [n for n in saved.__slots__ if isinstance(getattr(saved, n, None), torch.Tensor)]
-    ctx.save_for_backward(*(getattr(saved, n) for n in names))
-    ctx.names, ctx.rest = names, {n: getattr(saved, n, None) for n in saved.__slots__ if n not in names}
-    ctx.rest["output"] = None  # the next layer's, not this one's
-    ctx.kind = type(saved)
+    vectors = getattr(saved, "vectors", ())
+    rows = [n for n in saved.__slots__ if n == "arena" or n.endswith("_rows")]
+    ctx.save_for_backward(*vectors, *(getattr(saved, n) for n in rows))
+    ctx.rest = {n: getattr(saved, n) for n in saved.__slots__ if n not in rows and n not in ("vectors", "output")}
+    ctx.rows, ctx.kind = rows, type(saved)
 
 
 def _unstash(ctx):
     saved = ctx.kind()
     for name, value in ctx.rest.items():
         setattr(saved, name, value)
-    for name, value in zip(ctx.names, ctx.saved_tensors):
+    tensors = ctx.saved_tensors
+    vectors = len(tensors) - len(ctx.rows)
+    if vectors:
+        saved.vectors = tensors[:vectors]
+    for name, value in zip(ctx.rows, tensors[vectors:]):
         setattr(saved, name, value)
+    saved.output = None  # the next layer's, not this one's
     return saved
 
 
@@ -95,8 +100,8 @@ class _Postnorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, dy, *_):
         saved = _unstash(ctx)
-        if dy is None and saved.next_rstd is not None:  # y was not used
-            dy = torch.zeros(saved.shape, dtype=saved.branch_dtype, device=saved.next_rstd.device)
+        if dy is None and saved.meta[2]:  # y was not used
+            dy = torch.zeros(saved.shape, dtype=saved.branch_dtype, device=saved.arena.device)
         g = blocks.postnorm_residual_grad(dout, dy, saved)
         return (g.residual, g.branch, g.weight, g.bias, g.gate, g.next_weight, g.next_bias, None)
 

@@ -32,7 +32,6 @@ stream.  Sums are f32 in a fixed order: equal inputs give equal bits.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Any, NamedTuple, Optional
 
@@ -46,7 +45,7 @@ _DTYPE = {torch.float32: _lib.RF_F32, torch.bfloat16: _lib.RF_BF16, torch.float1
 _NORM = {"rms": _lib.RF_NORM_RMS, "layer": _lib.RF_NORM_LAYER}
 _POST = {"none": _lib.RF_NORM_NONE, **_NORM}
 _ACT = {"silu": _lib.RF_ACT_SILU, "gelu": _lib.RF_ACT_GELU, "gelu_tanh": _lib.RF_ACT_GELU_TANH}
-_SAVE = ("int8", "input", None)
+_SAVE = {None: 0, "int8": 1, "input": 2}
 
 
 class ActivationCheckpoint(NamedTuple):
@@ -80,20 +79,48 @@ class PostnormGrads(NamedTuple):
     next_bias: Any
 
 
-class NormSaved:
-    """What ``prenorm_grad`` / ``postnorm_residual_grad`` need.  ``output``:
-    the checkpoint of y, if one was asked for."""
+class _Saved:
+    """What a backward pass needs.  ``arena``: one byte tensor with the codes
+    of each kept row tensor, their exponents and, 16-byte aligned, the f32
+    statistics; ``output``: the checkpoint of the forward pass's output, if one
+    was asked for."""
 
-    __slots__ = ("args", "shape", "dtype", "branch_dtype", "branch", "branch_exponents", "hidden", "hidden_exponents",
-                 "post_mean", "post_rstd", "next_mean", "next_rstd", "weight", "bias", "gate", "next_weight",
-                 "next_bias", "output")
+    __slots__ = ()
+
+    def _kept(self, index: int, count: int):
+        """(codes, exponents) of the arena's checkpoint `index` of `count`."""
+        rows, blocks = math.prod(self.shape[:-1]), -(-self.shape[-1] // BLOCK)
+        codes = rows * blocks * BLOCK
+        at = count * codes + index * rows * blocks
+        return (self.arena[index * codes: (index + 1) * codes].view(torch.int8).view(rows, blocks * BLOCK),
+                self.arena[at: at + rows * blocks].view(rows, blocks))
 
 
-class GatedSaved:
-    """What ``gated_activation_grad`` needs.  ``output``: the checkpoint of h,
-    if one was asked for."""
+class NormSaved(_Saved):
+    """What ``prenorm_grad`` / ``postnorm_residual_grad`` need."""
 
-    __slots__ = ("activation", "shape", "dtype", "fused", "gate", "gate_exponents", "up", "up_exponents", "output")
+    # meta: gates, post, next, branch_scale, residual_scale, save
+    # vectors: weight, bias, gate, next_weight, next_bias
+    __slots__ = ("shape", "dtype", "branch_dtype", "meta", "vectors", "arena", "branch_rows", "hidden_rows", "output")
+
+    def _of(self, name: str, index: int):
+        if self.meta[5] == 2:
+            return (self.branch_rows if name == "branch" else self.hidden_rows), None
+        present = self.meta[1:3]
+        if not present[index]:
+            return None, None
+        return self._kept(index if present[0] else 0, sum(map(bool, present)))
+
+    branch = property(lambda self: self._of("branch", 0)[0])
+    branch_exponents = property(lambda self: self._of("branch", 0)[1])
+    hidden = property(lambda self: self._of("hidden", 1)[0])
+    hidden_exponents = property(lambda self: self._of("hidden", 1)[1])
+
+
+class GatedSaved(_Saved):
+    """What ``gated_activation_grad`` needs."""
+
+    __slots__ = ("activation", "shape", "dtype", "fused", "arena", "gate_rows", "up_rows", "output")
 
 
 # --------------------------------------------------------------- arguments ---
@@ -167,23 +194,19 @@ def _gates(gate, shape, device):
     return (gate.contiguous() if gates else gate), gates  # no gates: no rows
 
 
-def _check_save(save, checkpoint_output: bool):
-    if save not in _SAVE:
+def _check_save(save, checkpoint_output: bool) -> int:
+    mode = _SAVE.get(save)
+    if mode is None:
         raise ValueError(f"save must be 'int8', 'input' or None, got {save!r}")
-    if checkpoint_output and save is None:
+    if checkpoint_output and not mode:
         raise ValueError("checkpoint_output needs save='int8' or 'input'")
+    return mode
 
 
 def _norm_code(norm, table, what: str) -> int:
     if norm not in table:
         raise ValueError(f"{what} must be one of {', '.join(map(repr, table))}, got {norm!r}")
     return table[norm]
-
-
-def _new_codes(rows: int, cols: int, device):
-    blocks = -(-cols // BLOCK)
-    return (torch.empty((rows, blocks * BLOCK), dtype=torch.int8, device=device),
-            torch.empty((rows, blocks), dtype=torch.uint8, device=device))
 
 
 def _check_checkpoint(kept, device=None):
@@ -201,30 +224,45 @@ def _check_checkpoint(kept, device=None):
     return rows, shape[-1]
 
 
+def _host():
+    return _lib.pyblocks()
+
+
+def _must(got, what: str):
+    if got is None:  # `saved` or a checkpoint is not what its call made, or a size is past the kernels' range
+        raise ValueError(f"{what}: arguments that do not fit together, or a size out of range")
+    return got
+
+
+# Every call goes to the native host path first, which takes plain arguments
+# (contiguous tensors of the current device) as they are and returns None for
+# others.  Those are checked and laid out here, on their device, and go there
+# again with the shape of the outputs.
+
+
 # -------------------------------------------------------------- checkpoints ---
 def checkpoint_activations(x) -> ActivationCheckpoint:
     """x in 8-bit blocks of 32 columns."""
-    _tensor(x, "x")
-    code = _code(x.dtype, "x")
-    v, stride = _rows(x, "x")
-    cols = x.shape[-1]
-    rows = x.numel() // cols
-    codes, exps = _new_codes(rows, cols, x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().rf_checkpoint_store(v.data_ptr(), code, rows, cols, stride, codes.data_ptr(),
-                                                  exps.data_ptr(), _lib.stream_ptr()), "checkpoint_activations")
-    return ActivationCheckpoint(codes, exps, tuple(x.shape), x.dtype)
+    kept = _host().checkpoint_store(x, None)
+    if kept is None:
+        _tensor(x, "x")
+        _code(x.dtype, "x")
+        v, _ = _rows(x, "x")
+        with torch.cuda.device(x.device):
+            kept = _must(_host().checkpoint_store(v, tuple(x.shape)), "checkpoint_activations")
+    return ActivationCheckpoint(*kept, tuple(x.shape), x.dtype)
 
 
 def restore_activations(checkpoint: ActivationCheckpoint, *, dtype=None):
     """The values of a checkpoint, in its own dtype or another."""
     dtype = checkpoint.dtype if dtype is None else dtype
-    code = _code(dtype, "output")
-    rows, cols = _check_checkpoint(checkpoint)
-    out = torch.empty(checkpoint.shape, dtype=dtype, device=checkpoint.codes.device)
-    with torch.cuda.device(out.device):
-        _lib.check(_lib.lib().rf_checkpoint_load(checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr(), rows, cols,
-                                                 code, out.data_ptr(), _lib.stream_ptr()), "restore_activations")
+    _code(dtype, "output")
+    _check_checkpoint(checkpoint)
+    args = (checkpoint.codes, checkpoint.exponents, tuple(checkpoint.shape), dtype)
+    out = _host().checkpoint_load(*args)
+    if out is None:
+        with torch.cuda.device(checkpoint.codes.device):
+            out = _must(_host().checkpoint_load(*args), "restore_activations")
     return out
 
 
@@ -233,43 +271,32 @@ def linear_weight_grad(dy, checkpoint: ActivationCheckpoint, *, out=None, accumu
     ``dy`` [..., outs] and the checkpoint of x [..., cols].  ``out``: written,
     or added to with ``accumulate``; else a new tensor of ``dtype`` (dy's)."""
     _tensor(dy, "dy")
-    rows, cols = _check_checkpoint(checkpoint, dy.device)
-    if dy.dim() == 0 or dy.shape[:-1] != tuple(checkpoint.shape[:-1]):
+    _, cols = _check_checkpoint(checkpoint, dy.device)
+    if dy.dim() == 0 or tuple(dy.shape[:-1]) != tuple(checkpoint.shape[:-1]):
         raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {tuple(checkpoint.shape)}: their rows differ")
-    v, stride = _rows(dy, "dy")
     outs = dy.shape[-1]
-    if stride >= 1 << 24:  # the kernel addresses a few rows by 32 bits
-        v, stride = v.contiguous(), outs
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty((outs, cols), dtype=dy.dtype if dtype is None else dtype, device=dy.device)
+        if dtype is not None:
+            _code(dtype, "out")
     else:
         _tensor(out, "out", dy.device)
+        _code(out.dtype, "out")
         if out.shape != (outs, cols) or not out.is_contiguous():
             raise ValueError(f"out must be contiguous with shape {(outs, cols)}, got {tuple(out.shape)}")
         if dtype is not None and dtype != out.dtype:
             raise ValueError(f"out is {out.dtype}, dtype says {dtype}")
-    a = _lib.WeightGrad()
-    a.rows, a.outs, a.cols = rows, outs, cols
-    a.dy_dtype, a.out_dtype = _code(dy.dtype, "dy"), _code(out.dtype, "out")
-    a.dy, a.dy_stride = v.data_ptr(), stride
-    a.codes, a.exponents = checkpoint.codes.data_ptr(), checkpoint.exponents.data_ptr()
-    a.out, a.accumulate = out.data_ptr(), int(accumulate)
-    with torch.cuda.device(dy.device):
-        space, size = _workspace(_lib.lib().rf_linear_weight_grad_workspace, a, dy.device, "linear_weight_grad")
-        _lib.check(_lib.lib().rf_linear_weight_grad(a, space, size, _lib.stream_ptr()), "linear_weight_grad")
-    return out
-
-
-def _workspace(query, args, device, what: str):
-    """(device pointer, bytes) of a call's workspace: memory of the current
-    stream, which torch hands out again only behind the call's work."""
-    size = ctypes.c_int64()
-    _lib.check(query(args, size), what)
-    if not size.value:
-        return None, 0
-    return torch.empty(size.value, dtype=torch.uint8, device=device).data_ptr(), size.value
+    rest = (checkpoint.codes, checkpoint.exponents, cols, out, accumulate, dtype)
+    got = _host().weight_grad(dy, None, *rest)
+    if got is None:
+        _code(dy.dtype, "dy")
+        v, stride = _rows(dy, "dy")
+        if stride >= 1 << 24:  # the kernel addresses a few rows by 32 bits
+            v = v.contiguous()
+        with torch.cuda.device(dy.device):
+            got = _must(_host().weight_grad(v, tuple(dy.shape), *rest), "linear_weight_grad")
+    return got
 
 
 # ---------------------------------------------------------- gated activation ---
@@ -278,100 +305,65 @@ def gated_activation(gate, up=None, *, activation: str = "silu", save: Optional[
     """``h = act(gate) * up`` -> (h, saved).  Without ``up`` the gate's last
     dimension holds both, the gate first (one product's output).
     ``activation``: 'silu', 'gelu' (with the error function) or 'gelu_tanh'."""
-    _check_save(save, checkpoint_output)
-    if activation not in _ACT:
+    mode = _check_save(save, checkpoint_output)
+    act = _ACT.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(map(repr, _ACT))}, got {activation!r}")
-    _tensor(gate, "gate")
-    code = _code(gate.dtype, "gate")
-    fused = up is None
-    if fused:
-        if gate.dim() == 0 or gate.shape[-1] == 0 or gate.shape[-1] % 2:
+    g, u = gate, up
+    got = _host().gated_forward(gate, up, None, act, mode, checkpoint_output)
+    if got is None:
+        _tensor(gate, "gate")
+        _code(gate.dtype, "gate")
+        if up is None and (gate.dim() == 0 or gate.shape[-1] == 0 or gate.shape[-1] % 2):
             raise ValueError(f"without up the gate's last dimension holds both halves, got shape {tuple(gate.shape)}")
-        both, stride = _rows(gate, "gate")
-        cols = gate.shape[-1] // 2
-        both = both.as_strided((gate.numel() // (2 * cols), 2 * cols), (stride, 1))
-        g, u, gs, us = both[:, :cols], both[:, cols:], stride, stride
-    else:
-        g, gs = _rows(gate, "gate")
-        u, us = _like(up, gate.shape, gate.dtype, "up", gate.device)
-        cols = gate.shape[-1]
-    shape = (*gate.shape[:-1], cols)
-    rows, device = math.prod(shape[:-1]), gate.device
-    h = torch.empty(shape, dtype=gate.dtype, device=device)
-    a = _lib.Gated()
-    a.rows, a.cols, a.dtype, a.activation = rows, cols, code, _ACT[activation]
-    a.gate, a.up, a.gate_stride, a.up_stride, a.h = g.data_ptr(), u.data_ptr(), gs, us, h.data_ptr()
-    saved = None
-    if save is not None:
-        saved = GatedSaved()
-        saved.activation, saved.shape, saved.dtype, saved.fused = activation, shape, gate.dtype, fused
-        saved.output = saved.gate_exponents = saved.up_exponents = None
-        if save == "int8":
-            (saved.gate, saved.gate_exponents), (saved.up, saved.up_exponents) = (_new_codes(rows, cols, device)
-                                                                                  for _ in range(2))
-            a.gate_codes, a.gate_exponents = saved.gate.data_ptr(), saved.gate_exponents.data_ptr()
-            a.up_codes, a.up_exponents = saved.up.data_ptr(), saved.up_exponents.data_ptr()
-        else:
-            saved.gate, saved.up = g.as_strided((rows, cols), (gs, 1)), u.as_strided((rows, cols), (us, 1))
-        if checkpoint_output:
-            saved.output = ActivationCheckpoint(*_new_codes(rows, cols, device), shape, gate.dtype)
-            a.h_codes, a.h_exponents = saved.output.codes.data_ptr(), saved.output.exponents.data_ptr()
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().rf_gated_forward(a, _lib.stream_ptr()), "gated_activation")
+        g, _ = _rows(gate, "gate")
+        u = None if up is None else _like(up, gate.shape, gate.dtype, "up", gate.device)[0]
+        with torch.cuda.device(gate.device):
+            got = _must(_host().gated_forward(g, u, tuple(gate.shape), act, mode, checkpoint_output), "gated_activation")
+    h, arena, codes, exps = got
+    if not mode:
+        return h, None
+    saved = GatedSaved()
+    saved.activation, saved.shape, saved.dtype, saved.fused, saved.arena = act, h.shape, h.dtype, up is None, arena
+    saved.gate_rows = saved.up_rows = None
+    if mode == 2:
+        g = _rows(g, "gate")[0].view(-1, g.shape[-1]) if g.numel() else g.reshape(0, g.shape[-1])
+        cols = h.shape[-1]
+        saved.gate_rows = g[:, :cols]
+        saved.up_rows = g[:, cols:] if up is None else u.view(g.shape)
+    saved.output = ActivationCheckpoint(codes, exps, tuple(h.shape), h.dtype) if checkpoint_output else None
     return h, saved
 
 
 def gated_activation_grad(dh, saved: GatedSaved):
     """(dgate, dup); one tensor that holds both where the forward pass took one."""
-    shape, dtype, device = saved.shape, saved.dtype, saved.gate.device
-    v, stride = _like(dh, shape, dtype, "dh", device)
-    cols = shape[-1]
-    rows = math.prod(shape[:-1])
-    a = _lib.Gated()
-    a.rows, a.cols, a.dtype, a.activation = rows, cols, _DTYPE[dtype], _ACT[saved.activation]
-    if saved.gate_exponents is not None:
-        a.gate_codes, a.gate_exponents = saved.gate.data_ptr(), saved.gate_exponents.data_ptr()
-        a.up_codes, a.up_exponents = saved.up.data_ptr(), saved.up_exponents.data_ptr()
-    else:
-        a.gate, a.gate_stride = saved.gate.data_ptr(), saved.gate.stride(0)
-        a.up, a.up_stride = saved.up.data_ptr(), saved.up.stride(0)
-    a.dh, a.dh_stride = v.data_ptr(), stride
-    if saved.fused:
-        out = torch.empty((*shape[:-1], 2 * cols), dtype=dtype, device=device)
-        a.dgate, a.dup = out.data_ptr(), out.data_ptr() + cols * out.element_size()
-        a.dgate_stride = a.dup_stride = 2 * cols
-    else:
-        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
-        a.dgate, a.dup = out[0].data_ptr(), out[1].data_ptr()
-        a.dgate_stride = a.dup_stride = cols
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().rf_gated_backward(a, _lib.stream_ptr()), "gated_activation_grad")
-    return out
+    rest = (saved.activation, saved.fused, saved.arena, saved.gate_rows, saved.up_rows)
+    like = saved.gate_rows if saved.arena is None else saved.arena
+    got = None
+    if isinstance(dh, torch.Tensor) and dh.shape == saved.shape and dh.dtype == saved.dtype and dh.device == like.device:
+        got = _host().gated_backward(dh, None, *rest)
+    if got is None:
+        v, _ = _like(dh, saved.shape, saved.dtype, "dh", like.device)
+        with torch.cuda.device(like.device):
+            got = _must(_host().gated_backward(v, tuple(saved.shape), *rest), "gated_activation_grad")
+    return got
 
 
 # ---------------------------------------------------------------------- norms ---
-def _put_vector(a, name: str, v):
-    if v is not None:
-        setattr(a, name, v.data_ptr())
-        setattr(a, name + "_dtype", _DTYPE[v.dtype])
-
-
-def _stats(a, part: str, kind: int, rows: int, device, saved):
-    """The row statistics that the backward pass needs, one buffer a part."""
-    mean = kind == _lib.RF_NORM_LAYER
-    if kind not in (_lib.RF_NORM_RMS, _lib.RF_NORM_LAYER):
-        return
-    rstd = torch.empty(rows * (2 if mean else 1), dtype=torch.float32, device=device)
-    setattr(a, part + "_rstd", rstd.data_ptr())
-    setattr(saved, part + "_rstd", rstd)
-    if mean:
-        setattr(a, part + "_mean", rstd.data_ptr() + 4 * rows)
-
-
-def _new_saved():
+def _save_norm(got, shape, dtype, meta, vectors, branch, hidden):
+    """NormSaved of a forward pass's results."""
+    out, y, arena, gates, codes, exps = got
     saved = NormSaved()
-    for name in NormSaved.__slots__:
-        setattr(saved, name, None)
+    saved.shape, saved.dtype, saved.branch_dtype = shape, dtype, (y if branch is None else branch).dtype
+    saved.meta, saved.vectors, saved.arena = (gates, *meta), vectors, arena
+    saved.branch_rows = saved.hidden_rows = None
+    if meta[4] == 2:
+        cols = shape[-1]
+        if branch is not None:
+            saved.branch_rows = branch.reshape(branch.numel() // cols, cols)
+        if y is not None:
+            saved.hidden_rows = hidden.reshape(hidden.numel() // cols, cols)
+    saved.output = None if codes is None else ActivationCheckpoint(codes, exps, tuple(shape), y.dtype)
     return saved
 
 
@@ -381,50 +373,22 @@ def prenorm(x, weight=None, bias=None, *, norm: str = "rms", eps: float = 1e-6, 
     ``y = (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias`` for
     norm='layer', without the means for 'rms'.  ``dtype``: y's (x's; a 16-bit
     type beside a float32 x)."""
-    _check_save(save, checkpoint_output)
-    _tensor(x, "x")
-    device, cols = x.device, x.shape[-1] if x.dim() else 0
-    v, stride = _rows(x, "x")
-    rows = x.numel() // cols
-    a = _lib.Norm()
-    a.rows, a.cols = rows, cols
-    a.dtype, a.next, a.next_eps = _code(x.dtype, "x"), _norm_code(norm, _NORM, "norm"), eps
-    out_dtype = x.dtype if dtype is None else dtype
-    a.branch_dtype = _code(out_dtype, "y")
-    weight, bias = _vector(weight, cols, "weight", device), _vector(bias, cols, "bias", device)
-    _put_vector(a, "next_weight", weight)
-    _put_vector(a, "next_bias", bias)
-    y = torch.empty(x.shape, dtype=out_dtype, device=device)
-    a.hidden, a.hidden_stride, a.y = v.data_ptr(), stride, y.data_ptr()
-    saved = None
-    if save is not None:
-        saved = _new_saved()
-        saved.shape, saved.dtype, saved.branch_dtype = x.shape, x.dtype, out_dtype
-        saved.next_weight, saved.next_bias = weight, bias
-        _stats(a, "next", a.next, rows, device, saved)
-        _keep(a, "hidden", save, v, stride, rows, cols, device, saved)
-        _keep_output(a, checkpoint_output, rows, cols, x.shape, out_dtype, device, saved)
-        saved.args = (rows, cols, 0, _lib.RF_NORM_ABSENT, a.next, 1.0, 1.0)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().rf_norm_forward(a, _lib.stream_ptr()), "prenorm")
-    return y, saved
-
-
-def _keep(a, name: str, save: str, v, stride: int, rows: int, cols: int, device, saved):
-    if save == "int8":
-        codes, exps = _new_codes(rows, cols, device)
-        setattr(a, name + "_codes", codes.data_ptr())
-        setattr(a, name + "_exponents", exps.data_ptr())
-        setattr(saved, name, codes)
-        setattr(saved, name + "_exponents", exps)
-    else:
-        setattr(saved, name, v.as_strided((rows, cols), (stride, 1)))
-
-
-def _keep_output(a, wanted: bool, rows: int, cols: int, shape, dtype, device, saved):
-    if wanted:
-        saved.output = ActivationCheckpoint(*_new_codes(rows, cols, device), tuple(shape), dtype)
-        a.y_codes, a.y_exponents = saved.output.codes.data_ptr(), saved.output.exponents.data_ptr()
+    mode = _check_save(save, checkpoint_output)
+    rest = (0, _norm_code(norm, _NORM, "norm"), 0.0, eps, 1.0, 1.0, dtype, mode, checkpoint_output)
+    v, vectors = x, (None, None, None, weight, bias)
+    if dtype is not None:
+        _code(dtype, "y")
+    got = _host().norm_forward(x, None, None, vectors, *rest)
+    if got is None:
+        _tensor(x, "x")
+        _code(x.dtype, "x")
+        v, cols = _rows(x, "x")[0], x.shape[-1]
+        vectors = (None, None, None, _vector(weight, cols, "weight", x.device), _vector(bias, cols, "bias", x.device))
+        with torch.cuda.device(x.device):
+            got = _must(_host().norm_forward(v, None, tuple(x.shape), vectors, *rest), "prenorm")
+    if not mode:
+        return got[1], None
+    return got[1], _save_norm(got, x.shape, x.dtype, (*rest[:2], 1.0, 1.0, mode), vectors, None, v)
 
 
 def postnorm_residual(residual, branch, weight=None, bias=None, gate=None, *, norm: str = "rms", eps: float = 1e-6,
@@ -439,122 +403,71 @@ def postnorm_residual(residual, branch, weight=None, bias=None, gate=None, *, no
     last that share a gate ([sequences, 1, cols] for a gate per sequence).
     ``branch`` and y have one dtype: the residual's, or 16 bits beside a
     float32 residual."""
-    _check_save(save, checkpoint_output)
-    if checkpoint_output and next_norm is None:
-        raise ValueError("checkpoint_output needs next_norm")
-    _tensor(residual, "residual")
-    _tensor(branch, "branch", residual.device)
-    device, cols = residual.device, residual.shape[-1] if residual.dim() else 0
-    r, rs = _rows(residual, "residual")
-    u, us = _like(branch, residual.shape, branch.dtype, "branch", device)
-    rows = residual.numel() // cols
-    a = _lib.Norm()
-    a.rows, a.cols = rows, cols
-    a.dtype, a.branch_dtype = _code(residual.dtype, "residual"), _code(branch.dtype, "branch")
-    a.post, a.post_eps = _norm_code(norm, _POST, "norm"), eps
-    if a.post == _lib.RF_NORM_NONE and (weight is not None or bias is not None):
+    mode = _check_save(save, checkpoint_output)
+    post = _norm_code(norm, _POST, "norm")
+    follows = 0 if next_norm is None else _norm_code(next_norm, _NORM, "next_norm")
+    if not follows and (checkpoint_output or next_weight is not None or next_bias is not None):
+        raise ValueError("next_weight, next_bias and checkpoint_output need next_norm")
+    if post == _lib.RF_NORM_NONE and (weight is not None or bias is not None):
         raise ValueError("norm='none' takes no weight or bias")
-    a.branch_scale, a.residual_scale = branch_scale, residual_scale
-    weight, bias = _vector(weight, cols, "weight", device), _vector(bias, cols, "bias", device)
-    gate_rows, a.gates = _gates(gate, residual.shape, device)
-    _put_vector(a, "weight", weight)
-    _put_vector(a, "bias", bias)
-    _put_vector(a, "gate", gate_rows)
-    out = torch.empty(residual.shape, dtype=residual.dtype, device=device)
-    a.residual, a.residual_stride, a.branch, a.branch_stride = r.data_ptr(), rs, u.data_ptr(), us
-    a.hidden, a.hidden_stride = out.data_ptr(), cols
-    y = None
-    if next_norm is not None:
-        a.next, a.next_eps = _norm_code(next_norm, _NORM, "next_norm"), next_eps
-        next_weight = _vector(next_weight, cols, "next_weight", device)
-        next_bias = _vector(next_bias, cols, "next_bias", device)
-        _put_vector(a, "next_weight", next_weight)
-        _put_vector(a, "next_bias", next_bias)
-        y = torch.empty(residual.shape, dtype=branch.dtype, device=device)
-        a.y = y.data_ptr()
-    elif next_weight is not None or next_bias is not None:
-        raise ValueError("next_weight and next_bias need next_norm")
-    saved = None
-    if save is not None:
-        saved = _new_saved()
-        saved.shape, saved.dtype, saved.branch_dtype = residual.shape, residual.dtype, branch.dtype
-        saved.weight, saved.bias, saved.gate = weight, bias, gate_rows
-        saved.next_weight, saved.next_bias = next_weight, next_bias
-        _stats(a, "post", a.post, rows, device, saved)
-        _keep(a, "branch", save, u, us, rows, cols, device, saved)
-        if y is not None:
-            _stats(a, "next", a.next, rows, device, saved)
-            _keep(a, "hidden", save, out, cols, rows, cols, device, saved)
-            _keep_output(a, checkpoint_output, rows, cols, residual.shape, branch.dtype, device, saved)
-        saved.args = (rows, cols, a.gates, a.post, a.next, branch_scale, residual_scale)
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().rf_norm_forward(a, _lib.stream_ptr()), "postnorm_residual")
-    return out, y, saved
+    rest = (post, follows, eps, next_eps, branch_scale, residual_scale, None, mode, checkpoint_output)
+    r, u, vectors = residual, branch, (weight, bias, gate, next_weight, next_bias)
+    got = _host().norm_forward(residual, branch, None, vectors, *rest)
+    if got is None:
+        device = _tensor(residual, "residual").device
+        _tensor(branch, "branch", device)
+        _code(residual.dtype, "residual")
+        _code(branch.dtype, "branch")
+        r, cols = _rows(residual, "residual")[0], residual.shape[-1]
+        u, _ = _like(branch, residual.shape, branch.dtype, "branch", device)
+        vectors = (_vector(weight, cols, "weight", device), _vector(bias, cols, "bias", device),
+                   _gates(gate, residual.shape, device)[0], _vector(next_weight, cols, "next_weight", device),
+                   _vector(next_bias, cols, "next_bias", device))
+        with torch.cuda.device(device):
+            got = _must(_host().norm_forward(r, u, tuple(residual.shape), vectors, *rest), "postnorm_residual")
+    if not mode:
+        return got[0], got[1], None
+    saved = _save_norm(got, residual.shape, residual.dtype, (post, follows, branch_scale, residual_scale, mode), vectors,
+                       u, got[0])
+    return got[0], got[1], saved
 
 
-def _norm_grad(dhidden, dy, saved: NormSaved, what: str):
-    a = _lib.Norm()
-    a.rows, a.cols, a.gates, a.post, a.next, a.branch_scale, a.residual_scale = saved.args
-    rows, cols, device, shape = a.rows, a.cols, (saved.branch if a.post else saved.hidden).device, saved.shape
-    a.dtype, a.branch_dtype = _DTYPE[saved.dtype], _DTYPE[saved.branch_dtype]
-    keep = []
-    if dhidden is not None:
-        v, a.dhidden_stride = _like(dhidden, shape, saved.dtype, "dout" if a.post else "dresidual", device)
-        a.dhidden = v.data_ptr()
-        keep.append(v)
-    if a.next:
-        if dy is None:
-            raise ValueError("dy is missing")
-        v, a.dy_stride = _like(dy, shape, saved.branch_dtype, "dy", device)
-        a.dy = v.data_ptr()
-        keep.append(v)
-    elif dy is not None:
+def _norm_grad(dhidden, dy, saved: NormSaved):
+    post, follows = saved.meta[1:3]
+    if follows and dy is None:
+        raise ValueError("dy is missing")
+    if not follows and dy is not None:
         raise ValueError("dy without a next norm")
-    for part in ("post", "next"):
-        rstd = getattr(saved, part + "_rstd")
-        if rstd is not None:
-            setattr(a, part + "_rstd", rstd.data_ptr())
-            setattr(a, part + "_mean", rstd.data_ptr() + 4 * rows if rstd.numel() == 2 * rows else None)
-    for name in ("branch", "hidden"):
-        t, exps = getattr(saved, name), getattr(saved, name + "_exponents")
-        if exps is not None:
-            setattr(a, name + "_codes", t.data_ptr())
-            setattr(a, name + "_exponents", exps.data_ptr())
-        elif t is not None:
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + "_stride", t.stride(0))
-    grads = {}
-    for name in ("weight", "bias", "gate", "next_weight", "next_bias"):
-        v = getattr(saved, name)
-        grads[name] = None
-        if v is not None:
-            _put_vector(a, name, v)
-            grads[name] = torch.empty_like(v)
-            setattr(a, "d" + name, grads[name].data_ptr())
-    dresidual = torch.empty(shape, dtype=saved.dtype, device=device)
-    a.dresidual, dbranch = dresidual.data_ptr(), None
-    if a.post:
-        dbranch = torch.empty(shape, dtype=saved.branch_dtype, device=device)
-        a.dbranch = dbranch.data_ptr()
-    with torch.cuda.device(device):
-        space, size = _workspace(_lib.lib().rf_norm_backward_workspace, a, device, what)
-        _lib.check(_lib.lib().rf_norm_backward(a, space, size, _lib.stream_ptr()), what)
-    return dresidual, dbranch, grads
+    rest = (saved.vectors, saved.meta, saved.dtype, saved.branch_dtype, saved.arena, saved.branch_rows, saved.hidden_rows)
+    shape, device = saved.shape, saved.arena.device
+    got = None
+    lead = dy if follows else dhidden
+    if lead is None and not follows:
+        dhidden = lead = torch.zeros(shape, dtype=saved.dtype, device=device)
+    if isinstance(lead, torch.Tensor) and lead.shape == shape:
+        got = _host().norm_backward(dhidden, dy, None, *rest)
+    if got is None:
+        if dhidden is not None:
+            dhidden, _ = _like(dhidden, shape, saved.dtype, "dout" if post else "dresidual", device)
+        if follows:
+            dy, _ = _like(dy, shape, saved.branch_dtype, "dy", device)
+        with torch.cuda.device(device):
+            got = _must(_host().norm_backward(dhidden, dy, tuple(shape), *rest), "the norm's gradient")
+    return got
 
 
 def prenorm_grad(dy, saved: NormSaved, *, dresidual=None) -> PrenormGrads:
     """Gradients of ``prenorm``'s x, weight and bias.  ``dresidual``: another
     gradient at x (the residual path's), added to x's in the same pass."""
-    if saved.args[3] != _lib.RF_NORM_ABSENT:
+    if saved.meta[1] != _lib.RF_NORM_ABSENT:
         raise ValueError("saved is postnorm_residual's: use postnorm_residual_grad")
-    dx, _, g = _norm_grad(dresidual, dy, saved, "prenorm_grad")
-    return PrenormGrads(dx, g["next_weight"], g["next_bias"])
+    got = _norm_grad(dresidual, dy, saved)
+    return PrenormGrads(got[0], got[5], got[6])
 
 
 def postnorm_residual_grad(dout, dy, saved: NormSaved) -> PostnormGrads:
     """Gradients of ``postnorm_residual`` from those of out (None: zero) and,
     with a next norm, of y."""
-    if saved.args[3] == _lib.RF_NORM_ABSENT:
+    if saved.meta[1] == _lib.RF_NORM_ABSENT:
         raise ValueError("saved is prenorm's: use prenorm_grad")
-    dr, du, g = _norm_grad(dout, dy, saved, "postnorm_residual_grad")
-    return PostnormGrads(dr, du, g["weight"], g["bias"], g["gate"], g["next_weight"], g["next_bias"])
+    return PostnormGrads(*_norm_grad(dout, dy, saved))

@@ -28,6 +28,8 @@ HOST_SRC = os.path.join(CSRC, "rf_host.hip")
 # The native host fast path of the fused step: a CPython module built against
 # torch's C++ headers (tensor data pointers without a Python call).
 PYHOST_SRC = os.path.join(CSRC, "rf_pyhost.cpp")
+# The native host path of the residual-block operators, likewise.
+PYBLOCKS_SRC = os.path.join(CSRC, "rf_pyblocks.cpp")
 INST_SRC = os.path.join(CSRC, "rf_adam8_inst.hip")
 TILE_SRC = os.path.join(CSRC, "rf_tile_inst.hip")
 # One object per (apply, moment SR, exact) instance of the step kernels.
@@ -81,14 +83,14 @@ def _compile_jobs():
     return jobs
 
 
-def pyhost_path() -> str:
+def pyhost_path(name: str = "_rfhost") -> str:
     import sysconfig
 
-    return os.path.join(OUT_DIR, "_rfhost" + sysconfig.get_config_var("EXT_SUFFIX"))
+    return os.path.join(OUT_DIR, name + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def _pyhost_job():
-    """g++ command for the host fast-path module (compiled and linked at once)."""
+def _pyhost_job(name: str = "_rfhost", source: str = PYHOST_SRC):
+    """g++ command for a native host module (compiled and linked at once)."""
     import sysconfig
 
     import torch
@@ -99,11 +101,15 @@ def _pyhost_job():
                                                                f"-I{os.path.join(REPO, 'include')}"]
     libdirs = cpp_extension.library_paths()
     libs = [f"-L{d}" for d in libdirs] + [f"-Wl,-rpath,{d}" for d in libdirs]
-    out = pyhost_path() + ".tmp"
+    out = pyhost_path(name) + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, PYHOST_SRC, "-o", out, *libs,
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, source, "-o", out, *libs,
            "-ltorch_python", "-ltorch", "-lc10"]
     return cmd, out
+
+
+def _pyblocks_job():
+    return _pyhost_job("_rfblocks", PYBLOCKS_SRC)
 
 
 def _sources_of(obj: str) -> list:
@@ -123,6 +129,8 @@ def _sources_of(obj: str) -> list:
         return [TILE_SRC, *dev, *inc]
     if obj.endswith(".o"):
         return [INST_SRC, *dev, *inc]
+    if os.path.basename(obj).startswith("_rfblocks"):
+        return [PYBLOCKS_SRC, *inc, __file__]
     return [PYHOST_SRC, *inc, __file__]
 
 
@@ -140,10 +148,10 @@ def build(verbose: bool = False, jobs: int | None = None, incremental: bool = Fa
     os.makedirs(OBJ_DIR, exist_ok=True)
     max_par = jobs or min(len(_compile_jobs()), max(1, os.cpu_count() or 1))
     # the moment-SR objects compile longest: first, so that none runs alone at the end
-    pending = sorted(_compile_jobs(), key=lambda job: ("_m1_" not in job[1], "tile" in job[1])) + [_pyhost_job()]
+    pending = sorted(_compile_jobs(), key=lambda job: ("_m1_" not in job[1], "tile" in job[1]))
+    pending += [_pyhost_job(), _pyblocks_job()]
     if incremental:
-        pending = [(cmd, obj) for cmd, obj in pending
-                   if _stale(pyhost_path() if obj.endswith(".tmp") else obj)]
+        pending = [(cmd, obj) for cmd, obj in pending if _stale(obj.removesuffix(".tmp"))]
     def compile_one(job):
         cmd, obj = job
         if verbose:
@@ -157,8 +165,9 @@ def build(verbose: bool = False, jobs: int | None = None, incremental: bool = Fa
         for obj, out in failures:
             sys.stderr.write(f"--- {obj}\n{out}\n")
         raise RuntimeError(f"compilation failed for {len(failures)} object(s)")
-    if os.path.exists(pyhost_path() + ".tmp"):
-        os.replace(pyhost_path() + ".tmp", pyhost_path())
+    for path in (pyhost_path(), pyhost_path("_rfblocks")):
+        if os.path.exists(path + ".tmp"):
+            os.replace(path + ".tmp", path)
     tmp = LIB_PATH + ".tmp"
     objs = [obj for _, obj in _compile_jobs()]
     link = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", f"-Wl,-soname,{SONAME}", "-o", tmp, *objs]

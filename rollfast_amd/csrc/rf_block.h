@@ -29,6 +29,7 @@ typedef _Float16 f16;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_at __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32_at __attribute__((aligned(2)));
 typedef uint32_t u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -45,35 +46,88 @@ template <> struct Raw<float> { u32x4 a, b; };
 
 template <typename T> __device__ __forceinline__ Raw<T> zero8() { return Raw<T>{}; }
 
-// Elements p[0 .. 7]; those at and past `left` read as zero and are not
-// touched (left may be zero or negative).
-template <typename T> __device__ __forceinline__ Raw<T> load8(const T* p, int64_t left)
+// Loads go in two halves so that a row's loads, and the next row's, are in
+// flight together.  fetch8: eight columns from c of a row of at least eight, as
+// one unconditional load; a chunk that the row ends in, or before, is loaded
+// from the row's last eight columns instead.  (With a condition around it the
+// compiler could not count the loads in flight, and would wait for all.)
+// settle8: moves such a chunk's own columns to its front and clears the others;
+// only waves that hold one branch there.
+template <typename T> __device__ __forceinline__ Raw<T> fetch8(const T* row, int64_t c, int64_t cols)
+{
+    Raw<T> r;
+    const T* const p = row + min(c, cols - CHUNK);
+    r.a = *(const u32x4_at*)p;
+    if constexpr (sizeof(T) == 4) r.b = *(const u32x4_at*)(p + 4);
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void settle8(Raw<T>& r, int64_t c, int64_t cols)
+{
+    const int64_t left = cols - c;
+    if (left >= CHUNK || cols < CHUNK) return;  // (narrow rows: load8 put them in place)
+    if (left <= 0) {
+        r = Raw<T>{};
+        return;
+    }
+    const int by = CHUNK - (int)left;  // 1 .. 7
+    uint32_t w[CHUNK];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        w[k] = r.a[k];
+        if constexpr (sizeof(T) == 4) w[k + 4] = r.b[k];
+        else w[k + 4] = 0;
+    }
+    // whole words, by the bits of their number
+    const int words = sizeof(T) == 4 ? by : by >> 1;
+#pragma unroll
+    for (int bit = 1; bit < CHUNK; bit *= 2) {
+#pragma unroll
+        for (int k = 0; k < CHUNK; ++k) {
+            const uint32_t v = k + bit < CHUNK ? w[k + bit] : 0u;
+            w[k] = words & bit ? v : w[k];
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            r.a[k] = w[k];
+            r.b[k] = w[k + 4];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.a[k] = by & 1 ? (w[k] >> 16) | (w[k + 1] << 16) : w[k];
+    }
+}
+
+// Both at once, in rows of any width.
+template <typename T> __device__ __forceinline__ Raw<T> load8(const T* row, int64_t c, int64_t cols)
 {
     Raw<T> r{};
-    if (left >= CHUNK) {
-        if constexpr (sizeof(T) == 4) {
-            r.a = *(const u32x4_at*)p;
-            r.b = *(const u32x4_at*)(p + 4);
-        } else {
-            r.a = *(const u32x4_at*)p;
-        }
-    } else if (left > 0) {
-        const int n = (int)left;
-        if constexpr (sizeof(T) == 4) {
-            const uint32_t* q = (const uint32_t*)p;
+    if (cols >= CHUNK) {
+        r = fetch8(row, c, cols);
+        settle8(r, c, cols);
+        return r;
+    }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (k < n) r.a[k] = q[k];
-                if (k + 4 < n) r.b[k] = q[k + 4];
+    for (int k = 0; k < CHUNK - 1; ++k) {
+        if (c + k < cols) {
+            if constexpr (sizeof(T) == 4) {
+                const uint32_t w = ((const uint32_t*)row)[c + k];
+                if (k < 4) r.a[k & 3] = w;
+                else r.b[k & 3] = w;
+            } else {
+                r.a[k >> 1] |= (uint32_t)((const uint16_t*)row)[c + k] << (16 * (k & 1));
             }
-        } else {
-            const uint16_t* q = (const uint16_t*)p;
-#pragma unroll
-            for (int k = 0; k < CHUNK; ++k)
-                if (k < n) r.a[k >> 1] |= (uint32_t)q[k] << (16 * (k & 1));
         }
     }
     return r;
+}
+
+// As fetch8, in rows of any width.
+template <typename T> __device__ __forceinline__ Raw<T> fetch8_any(const T* row, int64_t c, int64_t cols)
+{
+    return cols >= CHUNK ? fetch8(row, c, cols) : load8(row, c, cols);
 }
 
 template <typename T> __device__ __forceinline__ void widen8(const Raw<T>& r, float (&v)[8])
@@ -130,6 +184,7 @@ template <typename T> __device__ __forceinline__ Raw<T> narrow8(const float (&v)
     return r;
 }
 
+// Stores the first `left` of eight elements.
 template <typename T> __device__ __forceinline__ void put8(T* p, const Raw<T>& r, int64_t left)
 {
     if (left >= CHUNK) {
@@ -138,34 +193,80 @@ template <typename T> __device__ __forceinline__ void put8(T* p, const Raw<T>& r
     } else if (left > 0) {
         const int n = (int)left;
         if constexpr (sizeof(T) == 4) {
-            uint32_t* q = (uint32_t*)p;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (k < n) q[k] = r.a[k];
-                if (k + 4 < n) q[k + 4] = r.b[k];
+            u32x4 v = r.a;
+            if (n & 4) {
+                *(u32x4_at*)p = v;
+                v = r.b;
+                p += 4;
             }
+            if (n & 2) {
+                *(u32x2_at*)p = u32x2{v[0], v[1]};
+                v[0] = v[2];
+                p += 2;
+            }
+            if (n & 1) *(uint32_t*)p = v[0];
         } else {
-            uint16_t* q = (uint16_t*)p;
-#pragma unroll
-            for (int k = 0; k < CHUNK; ++k)
-                if (k < n) q[k] = (uint16_t)(r.a[k >> 1] >> (16 * (k & 1)));
+            u32x4 v = r.a;
+            if (n & 4) {
+                *(u32x2_at*)p = u32x2{v[0], v[1]};
+                v[0] = v[2];
+                v[1] = v[3];
+                p += 4;
+            }
+            if (n & 2) {
+                *(u32_at*)p = v[0];
+                v[0] = v[1];
+                p += 2;
+            }
+            if (n & 1) *(uint16_t*)p = (uint16_t)v[0];
         }
     }
 }
 
-// Eight elements of a parameter vector whose type is known at run time
-// (RF_F32 / RF_BF16 / RF_F16); `fill` without one and past the end.
-__device__ __forceinline__ void vector8(const void* p, int dtype, int64_t at, int64_t left, float fill, float (&v)[8])
+// Columns of a parameter vector whose type is known at run time (RF_F32 /
+// RF_BF16 / RF_F16), or of one that is not there.  Loads of several vectors are
+// sent before the first is looked at: `elsewhere` is any eight 16-bit elements
+// that may be read instead of an absent vector's.
+struct Vector8 {
+    u32x4 a, b;
+
+    __device__ __forceinline__ void fetch(const void* p, int dtype, int64_t c, int64_t cols, const void* elsewhere)
+    {
+        const int size = p && dtype == RF_F32 ? 4 : 2;
+        const char* const q = p ? (const char*)p + min(c, cols - CHUNK) * size : (const char*)elsewhere;
+        a = *(const u32x4_at*)q;
+        b = *(const u32x4_at*)(q + (size == 4 ? 16 : 0));
+    }
+    __device__ __forceinline__ void get(const void* p, int dtype, int64_t c, int64_t cols, float fill, float (&v)[8])
+    {
+        if (!p) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = fill;
+        } else if (dtype == RF_F32) {
+            Raw<float> r{a, b};
+            settle8(r, c, cols);
+            widen8(r, v);
+        } else {
+            Raw<bf16> r{a};
+            settle8(r, c, cols);
+            if (dtype == RF_BF16) widen8(r, v);
+            else widen8(Raw<f16>{r.a}, v);
+        }
+    }
+};
+
+// The same at once, in rows of any width; zero past the end.
+__device__ __forceinline__ void vector8(const void* p, int dtype, int64_t c, int64_t cols, float fill, float (&v)[8])
 {
     if (!p) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = fill;
     } else if (dtype == RF_F32) {
-        widen8(load8((const float*)p + at, left), v);
+        widen8(load8((const float*)p, c, cols), v);
     } else if (dtype == RF_BF16) {
-        widen8(load8((const bf16*)p + at, left), v);
+        widen8(load8((const bf16*)p, c, cols), v);
     } else {
-        widen8(load8((const f16*)p + at, left), v);
+        widen8(load8((const f16*)p, c, cols), v);
     }
 }
 

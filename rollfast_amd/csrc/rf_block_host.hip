@@ -84,15 +84,13 @@ __global__ __launch_bounds__(256) void k_checkpoint_store(const T* __restrict__ 
     if (p.ch >= pitch / CHUNK) return;  // whole quads
     Raw<T> v[ROWS];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const int64_t r = p.row + i * blockDim.y;
-        v[i] = zero8<T>();
-        if (r < rows) v[i] = load8(x + r * stride + p.ch * CHUNK, cols - p.ch * CHUNK);
-    }
+    for (int i = 0; i < ROWS; ++i)
+        v[i] = fetch8_any(x + min(p.row + i * (int64_t)blockDim.y, rows - 1) * stride, p.ch * CHUNK, cols);
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int64_t r = p.row + i * blockDim.y;
         float f[8];
+        settle8(v[i], p.ch * CHUNK, cols);
         widen8(v[i], f);
         const Codes c = encode8(f);
         if (r < rows) put_codes(codes, exps, r, pitch, p.ch, c);
@@ -109,11 +107,7 @@ __global__ __launch_bounds__(256) void k_checkpoint_load(const int8_t* __restric
     if (p.ch >= pitch / CHUNK) return;
     Codes v[ROWS];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const int64_t r = p.row + i * blockDim.y;
-        v[i] = Codes{};
-        if (r < rows) v[i] = get_codes(codes, exps, r, pitch, p.ch);
-    }
+    for (int i = 0; i < ROWS; ++i) v[i] = get_codes(codes, exps, min(p.row + i * (int64_t)blockDim.y, rows - 1), pitch, p.ch);
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int64_t r = p.row + i * blockDim.y;
@@ -156,18 +150,17 @@ template <typename T, int ACT> __global__ __launch_bounds__(256) void k_gated_fo
     Raw<T> g[ROWS], u[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int64_t r = p.row + i * blockDim.y;
-        g[i] = u[i] = zero8<T>();
-        if (r < a.rows) {
-            g[i] = load8((const T*)a.gate + r * a.gate_stride + c, left);
-            u[i] = load8((const T*)a.up + r * a.up_stride + c, left);
-        }
+        const int64_t r = min(p.row + i * (int64_t)blockDim.y, a.rows - 1);
+        g[i] = fetch8_any((const T*)a.gate + r * a.gate_stride, c, a.cols);
+        u[i] = fetch8_any((const T*)a.up + r * a.up_stride, c, a.cols);
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int64_t r = p.row + i * blockDim.y;
         if (r >= a.rows) break;  // the same for the whole quad
         float x[8], y[8], h[8];
+        settle8(g[i], c, a.cols);
+        settle8(u[i], c, a.cols);
         widen8(g[i], x);
         widen8(u[i], y);
 #pragma unroll
@@ -201,21 +194,22 @@ __global__ __launch_bounds__(256) void k_gated_backward(const rf_gated a, uint32
     const int64_t c = p.ch * CHUNK, left = a.cols - c;
     if (left <= 0) return;
     Raw<T> d[ROWS];
-    Saved<T, SRC8> g[ROWS], u[ROWS];
+    Saved<T, SRC8, false> g[ROWS], u[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-        const int64_t r = min(p.row + i * blockDim.y, a.rows - 1);
-        d[i] = load8((const T*)a.dh + r * a.dh_stride + c, left);
-        g[i].load((const T*)a.gate, a.gate_stride, a.gate_codes, a.gate_exponents, r, pitch, p.ch, nch, a.cols);
-        u[i].load((const T*)a.up, a.up_stride, a.up_codes, a.up_exponents, r, pitch, p.ch, nch, a.cols);
+        const int64_t r = min(p.row + i * (int64_t)blockDim.y, a.rows - 1);
+        d[i] = fetch8_any((const T*)a.dh + r * a.dh_stride, c, a.cols);
+        g[i].fetch((const T*)a.gate, a.gate_stride, a.gate_codes, a.gate_exponents, r, pitch, p.ch, nch, a.cols);
+        u[i].fetch((const T*)a.up, a.up_stride, a.up_codes, a.up_exponents, r, pitch, p.ch, nch, a.cols);
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int64_t r = p.row + i * blockDim.y;
         if (r >= a.rows) break;
         float x[8], y[8], dh[8];
-        g[i].get(x);
-        u[i].get(y);
+        g[i].get(x, p.ch, a.cols);
+        u[i].get(y, p.ch, a.cols);
+        settle8(d[i], c, a.cols);
         widen8(d[i], dh);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -272,35 +266,49 @@ rf_status gated(const rf_gated* a, bool back, void* stream)
 constexpr int64_t MAX_REGISTER_COLS = 8192;  // 512 lanes, two chunks each
 constexpr size_t MAX_LDS = 64 * 1024;
 
-NormShape shape_of(const rf_norm& a, int cus)
+// Lanes and chunks of a row, measured on one GPU (us):
+// - one chunk a lane, or two: forward 16384 x 4096 bf16 122 / 128, 8192 x 768
+//   14.3 / 13.9 (two chunks in one wave need no barrier); backward in 16 bits,
+//   16384 x 4096 LayerNorm 298 / 194, 20000 x 1280 76 / 68; backward in f32,
+//   2317 x 1283 LayerNorm 25 / 39 (two chunks spill).
+// - threads a CU: forward 16384 x 4096 157 / 122 / 126 with 512 / 1024 / 2048;
+//   backward 159 / 180 with 512 / 768 (more partial rows to write and add).
+NormShape shape_of(const rf_norm& a, int cus, bool back)
 {
     NormShape s{};
     const int64_t nch = pitch_of(a.cols) / CHUNK;
-    s.tpr = nch <= 128 ? 64 : nch <= 256 ? 128 : nch <= 512 ? 256 : 512;
-    s.nv = a.cols > MAX_REGISTER_COLS ? 0 : nch <= s.tpr ? 1 : 2;
-    s.ny = s.tpr == 64 ? 4 : 1;
-    s.full = a.post == RF_NORM_LAYER || a.next == RF_NORM_LAYER || a.dbias || a.dnext_bias || (a.bias && a.dgate);
+    const bool two = nch > 512 || (nch > 64 && (back ? a.dtype != RF_F32 : nch <= 128));
+    const int64_t lanes = two ? (nch + 1) / 2 : nch;
+    s.tpr = (int)std::min<int64_t>(512, (lanes + 63) / 64 * 64);
+    s.nv = a.cols > MAX_REGISTER_COLS || a.cols < CHUNK ? 0 : two ? 2 : 1;
+    if (s.nv == 0) s.tpr = 512;
+    s.ny = s.tpr == 64 && s.nv ? 4 : 1;
+    s.full = a.post == RF_NORM_LAYER || a.next == RF_NORM_LAYER ||
+             (back ? a.dbias || a.dnext_bias || (a.bias && a.dgate) : a.bias || a.next_bias);
     s.src8 = a.post == RF_NORM_ABSENT ? a.hidden_codes != nullptr : a.branch_codes != nullptr;
-    s.workers = std::max<int64_t>(1, std::min<int64_t>((a.rows + s.ny - 1) / s.ny, (int64_t)cus * 2048 / (s.tpr * s.ny) * 2));
+    s.workers = std::max<int64_t>(1, std::min<int64_t>((a.rows + s.ny - 1) / s.ny, (int64_t)cus * 1024 / (s.tpr * s.ny)));
     if (s.nv == 0) s.workers = std::max<int64_t>(1, std::min<int64_t>(a.rows, (int64_t)cus * 4));
     return s;
 }
 
-// Rows are cut into pieces of a group, about two workgroups a CU; with more
-// groups than that a workgroup takes whole groups.
+// Rows are cut into pieces of a group, about 512 threads a CU and four rows a
+// piece at least; with more groups than pieces a workgroup takes whole groups.
+// Workgroups come in whole rounds of the CUs where there are more than one:
+// 2317 x 1283 LayerNorm in f32 took 25 us with 512 of them and 36 with 574.
 void plan_of(const rf_norm& a, int cus, NormShape& s, NormPlan& p)
 {
     p = NormPlan{};
     const bool exit = a.post != RF_NORM_ABSENT;
-    const int64_t target = (int64_t)cus * 2;
+    const int64_t target = (int64_t)cus * std::max(1, 512 / (s.tpr * s.ny));
     p.groups = exit ? std::max<int64_t>(1, a.gates) : 1;
     p.group_rows = a.rows / p.groups;
     if (p.groups > target) {
         p.pieces = 0;
         p.workers = (int32_t)target;
     } else {
-        const int64_t per = std::max<int64_t>(1, (p.group_rows + s.ny - 1) / s.ny);
-        p.pieces = (int32_t)std::min<int64_t>(per, std::max<int64_t>(1, target / p.groups));
+        int64_t all = std::min<int64_t>(target, std::max<int64_t>(1, a.rows / (4 * s.ny)));
+        if (all > cus) all = all / cus * cus;
+        p.pieces = (int32_t)std::max<int64_t>(1, all / p.groups);
         p.workers = (int32_t)(p.pieces * p.groups);
     }
     int n = 0;
@@ -322,75 +330,75 @@ int64_t workspace_of(const rf_norm& a, const NormShape& s, const NormPlan& p)
     return n * (int64_t)sizeof(float);
 }
 
-// Adds the partial rows.  A column's rows are dealt to 16 lanes: those of one
-// group, or, with many groups of few pieces, the groups themselves.
-constexpr int FIN_COLS = 64, FIN_LANES = 16;
+// Adds the partial rows: 32 columns a workgroup, 32 lanes a column.  The lanes
+// are dealt to the groups of rows (all of them to one group, or one to each of
+// 32 groups at a time), and within a group to its pieces.
+constexpr int FIN_COLS = 32, FIN_LANES = 32;
+
+// Partial rows w0 + i * step below w1, eight loads in flight.
+__device__ __forceinline__ float add_rows(const float* __restrict__ p, int64_t w0, int64_t w1, int64_t step, int64_t pitch)
+{
+    float s = 0.0f;
+    for (int64_t w = w0; w < w1; w += 8 * step) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = w + i * step < w1 ? p[(w + i * step) * pitch] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    return s;
+}
 
 __global__ __launch_bounds__(FIN_COLS* FIN_LANES) void k_norm_finish(const rf_norm a, const NormPlan p,
                                                                     const float* __restrict__ partial)
 {
-    __shared__ float lds[FIN_LANES][FIN_COLS];
-    const int64_t c = (int64_t)blockIdx.x * FIN_COLS + threadIdx.x, cols = a.cols;
-    const int ty = threadIdx.y;
+    __shared__ float lds[4][FIN_LANES][FIN_COLS];
+    const int tx = threadIdx.x, ty = threadIdx.y;
+    const int64_t cols = a.cols, c = (int64_t)blockIdx.x * FIN_COLS + tx, at = min(c, cols - 1), pitch = p.vectors * cols;
     const bool in = c < cols;
-    auto sum = [&](float v) {  // over the lanes of a column, in their order
-        __syncthreads();
-        lds[ty][threadIdx.x] = v;
-        __syncthreads();
-        float s = 0.0f;
-        for (int i = 0; i < FIN_LANES; ++i) s += lds[i][threadIdx.x];
-        return s;
-    };
-    auto rows = [&](int index, int64_t w0, int64_t w1, int64_t from, int64_t step) {
-        float s = 0.0f;
-        if (in && index >= 0)
-            for (int64_t w = w0 + from; w < min(w1, (int64_t)p.workers); w += step) s += partial[(w * p.vectors + index) * cols + c];
-        return s;
-    };
-    if (p.i_w2 >= 0) {
-        const float v = sum(rows(p.i_w2, 0, p.workers, ty, FIN_LANES));
-        if (in && ty == 0) put_scalar(a.dnext_weight, a.next_weight_dtype, c, v);
-    }
-    if (p.i_b2 >= 0) {
-        const float v = sum(rows(p.i_b2, 0, p.workers, ty, FIN_LANES));
-        if (in && ty == 0) put_scalar(a.dnext_bias, a.next_bias_dtype, c, v);
-    }
-    if (p.i_p < 0) return;
-    const float w = in && a.weight ? scalar_at(a.weight, a.weight_dtype, c) : 1.0f;
-    const float b = in && a.bias ? scalar_at(a.bias, a.bias_dtype, c) : 0.0f;
-    auto gate = [&](int64_t g) { return in && a.gate ? scalar_at(a.gate, a.gate_dtype, g * cols + c) : 1.0f; };
-    auto put_gate = [&](int64_t g, float P, float Q) {
-        if (in && a.dgate) put_scalar(a.dgate, a.gate_dtype, g * cols + c, a.branch_scale * fmaf(w, P, b * Q));
-    };
-    float dw, db;
-    if (p.pieces == 0) {  // the gate is in the sums already
-        dw = sum(rows(p.i_p, 0, p.workers, ty, FIN_LANES));
-        db = sum(rows(p.i_q, 0, p.workers, ty, FIN_LANES));
-    } else if (p.pieces >= FIN_LANES || p.groups == 1) {
-        dw = db = 0.0f;
-        for (int64_t g = 0; g < p.groups; ++g) {
-            const float P = sum(rows(p.i_p, g * p.pieces, (g + 1) * p.pieces, ty, FIN_LANES));
-            const float Q = p.i_q >= 0 ? sum(rows(p.i_q, g * p.pieces, (g + 1) * p.pieces, ty, FIN_LANES)) : 0.0f;
-            if (ty == 0) put_gate(g, P, Q);
-            dw = fmaf(gate(g), P, dw);
-            db = fmaf(gate(g), Q, db);
+    const bool post = p.i_p >= 0, has_q = p.i_q >= 0;
+    // whole groups: the gate is in the sums already, and its gradient is written
+    const bool gated = p.pieces > 0 && a.gate;
+    const int64_t groups = p.pieces > 0 ? p.groups : 1, pieces = p.pieces > 0 ? p.pieces : p.workers;
+    const int lanes = (int)max((int64_t)1, FIN_LANES / groups), slots = FIN_LANES / lanes;
+    const int slot = ty / lanes, sub = ty % lanes;
+    const float w = post && a.weight ? scalar_at(a.weight, a.weight_dtype, at) : 1.0f;
+    const float b = post && a.bias ? scalar_at(a.bias, a.bias_dtype, at) : 0.0f;
+    lds[0][ty][tx] = p.i_w2 >= 0 ? add_rows(partial + p.i_w2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
+    lds[1][ty][tx] = p.i_b2 >= 0 ? add_rows(partial + p.i_b2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
+    float dw = 0.0f, db = 0.0f;
+    if (post) {
+        for (int64_t first = 0; first < groups; first += slots) {
+            const int64_t g = first + slot, w0 = g * pieces;
+            const bool mine = slot < slots && g < groups;
+            const int64_t w1 = mine ? min(w0 + pieces, (int64_t)p.workers) : 0;
+            lds[2][ty][tx] = add_rows(partial + p.i_p * cols + at, w0 + sub, w1, lanes, pitch);
+            lds[3][ty][tx] = has_q ? add_rows(partial + p.i_q * cols + at, w0 + sub, w1, lanes, pitch) : 0.0f;
+            __syncthreads();
+            if (mine && sub == 0) {
+                float P = 0.0f, Q = 0.0f;
+                for (int i = 0; i < lanes; ++i) {
+                    P += lds[2][ty + i][tx];
+                    Q += lds[3][ty + i][tx];
+                }
+                const float gt = gated ? scalar_at(a.gate, a.gate_dtype, g * cols + at) : 1.0f;
+                if (gated && a.dgate && in) put_scalar(a.dgate, a.gate_dtype, g * cols + c, a.branch_scale * fmaf(w, P, b * Q));
+                dw = fmaf(gt, P, dw);
+                db = fmaf(gt, Q, db);
+            }
+            __syncthreads();
         }
-    } else {
-        float sw = 0.0f, sb = 0.0f;
-        for (int64_t g = ty; g < p.groups; g += FIN_LANES) {
-            const float P = rows(p.i_p, g * p.pieces, (g + 1) * p.pieces, 0, 1);
-            const float Q = rows(p.i_q, g * p.pieces, (g + 1) * p.pieces, 0, 1);
-            put_gate(g, P, Q);
-            sw = fmaf(gate(g), P, sw);
-            sb = fmaf(gate(g), Q, sb);
-        }
-        dw = sum(sw);
-        db = sum(sb);
     }
-    if (in && ty == 0) {
-        if (a.dweight) put_scalar(a.dweight, a.weight_dtype, c, a.branch_scale * dw);
-        if (a.dbias) put_scalar(a.dbias, a.bias_dtype, c, a.branch_scale * db);
-    }
+    lds[2][ty][tx] = dw;
+    lds[3][ty][tx] = db;
+    __syncthreads();
+    if (ty >= 4 || !in) return;
+    void* const out = ty == 0 ? a.dnext_weight : ty == 1 ? a.dnext_bias : ty == 2 ? a.dweight : a.dbias;
+    const int dtype = ty == 0 ? a.next_weight_dtype : ty == 1 ? a.next_bias_dtype : ty == 2 ? a.weight_dtype : a.bias_dtype;
+    if (!out) return;
+    float s = 0.0f;
+    for (int i = 0; i < FIN_LANES; ++i) s += lds[ty][i][tx];
+    put_scalar(out, dtype, c, ty < 2 ? s : a.branch_scale * s);
 }
 
 bool has_pair(const rf_norm& a)
@@ -508,7 +516,7 @@ rf_status rf_norm_forward(const rf_norm* args, void* stream)
     if (!a.hidden || (exit && (!a.residual || !a.branch)) || (next && !a.y)) return bad("null buffer");
     int cus = 0;
     if (const rf_status s = rf::device_cus(&cus); s != RF_OK) return s;
-    forward_of(a)(a, shape_of(a, cus), (hipStream_t)stream);
+    forward_of(a)(a, shape_of(a, cus, false), (hipStream_t)stream);
     BLK_TRY(hipGetLastError());
     return RF_OK;
 }
@@ -519,7 +527,7 @@ rf_status rf_norm_backward_workspace(const rf_norm* args, int64_t* bytes)
     if (const rf_status s = check_backward(args); s != RF_OK) return s;
     int cus = 0;
     if (const rf_status s = rf::device_cus(&cus); s != RF_OK) return s;
-    NormShape s = shape_of(*args, cus);
+    NormShape s = shape_of(*args, cus, true);
     NormPlan p;
     plan_of(*args, cus, s, p);
     *bytes = workspace_of(*args, s, p);
@@ -539,7 +547,7 @@ rf_status rf_norm_backward(const rf_norm* args, void* workspace, int64_t workspa
         return bad("null statistics");
     int cus = 0;
     if (const rf_status s = rf::device_cus(&cus); s != RF_OK) return s;
-    NormShape s = shape_of(a, cus);
+    NormShape s = shape_of(a, cus, true);
     NormPlan p;
     plan_of(a, cus, s, p);
     if (workspace_bytes < workspace_of(a, s, p) || (workspace_of(a, s, p) && !workspace)) return bad("workspace too small");

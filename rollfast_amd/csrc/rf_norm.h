@@ -65,91 +65,129 @@ template <int NS> __device__ __forceinline__ void row_sums(float (&s)[NS], float
     }
 }
 
-template <typename T> __device__ __forceinline__ T* row_of(T* p, int64_t row, int64_t stride) { return p + row * stride; }
+__device__ __forceinline__ const void* gate_row(const rf_norm& a, int64_t g)
+{
+    return a.gate ? (const char*)a.gate + g * a.cols * (a.gate_dtype == RF_F32 ? 4 : 2) : nullptr;
+}
 
 // ------------------------------------------------------------- forward -----
 // blockDim (tpr, ny): tpr lanes a row; ny > 1 only where a wave holds a row.
-template <typename T, typename U, bool EXIT, bool NEXT, int NV>
+// FULL: LayerNorm or a bias somewhere.  The next row's loads are sent before
+// this row's sums.
+template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, int NV>
 __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
 {
     __shared__ float red[2][MAX_WAVES][8];
     int half = 0;
-    const int tid = threadIdx.x, tpr = blockDim.x;
+    const int tid = threadIdx.x, tpr = blockDim.x, ty = __builtin_amdgcn_readfirstlane(threadIdx.y), ny = blockDim.y;
     const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
     const float inv_cols = 1.0f / (float)cols;
-    const int64_t r0 = part(a.rows, blockIdx.x, gridDim.x), r1 = part(a.rows, blockIdx.x + 1, gridDim.x);
+    const int64_t r0 = part(a.rows, blockIdx.x, gridDim.x) + ty, r1 = part(a.rows, blockIdx.x + 1, gridDim.x);
+    if (r0 >= r1) return;  // a wave of its own (ny > 1): no other waits for it
     const int64_t group_rows = a.gates > 1 ? a.rows / a.gates : 0;
-    float A[NV][8], B[NV][8], w2[NV][8], b2[NV][8];
-    int64_t group = -1;
-    auto load_post = [&](int64_t g) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            float gt[8];
-            vector8(a.weight, a.weight_dtype, c, cols - c, 1.0f, A[j]);
-            vector8(a.bias, a.bias_dtype, c, cols - c, 0.0f, B[j]);
-            vector8(a.gate, a.gate_dtype, g * cols + c, cols - c, 1.0f, gt);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                A[j][k] *= a.branch_scale * gt[k];
-                B[j][k] *= a.branch_scale * gt[k];
-            }
-        }
+    struct Row {
+        Raw<T> r[NV];
+        Raw<U> u[EXIT ? NV : 1];
     };
-    if constexpr (EXIT) {
-        if (group_rows == 0) load_post(0);
-    }
-    if constexpr (NEXT) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            vector8(a.next_weight, a.next_weight_dtype, c, cols - c, 1.0f, w2[j]);
-            vector8(a.next_bias, a.next_bias_dtype, c, cols - c, 0.0f, b2[j]);
-        }
-    }
-    for (int64_t r = r0 + threadIdx.y; r < r1; r += blockDim.y) {
-        Raw<T> rr[NV];
-        Raw<U> ur[EXIT ? NV : 1];
+    auto load = [&](int64_t r) {
+        Row x;
         const T* rp = EXIT ? (const T*)a.residual + r * a.residual_stride : (const T*)a.hidden + r * a.hidden_stride;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            rr[j] = load8(rp + c, cols - c);
-            if constexpr (EXIT) ur[j] = load8((const U*)a.branch + r * a.branch_stride + c, cols - c);
+            x.r[j] = fetch8(rp, c, cols);
+            if constexpr (EXIT) x.u[j] = fetch8((const U*)a.branch + r * a.branch_stride, c, cols);
+        }
+        return x;
+    };
+    Row now = load(r0);
+    const void* const some = EXIT ? a.residual : a.hidden;
+    float w2[NEXT ? NV : 1][8], b2[NEXT && FULL ? NV : 1][8];
+    if constexpr (NEXT) {
+        Vector8 w[NV], b[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            w[j].fetch(a.next_weight, a.next_weight_dtype, c, cols, some);
+            if constexpr (FULL) b[j].fetch(a.next_bias, a.next_bias_dtype, c, cols, some);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            w[j].get(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, w2[j]);
+            if constexpr (FULL) b[j].get(a.next_bias, a.next_bias_dtype, c, cols, 0.0f, b2[j]);
+        }
+    }
+    // mean and 1 / sqrt(variance + eps) of a row; columns past the end are zero
+    auto stats = [&](const auto& x, bool layer, float eps, float& mean, float& rstd) {
+        mean = 0.0f;
+        if (layer) {
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                float v[8];
+                widen8(x[j], v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[0] += v[k];
+            }
+            row_sums(s, red, half);
+            mean = s[0] * inv_cols;
+        }
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
+            float v[8];
+            widen8(x[j], v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float d = FULL ? (k < left ? v[k] - mean : 0.0f) : v[k];
+                s[0] = fmaf(d, d, s[0]);
+            }
+        }
+        row_sums(s, red, half);
+        rstd = 1.0f / sqrtf(s[0] * inv_cols + eps);
+    };
+    for (int64_t r = r0; r < r1;) {
+    // the rows of one gate
+    const int64_t g = group_rows ? r / group_rows : 0, end = group_rows ? min(r1, (g + 1) * group_rows) : r1;
+    float A[EXIT ? NV : 1][8], B[EXIT && FULL ? NV : 1][8];
+    if constexpr (EXIT) {
+        Vector8 w[NV], b[NV], gt[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            w[j].fetch(a.weight, a.weight_dtype, c, cols, some);
+            gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, some);
+            if constexpr (FULL) b[j].fetch(a.bias, a.bias_dtype, c, cols, some);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            float v[8];
+            w[j].get(a.weight, a.weight_dtype, c, cols, 1.0f, A[j]);
+            gt[j].get(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
+            if constexpr (FULL) b[j].get(a.bias, a.bias_dtype, c, cols, 0.0f, B[j]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] *= a.branch_scale;
+                A[j][k] *= v[k];
+                if constexpr (FULL) B[j][k] *= v[k];
+            }
+        }
+    }
+    for (; r < end; r += ny) {
+        const Row ahead = load(r + ny < r1 ? r + ny : r);  // the last row again: still cached
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            settle8(now.r[j], c, cols);
+            if constexpr (EXIT) settle8(now.u[j], c, cols);
         }
         if constexpr (EXIT) {
-            if (group_rows && r / group_rows != group) {
-                group = r / group_rows;
-                load_post(group);
-            }
             float mean = 0.0f, rstd = 1.0f;
-            if (a.post == RF_NORM_LAYER) {
-                float s[1] = {0.0f};
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    float u[8];
-                    widen8(ur[j], u);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) s[0] += u[k];
-                }
-                row_sums(s, red, half);
-                mean = s[0] * inv_cols;
-            }
             if (a.post != RF_NORM_NONE) {
-                float s[1] = {0.0f};
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
-                    float u[8];
-                    widen8(ur[j], u);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float d = k < left ? u[k] - mean : 0.0f;
-                        s[0] = fmaf(d, d, s[0]);
-                    }
-                }
-                row_sums(s, red, half);
-                rstd = 1.0f / sqrtf(s[0] * inv_cols + a.post_eps);
+                stats(now.u, FULL && a.post == RF_NORM_LAYER, a.post_eps, mean, rstd);
                 if (tid == 0) {
                     if (a.post_rstd) a.post_rstd[r] = rstd;
                     if (a.post_mean) a.post_mean[r] = mean;
@@ -160,45 +198,23 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
                 const int64_t ch = tid + j * tpr, c = ch * CHUNK;
                 if (ch < nch) {
                     float u[8], x[8], o[8];
-                    widen8(ur[j], u);
-                    widen8(rr[j], x);
+                    widen8(now.u[j], u);
+                    widen8(now.r[j], x);
                     if (a.branch_codes) put_codes(a.branch_codes, a.branch_exponents, r, pitch, ch, encode8(u));
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        o[k] = c + k < cols ? fmaf(a.residual_scale, x[k], fmaf((u[k] - mean) * rstd, A[j][k], B[j][k])) : 0.0f;
-                    rr[j] = narrow8<T>(o);
-                    put8((T*)a.hidden + r * cols + c, rr[j], cols - c);
+                    for (int k = 0; k < 8; ++k) {
+                        const float n = FULL ? fmaf((u[k] - mean) * rstd, A[j][k], B[FULL ? j : 0][k]) : u[k] * rstd * A[j][k];
+                        o[k] = fmaf(a.residual_scale, x[k], n);
+                        if (FULL && c + k >= cols) o[k] = 0.0f;
+                    }
+                    now.r[j] = narrow8<T>(o);
+                    put8((T*)a.hidden + r * cols + c, now.r[j], cols - c);
                 }
             }
         }
         if constexpr (NEXT) {
-            float mean = 0.0f;
-            if (a.next == RF_NORM_LAYER) {
-                float s[1] = {0.0f};
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    float v[8];
-                    widen8(rr[j], v);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) s[0] += v[k];
-                }
-                row_sums(s, red, half);
-                mean = s[0] * inv_cols;
-            }
-            float s[1] = {0.0f};
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
-                float v[8];
-                widen8(rr[j], v);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float d = k < left ? v[k] - mean : 0.0f;
-                    s[0] = fmaf(d, d, s[0]);
-                }
-            }
-            row_sums(s, red, half);
-            const float rstd = 1.0f / sqrtf(s[0] * inv_cols + a.next_eps);
+            float mean, rstd;
+            stats(now.r, FULL && a.next == RF_NORM_LAYER, a.next_eps, mean, rstd);
             if (tid == 0) {
                 if (a.next_rstd) a.next_rstd[r] = rstd;
                 if (a.next_mean) a.next_mean[r] = mean;
@@ -208,11 +224,13 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
                 const int64_t ch = tid + j * tpr, c = ch * CHUNK;
                 if (ch < nch) {
                     float v[8], y[8];
-                    widen8(rr[j], v);
+                    widen8(now.r[j], v);
                     if (a.hidden_codes) put_codes(a.hidden_codes, a.hidden_exponents, r, pitch, ch, encode8(v));
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        y[k] = c + k < cols ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[j][k]) : 0.0f;
+                    for (int k = 0; k < 8; ++k) {
+                        y[k] = FULL ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[FULL ? j : 0][k]) : v[k] * rstd * w2[j][k];
+                        if (FULL && c + k >= cols) y[k] = 0.0f;
+                    }
                     const Raw<U> yr = narrow8<U>(y);
                     put8((U*)a.y + r * cols + c, yr, cols - c);
                     if (a.y_codes) {
@@ -222,6 +240,8 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
                 }
             }
         }
+        now = ahead;
+    }
     }
 }
 
@@ -242,7 +262,7 @@ __global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
             float s[1] = {0.0f};
             for (int64_t ch = tid; ch < nch; ch += tpr) {
                 float v[8];
-                widen8(load8(p + ch * CHUNK, cols - ch * CHUNK), v);
+                widen8(load8(p, ch * CHUNK, cols), v);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) s[0] += v[k];
             }
@@ -253,7 +273,7 @@ __global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
         for (int64_t ch = tid; ch < nch; ch += tpr) {
             const int64_t left = cols - ch * CHUNK;
             float v[8];
-            widen8(load8(p + ch * CHUNK, left), v);
+            widen8(load8(p, ch * CHUNK, cols), v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float d = k < left ? v[k] - mean : 0.0f;
@@ -280,11 +300,11 @@ __global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
             for (int64_t ch = tid; ch < nch; ch += tpr) {
                 const int64_t c = ch * CHUNK, left = cols - c;
                 float u[8], x[8], w[8], b[8], gt[8], o[8];
-                widen8(load8(up + c, left), u);
-                widen8(load8(rp + c, left), x);
-                vector8(a.weight, a.weight_dtype, c, left, 1.0f, w);
-                vector8(a.bias, a.bias_dtype, c, left, 0.0f, b);
-                vector8(a.gate, a.gate_dtype, g * cols + c, left, 1.0f, gt);
+                widen8(load8(up, c, cols), u);
+                widen8(load8(rp, c, cols), x);
+                vector8(a.weight, a.weight_dtype, c, cols, 1.0f, w);
+                vector8(a.bias, a.bias_dtype, c, cols, 0.0f, b);
+                vector8(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, gt);
                 if (a.branch_codes) put_codes(a.branch_codes, a.branch_exponents, r, pitch, ch, encode8(u));
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -304,9 +324,9 @@ __global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
             for (int64_t ch = tid; ch < nch; ch += tpr) {
                 const int64_t c = ch * CHUNK, left = cols - c;
                 float v[8], w[8], b[8], y[8];
-                widen8(load8((const T*)hp + c, left), v);
-                vector8(a.next_weight, a.next_weight_dtype, c, left, 1.0f, w);
-                vector8(a.next_bias, a.next_bias_dtype, c, left, 0.0f, b);
+                widen8(load8((const T*)hp, c, cols), v);
+                vector8(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, w);
+                vector8(a.next_bias, a.next_bias_dtype, c, cols, 0.0f, b);
                 if (a.hidden_codes) put_codes(a.hidden_codes, a.hidden_exponents, r, pitch, ch, encode8(v));
 #pragma unroll
                 for (int k = 0; k < 8; ++k) y[k] = k < left ? fmaf((v[k] - mean) * rstd, w[k], b[k]) : 0.0f;
@@ -322,25 +342,30 @@ __global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
 }
 
 // ------------------------------------------------------------ backward -----
-// The saved row of a norm: a checkpoint, or the tensor itself.
-template <typename T, bool SRC8> struct Saved {
+// A chunk of a saved row: of a checkpoint, or of the tensor itself.  WIDE: rows
+// of at least eight columns.
+template <typename T, bool SRC8, bool WIDE> struct Saved {
     Raw<T> t;
-    __device__ __forceinline__ void load(const T* p, int64_t stride, const int8_t*, const uint8_t*, int64_t r, int64_t,
-                                         int64_t ch, int64_t, int64_t cols)
+    __device__ __forceinline__ void fetch(const T* p, int64_t stride, const int8_t*, const uint8_t*, int64_t r, int64_t,
+                                          int64_t ch, int64_t, int64_t cols)
     {
-        t = load8(p + r * stride + ch * CHUNK, cols - ch * CHUNK);
+        t = WIDE ? fetch8(p + r * stride, ch * CHUNK, cols) : fetch8_any(p + r * stride, ch * CHUNK, cols);
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const { widen8(t, v); }
+    __device__ __forceinline__ void get(float (&v)[8], int64_t ch, int64_t cols)
+    {
+        settle8(t, ch * CHUNK, cols);
+        widen8(t, v);
+    }
 };
-template <typename T> struct Saved<T, true> {
+template <typename T, bool WIDE> struct Saved<T, true, WIDE> {
     Codes t;
-    __device__ __forceinline__ void load(const T*, int64_t, const int8_t* codes, const uint8_t* exps, int64_t r,
-                                         int64_t pitch, int64_t ch, int64_t nch, int64_t)
+    __device__ __forceinline__ void fetch(const T*, int64_t, const int8_t* codes, const uint8_t* exps, int64_t r,
+                                          int64_t pitch, int64_t ch, int64_t nch, int64_t)
     {
-        t = Codes{};
-        if (ch < nch) t = get_codes(codes, exps, r, pitch, ch);
+        t = get_codes(codes, exps, r, pitch, min(ch, nch - 1));
+        if (ch >= nch) t.e = 0;  // reads as zero
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const { decode8(t, v); }
+    __device__ __forceinline__ void get(float (&v)[8], int64_t, int64_t) const { decode8(t, v); }
 };
 
 // FULL: LayerNorm or a bias somewhere (the sums of g, t and their columns).
@@ -350,7 +375,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
     __shared__ float red[2][MAX_WAVES][8];
     extern __shared__ float cols_lds[];
     int half = 0;
-    const int tid = threadIdx.x, tpr = blockDim.x, ty = threadIdx.y, ny = blockDim.y;
+    const int tid = threadIdx.x, tpr = blockDim.x, ty = __builtin_amdgcn_readfirstlane(threadIdx.y), ny = blockDim.y;
     const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
     const float inv_cols = 1.0f / (float)cols;
     const bool post_layer = FULL && EXIT && a.post == RF_NORM_LAYER, next_layer = FULL && NEXT && a.next == RF_NORM_LAYER;
@@ -359,17 +384,58 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
     float P[EXIT ? NV : 1][8] = {}, Q[EXIT && FULL ? NV : 1][8] = {};
     float W2[NEXT ? NV : 1][8] = {}, B2[NEXT && FULL ? NV : 1][8] = {};
     float h[EXIT ? NV : 1][8], w2[NEXT ? NV : 1][8];
-    if constexpr (NEXT) {
+    // This wave's (or workgroup's) rows: whole groups in a run, or every ny-th
+    // row of a piece of one group.
+    int64_t r0, r1, g;
+    const int64_t step = whole_groups ? 1 : ny;
+    if (whole_groups) {
+        const int64_t ga = part(plan.groups, blockIdx.x, gridDim.x), gb = part(plan.groups, blockIdx.x + 1, gridDim.x);
+        g = ga + part(gb - ga, ty, ny);
+        r0 = g * plan.group_rows;
+        r1 = (ga + part(gb - ga, ty + 1, ny)) * plan.group_rows;
+    } else {
+        const int64_t piece = blockIdx.x % plan.pieces;
+        g = blockIdx.x / plan.pieces;
+        r0 = g * plan.group_rows + part(plan.group_rows, piece, plan.pieces) + ty;
+        r1 = g * plan.group_rows + part(plan.group_rows, piece + 1, plan.pieces);
+    }
+    struct Row {
+        Raw<T> dh[NV];
+        Raw<U> dy[NEXT ? NV : 1];
+        Saved<U, SRC8, true> u[EXIT ? NV : 1];
+        Saved<T, SRC8, true> h[NEXT ? NV : 1];
+        float rstd1, mean1, rstd2, mean2;
+    };
+    auto load = [&](int64_t r) {
+        Row x;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            vector8(a.next_weight, a.next_weight_dtype, c, cols - c, 1.0f, w2[j]);
+            const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+            // without one: any rows that may be read, cleared below
+            x.dh[j] = fetch8(a.dhidden ? (const T*)a.dhidden + r * a.dhidden_stride : (const T*)a.dresidual + r * cols, c, cols);
+            if constexpr (NEXT) {
+                x.dy[j] = fetch8((const U*)a.dy + r * a.dy_stride, c, cols);
+                x.h[j].fetch((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch, cols);
+            }
+            if constexpr (EXIT)
+                x.u[j].fetch((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch, cols);
         }
+        x.rstd1 = post_norm ? a.post_rstd[r] : 1.0f;
+        x.mean1 = post_layer ? a.post_mean[r] : 0.0f;
+        x.rstd2 = NEXT ? a.next_rstd[r] : 0.0f;
+        x.mean2 = next_layer ? a.next_mean[r] : 0.0f;
+        return x;
+    };
+    Row now;
+    if (r0 < r1) now = load(r0);  // (a wave without rows has sums of zero)
+    if constexpr (NEXT) {
+        Vector8 w[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) w[j].fetch(a.next_weight, a.next_weight_dtype, (int64_t)(tid + j * tpr) * CHUNK, cols, a.dy);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            w[j].get(a.next_weight, a.next_weight_dtype, (int64_t)(tid + j * tpr) * CHUNK, cols, 1.0f, w2[j]);
     }
-    // groups of this workgroup and the rows of each
-    const int64_t g0 = whole_groups ? part(plan.groups, blockIdx.x, gridDim.x) + ty
-                                    : blockIdx.x / max(plan.pieces, 1);
-    const int64_t g1 = whole_groups ? part(plan.groups, blockIdx.x + 1, gridDim.x) : g0 + 1;
     // whole groups: the sums over groups, of this wave's or workgroup's columns
     float* const sums_p = cols_lds + (int64_t)ty * (FULL ? 2 : 1) * pitch;
     float* const sums_q = sums_p + pitch;
@@ -386,145 +452,136 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
             }
         }
     }
-    for (int64_t g = g0; g < g1; g += whole_groups ? ny : 1) {
-        int64_t r0 = g * plan.group_rows, r1 = r0 + plan.group_rows;
-        if (!whole_groups) {
-            const int64_t piece = blockIdx.x % max(plan.pieces, 1);
-            r1 = r0 + part(plan.group_rows, piece + 1, plan.pieces);
-            r0 += part(plan.group_rows, piece, plan.pieces) + ty;
+    for (int64_t r = r0; r < r1; ++g) {
+    const int64_t end = whole_groups ? r + plan.group_rows : r1;
+    if constexpr (EXIT) {
+        Vector8 w[NV], gt[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            w[j].fetch(a.weight, a.weight_dtype, c, cols, a.dbranch);
+            gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, a.dbranch);
         }
-        if constexpr (EXIT) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-                float gt[8];
-                vector8(a.weight, a.weight_dtype, c, cols - c, 1.0f, h[j]);
-                vector8(a.gate, a.gate_dtype, g * cols + c, cols - c, 1.0f, gt);
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            float v[8];
+            w[j].get(a.weight, a.weight_dtype, c, cols, 1.0f, h[j]);
+            gt[j].get(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) h[j][k] = c + k < cols ? h[j][k] * a.branch_scale * gt[k] : 0.0f;
+            for (int k = 0; k < 8; ++k) h[j][k] = c + k < cols ? h[j][k] * a.branch_scale * v[k] : 0.0f;
+        }
+    }
+    for (; r < end; r += step) {
+        const Row ahead = load(r + step < r1 ? r + step : r);
+        const float rstd1 = now.rstd1, mean1 = now.mean1, rstd2 = now.rstd2, mean2 = now.mean2;
+        float e[NV][8], x[NEXT ? NV : 1][8], u[EXIT ? NV : 1][8];
+        // g2 xhat, h e uhat, h xhat uhat; FULL: g2, h uhat, h e, h, h xhat
+        float s[FULL ? 8 : 3] = {};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t ch = tid + j * tpr, left = cols - ch * CHUNK;
+            settle8(now.dh[j], ch * CHUNK, cols);
+            widen8(now.dh[j], e[j]);
+            if (!a.dhidden) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[j][k] = 0.0f;
             }
-        }
-        for (int64_t r = r0; r < r1; r += whole_groups ? 1 : ny) {
-            Raw<T> dhr[NV];
-            Raw<U> dyr[NEXT ? NV : 1];
-            Saved<U, SRC8> us[EXIT ? NV : 1];
-            Saved<T, SRC8> hs[NEXT ? NV : 1];
+            if constexpr (NEXT) {
+                float dy[8];
+                settle8(now.dy[j], ch * CHUNK, cols);
+                widen8(now.dy[j], dy);
+                now.h[j].get(x[j], ch, cols);
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
-                dhr[j] = zero8<T>();
-                if (a.dhidden) dhr[j] = load8((const T*)a.dhidden + r * a.dhidden_stride + c, cols - c);
-                if constexpr (NEXT) {
-                    dyr[j] = load8((const U*)a.dy + r * a.dy_stride + c, cols - c);
-                    hs[j].load((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch,
-                               cols);
+                for (int k = 0; k < 8; ++k) {
+                    x[j][k] = FULL ? (k < left ? (x[j][k] - mean2) * rstd2 : 0.0f) : x[j][k] * rstd2;
+                    const float g2 = dy[k] * w2[j][k];
+                    W2[j][k] = fmaf(dy[k], x[j][k], W2[j][k]);
+                    if constexpr (FULL) {
+                        B2[j][k] += dy[k];
+                        s[3] += g2;
+                    }
+                    s[0] = fmaf(g2, x[j][k], s[0]);
+                    e[j][k] = fmaf(rstd2, g2, e[j][k]);
                 }
-                if constexpr (EXIT)
-                    us[j].load((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch,
-                               cols);
             }
-            const float rstd1 = post_norm ? a.post_rstd[r] : 1.0f, mean1 = post_layer ? a.post_mean[r] : 0.0f;
-            const float rstd2 = NEXT ? a.next_rstd[r] : 0.0f, mean2 = next_layer ? a.next_mean[r] : 0.0f;
-            float e[NV][8], x[NEXT ? NV : 1][8], u[EXIT ? NV : 1][8];
-            // g2 xhat, h e uhat, h xhat uhat; FULL: g2, h uhat, h e, h, h xhat
-            float s[FULL ? 8 : 3] = {};
+            if constexpr (EXIT) {
+                now.u[j].get(u[j], ch, cols);
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
-                widen8(dhr[j], e[j]);
-                if constexpr (NEXT) {
-                    float dy[8];
-                    widen8(dyr[j], dy);
-                    hs[j].get(x[j]);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        x[j][k] = k < left ? (x[j][k] - mean2) * rstd2 : 0.0f;
-                        const float g2 = dy[k] * w2[j][k];
-                        W2[j][k] = fmaf(dy[k], x[j][k], W2[j][k]);
-                        if constexpr (FULL) {
-                            B2[j][k] += dy[k];
-                            s[3] += k < left ? g2 : 0.0f;
-                        }
-                        s[0] = fmaf(g2, x[j][k], s[0]);
-                        e[j][k] = fmaf(rstd2, g2, e[j][k]);
+                for (int k = 0; k < 8; ++k) {
+                    u[j][k] = FULL ? (k < left ? (u[j][k] - mean1) * rstd1 : 0.0f) : u[j][k] * rstd1;
+                    const float hu = h[j][k] * u[j][k];
+                    s[1] = fmaf(e[j][k], hu, s[1]);
+                    if constexpr (NEXT) s[2] = fmaf(x[j][k], hu, s[2]);
+                    if constexpr (FULL) {
+                        s[4] += hu;
+                        s[5] = fmaf(h[j][k], e[j][k], s[5]);
+                        s[6] += h[j][k];
+                        if constexpr (NEXT) s[7] = fmaf(h[j][k], x[j][k], s[7]);
                     }
                 }
+            }
+        }
+        row_sums(s, red, half);
+        const float k1 = NEXT ? rstd2 * (s[0] * inv_cols) : 0.0f;
+        float k0 = 0.0f, m1 = s[1] - k1 * s[2], m0 = 0.0f;
+        if constexpr (FULL) {
+            k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
+            m1 -= k0 * s[4];
+            m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
+        }
+        m1 = post_norm ? m1 * inv_cols : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+            if (ch < nch) {
+                float o[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (NEXT) e[j][k] -= fmaf(k1, x[j][k], k0);
+                    o[k] = EXIT ? a.residual_scale * e[j][k] : e[j][k];
+                }
+                put8((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
                 if constexpr (EXIT) {
-                    us[j].get(u[j]);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        u[j][k] = k < left ? (u[j][k] - mean1) * rstd1 : 0.0f;
-                        const float hu = h[j][k] * u[j][k];
-                        s[1] = fmaf(e[j][k], hu, s[1]);
-                        if constexpr (NEXT) s[2] = fmaf(x[j][k], hu, s[2]);
-                        if constexpr (FULL) {
-                            s[4] += hu;
-                            s[5] = fmaf(h[j][k], e[j][k], s[5]);
-                            s[6] += h[j][k];
-                            if constexpr (NEXT) s[7] = fmaf(h[j][k], x[j][k], s[7]);
-                        }
+                        P[j][k] = fmaf(u[j][k], e[j][k], P[j][k]);
+                        if constexpr (FULL) Q[j][k] += e[j][k];
+                        o[k] = rstd1 * (FULL ? fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1 : fmaf(h[j][k], e[j][k], -(u[j][k] * m1)));
                     }
+                    put8((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
                 }
             }
-            row_sums(s, red, half);
-            const float k1 = NEXT ? rstd2 * (s[0] * inv_cols) : 0.0f;
-            float k0 = 0.0f, m1 = s[1] - k1 * s[2], m0 = 0.0f;
-            if constexpr (FULL) {
-                k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
-                m1 -= k0 * s[4];
-                m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
-            }
-            m1 = post_norm ? m1 * inv_cols : 0.0f;
+        }
+        now = ahead;
+    }
+    if constexpr (EXIT) {
+        if (whole_groups) {  // this group is complete: its gate's gradient, and its share of the sums
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int64_t ch = tid + j * tpr, c = ch * CHUNK;
                 if (ch < nch) {
-                    float o[8];
+                    float w[8], b[8], gt[8];
+                    vector8(a.weight, a.weight_dtype, c, cols, 1.0f, w);
+                    vector8(a.bias, a.bias_dtype, c, cols, 0.0f, b);
+                    vector8(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, gt);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        if constexpr (NEXT) e[j][k] -= fmaf(k1, x[j][k], k0);
-                        o[k] = EXIT ? a.residual_scale * e[j][k] : e[j][k];
-                    }
-                    put8((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
-                    if constexpr (EXIT) {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            P[j][k] = fmaf(u[j][k], e[j][k], P[j][k]);
-                            if constexpr (FULL) Q[j][k] += e[j][k];
-                            o[k] = rstd1 * (fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1);
-                        }
-                        put8((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
-                    }
-                }
-            }
-        }
-        if constexpr (EXIT) {
-            if (whole_groups) {  // this group is complete: its gate's gradient, and its share of the sums
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
-                    if (ch < nch) {
-                        float w[8], b[8], gt[8];
-                        vector8(a.weight, a.weight_dtype, c, cols - c, 1.0f, w);
-                        vector8(a.bias, a.bias_dtype, c, cols - c, 0.0f, b);
-                        vector8(a.gate, a.gate_dtype, g * cols + c, cols - c, 1.0f, gt);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float q = FULL ? Q[FULL ? j : 0][k] : 0.0f;
-                            if (a.dgate && c + k < cols)
-                                put_scalar(a.dgate, a.gate_dtype, g * cols + c + k,
-                                           a.branch_scale * fmaf(w[k], P[j][k], b[k] * q));
-                            sums_p[c + k] = fmaf(gt[k], P[j][k], sums_p[c + k]);
-                            P[j][k] = 0.0f;
-                            if constexpr (FULL) {
-                                sums_q[c + k] = fmaf(gt[k], q, sums_q[c + k]);
-                                Q[j][k] = 0.0f;
-                            }
+                        const float q = FULL ? Q[FULL ? j : 0][k] : 0.0f;
+                        if (a.dgate && c + k < cols)
+                            put_scalar(a.dgate, a.gate_dtype, g * cols + c + k,
+                                       a.branch_scale * fmaf(w[k], P[j][k], b[k] * q));
+                        sums_p[c + k] = fmaf(gt[k], P[j][k], sums_p[c + k]);
+                        P[j][k] = 0.0f;
+                        if constexpr (FULL) {
+                            sums_q[c + k] = fmaf(gt[k], q, sums_q[c + k]);
+                            Q[j][k] = 0.0f;
                         }
                     }
                 }
             }
         }
+    }
     }
     if constexpr (EXIT) {
         if (whole_groups) {
@@ -633,14 +690,14 @@ __global__ __launch_bounds__(512) void k_norm_backward_wide(const rf_norm a, con
                 const int64_t c = ch * CHUNK, left = cols - c;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) e[k] = x[k] = u[k] = h[k] = dy[k] = g2[k] = 0.0f;
-                if (a.dhidden) widen8(load8((const T*)a.dhidden + r * a.dhidden_stride + c, left), e);
+                if (a.dhidden) widen8(load8((const T*)a.dhidden + r * a.dhidden_stride, c, cols), e);
                 if constexpr (NEXT) {
                     float w[8];
-                    Saved<T, SRC8> hs;
-                    hs.load((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch, cols);
-                    hs.get(x);
-                    widen8(load8((const U*)a.dy + r * a.dy_stride + c, left), dy);
-                    vector8(a.next_weight, a.next_weight_dtype, c, left, 1.0f, w);
+                    Saved<T, SRC8, false> hs;
+                    hs.fetch((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch, cols);
+                    hs.get(x, ch, cols);
+                    widen8(load8((const U*)a.dy + r * a.dy_stride, c, cols), dy);
+                    vector8(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, w);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         x[k] = k < left ? (x[k] - mean2) * rstd2 : 0.0f;
@@ -650,11 +707,11 @@ __global__ __launch_bounds__(512) void k_norm_backward_wide(const rf_norm a, con
                 }
                 if constexpr (EXIT) {
                     float gt[8];
-                    Saved<U, SRC8> us;
-                    us.load((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch, cols);
-                    us.get(u);
-                    vector8(a.weight, a.weight_dtype, c, left, 1.0f, h);
-                    vector8(a.gate, a.gate_dtype, g * cols + c, left, 1.0f, gt);
+                    Saved<U, SRC8, false> us;
+                    us.fetch((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch, cols);
+                    us.get(u, ch, cols);
+                    vector8(a.weight, a.weight_dtype, c, cols, 1.0f, h);
+                    vector8(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, gt);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         u[k] = k < left ? (u[k] - mean1) * rstd1 : 0.0f;
