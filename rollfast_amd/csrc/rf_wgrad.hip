@@ -21,28 +21,31 @@ using rf::report;
 
 namespace {
 
-constexpr int STEP = 64;              // rows t of a step: eight octets
-constexpr int COL_BYTES = STEP * 2;   // LDS bytes of a column's step
+constexpr int STEP = 32;             // rows t of a step: four octets
+constexpr int COL_BYTES = STEP * 2;  // LDS bytes of a column's step
 
 typedef __attribute__((ext_vector_type(8))) bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 
-// LDS place of octet o of column c: two columns share 256 bytes, sixteen slots
-// of 16 bytes, all banks once; column c's octet o is in slot
-//   (8 c0 + o) ^ (c2 + 2 c3 + 4 (c1 ^ c4) + 8 c5)     (ci: bit i of c).
-// Lanes write columns 4 l + i and read columns 16 j + l, and either way sixteen
-// neighbouring lanes touch the sixteen different slots.  What a lane's own bits
-// give is computed once; i, j and the half of the octets xor 4 and 8 onto it,
-// so four addresses and immediate offsets reach everything.
+// LDS place of octet o of column c: four columns share 256 bytes, sixteen slots
+// of 16 bytes, all banks once.  With ci, oi the bits of c and o the slot is the
+// xor of the numbers
+//   o0 1, o1 2, c0 4, c1 8, c2 3, c3 2, c4 4, c5 8.
+// Lanes write columns 4 l + i and read columns 16 j + l % 16 of octet l / 16.
+// 16-byte writes go by eight neighbouring lanes, 16-byte reads by the lanes 0-3,
+// 12-15, 20-23, 24-27 (4-11, 16-19, 28-31; the same from 32 on), as counted
+// conflicts of pairs of lanes show; either set touches different slots.  What a
+// lane's own bits give is computed once, and four addresses with immediate
+// offsets reach everything.
 struct Places {
-    int at[4];  // by the two bits xored onto the slot, 4 and 8
+    int at[4];
 };
 
 __device__ __forceinline__ Places places(int base, int slot)
 {
     Places p;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) p.at[k] = base + ((slot ^ (4 * k)) * 16);
+    for (int k = 0; k < 4; ++k) p.at[k] = base + ((slot ^ (k * 4)) * 16);
     return p;
 }
 
@@ -108,190 +111,269 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t first, uint32_t second)
     return __builtin_amdgcn_perm(second, first, 0x07060302u);
 }
 
-// f32 bits cut to their leading eight significant bits (Inf and NaN stay what they are).
-__device__ __forceinline__ uint32_t head(uint32_t x)
+// What is left of x (f32 bits) behind its high half, its leading eight
+// significant bits: exact; zero behind an infinity (behind a NaN, a NaN).
+__device__ __forceinline__ uint32_t rest(uint32_t x)
 {
-    const uint32_t quiet = (x & 0x7FFFFFFFu) > 0x7F800000u ? 0x00400000u : 0u;
-    return (x | quiet) & 0xFFFF0000u;
+    const float r = __uint_as_float(x) - __uint_as_float(x & 0xFFFF0000u);
+    return __builtin_isinf(__uint_as_float(x)) ? 0u : __float_as_uint(r);
 }
 
-// What the head leaves: exact; nothing behind an Inf or NaN.
-__device__ __forceinline__ uint32_t rest(uint32_t x, uint32_t h)
-{
-    const float r = __uint_as_float(x) - __uint_as_float(h);
-    return (h & 0x7F800000u) == 0x7F800000u ? 0u : __float_as_uint(r);
-}
+// A side's data of one step: eight rows of this lane's four columns.
+template <typename T> struct StagedD { Quad<T> q[8]; };
+struct StagedX { uint32_t c[8], e[2]; };  // codes of the rows, exponents of rows lane % 4 and 4 + lane % 4
 
-// A tile of TK columns x TN outputs per workgroup, WAVES_K x WAVES_N waves.
-// Steps go through two LDS buffers: while one is multiplied, the next step's
-// registers are converted into the other and the loads of the step after that
-// are sent.  The two waves of a SIMD do the two things in opposite order, so
-// that one's conversion runs beside the other's matrix instructions.
-template <typename T, int TK, int TN, int WAVES_K, int WAVES_N>
+// A tile of TILE columns x TILE outputs per workgroup, WAVES_K x WAVES_N waves;
+// the first half of the waves stages the codes, the second half dy.  A wave of
+// each half runs on every SIMD.
+//
+// Step q multiplies LDS buffer q % 3.  In the same step the registers loaded for
+// step q + 2 go into buffer (q + 2) % 3, the loads of step q + 4 are sent, and
+// the first fragments of step q + 1 are read, whose buffer the barrier at the
+// end of step q - 1 completed: nothing in a step waits for what was begun in it.
+// The rows past the last whole step are step 0 of the last split, so that the
+// loop's loads need no guard.
+// EDGE: dy's rows are no multiple of four elements.
+template <typename T, int TILE, int WAVES_K, int WAVES_N, bool EDGE>
 __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE) void k_wgrad(const rf_weight_grad a, float* __restrict__ partial,
                                                                  uint32_t tiles_k, uint32_t tiles, uint32_t splits)
 {
-    constexpr int NP = Pieces<T>::n, THREADS = WAVES_K * WAVES_N * WAVE;
-    constexpr int WK = TK / WAVES_K, WN = TN / WAVES_N, FK = WK / 16, FN = WN / 16;
-    constexpr int X_BYTES = TK * COL_BYTES, D_BYTES = TN * COL_BYTES, BUFFER = X_BYTES + NP * D_BYTES;
-    static_assert(TK / 4 * 8 == THREADS && TN / 4 * 8 == THREADS, "a lane stages one octet of four columns of each side");
+    constexpr int NP = Pieces<T>::n, HALF = WAVES_K * WAVES_N * WAVE / 2;
+    constexpr int WK = TILE / WAVES_K, WN = TILE / WAVES_N, FK = WK / 16, FN = WN / 16;
+    constexpr int PLANE = TILE * COL_BYTES, BUFFER = (1 + NP) * PLANE;
+    static_assert(TILE == HALF, "a lane stages one octet of four columns of its side");
+    static_assert(WK % 64 == 0 && WN % 64 == 0, "bits c4 and c5 are the fragment's number");
     extern __shared__ char lds[];
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
-    const uint32_t tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-    const int64_t k0 = (int64_t)(tile % tiles_k) * TK, n0 = (int64_t)(tile / tiles_k) * TN;
+    // Workgroups go to the eight XCDs in turn: an XCD takes neighbouring tiles,
+    // which share rows of dy in its L2.
+    const uint32_t all = tiles * splits, xcd = blockIdx.x % 8, each = all / 8;
+    const uint32_t id = blockIdx.x < each * 8 ? xcd * each + blockIdx.x / 8 : blockIdx.x;
+    const uint32_t tile = id % tiles, split = id / tiles;
+    const int64_t k0 = (int64_t)(tile % tiles_k) * TILE, n0 = (int64_t)(tile / tiles_k) * TILE;
     const int64_t pitch = pitch_of(a.cols), blocks = pitch / BLOCK;
-    const int64_t all = (a.rows + STEP - 1) / STEP;
-    const int64_t s0 = all * split / splits, s1 = all * (split + 1) / splits;
+    const int64_t whole_steps = a.rows / STEP;
+    const int64_t f0 = whole_steps * split / splits, f1 = whole_steps * (split + 1) / splits;
+    const int tail = split + 1 == splits && a.rows % STEP ? 1 : 0;
+    const int64_t steps = f1 - f0 + tail;
 
-    // ---- staging: this lane's octet and its four columns on either side.
-    // Columns past the end are loaded from valid places and never stored; the
-    // last four of dy's row stand in for a group of columns that the row ends
-    // in, shifted into place.
-    const int oct = tid / (TK / 4), col = tid % (TK / 4) * 4;
+    // ---- staging: this lane's octet and its four columns.  Columns past the
+    // end are loaded from valid places and never stored; the last four of dy's
+    // row stand in for a group of columns that the row ends in, moved into place.
+    const int oct = tid % HALF / (TILE / 4), col = tid % (TILE / 4) * 4;
     const int64_t xc = min(k0 + col, pitch - 4), dc = max(min(n0 + col, a.outs - 4), (int64_t)0);
-    const bool narrow = a.outs < 4, edge = n0 + TN > a.outs && (a.outs & 3) != 0;
+    const bool narrow = EDGE && a.outs < 4;
     const int by = (int)min(n0 + col - dc, (int64_t)3);
-    const int have = (int)max(min(a.outs - (n0 + col), (int64_t)4), (int64_t)0);
     const int64_t d_pitch = a.dy_stride * (int64_t)sizeof(T);
     // bytes of this lane's first row from the step's first row (32 bits: see check())
-    const uint32_t x_off = (uint32_t)(oct * 8 * pitch + xc), e_off = (uint32_t)(oct * 8 * blocks + xc / BLOCK);
-    const uint32_t d_off = (uint32_t)(oct * 8 * d_pitch + dc * (int64_t)sizeof(T));
-    uint32_t xr[8], er[8];
-    Quad<T> dr[8];
-    auto load = [&](int64_t step) {
+    uint32_t x_off = (uint32_t)(oct * 8 * pitch + xc);
+    uint32_t e_off = (uint32_t)((oct * 8 + lane % 4) * blocks + xc / BLOCK);  // (one block for the four lanes)
+    uint32_t d_off = (uint32_t)(oct * 8 * d_pitch + dc * (int64_t)sizeof(T));
+    // row i of a step: a scalar base and a 32-bit lane offset (hide() keeps the
+    // compiler from extending it outside the loop and adding in 64 bits)
+    auto hide = [&] { asm volatile("" : "+v"(x_off), "+v"(e_off), "+v"(d_off)); };
+    auto load_x = [&](int64_t step, StagedX& r, int i) {
         const char* const x = (const char*)a.codes + step * STEP * pitch;
         const char* const e = (const char*)a.exponents + step * STEP * blocks;
+        r.c[i] = *(const uint32_t*)(x + i * pitch + x_off);
+        if (i % 4 == 0) r.e[i / 4] = *(const uint8_t*)(e + i * blocks + e_off);
+    };
+    auto load_d = [&](int64_t step, StagedD<T>& r, int i) {
         const char* const d = (const char*)a.dy + step * STEP * d_pitch;
-        if (step * STEP + STEP <= a.rows && !narrow) {
+        if (EDGE && narrow) r.q[i] = load_some((const T*)(d + i * d_pitch + d_off), (int)a.outs);
+        else r.q[i] = load_quad((const T*)(d + i * d_pitch + d_off));
+    };
+    // the rows behind the last whole step; zeros behind them
+    auto load_tail_x = [&](StagedX& r) {
+        const int64_t t = whole_steps * STEP + oct * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                xr[i] = *(const uint32_t*)(x + i * pitch + x_off);
-                er[i] = *(const uint8_t*)(e + i * blocks + e_off);
-                dr[i] = load_quad((const T*)(d + i * d_pitch + d_off));
-            }
-            if (edge) {
+        for (int i = 0; i < 8; ++i) {
+            r.c[i] = 0;
+            if (t + i < a.rows) r.c[i] = *(const uint32_t*)(a.codes + (t + i) * pitch + xc);
+        }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dr[i] = drop(dr[i], by);
-            }
-        } else {  // the last rows, or a row of fewer than four outputs
-            const int64_t t = step * STEP + oct * 8;
+        for (int i = 0; i < 2; ++i) {
+            r.e[i] = 0;
+            if (t + 4 * i + lane % 4 < a.rows) r.e[i] = a.exponents[(t + 4 * i + lane % 4) * blocks + xc / BLOCK];
+        }
+    };
+    auto load_tail_d = [&](StagedD<T>& r) {
+        const int64_t t = whole_steps * STEP + oct * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                xr[i] = er[i] = 0;
-                dr[i] = Quad<T>{};
-                if (t + i < a.rows) {
-                    xr[i] = *(const uint32_t*)(x + i * pitch + x_off);
-                    er[i] = *(const uint8_t*)(e + i * blocks + e_off);
-                    dr[i] = load_some((const T*)a.dy + (t + i) * a.dy_stride + (have ? n0 + col : 0), have);
-                }
+        for (int i = 0; i < 8; ++i) {
+            r.q[i] = Quad<T>{};
+            if (t + i < a.rows) {
+                const T* const p = (const T*)a.dy + (t + i) * a.dy_stride + dc;
+                r.q[i] = a.outs < 4 ? load_some(p, (int)a.outs) : load_quad(p);
             }
         }
     };
     // col is a multiple of four: bits c2 .. c5 are the lane's
-    const Places put = places(col / 2 * 256, oct ^ (((col >> 2) & 3) | ((col >> 4) & 1) << 2 | ((col >> 5) & 1) << 3));
-    auto stage = [&](char* buf) {
-        float step[8];
+    const Places put = places(col / 4 * 256, oct ^ ((col >> 2) & 1) * 3 ^ ((col >> 3) & 1) * 2 ^ ((col >> 4) & 3) * 4);
+    // column c of the four
+    auto stage_x = [&](char* buf, const StagedX& r, int c) {
+        const uint32_t e[8] = {dpp<0x00>(r.e[0]), dpp<0x55>(r.e[0]), dpp<0xAA>(r.e[0]), dpp<0xFF>(r.e[0]),
+                               dpp<0x00>(r.e[1]), dpp<0x55>(r.e[1]), dpp<0xAA>(r.e[1]), dpp<0xFF>(r.e[1])};
+        u32x4 v;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) step[i] = __uint_as_float(er[i] << 23);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            u32x4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float lo = (float)(int8_t)(xr[2 * i] >> (8 * c)) * step[2 * i];
-                const float hi = (float)(int8_t)(xr[2 * i + 1] >> (8 * c)) * step[2 * i + 1];
-                v[i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
-            }
-            *(u32x4*)(buf + put.at[(c >> 1) | (c & 1) << 1] + (c >> 1) * 256) = v;
+        for (int i = 0; i < 4; ++i) {
+            const float lo = (float)(int8_t)(r.c[2 * i] >> (8 * c)) * __uint_as_float(e[2 * i] << 23);
+            const float hi = (float)(int8_t)(r.c[2 * i + 1] >> (8 * c)) * __uint_as_float(e[2 * i + 1] << 23);
+            v[i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
         }
-        char* const d = buf + X_BYTES;
+        *(u32x4*)(buf + put.at[c]) = v;
+    };
+    auto stage_d = [&](char* buf, StagedD<T>& r, int c) {
+        if (EDGE && c == 0) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            u32x4 v[NP];
+            for (int i = 0; i < 8; ++i) r.q[i] = drop(r.q[i], by);
+        }
+        u32x4 v[NP];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (NP == 1) {
-                    v[0][i] = __builtin_amdgcn_perm(dr[2 * i + 1].w[c / 2], dr[2 * i].w[c / 2],
-                                                    c & 1 ? 0x07060302u : 0x05040100u);
-                } else {
-                    uint32_t x[2];
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (NP == 1) {
+                v[0][i] = __builtin_amdgcn_perm(r.q[2 * i + 1].w[c / 2], r.q[2 * i].w[c / 2],
+                                                c & 1 ? 0x07060302u : 0x05040100u);
+            } else {
+                uint32_t x[2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        if constexpr (NP == 3) {
-                            x[j] = dr[2 * i + j].w[c];
-                        } else {
-                            const uint16_t h = (uint16_t)(dr[2 * i + j].w[c / 2] >> (16 * (c & 1)));
-                            f16 f;
-                            __builtin_memcpy(&f, &h, 2);
-                            x[j] = __float_as_uint((float)f);
-                        }
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (NP == 3) {
+                        x[j] = r.q[2 * i + j].w[c];
+                    } else {
+                        const uint16_t h = (uint16_t)(r.q[2 * i + j].w[c / 2] >> (16 * (c & 1)));
+                        f16 f;
+                        __builtin_memcpy(&f, &h, 2);
+                        x[j] = __float_as_uint((float)f);
                     }
+                }
 #pragma unroll
-                    for (int p = 0; p < NP; ++p) {
-                        const uint32_t h0 = head(x[0]), h1 = head(x[1]);
-                        v[p][i] = high_halves(h0, h1);
-                        if (p + 1 < NP) {
-                            x[0] = rest(x[0], h0);
-                            x[1] = rest(x[1], h1);
-                        }
+                for (int p = 0; p < NP; ++p) {
+                    v[p][i] = high_halves(x[0], x[1]);
+                    if (p + 1 < NP) {
+                        x[0] = rest(x[0]);
+                        x[1] = rest(x[1]);
                     }
                 }
             }
-#pragma unroll
-            for (int p = 0; p < NP; ++p) *(u32x4*)(d + p * D_BYTES + put.at[(c >> 1) | (c & 1) << 1] + (c >> 1) * 256) = v[p];
         }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *(u32x4*)(buf + (1 + p) * PLANE + put.at[c]) = v[p];
     };
 
     // ---- the product: lane l holds column l % 16 of a fragment, octet l / 16
     const int wk = wave / WAVES_N * WK, wn = wave % WAVES_N * WN;
-    static_assert(WK % 64 == 0 && WN % 64 == 0, "bits c4 and c5 are the fragment's number");
-    const int slot = (((lane & 1) << 3) | (lane >> 4)) ^ (((lane >> 2) & 3) | ((lane >> 1) & 1) << 2);
-    const Places get_x = places(wk / 2 * 256 + (lane & 15) / 2 * 256, slot);
-    const Places get_d = places(X_BYTES + wn / 2 * 256 + (lane & 15) / 2 * 256, slot);
+    const int slot = (lane >> 4) ^ (lane & 3) * 4 ^ ((lane >> 2) & 1) * 3 ^ ((lane >> 3) & 1) * 2;
+    const Places get_x = places(wk / 4 * 256 + (lane & 15) / 4 * 256, slot);
+    const Places get_d = places(PLANE + wn / 4 * 256 + (lane & 15) / 4 * 256, slot);
+    auto read_x = [&](const char* buf, int i) { return *(const bf16x8*)(buf + get_x.at[i & 3] + i * 1024); };
+    auto read_d = [&](const char* buf, int p, int j) { return *(const bf16x8*)(buf + get_d.at[j & 3] + p * PLANE + j * 1024); };
     f32x4 acc[FK][FN];
 #pragma unroll
     for (int i = 0; i < FK; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto multiply = [&](const char* buf) {
+
+    // One side's run through the steps.
+    struct Fragments {
+        bf16x8 y[NP][FN], x[2];  // all of a step's on dy's side, the first two on the codes'
+    };
+    auto run = [&](auto load, auto load_tail, auto stage, auto& even, auto& odd) {
+        // step p of this split, clamped: what lies past its end is staged and never read
+        auto clamped = [&](int64_t p) { return max(min(f0 + p - tail, f1 - 1), (int64_t)0); };
+        auto fetch = [&](int64_t p, auto& r) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            bf16x8 x[FK];
+            for (int i = 0; i < 8; ++i) load(clamped(p), r, i);
+        };
+        auto stage_all = [&](char* buf, auto& r) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) stage(buf, r, c);
+        };
+        char *now = lds, *next = lds + BUFFER, *after = lds + 2 * BUFFER;
+        if (tail) load_tail(even);
+        else fetch(0, even);
+        if (whole_steps) fetch(1, odd);
+        stage_all(now, even);
+        if (whole_steps) {
+            fetch(2, even);
+            stage_all(next, odd);
+            fetch(3, odd);
+        }
+        __syncthreads();
+        Fragments f, g;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) f.y[p][j] = read_d(now, p, j);
+        f.x[0] = read_x(now, 0);
+        f.x[1] = read_x(now, 1);
+        // The matrix instructions of fragment row i, then a piece of the other
+        // work of the step that the matrix cores run beside.
+        auto step = [&](int64_t q, auto& regs, Fragments& f, Fragments& g) {
+            const int64_t ahead = clamped(q + 4);
+            hide();
+#pragma unroll
+            for (int i = 0; i < FK; ++i) {
+                const bf16x8 xi = f.x[i & 1];
+                if (i + 2 < FK) f.x[i & 1] = read_x(now, i + 2);
+                else g.x[i & 1] = read_x(next, i + 2 - FK);
+                if (i + 2 >= FK) {
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int j = (i + 2 - FK) * FN / 2; j < (i + 3 - FK) * FN / 2; ++j) g.y[p][j] = read_d(next, p, j);
+                }
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xi, f.y[p][j], acc[i][j], 0, 0, 0);
+                // FK is 8 or 4: four columns in the first half, or a quarter each; then the loads
+                if (i < 4) stage(after, regs, i);
+                if (FK == 8 && i >= 4) {
+                    load(ahead, regs, 2 * (i - 4));
+                    load(ahead, regs, 2 * (i - 4) + 1);
+                }
+                if (FK == 4 && i == 3) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) load(ahead, regs, k);
+                }
+#pragma unroll
+                for (int k = 0; k < NP * FN; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction,
+                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // up to six vector ones beside it
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            char* const t = now;
+            now = next;
+            next = after;
+            after = t;
+            __syncthreads();
+        };
+        if (whole_steps) {
+            for (int64_t q = 0; q < steps; q += 2) {
+                step(q, even, f, g);
+                if (q + 1 < steps) step(q + 1, odd, g, f);
+            }
+        } else {  // fewer rows than a step
 #pragma unroll
             for (int i = 0; i < FK; ++i)
-                x[i] = *(const bf16x8*)(buf + get_x.at[(half ^ (i & 1)) | ((i >> 1) & 1) << 1] + i * 2048);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
+                for (int p = 0; p < NP; ++p)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    const bf16x8 y = *(const bf16x8*)(buf + get_d.at[(half ^ (j & 1)) | ((j >> 1) & 1) << 1] +
-                                                      p * D_BYTES + j * 2048);
-#pragma unroll
-                    for (int i = 0; i < FK; ++i)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y, acc[i][j], 0, 0, 0);
-                }
-            }
+                    for (int j = 0; j < FN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(i < 2 ? f.x[i & 1] : read_x(now, i), f.y[p][j],
+                                                                           acc[i][j], 0, 0, 0);
         }
     };
-
-    if (s0 < s1) {
-        load(s0);
-        stage(lds);
-        if (s0 + 1 < s1) load(s0 + 1);
-        __syncthreads();
-        for (int64_t s = s0; s < s1; ++s) {
-            char* const now = lds + ((s - s0) & 1) * BUFFER;
-            char* const next = lds + ((s - s0 + 1) & 1) * BUFFER;
-            if (wave < WAVES_K * WAVES_N / 2) {
-                if (s + 1 < s1) stage(next);
-                if (s + 2 < s1) load(s + 2);
-                multiply(now);
-            } else {
-                multiply(now);
-                if (s + 1 < s1) stage(next);
-                if (s + 2 < s1) load(s + 2);
-            }
-            __syncthreads();
+    if (steps > 0) {
+        if (wave < WAVES_K * WAVES_N / 2) {
+            StagedX even, odd;
+            run(load_x, load_tail_x, stage_x, even, odd);
+        } else {
+            StagedD<T> even, odd;
+            run(load_d, load_tail_d, stage_d, even, odd);
         }
     }
 
@@ -362,34 +444,55 @@ struct Plan {
     int64_t workspace;
 };
 
+// The cheapest of the tiles and splits by what they take (us, measured on one
+// GPU): 5 for a round of workgroups, `step` for 32 rows, and, split, 3 and the
+// partial sums at 4 TB/s.  Workgroups at a time: one a CU with 256 x 256 tiles
+// and with two or three pieces, else two.
 Plan plan_of(const rf_weight_grad& a, int cus)
 {
-    Plan p{};
-    auto count = [&](int64_t tk, int64_t tn) {
-        p.tiles_k = (uint32_t)((a.cols + tk - 1) / tk);
-        p.tiles = p.tiles_k * (uint32_t)((a.outs + tn - 1) / tn);
-    };
-    count(256, 256);
-    p.big = a.dy_dtype == RF_BF16 && (int64_t)p.tiles * 4 >= (int64_t)cus * 3;
-    if (!p.big) count(128, 128);
-    // few tiles: the rows are split so that the chip is filled, four steps a split at least
-    const int64_t steps = (a.rows + STEP - 1) / STEP, room = (int64_t)cus * (p.big || a.dy_dtype != RF_BF16 ? 1 : 2);
-    p.splits = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(steps / 4, room / p.tiles));
-    p.workspace = p.splits > 1 ? (int64_t)p.splits * a.outs * a.cols * 4 : 0;
-    return p;
+    Plan best{};
+    double least = 1e30;
+    const int64_t steps = (a.rows + STEP - 1) / STEP;
+    for (int big = 0; big < (a.dy_dtype == RF_BF16 ? 2 : 1); ++big) {
+        Plan p{};
+        const int64_t tile = big ? 256 : 128;
+        p.big = big != 0;
+        p.tiles_k = (uint32_t)((a.cols + tile - 1) / tile);
+        p.tiles = p.tiles_k * (uint32_t)((a.outs + tile - 1) / tile);
+        const int64_t room = (int64_t)cus * (big || a.dy_dtype != RF_BF16 ? 1 : 2);
+        const double step = big ? 1.05 : a.dy_dtype == RF_F32 ? 1.2 : 0.9;
+        for (int64_t n = 1; n <= std::min<int64_t>(std::max<int64_t>(1, steps), 64); ++n) {
+            const double rounds = (double)((p.tiles * n + room - 1) / room);
+            const double us = rounds * (5 + step * (double)((steps + n - 1) / n)) +
+                              (n > 1 ? 3 + (double)n * (double)a.outs * (double)a.cols * 8 / 4e6 : 0);
+            if (us < least) {
+                least = us;
+                best = p;
+                best.splits = (uint32_t)n;
+            }
+        }
+    }
+    best.workspace = best.splits > 1 ? (int64_t)best.splits * a.outs * a.cols * 4 : 0;
+    return best;
 }
 
-template <typename T, int TK, int TN, int WK, int WN>
+template <typename T, int TILE, int WK, int WN, bool EDGE>
 rf_status launch(const rf_weight_grad& a, const Plan& p, float* partial, hipStream_t st)
 {
-    constexpr size_t LDS = 2 * (size_t)(TK + Pieces<T>::n * TN) * COL_BYTES;
-    const auto f = k_wgrad<T, TK, TN, WK, WN>;
+    constexpr size_t LDS = 3 * (size_t)(1 + Pieces<T>::n) * TILE * COL_BYTES;
+    const auto f = k_wgrad<T, TILE, WK, WN, EDGE>;
     if (LDS > 64 * 1024) {
         static const hipError_t e = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
         if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
     }
     f<<<p.tiles * p.splits, WK * WN * WAVE, LDS, st>>>(a, partial, p.tiles_k, p.tiles, p.splits);
     return RF_OK;
+}
+
+template <typename T, int TILE, int WK, int WN>
+rf_status launch(const rf_weight_grad& a, const Plan& p, float* partial, hipStream_t st)
+{
+    return a.outs % 4 ? launch<T, TILE, WK, WN, true>(a, p, partial, st) : launch<T, TILE, WK, WN, false>(a, p, partial, st);
 }
 
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
@@ -436,10 +539,10 @@ rf_status rf_linear_weight_grad(const rf_weight_grad* args, void* workspace, int
     hipStream_t st = (hipStream_t)stream;
     float* const partial = (float*)workspace;
     rf_status s;
-    if (a.dy_dtype == RF_F32) s = launch<float, 128, 128, 2, 2>(a, p, partial, st);
-    else if (a.dy_dtype == RF_F16) s = launch<f16, 128, 128, 2, 2>(a, p, partial, st);
-    else if (p.big) s = launch<bf16, 256, 256, 2, 4>(a, p, partial, st);
-    else s = launch<bf16, 128, 128, 2, 2>(a, p, partial, st);
+    if (a.dy_dtype == RF_F32) s = launch<float, 128, 2, 2>(a, p, partial, st);
+    else if (a.dy_dtype == RF_F16) s = launch<f16, 128, 2, 2>(a, p, partial, st);
+    else if (p.big) s = launch<bf16, 256, 2, 4>(a, p, partial, st);
+    else s = launch<bf16, 128, 2, 2>(a, p, partial, st);
     if (s != RF_OK) return s;
     if (p.splits > 1) {
         const int64_t grid = (a.outs * a.cols + 1023) / 1024;
