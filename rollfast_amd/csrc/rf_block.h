@@ -224,7 +224,7 @@ template <typename T> __device__ __forceinline__ void put8(T* p, const Raw<T>& r
 }
 
 // Columns of a parameter vector whose type is known at run time (RF_F32 /
-// RF_BF16 / RF_F16), or of one that is not there.  Loads of several vectors are
+// RF_BF16 / RF_F16), or `fill` for one that is not there; zero past the end.  Loads of several vectors are
 // sent before the first is looked at: `elsewhere` is any eight 16-bit elements
 // that may be read instead of an absent vector's.
 struct Vector8 {
@@ -241,7 +241,7 @@ struct Vector8 {
     {
         if (!p) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = fill;
+            for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? fill : 0.0f;
         } else if (dtype == RF_F32) {
             Raw<float> r{a, b};
             settle8(r, c, cols);

@@ -28,7 +28,20 @@ namespace rfb {
 
 constexpr int MAX_WAVES = 8;  // waves of a row in the register kernels
 
-// How the rows of a backward pass are dealt out.
+// n things dealt to `of` takers in runs; the first `more` get one more than `each`.
+// (Kernels divide nothing: a 64-bit division is 140 instructions.)
+struct Share {
+    uint32_t each, more;
+};
+
+__host__ __device__ inline Share share_of(int64_t n, int64_t of)
+{
+    return {(uint32_t)(n / of), (uint32_t)(n % of)};
+}
+
+__device__ __forceinline__ int64_t first_of(const Share& s, uint32_t i) { return (int64_t)s.each * i + min(i, s.more); }
+
+// How the rows of a pass are dealt out.
 struct NormPlan {
     int32_t pieces;    // pieces of a group, each a workgroup (0: workgroups take whole groups)
     int32_t workers;   // workgroups = partial rows
@@ -36,9 +49,8 @@ struct NormPlan {
     int32_t i_p, i_q, i_w2, i_b2;  // their indices, -1 absent
     int64_t group_rows;            // rows that share a gate
     int64_t groups;
+    Share rows;                    // forward: a workgroup's rows; backward: a piece's rows, or a workgroup's groups
 };
-
-__device__ __forceinline__ int64_t part(int64_t n, int64_t i, int64_t of) { return n * i / of; }
 
 // Sums of NS values over the tpr lanes of a row.  `red` has two halves used
 // in turn, so one barrier a call is enough: a half is written again only
@@ -73,18 +85,18 @@ __device__ __forceinline__ const void* gate_row(const rf_norm& a, int64_t g)
 // ------------------------------------------------------------- forward -----
 // blockDim (tpr, ny): tpr lanes a row; ny > 1 only where a wave holds a row.
 // FULL: LayerNorm or a bias somewhere.  The next row's loads are sent before
-// this row's sums.
+// this row's sums.  Past the end of a row the elements and the vectors are
+// zero, and so is what they give.
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, int NV>
-__global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
+__global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Share share, const uint32_t group_rows)
 {
     __shared__ float red[2][MAX_WAVES][8];
     int half = 0;
     const int tid = threadIdx.x, tpr = blockDim.x, ty = __builtin_amdgcn_readfirstlane(threadIdx.y), ny = blockDim.y;
     const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
     const float inv_cols = 1.0f / (float)cols;
-    const int64_t r0 = part(a.rows, blockIdx.x, gridDim.x) + ty, r1 = part(a.rows, blockIdx.x + 1, gridDim.x);
+    const int64_t r0 = first_of(share, blockIdx.x) + ty, r1 = first_of(share, blockIdx.x + 1);
     if (r0 >= r1) return;  // a wave of its own (ny > 1): no other waits for it
-    const int64_t group_rows = a.gates > 1 ? a.rows / a.gates : 0;
     struct Row {
         Raw<T> r[NV];
         Raw<U> u[EXIT ? NV : 1];
@@ -137,20 +149,25 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
-            float v[8];
+            float v[8], t = 0.0f;
             widen8(x[j], v);
+            if (FULL && (cols & (CHUNK - 1))) {  // the row may end inside the chunk
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = k < left ? v[k] : mean;
+            }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float d = FULL ? (k < left ? v[k] - mean : 0.0f) : v[k];
-                s[0] = fmaf(d, d, s[0]);
+                const float d = FULL ? v[k] - mean : v[k];
+                t = fmaf(d, d, t);
             }
+            s[0] += FULL && left <= 0 ? 0.0f : t;
         }
         row_sums(s, red, half);
         rstd = 1.0f / sqrtf(s[0] * inv_cols + eps);
     };
     for (int64_t r = r0; r < r1;) {
     // the rows of one gate
-    const int64_t g = group_rows ? r / group_rows : 0, end = group_rows ? min(r1, (g + 1) * group_rows) : r1;
+    const int64_t g = group_rows ? (uint32_t)r / group_rows : 0, end = group_rows ? min(r1, (g + 1) * group_rows) : r1;
     float A[EXIT ? NV : 1][8], B[EXIT && FULL ? NV : 1][8];
     if constexpr (EXIT) {
         Vector8 w[NV], b[NV], gt[NV];
@@ -205,7 +222,6 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
                     for (int k = 0; k < 8; ++k) {
                         const float n = FULL ? fmaf((u[k] - mean) * rstd, A[j][k], B[FULL ? j : 0][k]) : u[k] * rstd * A[j][k];
                         o[k] = fmaf(a.residual_scale, x[k], n);
-                        if (FULL && c + k >= cols) o[k] = 0.0f;
                     }
                     now.r[j] = narrow8<T>(o);
                     put8((T*)a.hidden + r * cols + c, now.r[j], cols - c);
@@ -229,7 +245,6 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         y[k] = FULL ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[FULL ? j : 0][k]) : v[k] * rstd * w2[j][k];
-                        if (FULL && c + k >= cols) y[k] = 0.0f;
                     }
                     const Raw<U> yr = narrow8<U>(y);
                     put8((U*)a.y + r * cols + c, yr, cols - c);
@@ -368,6 +383,8 @@ template <typename T, bool WIDE> struct Saved<T, true, WIDE> {
     __device__ __forceinline__ void get(float (&v)[8], int64_t, int64_t) const { decode8(t, v); }
 };
 
+// Past the end of a row dy, dhidden and h are zero, so xhat and uhat may be
+// anything finite there.
 // FULL: LayerNorm or a bias somewhere (the sums of g, t and their columns).
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, int NV>
 __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const NormPlan plan, float* __restrict__ partial)
@@ -389,15 +406,15 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
     int64_t r0, r1, g;
     const int64_t step = whole_groups ? 1 : ny;
     if (whole_groups) {
-        const int64_t ga = part(plan.groups, blockIdx.x, gridDim.x), gb = part(plan.groups, blockIdx.x + 1, gridDim.x);
-        g = ga + part(gb - ga, ty, ny);
+        const int64_t ga = first_of(plan.rows, blockIdx.x), n = first_of(plan.rows, blockIdx.x + 1) - ga;
+        g = ga + (ny == 4 ? n * ty / 4 : 0);
         r0 = g * plan.group_rows;
-        r1 = (ga + part(gb - ga, ty + 1, ny)) * plan.group_rows;
+        r1 = (ga + (ny == 4 ? n * (ty + 1) / 4 : n)) * plan.group_rows;
     } else {
-        const int64_t piece = blockIdx.x % plan.pieces;
-        g = blockIdx.x / plan.pieces;
-        r0 = g * plan.group_rows + part(plan.group_rows, piece, plan.pieces) + ty;
-        r1 = g * plan.group_rows + part(plan.group_rows, piece + 1, plan.pieces);
+        const uint32_t piece = blockIdx.x % (uint32_t)plan.pieces;
+        g = blockIdx.x / (uint32_t)plan.pieces;
+        r0 = g * plan.group_rows + first_of(plan.rows, piece) + ty;
+        r1 = g * plan.group_rows + first_of(plan.rows, piece + 1);
     }
     struct Row {
         Raw<T> dh[NV];
@@ -469,7 +486,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
             w[j].get(a.weight, a.weight_dtype, c, cols, 1.0f, h[j]);
             gt[j].get(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) h[j][k] = c + k < cols ? h[j][k] * a.branch_scale * v[k] : 0.0f;
+            for (int k = 0; k < 8; ++k) h[j][k] *= a.branch_scale * v[k];
         }
     }
     for (; r < end; r += step) {
@@ -480,7 +497,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
         float s[FULL ? 8 : 3] = {};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t ch = tid + j * tpr, left = cols - ch * CHUNK;
+            const int64_t ch = tid + j * tpr;
             settle8(now.dh[j], ch * CHUNK, cols);
             widen8(now.dh[j], e[j]);
             if (!a.dhidden) {
@@ -494,7 +511,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
                 now.h[j].get(x[j], ch, cols);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    x[j][k] = FULL ? (k < left ? (x[j][k] - mean2) * rstd2 : 0.0f) : x[j][k] * rstd2;
+                    x[j][k] = FULL ? (x[j][k] - mean2) * rstd2 : x[j][k] * rstd2;
                     const float g2 = dy[k] * w2[j][k];
                     W2[j][k] = fmaf(dy[k], x[j][k], W2[j][k]);
                     if constexpr (FULL) {
@@ -509,7 +526,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
                 now.u[j].get(u[j], ch, cols);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    u[j][k] = FULL ? (k < left ? (u[j][k] - mean1) * rstd1 : 0.0f) : u[j][k] * rstd1;
+                    u[j][k] = FULL ? (u[j][k] - mean1) * rstd1 : u[j][k] * rstd1;
                     const float hu = h[j][k] * u[j][k];
                     s[1] = fmaf(e[j][k], hu, s[1]);
                     if constexpr (NEXT) s[2] = fmaf(x[j][k], hu, s[2]);
@@ -669,17 +686,17 @@ __global__ __launch_bounds__(512) void k_norm_backward_wide(const rf_norm a, con
             for (int v = 0; v < plan.vectors; ++v) mine[v * cols + c] = 0.0f;
             if (whole_groups) group_sums[c] = group_sums[cols + c] = 0.0f;
         }
-    const int64_t g0 = whole_groups ? part(plan.groups, blockIdx.x, gridDim.x) : blockIdx.x / max(plan.pieces, 1);
-    const int64_t g1 = whole_groups ? part(plan.groups, blockIdx.x + 1, gridDim.x) : g0 + 1;
+    const int64_t g0 = whole_groups ? first_of(plan.rows, blockIdx.x) : blockIdx.x / max(plan.pieces, 1);
+    const int64_t g1 = whole_groups ? first_of(plan.rows, blockIdx.x + 1) : g0 + 1;
     float* const sum_p = whole_groups ? group_sums : mine + (int64_t)max(plan.i_p, 0) * cols;
     float* const sum_q = whole_groups ? group_sums + cols : mine + (int64_t)max(plan.i_q, 0) * cols;
     const bool want_q = whole_groups || plan.i_q >= 0;
     for (int64_t g = g0; g < g1; ++g) {
         int64_t r0 = g * plan.group_rows, r1 = r0 + plan.group_rows;
         if (!whole_groups) {
-            const int64_t piece = blockIdx.x % max(plan.pieces, 1);
-            r1 = r0 + part(plan.group_rows, piece + 1, plan.pieces);
-            r0 += part(plan.group_rows, piece, plan.pieces);
+            const uint32_t piece = blockIdx.x % max(plan.pieces, 1);
+            r1 = r0 + first_of(plan.rows, piece + 1);
+            r0 += first_of(plan.rows, piece);
         }
         for (int64_t r = r0; r < r1; ++r) {
             const float rstd1 = post_norm ? a.post_rstd[r] : 1.0f, mean1 = post_layer ? a.post_mean[r] : 0.0f;

@@ -15,11 +15,13 @@ using U = Elem<RFI_U>::type;
 template <bool EXIT, bool NEXT> static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
 {
     const dim3 grid((unsigned)s.workers), block(s.tpr, s.ny);
+    const Share rows = share_of(a.rows, s.workers);
+    const uint32_t per_gate = a.gates > 1 ? (uint32_t)(a.rows / a.gates) : 0;
     if (s.nv == 0) k_norm_forward_wide<T, U, EXIT, NEXT><<<grid, block, 0, st>>>(a);
-    else if (s.nv == 1 && s.full) k_norm_forward<T, U, EXIT, NEXT, true, 1><<<grid, block, 0, st>>>(a);
-    else if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, false, 1><<<grid, block, 0, st>>>(a);
-    else if (s.full) k_norm_forward<T, U, EXIT, NEXT, true, 2><<<grid, block, 0, st>>>(a);
-    else k_norm_forward<T, U, EXIT, NEXT, false, 2><<<grid, block, 0, st>>>(a);
+    else if (s.nv == 1 && s.full) k_norm_forward<T, U, EXIT, NEXT, true, 1><<<grid, block, 0, st>>>(a, rows, per_gate);
+    else if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, false, 1><<<grid, block, 0, st>>>(a, rows, per_gate);
+    else if (s.full) k_norm_forward<T, U, EXIT, NEXT, true, 2><<<grid, block, 0, st>>>(a, rows, per_gate);
+    else k_norm_forward<T, U, EXIT, NEXT, false, 2><<<grid, block, 0, st>>>(a, rows, per_gate);
 }
 
 template <bool EXIT, bool NEXT, bool FULL, bool SRC8>

@@ -119,6 +119,51 @@ __device__ __forceinline__ uint32_t rest(uint32_t x)
     return __builtin_isinf(__uint_as_float(x)) ? 0u : __float_as_uint(r);
 }
 
+// Writes a wave's accumulators, columns from k and outputs from n on: a lane
+// holds four neighbouring columns of an output's row.  `partial`: this split's
+// sums, or null for the result.
+template <int FK, int FN>
+__device__ __forceinline__ void store_tile(const rf_weight_grad& a, float* __restrict__ partial, const f32x4 (&acc)[FK][FN],
+                                           int64_t k_from, int64_t n_from)
+{
+    const int lane = threadIdx.x % WAVE;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int64_t n = n_from + 16 * j + lane % 16;
+        if (n >= a.outs) continue;
+#pragma unroll
+        for (int i = 0; i < FK; ++i) {
+            const int64_t k = k_from + 16 * i + lane / 16 * 4, left = a.cols - k, at = n * a.cols + k;
+            if (partial) {
+                float* const o = partial + at;
+                if (left >= 4) {
+                    *(u32x4_at*)o = __builtin_bit_cast(u32x4, acc[i][j]);
+                } else {
+                    for (int r = 0; r < 4; ++r)
+                        if (r < left) o[r] = acc[i][j][r];
+                }
+                continue;
+            }
+            if (a.out_dtype == RF_F32 && left >= 4) {
+                float* const o = (float*)a.out + at;
+                f32x4 v = acc[i][j];
+                if (a.accumulate) v += __builtin_bit_cast(f32x4, (u32x4) * (const u32x4_at*)o);
+                *(u32x4_at*)o = __builtin_bit_cast(u32x4, v);
+            } else if (a.out_dtype == RF_BF16 && left >= 4 && !a.accumulate) {
+                const f32x4 v = acc[i][j];
+                const bf16x2 lo = __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2);
+                const bf16x2 hi = __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2);
+                *(u32x2_h*)((bf16*)a.out + at) = u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+            } else {
+                for (int r = 0; r < 4; ++r)
+                    if (r < left)
+                        put_scalar(a.out, a.out_dtype, at + r,
+                                   a.accumulate ? scalar_at(a.out, a.out_dtype, at + r) + acc[i][j][r] : acc[i][j][r]);
+            }
+        }
+    }
+}
+
 // A side's data of one step: eight rows of this lane's four columns.
 template <typename T> struct StagedD { Quad<T> q[8]; };
 struct StagedX { uint32_t c[8], e[2]; };  // codes of the rows, exponents of rows lane % 4 and 4 + lane % 4
@@ -377,43 +422,230 @@ __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE) void k_wgrad(const rf_weigh
         }
     }
 
-    // ---- a lane holds four neighbouring columns of an output's row
-    const bool whole = splits == 1;
+    store_tile(a, splits == 1 ? nullptr : partial + (int64_t)split * a.outs * a.cols, acc, k0 + wk, n0 + wn);
+}
+
+// The same for bf16 gradients whose rows are whole 16-byte units, tiles of
+// 256 x 256: every load goes straight to LDS (1 KB a wave instruction, no
+// registers), several steps ahead.
+//
+// dy's rows stay as they are, [32 t][256 n], and are transposed as they are
+// read: ds_read_b64_tr_b16 gives a lane four t of one column.  The codes and
+// exponents land in rings of their own and go from there through registers to
+// the same layout as above: a lane converts four rows of four columns.
+//   step q:  loads of dy of step q + 3 and of the codes of step q + 5 sent;
+//            codes of step q + 2 converted; products of step q; first fragments
+//            of step q + 1 read; at its end the wave waits for its loads of dy
+//            of step q + 2 and of the codes of step q + 3 (all but its last six),
+//            and the barrier makes them everybody's.
+// 32-byte units of dy's rows are xored by (t0, t1, t3) so that the sixteen rows
+// of a transposed read lie in different banks.
+//
+// The compiler must not count or order these loads (it would wait for all of
+// them before each LDS read): they are written in assembly, have no results,
+// and the waits for them are explicit.  (m0, which they set, is otherwise unused
+// here.)
+constexpr int DIRECT = 256, DIRECT_WAVES = 8;
+constexpr int D_SLOT = STEP * DIRECT * 2, X_SLOT = STEP * DIRECT, E_SLOT = DIRECT_WAVES * WAVE * 4;
+constexpr int D_RING = 4, X_RING = 4;
+constexpr int AT_D = 0, AT_X = AT_D + D_RING * D_SLOT, AT_E = AT_X + X_RING * X_SLOT, AT_B = AT_E + X_RING * E_SLOT;
+constexpr int DIRECT_LDS = AT_B + 3 * DIRECT * COL_BYTES;
+static_assert(DIRECT_LDS <= 160 * 1024, "one workgroup a CU");
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+__device__ __forceinline__ void load_16_to_lds(uint32_t to, uint32_t off, const char* base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+
+__device__ __forceinline__ void load_byte_to_lds(uint32_t to, uint32_t off, const char* base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+
+__global__ __launch_bounds__(DIRECT_WAVES* WAVE) void k_wgrad_direct(const rf_weight_grad a, float* __restrict__ partial,
+                                                                    uint32_t tiles_k, uint32_t tiles, uint32_t splits)
+{
+    constexpr int WK = 128, WN = 64, FK = WK / 16, FN = WN / 16;
+    extern __shared__ char lds[];
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const uint32_t all = tiles * splits, xcd = blockIdx.x % 8, each = all / 8;  // as in k_wgrad
+    const uint32_t id = blockIdx.x < each * 8 ? xcd * each + blockIdx.x / 8 : blockIdx.x;
+    const uint32_t tile = id % tiles, split = id / tiles;
+    const int64_t k0 = (int64_t)(tile % tiles_k) * DIRECT, n0 = (int64_t)(tile / tiles_k) * DIRECT;
+    const int64_t pitch = pitch_of(a.cols), blocks = pitch / BLOCK, d_pitch = a.dy_stride * 2;
+    const int64_t whole_steps = a.rows / STEP;
+    const int64_t f0 = whole_steps * split / splits, f1 = whole_steps * (split + 1) / splits;
+    const int tail = split + 1 == splits && a.rows % STEP ? 1 : 0;
+    const int64_t steps = f1 - f0 + tail;
+
+    // ---- loads: this wave's rows 4 w .. 4 w + 3 of a step.  Columns past the
+    // end come from valid places and are never stored.
+    const int row0 = 4 * wave;
+    auto unit = [](int t) { return (t & 3) | ((t >> 3) & 1) << 2; };  // xored onto a row's 32-byte units
+    auto d_from = [&](int t) {  // byte of dy's row that this lane's 16 bytes of row t come from
+        return min((int64_t)n0 * 2 + ((lane % 32) ^ (2 * unit(t))) * 16, a.outs * 2 - 16);
+    };
+    const uint32_t d_off0 = (uint32_t)((row0 + lane / 32) * d_pitch + d_from(row0 + lane / 32));
+    const uint32_t d_off1 = (uint32_t)((row0 + 2 + lane / 32) * d_pitch + d_from(row0 + 2 + lane / 32));
+    const int64_t x_from = min(k0 + lane % 16 * 16, pitch - 16), e_from = min(k0 + 4 * lane, pitch - 4) / BLOCK;
+    const uint32_t x_off = (uint32_t)((row0 + lane / 16) * pitch + x_from);
+    const uint32_t e_off = (uint32_t)((row0 + lane % 4) * blocks + e_from);
+    const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)lds);
+    // step p of this split, clamped: what lies past its end is loaded and never read
+    auto clamped = [&](int64_t p) { return max(min(f0 + p - tail, f1 - 1), (int64_t)0); };
+    auto load_d = [&](int64_t p) {
+        const char* const d = (const char*)a.dy + clamped(p) * STEP * d_pitch;
+        const uint32_t to = base + AT_D + (uint32_t)(p % D_RING) * D_SLOT + row0 * (DIRECT * 2);
+        load_16_to_lds(to, d_off0, d);
+        load_16_to_lds(to + 2 * DIRECT * 2, d_off1, d);
+    };
+    auto load_x = [&](int64_t p) {
+        const int64_t s = clamped(p) * STEP;
+        load_16_to_lds(base + AT_X + (uint32_t)(p % X_RING) * X_SLOT + row0 * DIRECT, x_off, (const char*)a.codes + s * pitch);
+        load_byte_to_lds(base + AT_E + (uint32_t)(p % X_RING) * E_SLOT + wave * WAVE * 4, e_off,
+                         (const char*)a.exponents + s * blocks);
+    };
+    // the rows behind the last whole step, as step 0; zeros behind them
+    auto load_tail = [&] {
+        const int64_t t0 = whole_steps * STEP;
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const int64_t n = n0 + wn + 16 * j + lane % 16;
-        if (n >= a.outs) continue;
-#pragma unroll
-        for (int i = 0; i < FK; ++i) {
-            const int64_t k = k0 + wk + 16 * i + lane / 16 * 4, left = a.cols - k, at = n * a.cols + k;
-            if (!whole) {
-                float* const o = partial + (int64_t)split * a.outs * a.cols + at;
-                if (left >= 4) {
-                    *(u32x4_at*)o = __builtin_bit_cast(u32x4, acc[i][j]);
-                } else {
-                    for (int r = 0; r < 4; ++r)
-                        if (r < left) o[r] = acc[i][j][r];
-                }
-                continue;
-            }
-            if (a.out_dtype == RF_F32 && left >= 4) {
-                float* const o = (float*)a.out + at;
-                f32x4 v = acc[i][j];
-                if (a.accumulate) v += __builtin_bit_cast(f32x4, (u32x4) * (const u32x4_at*)o);
-                *(u32x4_at*)o = __builtin_bit_cast(u32x4, v);
-            } else if (a.out_dtype == RF_BF16 && left >= 4 && !a.accumulate) {
-                const f32x4 v = acc[i][j];
-                const bf16x2 lo = __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2);
-                const bf16x2 hi = __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2);
-                *(u32x2_h*)((bf16*)a.out + at) = u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
-            } else {
-                for (int r = 0; r < 4; ++r)
-                    if (r < left)
-                        put_scalar(a.out, a.out_dtype, at + r,
-                                   a.accumulate ? scalar_at(a.out, a.out_dtype, at + r) + acc[i][j][r] : acc[i][j][r]);
-            }
+        for (int j = 0; j < 2; ++j) {
+            const int t = row0 + 2 * j + lane / 32;
+            u32x4 v{};
+            if (t0 + t < a.rows) v = *(const u32x4*)((const char*)a.dy + (t0 + t) * d_pitch + d_from(t));
+            *(u32x4*)(lds + AT_D + t * (DIRECT * 2) + lane % 32 * 16) = v;
         }
+        const int t = row0 + lane / 16, te = row0 + lane % 4;
+        u32x4 v{};
+        if (t0 + t < a.rows) v = *(const u32x4*)(a.codes + (t0 + t) * pitch + x_from);
+        *(u32x4*)(lds + AT_X + t * DIRECT + lane % 16 * 16) = v;
+        *(uint32_t*)(lds + AT_E + (wave * WAVE + lane) * 4) = t0 + te < a.rows ? a.exponents[(t0 + te) * blocks + e_from] : 0u;
+    };
+
+    // ---- conversion: rows 4 w .. 4 w + 3 of columns 4 l .. 4 l + 3, half of octet w / 2
+    const int col = 4 * lane;
+    const Places put = places(AT_B + col / 4 * 256 + (wave & 1) * 8, (wave >> 1) ^ ((col >> 2) & 1) * 3 ^ ((col >> 3) & 1) * 2 ^
+                                                                          ((col >> 4) & 3) * 4);
+    const int raw_x = AT_X + row0 * DIRECT + col, raw_e = AT_E + (wave * WAVE + lane) * 4;
+    struct Raw4 { uint32_t c[4], e; };
+    auto read_raw = [&](int slot, Raw4& r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.c[i] = *(const uint32_t*)(lds + raw_x + slot * X_SLOT + i * DIRECT);
+        r.e = *(const uint32_t*)(lds + raw_e + slot * E_SLOT);
+    };
+    auto convert = [&](int buf, const Raw4& r, int c) {
+        const uint32_t e[4] = {dpp<0x00>(r.e), dpp<0x55>(r.e), dpp<0xAA>(r.e), dpp<0xFF>(r.e)};
+        u32x2 v;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float lo = (float)(int8_t)(r.c[2 * i] >> (8 * c)) * __uint_as_float(e[2 * i] << 23);
+            const float hi = (float)(int8_t)(r.c[2 * i + 1] >> (8 * c)) * __uint_as_float(e[2 * i + 1] << 23);
+            v[i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
+        }
+        *(u32x2*)(lds + buf * (DIRECT * COL_BYTES) + put.at[c]) = v;
+    };
+
+    // ---- the product: lane l holds column l % 16 of a fragment, octet l / 16
+    const int wk = wave / 4 * WK, wn = wave % 4 * WN;
+    const Places get_x = places(AT_B + wk / 4 * 256 + (lane & 15) / 4 * 256,
+                                (lane >> 4) ^ (lane & 3) * 4 ^ ((lane >> 2) & 1) * 3 ^ ((lane >> 3) & 1) * 2);
+    int get_d[FN];  // four t of column wn + 16 j + l % 16, as the transposed read wants them addressed
+    {
+        const int t = 8 * (lane >> 4) + ((lane & 15) >> 2);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) get_d[j] = AT_D + t * (DIRECT * 2) + ((wn / 16 + j) ^ unit(t)) * 32 + (lane & 3) * 8;
     }
+    auto read_x = [&](int buf, int i) {
+        return *(const bf16x8*)(lds + buf * (DIRECT * COL_BYTES) + get_x.at[i & 3] + i * 1024);
+    };
+    auto read_d = [&](int slot, int j) {
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        union { s16x4 h[2]; bf16x8 v; } u;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)  // rows t + 4 half: the same xor
+            u.h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(lds_char*)(lds + slot * D_SLOT + get_d[j] + half * 4 * DIRECT * 2));
+        return u.v;
+    };
+    f32x4 acc[FK][FN];
+#pragma unroll
+    for (int i = 0; i < FK; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    if (steps > 0) {
+        if (tail) {
+            load_tail();
+        } else {
+            load_d(0);
+            load_x(0);
+        }
+        load_d(1);
+        load_d(2);
+        load_x(1);
+        load_x(2);
+        load_x(3);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        Raw4 raw;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            read_raw(p, raw);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) convert(p, raw, c);
+        }
+        __syncthreads();
+        load_x(4);
+        struct Fragments {
+            bf16x8 y[FN], x[2];
+        };
+        Fragments f, g;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) f.y[j] = read_d(0, j);
+        f.x[0] = read_x(0, 0);
+        f.x[1] = read_x(0, 1);
+        int b = 0;  // q % 3
+        auto step = [&](int64_t q, Fragments& f, Fragments& g) {
+            const int b1 = b == 2 ? 0 : b + 1, b2 = b1 == 2 ? 0 : b1 + 1;
+            load_d(q + 3);
+            load_x(q + 5);
+            read_raw((int)((q + 2) % X_RING), raw);
+#pragma unroll
+            for (int i = 0; i < FK; ++i) {
+                const bf16x8 xi = f.x[i & 1];
+                if (i + 2 < FK) f.x[i & 1] = read_x(b, i + 2);
+                else g.x[i & 1] = read_x(b1, i + 2 - FK);
+                if (i + 2 >= FK) {
+#pragma unroll
+                    for (int j = (i + 2 - FK) * FN / 2; j < (i + 3 - FK) * FN / 2; ++j)
+                        g.y[j] = read_d((int)((q + 1) % D_RING), j);
+                }
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xi, f.y[j], acc[i][j], 0, 0, 0);
+                if (i >= 1 && i < 5) convert(b2, raw, i - 1);
+#pragma unroll
+                for (int k = 0; k < FN; ++k) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction,
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // up to four vector ones beside it
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+            __syncthreads();
+            b = b1;
+        };
+        for (int64_t q = 0; q < steps; q += 2) {
+            step(q, f, g);
+            if (q + 1 < steps) step(q + 1, g, f);
+        }
+        // nothing may land in LDS that is another workgroup's by then
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    store_tile(a, splits == 1 ? nullptr : partial + (int64_t)split * a.outs * a.cols, acc, k0 + wk, n0 + wn);
 }
 
 // Adds the splits' partial sums in their order.
@@ -424,14 +656,24 @@ __global__ __launch_bounds__(256) void k_wgrad_join(const rf_weight_grad a, cons
     if (at >= n) return;
     const int left = (int)min((int64_t)4, n - at);
     float s[4] = {};
-    for (uint32_t p = 0; p < splits; ++p) {
-        const float* const q = partial + (int64_t)p * n + at;
-        if (left == 4) {
-            const f32x4 v = __builtin_bit_cast(f32x4, (u32x4) * (const u32x4_at*)q);
-            for (int i = 0; i < 4; ++i) s[i] += v[i];
-        } else {
-            for (int i = 0; i < left; ++i) s[i] += q[i];
+    for (uint32_t p = 0; p < splits; p += 8) {  // eight loads in flight
+        f32x4 v[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            v[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (p + k < splits) {
+                const float* const q = partial + (int64_t)(p + k) * n + at;
+                if (left == 4) {
+                    v[k] = __builtin_bit_cast(f32x4, (u32x4) * (const u32x4_at*)q);
+                } else {
+                    for (int i = 0; i < 3; ++i)
+                        if (i < left) v[k][i] = q[i];
+                }
+            }
         }
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+            for (int i = 0; i < 4; ++i) s[i] += v[k][i];
     }
     for (int i = 0; i < left; ++i)
         put_scalar(a.out, a.out_dtype, at + i, a.accumulate ? scalar_at(a.out, a.out_dtype, at + i) + s[i] : s[i]);
@@ -439,7 +681,7 @@ __global__ __launch_bounds__(256) void k_wgrad_join(const rf_weight_grad a, cons
 
 // Tile and split of a call.
 struct Plan {
-    bool big;
+    bool big, direct;
     uint32_t tiles_k, tiles, splits;
     int64_t workspace;
 };
@@ -460,6 +702,7 @@ Plan plan_of(const rf_weight_grad& a, int cus)
         p.tiles_k = (uint32_t)((a.cols + tile - 1) / tile);
         p.tiles = p.tiles_k * (uint32_t)((a.outs + tile - 1) / tile);
         const int64_t room = (int64_t)cus * (big || a.dy_dtype != RF_BF16 ? 1 : 2);
+        p.direct = big && a.rows >= STEP && a.outs % 8 == 0 && a.dy_stride % 8 == 0 && ((uintptr_t)a.dy & 15) == 0;
         const double step = big ? 1.05 : a.dy_dtype == RF_F32 ? 1.2 : 0.9;
         for (int64_t n = 1; n <= std::min<int64_t>(std::max<int64_t>(1, steps), 64); ++n) {
             const double rounds = (double)((p.tiles * n + room - 1) / room);
@@ -486,6 +729,15 @@ rf_status launch(const rf_weight_grad& a, const Plan& p, float* partial, hipStre
         if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
     }
     f<<<p.tiles * p.splits, WK * WN * WAVE, LDS, st>>>(a, partial, p.tiles_k, p.tiles, p.splits);
+    return RF_OK;
+}
+
+rf_status launch_direct(const rf_weight_grad& a, const Plan& p, float* partial, hipStream_t st)
+{
+    static const hipError_t e =
+        hipFuncSetAttribute((const void*)k_wgrad_direct, hipFuncAttributeMaxDynamicSharedMemorySize, DIRECT_LDS);
+    if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
+    k_wgrad_direct<<<p.tiles * p.splits, DIRECT_WAVES * WAVE, DIRECT_LDS, st>>>(a, partial, p.tiles_k, p.tiles, p.splits);
     return RF_OK;
 }
 
@@ -541,6 +793,7 @@ rf_status rf_linear_weight_grad(const rf_weight_grad* args, void* workspace, int
     rf_status s;
     if (a.dy_dtype == RF_F32) s = launch<float, 128, 2, 2>(a, p, partial, st);
     else if (a.dy_dtype == RF_F16) s = launch<f16, 128, 2, 2>(a, p, partial, st);
+    else if (p.direct) s = launch_direct(a, p, partial, st);
     else if (p.big) s = launch<bf16, 256, 2, 4>(a, p, partial, st);
     else s = launch<bf16, 128, 2, 2>(a, p, partial, st);
     if (s != RF_OK) return s;

@@ -192,6 +192,36 @@ def test_weight_grad_accumulates(t, n, k, dtype, out):
     close(acc, d(dy).t() @ kept(x), slack, "overwritten")
 
 
+@pytest.mark.parametrize("t,n,k", [(32, 4096, 4096), (333, 4096, 4096), (290, 4104, 3936), (64, 3969, 4100), (450, 4098, 4001)])
+def test_weight_grad_large_tiles(t, n, k):
+    """Enough outputs for the largest tiles: rows of whole 16-byte units and
+    others, tails of rows, columns and outputs; strided and offset rows."""
+    wgrad_case(t, n, k, BF16, F32)
+    x = rand((t, k), BF16, 11)
+    ck = rf().checkpoint_activations(x)
+    base = rand((t, n + 24), BF16, 12, 1e-2)
+    for off in (8, 3):
+        dy = base[:, off: off + n]
+        a, b = d(dy), kept(x)
+        close(rf().linear_weight_grad(dy, ck, dtype=F32), a.t() @ b, (t + 8) * U * (a.abs().t() @ b.abs()), (t, n, k, off))
+
+
+def test_weight_grad_large_tiles_are_those_of_the_small():
+    """The sums of a column do not depend on the tile but for their order: an
+    Inf and a NaN reach their rows of outputs and nothing else."""
+    t, n, k = 300, 4096, 4096
+    dy, x = rand((t, n), BF16, 1, 1e-2), rand((t, k), BF16, 2)
+    dy[299, 7], dy[5, 4000] = math.inf, math.nan
+    x[:, 0] = x[:, 0].abs() + 0.5
+    got = rf().linear_weight_grad(dy, rf().checkpoint_activations(x), dtype=F32)
+    assert not torch.isfinite(got[7, 0]) and torch.isnan(got[4000]).all()
+    mask = torch.ones(n, dtype=torch.bool)
+    mask[[7, 4000]] = False
+    assert torch.isfinite(got.cpu()[mask]).all()
+    small = rf().linear_weight_grad(dy[:, 64:192].contiguous(), rf().checkpoint_activations(x), dtype=F32)
+    assert (got[64:192] - small).abs().max() <= 2 * (t + 8) * U * (d(dy[:, 64:192]).abs().t() @ kept(x).abs()).max()
+
+
 def test_weight_grad_of_no_rows():
     ck = rf().checkpoint_activations(torch.empty(0, 40, device="cuda"))
     dy = torch.empty(0, 9, device="cuda", dtype=BF16)
