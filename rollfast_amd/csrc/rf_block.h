@@ -62,9 +62,15 @@ template <typename T> __device__ __forceinline__ Raw<T> fetch8(const T* row, int
     return r;
 }
 
-template <typename T> __device__ __forceinline__ void settle8(Raw<T>& r, int64_t c, int64_t cols)
+// TAIL: rows may end inside a chunk (cols % 8); without, the lane masks for it
+// take no registers.
+template <bool TAIL = true, typename T> __device__ __forceinline__ void settle8(Raw<T>& r, int64_t c, int64_t cols)
 {
     const int64_t left = cols - c;
+    if (!TAIL) {
+        if (left <= 0) r = Raw<T>{};
+        return;
+    }
     if (left >= CHUNK || cols < CHUNK) return;  // (narrow rows: load8 put them in place)
     if (left <= 0) {
         r = Raw<T>{};
@@ -185,12 +191,12 @@ template <typename T> __device__ __forceinline__ Raw<T> narrow8(const float (&v)
 }
 
 // Stores the first `left` of eight elements.
-template <typename T> __device__ __forceinline__ void put8(T* p, const Raw<T>& r, int64_t left)
+template <bool TAIL = true, typename T> __device__ __forceinline__ void put8(T* p, const Raw<T>& r, int64_t left)
 {
-    if (left >= CHUNK) {
+    if (TAIL ? left >= CHUNK : left > 0) {
         *(u32x4_at*)p = r.a;
         if constexpr (sizeof(T) == 4) *(u32x4_at*)(p + 4) = r.b;
-    } else if (left > 0) {
+    } else if (TAIL && left > 0) {
         const int n = (int)left;
         if constexpr (sizeof(T) == 4) {
             u32x4 v = r.a;
@@ -237,18 +243,19 @@ struct Vector8 {
         a = *(const u32x4_at*)q;
         b = *(const u32x4_at*)(q + (size == 4 ? 16 : 0));
     }
+    template <bool TAIL>
     __device__ __forceinline__ void get(const void* p, int dtype, int64_t c, int64_t cols, float fill, float (&v)[8])
     {
         if (!p) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? fill : 0.0f;
+            for (int k = 0; k < 8; ++k) v[k] = c + (TAIL ? k : 0) < cols ? fill : 0.0f;
         } else if (dtype == RF_F32) {
             Raw<float> r{a, b};
-            settle8(r, c, cols);
+            settle8<TAIL>(r, c, cols);
             widen8(r, v);
         } else {
             Raw<bf16> r{a};
-            settle8(r, c, cols);
+            settle8<TAIL>(r, c, cols);
             if (dtype == RF_BF16) widen8(r, v);
             else widen8(Raw<f16>{r.a}, v);
         }

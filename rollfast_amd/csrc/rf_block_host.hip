@@ -375,7 +375,8 @@ int64_t workspace_of(const rf_norm& a, const NormShape& s, const NormPlan& p)
 
 // Adds the partial rows: 32 columns a workgroup, 32 lanes a column.  The lanes
 // are dealt to the groups of rows (all of them to one group, or one to each of
-// 32 groups at a time), and within a group to its pieces.
+// 32 groups at a time), and within a group to its pieces.  blockIdx.y: 0 the next
+// norm's vectors, 1 the post norm's and the gate (not launched without).
 constexpr int FIN_COLS = 32, FIN_LANES = 32;
 
 // Partial rows w0 + i * step below w1, eight loads in flight.
@@ -399,18 +400,28 @@ __global__ __launch_bounds__(FIN_COLS* FIN_LANES) void k_norm_finish(const rf_no
     const int tx = threadIdx.x, ty = threadIdx.y;
     const int64_t cols = a.cols, c = (int64_t)blockIdx.x * FIN_COLS + tx, at = min(c, cols - 1), pitch = p.vectors * cols;
     const bool in = c < cols;
-    const bool post = p.i_p >= 0, has_q = p.i_q >= 0;
+    const bool has_q = p.i_q >= 0;
     // whole groups: the gate is in the sums already, and its gradient is written
     const bool gated = p.pieces > 0 && a.gate;
     const int64_t groups = p.pieces > 0 ? p.groups : 1, pieces = p.pieces > 0 ? p.pieces : p.workers;
     const int lanes = (int)max((int64_t)1, FIN_LANES / groups), slots = FIN_LANES / lanes;
     const int slot = ty / lanes, sub = ty % lanes;
-    const float w = post && a.weight ? scalar_at(a.weight, a.weight_dtype, at) : 1.0f;
-    const float b = post && a.bias ? scalar_at(a.bias, a.bias_dtype, at) : 0.0f;
-    lds[0][ty][tx] = p.i_w2 >= 0 ? add_rows(partial + p.i_w2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
-    lds[1][ty][tx] = p.i_b2 >= 0 ? add_rows(partial + p.i_b2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
+    const float w = a.weight ? scalar_at(a.weight, a.weight_dtype, at) : 1.0f;
+    const float b = a.bias ? scalar_at(a.bias, a.bias_dtype, at) : 0.0f;
+    if (blockIdx.y == 0) {  // the next norm's vectors
+        lds[0][ty][tx] = p.i_w2 >= 0 ? add_rows(partial + p.i_w2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
+        lds[1][ty][tx] = p.i_b2 >= 0 ? add_rows(partial + p.i_b2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
+        __syncthreads();
+        void* const out = ty == 0 ? a.dnext_weight : a.dnext_bias;
+        if (ty < 2 && in && out) {
+            float s = 0.0f;
+            for (int i = 0; i < FIN_LANES; ++i) s += lds[ty][i][tx];
+            put_scalar(out, ty == 0 ? a.next_weight_dtype : a.next_bias_dtype, c, s);
+        }
+        return;
+    }
     float dw = 0.0f, db = 0.0f;
-    if (post) {
+    {
         for (int64_t first = 0; first < groups; first += slots) {
             const int64_t g = first + slot, w0 = g * pieces;
             const bool mine = slot < slots && g < groups;
@@ -435,13 +446,11 @@ __global__ __launch_bounds__(FIN_COLS* FIN_LANES) void k_norm_finish(const rf_no
     lds[2][ty][tx] = dw;
     lds[3][ty][tx] = db;
     __syncthreads();
-    if (ty >= 4 || !in) return;
-    void* const out = ty == 0 ? a.dnext_weight : ty == 1 ? a.dnext_bias : ty == 2 ? a.dweight : a.dbias;
-    const int dtype = ty == 0 ? a.next_weight_dtype : ty == 1 ? a.next_bias_dtype : ty == 2 ? a.weight_dtype : a.bias_dtype;
-    if (!out) return;
+    void* const out = ty == 0 ? a.dweight : a.dbias;
+    if (ty >= 2 || !in || !out) return;
     float s = 0.0f;
-    for (int i = 0; i < FIN_LANES; ++i) s += lds[ty][i][tx];
-    put_scalar(out, dtype, c, ty < 2 ? s : a.branch_scale * s);
+    for (int i = 0; i < FIN_LANES; ++i) s += lds[2 + ty][i][tx];
+    put_scalar(out, ty == 0 ? a.weight_dtype : a.bias_dtype, c, a.branch_scale * s);
 }
 
 bool has_pair(const rf_norm& a)
@@ -586,7 +595,8 @@ rf_status rf_norm_backward(const rf_norm* args, void* workspace, int64_t workspa
     }
     if (p.vectors) {
         const unsigned tiles = (unsigned)((a.cols + FIN_COLS - 1) / FIN_COLS);
-        k_norm_finish<<<dim3(tiles), dim3(FIN_COLS, FIN_LANES), 0, st>>>(a, p, (const float*)workspace);
+        // y = 0: the next norm's vectors, y = 1: the post norm's and the gate
+        k_norm_finish<<<dim3(tiles, p.i_p >= 0 ? 2 : 1), dim3(FIN_COLS, FIN_LANES), 0, st>>>(a, p, (const float*)workspace);
     }
     BLK_TRY(hipGetLastError());
     return RF_OK;

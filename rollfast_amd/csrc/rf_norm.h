@@ -87,7 +87,7 @@ __device__ __forceinline__ const void* gate_row(const rf_norm& a, int64_t g)
 // FULL: LayerNorm or a bias somewhere.  The next row's loads are sent before
 // this row's sums.  Past the end of a row the elements and the vectors are
 // zero, and so is what they give.
-template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, int NV>
+template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool TAIL, int NV>
 __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Share share, const uint32_t group_rows)
 {
     __shared__ float red[2][MAX_WAVES][8];
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            w[j].get(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, w2[j]);
-            if constexpr (FULL) b[j].get(a.next_bias, a.next_bias_dtype, c, cols, 0.0f, b2[j]);
+            w[j].template get<TAIL>(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, w2[j]);
+            if constexpr (FULL) b[j].template get<TAIL>(a.next_bias, a.next_bias_dtype, c, cols, 0.0f, b2[j]);
         }
     }
     // mean and 1 / sqrt(variance + eps) of a row; columns past the end are zero
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
             const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
             float v[8], t = 0.0f;
             widen8(x[j], v);
-            if (FULL && (cols & (CHUNK - 1))) {  // the row may end inside the chunk
+            if (FULL && TAIL) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = k < left ? v[k] : mean;
             }
@@ -182,9 +182,9 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
         for (int j = 0; j < NV; ++j) {
             const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
             float v[8];
-            w[j].get(a.weight, a.weight_dtype, c, cols, 1.0f, A[j]);
-            gt[j].get(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
-            if constexpr (FULL) b[j].get(a.bias, a.bias_dtype, c, cols, 0.0f, B[j]);
+            w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, A[j]);
+            gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
+            if constexpr (FULL) b[j].template get<TAIL>(a.bias, a.bias_dtype, c, cols, 0.0f, B[j]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 v[k] *= a.branch_scale;
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            settle8(now.r[j], c, cols);
-            if constexpr (EXIT) settle8(now.u[j], c, cols);
+            settle8<TAIL>(now.r[j], c, cols);
+            if constexpr (EXIT) settle8<TAIL>(now.u[j], c, cols);
         }
         if constexpr (EXIT) {
             float mean = 0.0f, rstd = 1.0f;
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
                         o[k] = fmaf(a.residual_scale, x[k], n);
                     }
                     now.r[j] = narrow8<T>(o);
-                    put8((T*)a.hidden + r * cols + c, now.r[j], cols - c);
+                    put8<TAIL>((T*)a.hidden + r * cols + c, now.r[j], cols - c);
                 }
             }
         }
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
                         y[k] = FULL ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[FULL ? j : 0][k]) : v[k] * rstd * w2[j][k];
                     }
                     const Raw<U> yr = narrow8<U>(y);
-                    put8((U*)a.y + r * cols + c, yr, cols - c);
+                    put8<TAIL>((U*)a.y + r * cols + c, yr, cols - c);
                     if (a.y_codes) {
                         widen8(yr, y);
                         put_codes(a.y_codes, a.y_exponents, r, pitch, ch, encode8(y));
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(512) void k_norm_forward_wide(const rf_norm a)
 // ------------------------------------------------------------ backward -----
 // A chunk of a saved row: of a checkpoint, or of the tensor itself.  WIDE: rows
 // of at least eight columns.
-template <typename T, bool SRC8, bool WIDE> struct Saved {
+template <typename T, bool SRC8, bool WIDE, bool TAIL = true> struct Saved {
     Raw<T> t;
     __device__ __forceinline__ void fetch(const T* p, int64_t stride, const int8_t*, const uint8_t*, int64_t r, int64_t,
                                           int64_t ch, int64_t, int64_t cols)
@@ -368,11 +368,11 @@ template <typename T, bool SRC8, bool WIDE> struct Saved {
     }
     __device__ __forceinline__ void get(float (&v)[8], int64_t ch, int64_t cols)
     {
-        settle8(t, ch * CHUNK, cols);
+        settle8<TAIL>(t, ch * CHUNK, cols);
         widen8(t, v);
     }
 };
-template <typename T, bool WIDE> struct Saved<T, true, WIDE> {
+template <typename T, bool WIDE, bool TAIL> struct Saved<T, true, WIDE, TAIL> {
     Codes t;
     __device__ __forceinline__ void fetch(const T*, int64_t, const int8_t* codes, const uint8_t* exps, int64_t r,
                                           int64_t pitch, int64_t ch, int64_t nch, int64_t)
@@ -386,7 +386,7 @@ template <typename T, bool WIDE> struct Saved<T, true, WIDE> {
 // Past the end of a row dy, dhidden and h are zero, so xhat and uhat may be
 // anything finite there.
 // FULL: LayerNorm or a bias somewhere (the sums of g, t and their columns).
-template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, int NV>
+template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL, int NV>
 __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const NormPlan plan, float* __restrict__ partial)
 {
     __shared__ float red[2][MAX_WAVES][8];
@@ -419,8 +419,8 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
     struct Row {
         Raw<T> dh[NV];
         Raw<U> dy[NEXT ? NV : 1];
-        Saved<U, SRC8, true> u[EXIT ? NV : 1];
-        Saved<T, SRC8, true> h[NEXT ? NV : 1];
+        Saved<U, SRC8, true, TAIL> u[EXIT ? NV : 1];
+        Saved<T, SRC8, true, TAIL> h[NEXT ? NV : 1];
         float rstd1, mean1, rstd2, mean2;
     };
     auto load = [&](int64_t r) {
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
         for (int j = 0; j < NV; ++j) w[j].fetch(a.next_weight, a.next_weight_dtype, (int64_t)(tid + j * tpr) * CHUNK, cols, a.dy);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            w[j].get(a.next_weight, a.next_weight_dtype, (int64_t)(tid + j * tpr) * CHUNK, cols, 1.0f, w2[j]);
+            w[j].template get<TAIL>(a.next_weight, a.next_weight_dtype, (int64_t)(tid + j * tpr) * CHUNK, cols, 1.0f, w2[j]);
     }
     // whole groups: the sums over groups, of this wave's or workgroup's columns
     float* const sums_p = cols_lds + (int64_t)ty * (FULL ? 2 : 1) * pitch;
@@ -483,8 +483,8 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
         for (int j = 0; j < NV; ++j) {
             const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
             float v[8];
-            w[j].get(a.weight, a.weight_dtype, c, cols, 1.0f, h[j]);
-            gt[j].get(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
+            w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, h[j]);
+            gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) h[j][k] *= a.branch_scale * v[k];
         }
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t ch = tid + j * tpr;
-            settle8(now.dh[j], ch * CHUNK, cols);
+            settle8<TAIL>(now.dh[j], ch * CHUNK, cols);
             widen8(now.dh[j], e[j]);
             if (!a.dhidden) {
 #pragma unroll
@@ -506,7 +506,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
             }
             if constexpr (NEXT) {
                 float dy[8];
-                settle8(now.dy[j], ch * CHUNK, cols);
+                settle8<TAIL>(now.dy[j], ch * CHUNK, cols);
                 widen8(now.dy[j], dy);
                 now.h[j].get(x[j], ch, cols);
 #pragma unroll
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
                     if constexpr (NEXT) e[j][k] -= fmaf(k1, x[j][k], k0);
                     o[k] = EXIT ? a.residual_scale * e[j][k] : e[j][k];
                 }
-                put8((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
+                put8<TAIL>((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
                 if constexpr (EXIT) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
                         if constexpr (FULL) Q[j][k] += e[j][k];
                         o[k] = rstd1 * (FULL ? fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1 : fmaf(h[j][k], e[j][k], -(u[j][k] * m1)));
                     }
-                    put8((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
+                    put8<TAIL>((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
                 }
             }
         }
@@ -649,7 +649,7 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
                         v.a[i] = __float_as_uint(acc[j][i]);
                         v.b[i] = __float_as_uint(acc[j][i + 4]);
                     }
-                    put8(out + index * cols + c, v, cols - c);
+                    put8<TAIL>(out + index * cols + c, v, cols - c);
                 }
             }
         }

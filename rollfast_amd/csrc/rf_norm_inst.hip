@@ -12,37 +12,56 @@ template <> struct Elem<RF_F16> { using type = f16; };
 using T = Elem<RFI_T>::type;
 using U = Elem<RFI_U>::type;
 
-template <bool EXIT, bool NEXT> static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
+template <bool EXIT, bool NEXT, bool FULL, bool TAIL>
+static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
 {
     const dim3 grid((unsigned)s.workers), block(s.tpr, s.ny);
     const Share rows = share_of(a.rows, s.workers);
     const uint32_t per_gate = a.gates > 1 ? (uint32_t)(a.rows / a.gates) : 0;
-    if (s.nv == 0) k_norm_forward_wide<T, U, EXIT, NEXT><<<grid, block, 0, st>>>(a);
-    else if (s.nv == 1 && s.full) k_norm_forward<T, U, EXIT, NEXT, true, 1><<<grid, block, 0, st>>>(a, rows, per_gate);
-    else if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, false, 1><<<grid, block, 0, st>>>(a, rows, per_gate);
-    else if (s.full) k_norm_forward<T, U, EXIT, NEXT, true, 2><<<grid, block, 0, st>>>(a, rows, per_gate);
-    else k_norm_forward<T, U, EXIT, NEXT, false, 2><<<grid, block, 0, st>>>(a, rows, per_gate);
+    if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 1><<<grid, block, 0, st>>>(a, rows, per_gate);
+    else k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 2><<<grid, block, 0, st>>>(a, rows, per_gate);
 }
 
-template <bool EXIT, bool NEXT, bool FULL, bool SRC8>
+template <bool EXIT, bool NEXT> static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
+{
+    if (s.nv == 0) {
+        k_norm_forward_wide<T, U, EXIT, NEXT><<<dim3((unsigned)s.workers), dim3(s.tpr), 0, st>>>(a);
+    } else if (a.cols % CHUNK) {
+        if (s.full) forward<EXIT, NEXT, true, true>(a, s, st);
+        else forward<EXIT, NEXT, false, true>(a, s, st);
+    } else {
+        if (s.full) forward<EXIT, NEXT, true, false>(a, s, st);
+        else forward<EXIT, NEXT, false, false>(a, s, st);
+    }
+}
+
+template <bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL>
 static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
 {
     const dim3 grid((unsigned)p.workers), block(s.tpr, s.ny);
-    if (s.nv == 1) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, 1><<<grid, block, s.lds, st>>>(a, p, partial);
-    else if (s.nv == 2) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, 2><<<grid, block, s.lds, st>>>(a, p, partial);
-    else k_norm_backward_wide<T, U, EXIT, NEXT, SRC8><<<grid, block, 0, st>>>(a, p, partial);
+    if (s.nv == 1) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, TAIL, 1><<<grid, block, s.lds, st>>>(a, p, partial);
+    else k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, TAIL, 2><<<grid, block, s.lds, st>>>(a, p, partial);
+}
+
+template <bool EXIT, bool NEXT, bool SRC8>
+static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
+{
+    if (s.nv == 0) {
+        k_norm_backward_wide<T, U, EXIT, NEXT, SRC8><<<dim3((unsigned)p.workers), dim3(s.tpr), 0, st>>>(a, p, partial);
+    } else if (a.cols % CHUNK) {
+        if (s.full) backward<EXIT, NEXT, true, SRC8, true>(a, s, p, partial, st);
+        else backward<EXIT, NEXT, false, SRC8, true>(a, s, p, partial, st);
+    } else {
+        if (s.full) backward<EXIT, NEXT, true, SRC8, false>(a, s, p, partial, st);
+        else backward<EXIT, NEXT, false, SRC8, false>(a, s, p, partial, st);
+    }
 }
 
 template <bool EXIT, bool NEXT>
 static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
 {
-    if (s.full) {
-        if (s.src8) backward<EXIT, NEXT, true, true>(a, s, p, partial, st);
-        else backward<EXIT, NEXT, true, false>(a, s, p, partial, st);
-    } else {
-        if (s.src8) backward<EXIT, NEXT, false, true>(a, s, p, partial, st);
-        else backward<EXIT, NEXT, false, false>(a, s, p, partial, st);
-    }
+    if (s.src8) backward<EXIT, NEXT, true>(a, s, p, partial, st);
+    else backward<EXIT, NEXT, false>(a, s, p, partial, st);
 }
 
 #define RFI_CAT2(a, b, c) a##b##_##c

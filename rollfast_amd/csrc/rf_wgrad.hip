@@ -687,7 +687,7 @@ struct Plan {
 };
 
 // The cheapest of the tiles and splits by what they take (us, measured on one
-// GPU): 5 for a round of workgroups, `step` for 32 rows, and, split, 3 and the
+// GPU): 7 for a round of workgroups, `step` for 32 rows, and, split, 3 and the
 // partial sums at 4 TB/s.  Workgroups at a time: one a CU with 256 x 256 tiles
 // and with two or three pieces, else two.
 Plan plan_of(const rf_weight_grad& a, int cus)
@@ -703,10 +703,10 @@ Plan plan_of(const rf_weight_grad& a, int cus)
         p.tiles = p.tiles_k * (uint32_t)((a.outs + tile - 1) / tile);
         const int64_t room = (int64_t)cus * (big || a.dy_dtype != RF_BF16 ? 1 : 2);
         p.direct = big && a.rows >= STEP && a.outs % 8 == 0 && a.dy_stride % 8 == 0 && ((uintptr_t)a.dy & 15) == 0;
-        const double step = big ? 1.05 : a.dy_dtype == RF_F32 ? 1.2 : 0.9;
+        const double step = big ? 1.0 : a.dy_dtype == RF_F32 ? 2.4 : a.dy_dtype == RF_F16 ? 1.4 : 0.9;
         for (int64_t n = 1; n <= std::min<int64_t>(std::max<int64_t>(1, steps), 64); ++n) {
             const double rounds = (double)((p.tiles * n + room - 1) / room);
-            const double us = rounds * (5 + step * (double)((steps + n - 1) / n)) +
+            const double us = rounds * (7 + step * (double)((steps + n - 1) / n)) +
                               (n > 1 ? 3 + (double)n * (double)a.outs * (double)a.cols * 8 / 4e6 : 0);
             if (us < least) {
                 least = us;
