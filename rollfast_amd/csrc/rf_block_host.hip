@@ -464,6 +464,8 @@ rf_status check_norm(const rf_norm* a)
     if (!sane(a->rows, a->cols)) return bad("rows or cols out of range");
     if (a->post < RF_NORM_ABSENT || a->post > RF_NORM_LAYER) return bad("unknown post norm");
     if (a->next != RF_NORM_ABSENT && a->next != RF_NORM_RMS && a->next != RF_NORM_LAYER) return bad("unknown next norm");
+    if ((a->post >= RF_NORM_RMS && !(a->post_eps >= 0.0f)) || (a->next >= RF_NORM_RMS && !(a->next_eps >= 0.0f)))
+        return bad("eps must not be negative");
     if (a->post == RF_NORM_ABSENT && a->next == RF_NORM_ABSENT) return bad("neither a post norm nor a next norm");
     if (!has_pair(*a))
         return report(RF_ERR_UNSUPPORTED, "dtype must be f32, bf16 or f16, and the branch's the same or 16-bit beside f32");

@@ -13,6 +13,7 @@
 // codes pass through registers for their conversion anyway, so it costs them
 // nothing, and dy half an instruction per element.
 #include <algorithm>
+#include <atomic>
 
 #include "rf_block.h"
 
@@ -180,7 +181,7 @@ struct StagedX { uint32_t c[8], e[2]; };  // codes of the rows, exponents of row
 // loop's loads need no guard.
 // EDGE: dy's rows are no multiple of four elements.
 template <typename T, int TILE, int WAVES_K, int WAVES_N, bool EDGE>
-__global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE) void k_wgrad(const rf_weight_grad a, float* __restrict__ partial,
+__global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) void k_wgrad(const rf_weight_grad a, float* __restrict__ partial,
                                                                  uint32_t tiles_k, uint32_t tiles, uint32_t splits)
 {
     constexpr int NP = Pieces<T>::n, HALF = WAVES_K * WAVES_N * WAVE / 2;
@@ -689,7 +690,7 @@ struct Plan {
 // The cheapest of the tiles and splits by what they take (us, measured on one
 // GPU): 7 for a round of workgroups, `step` for 32 rows, and, split, 3 and the
 // partial sums at 4 TB/s.  Workgroups at a time: one a CU with 256 x 256 tiles
-// and with two or three pieces, else two.
+// and with three pieces (LDS), else two.
 Plan plan_of(const rf_weight_grad& a, int cus)
 {
     Plan best{};
@@ -701,7 +702,7 @@ Plan plan_of(const rf_weight_grad& a, int cus)
         p.big = big != 0;
         p.tiles_k = (uint32_t)((a.cols + tile - 1) / tile);
         p.tiles = p.tiles_k * (uint32_t)((a.outs + tile - 1) / tile);
-        const int64_t room = (int64_t)cus * (big || a.dy_dtype != RF_BF16 ? 1 : 2);
+        const int64_t room = (int64_t)cus * (big || a.dy_dtype == RF_F32 ? 1 : 2);
         p.direct = big && a.rows >= STEP && a.outs % 8 == 0 && a.dy_stride % 8 == 0 && ((uintptr_t)a.dy & 15) == 0;
         const double step = big ? 1.0 : a.dy_dtype == RF_F32 ? 2.4 : a.dy_dtype == RF_F16 ? 1.4 : 0.9;
         for (int64_t n = 1; n <= std::min<int64_t>(std::max<int64_t>(1, steps), 64); ++n) {
@@ -719,24 +720,35 @@ Plan plan_of(const rf_weight_grad& a, int cus)
     return best;
 }
 
+// Allows a kernel more than 64 KB of LDS, once on each device.
+rf_status allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done)
+{
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return rf::report_hip(e, "hipGetDevice");
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bytes <= 64 * 1024 || (done.load(std::memory_order_relaxed) & bit)) return RF_OK;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return RF_OK;
+}
+
 template <typename T, int TILE, int WK, int WN, bool EDGE>
 rf_status launch(const rf_weight_grad& a, const Plan& p, float* partial, hipStream_t st)
 {
     constexpr size_t LDS = 3 * (size_t)(1 + Pieces<T>::n) * TILE * COL_BYTES;
+    static std::atomic<uint64_t> done;
     const auto f = k_wgrad<T, TILE, WK, WN, EDGE>;
-    if (LDS > 64 * 1024) {
-        static const hipError_t e = hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
-        if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
-    }
+    if (const rf_status s = allow_lds((const void*)f, LDS, done); s != RF_OK) return s;
     f<<<p.tiles * p.splits, WK * WN * WAVE, LDS, st>>>(a, partial, p.tiles_k, p.tiles, p.splits);
     return RF_OK;
 }
 
 rf_status launch_direct(const rf_weight_grad& a, const Plan& p, float* partial, hipStream_t st)
 {
-    static const hipError_t e =
-        hipFuncSetAttribute((const void*)k_wgrad_direct, hipFuncAttributeMaxDynamicSharedMemorySize, DIRECT_LDS);
-    if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
+    static std::atomic<uint64_t> done;
+    if (const rf_status s = allow_lds((const void*)k_wgrad_direct, DIRECT_LDS, done); s != RF_OK) return s;
     k_wgrad_direct<<<p.tiles * p.splits, DIRECT_WAVES * WAVE, DIRECT_LDS, st>>>(a, partial, p.tiles_k, p.tiles, p.splits);
     return RF_OK;
 }

@@ -591,6 +591,61 @@ def test_norm_rows_that_are_zero_or_not_finite():
         assert torch.isfinite(g.x[[0, 1, 2, 5]]).all() and torch.isnan(g.x[4]).all()
 
 
+def test_vectors_of_any_stride():
+    """Strided weights, biases and gates give the bits of contiguous ones."""
+    x, u = rand((30, 100), BF16, 1), rand((30, 100), BF16, 2)
+    v = rand((100, 7), F32, 3, 0.2, 1.0)
+    gate = rand((100, 3, 30), F32, 4).permute(2, 1, 0)[:, :1]
+    args = {"norm": "layer", "next_norm": "layer"}
+    r, b = x.view(30, 1, 100), u.view(30, 1, 100)
+    first = rf().postnorm_residual(r, b, v[:, 0], v[:, 1], gate, next_weight=v[:, 2], next_bias=v[:, 3], **args)
+    c = [v[:, i].contiguous() for i in range(4)]
+    second = rf().postnorm_residual(r, b, c[0], c[1], gate.contiguous(), next_weight=c[2], next_bias=c[3], **args)
+    assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
+    for p, q in zip(rf().postnorm_residual_grad(r, b, first[2]), rf().postnorm_residual_grad(r, b, second[2])):
+        assert torch.equal(p, q)
+
+
+# --------------------------------------------------------- past 32-bit offsets ---
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: rows near the end are those of a
+    call on them alone."""
+    rows, cols = 270_000, 8192  # 2.2e9 elements
+    last = slice(rows - 40, rows)
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda")
+    for i in range(0, rows, 27_000):
+        x[i: i + 27_000] = rand((1, cols), BF16, i) * torch.linspace(0.5, 2, 27_000, device="cuda").to(BF16)[:, None]
+    ck = rf().checkpoint_activations(x)
+    end = rf().checkpoint_activations(x[last])
+    assert torch.equal(ck.codes[last], end.codes) and torch.equal(ck.exponents[last], end.exponents)
+    y = rf().restore_activations(ck)
+    assert torch.equal(y[last], rf().restore_activations(end))
+    del y
+    w = rand((cols,), F32, 1, 0.1, 1.0)
+    y, saved = rf().prenorm(x, w)
+    y2, saved2 = rf().prenorm(x[last], w)
+    assert torch.equal(y[last], y2)
+    dx = rf().prenorm_grad(y, saved).x
+    assert torch.equal(dx[last], rf().prenorm_grad(y2, saved2).x)
+    del y, saved, dx
+    h, kept_h = rf().gated_activation(x, x)
+    h2, kept_h2 = rf().gated_activation(x[last], x[last])
+    assert torch.equal(h[last], h2)
+    dg, _ = rf().gated_activation_grad(h, kept_h)
+    assert torch.equal(dg[last], rf().gated_activation_grad(h2, kept_h2)[0])
+    del h, kept_h, dg, x
+    # the sum over all rows, in two calls: f32 sums in another order
+    dy = rand((rows, 1), F32, 2).to(BF16).expand(rows, 8).contiguous()
+    whole = rf().linear_weight_grad(dy, ck, dtype=F32)
+    half = rows // 2
+    parts = torch.zeros(8, cols, device="cuda")
+    for s in (slice(0, half), slice(half, rows)):
+        part = rf().ActivationCheckpoint(ck.codes[s], ck.exponents[s], (ck.codes[s].shape[0], cols), BF16)
+        rf().linear_weight_grad(dy[s], part, out=parts, accumulate=True)
+    size = (dy[:, :1].float().abs().sum() * 8).item()  # |x| below 8
+    assert (whole - parts).abs().max().item() <= 2 * rows ** 0.5 * U * size
+
+
 # ------------------------------------------------- gradients by differences ---
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 def test_gradients_by_differences(norm):

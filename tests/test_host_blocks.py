@@ -93,7 +93,8 @@ def test_norm_refusals():
                        ({"gates": 2}, "gates"), ({"gate": P}, "gates"), ({"post": 0, "weight": P}, "without"),
                        ({"post": 1, "bias": P}, "without"), ({"branch_codes": P}, "together"),
                        ({"hidden_codes": P + 4, "hidden_exponents": P}, "aligned"), ({"hidden": None}, "null"),
-                       ({"y": None}, "null"), ({"branch": None}, "null")):
+                       ({"y": None}, "null"), ({"branch": None}, "null"), ({"post_eps": -1.0}, "eps"),
+                       ({"next_eps": float("nan")}, "eps")):
         refused(L.rf_norm_forward(norm(**over), None), text)
     refused(L.rf_norm_forward(norm(dtype=1, branch_dtype=0), None), "dtype", 3)
     refused(L.rf_norm_forward(norm(weight=P, weight_dtype=9), None), "dtype", 3)
