@@ -497,17 +497,22 @@ __global__ __launch_bounds__(DIRECT_WAVES* WAVE) void k_wgrad_direct(const rf_we
     const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)lds);
     // step p of this split, clamped: what lies past its end is loaded and never read
     auto clamped = [&](int64_t p) { return max(min(f0 + p - tail, f1 - 1), (int64_t)0); };
-    auto load_d = [&](int64_t p) {
+    auto load_d = [&](int64_t p, int half) {
         const char* const d = (const char*)a.dy + clamped(p) * STEP * d_pitch;
         const uint32_t to = base + AT_D + (uint32_t)(p % D_RING) * D_SLOT + row0 * (DIRECT * 2);
-        load_16_to_lds(to, d_off0, d);
-        load_16_to_lds(to + 2 * DIRECT * 2, d_off1, d);
+        load_16_to_lds(to + half * 2 * DIRECT * 2, half ? d_off1 : d_off0, d);
+    };
+    auto load_codes = [&](int64_t p) {
+        load_16_to_lds(base + AT_X + (uint32_t)(p % X_RING) * X_SLOT + row0 * DIRECT, x_off,
+                       (const char*)a.codes + clamped(p) * STEP * pitch);
+    };
+    auto load_exponents = [&](int64_t p) {
+        load_byte_to_lds(base + AT_E + (uint32_t)(p % X_RING) * E_SLOT + wave * WAVE * 4, e_off,
+                         (const char*)a.exponents + clamped(p) * STEP * blocks);
     };
     auto load_x = [&](int64_t p) {
-        const int64_t s = clamped(p) * STEP;
-        load_16_to_lds(base + AT_X + (uint32_t)(p % X_RING) * X_SLOT + row0 * DIRECT, x_off, (const char*)a.codes + s * pitch);
-        load_byte_to_lds(base + AT_E + (uint32_t)(p % X_RING) * E_SLOT + wave * WAVE * 4, e_off,
-                         (const char*)a.exponents + s * blocks);
+        load_codes(p);
+        load_exponents(p);
     };
     // the rows behind the last whole step, as step 0; zeros behind them
     auto load_tail = [&] {
@@ -581,11 +586,14 @@ __global__ __launch_bounds__(DIRECT_WAVES* WAVE) void k_wgrad_direct(const rf_we
         if (tail) {
             load_tail();
         } else {
-            load_d(0);
+            load_d(0, 0);
+            load_d(0, 1);
             load_x(0);
         }
-        load_d(1);
-        load_d(2);
+        for (int p = 1; p < 3; ++p) {
+            load_d(p, 0);
+            load_d(p, 1);
+        }
         load_x(1);
         load_x(2);
         load_x(3);
@@ -611,8 +619,6 @@ __global__ __launch_bounds__(DIRECT_WAVES* WAVE) void k_wgrad_direct(const rf_we
         int b = 0;  // q % 3
         auto step = [&](int64_t q, Fragments& f, Fragments& g) {
             const int b1 = b == 2 ? 0 : b + 1, b2 = b1 == 2 ? 0 : b1 + 1;
-            load_d(q + 3);
-            load_x(q + 5);
             read_raw((int)((q + 2) % X_RING), raw);
 #pragma unroll
             for (int i = 0; i < FK; ++i) {
@@ -628,10 +634,15 @@ __global__ __launch_bounds__(DIRECT_WAVES* WAVE) void k_wgrad_direct(const rf_we
                 for (int j = 0; j < FN; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xi, f.y[j], acc[i][j], 0, 0, 0);
                 if (i >= 1 && i < 5) convert(b2, raw, i - 1);
+                // one load at a time: a wave that sends them together waits until the others' are taken
+                if (i == 0) load_d(q + 3, 0);
+                if (i == 2) load_d(q + 3, 1);
+                if (i == 4) load_codes(q + 5);
+                if (i == 6) load_exponents(q + 5);
 #pragma unroll
                 for (int k = 0; k < FN; ++k) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction,
-                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // up to four vector ones beside it
+                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // up to six vector ones beside it
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
