@@ -14,6 +14,7 @@
 // nothing, and dy half an instruction per element.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "rf_block.h"
 
@@ -118,6 +119,32 @@ __device__ __forceinline__ uint32_t rest(uint32_t x)
 {
     const float r = __uint_as_float(x) - __uint_as_float(x & 0xFFFF0000u);
     return __builtin_isinf(__uint_as_float(x)) ? 0u : __float_as_uint(r);
+}
+
+// Steps 0 .. n - 1 in turn.  LAST: the steps that have no two behind them are
+// told so (copies of the loop's body, which f32's kernel has registers for).
+template <bool LAST, typename Even, typename Odd> __device__ __forceinline__ void in_pairs(int64_t n, Even even, Odd odd)
+{
+    int64_t q = 0;
+    if constexpr (!LAST) {
+        for (; q < n; q += 2) {
+            even(q, std::true_type{});
+            if (q + 1 < n) odd(q + 1, std::true_type{});
+        }
+    } else {
+        for (; q + 3 < n; q += 2) {
+            even(q, std::true_type{});
+            odd(q + 1, std::true_type{});
+        }
+        if (q + 2 < n) {
+            even(q, std::true_type{});
+            odd(q + 1, std::false_type{});
+            even(q + 2, std::false_type{});
+        } else {
+            even(q, std::false_type{});
+            if (q + 1 < n) odd(q + 1, std::false_type{});
+        }
+    }
 }
 
 // Writes a wave's accumulators, columns from k and outputs from n on: a lane
@@ -355,7 +382,9 @@ __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) v
         f.x[1] = read_x(now, 1);
         // The matrix instructions of fragment row i, then a piece of the other
         // work of the step that the matrix cores run beside.
-        auto step = [&](int64_t q, auto& regs, Fragments& f, Fragments& g) {
+        // Without MORE there is no step q + 2 to stage.
+        auto step = [&](int64_t q, auto& regs, Fragments& f, Fragments& g, auto more) {
+            constexpr bool MORE = decltype(more)::value;
             const int64_t ahead = clamped(q + 4);
             hide();
 #pragma unroll
@@ -375,12 +404,12 @@ __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) v
                     for (int j = 0; j < FN; ++j)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xi, f.y[p][j], acc[i][j], 0, 0, 0);
                 // FK is 8 or 4: four columns in the first half, or a quarter each; then the loads
-                if (i < 4) stage(after, regs, i);
-                if (FK == 8 && i >= 4) {
+                if (MORE && i < 4) stage(after, regs, i);
+                if (MORE && FK == 8 && i >= 4) {
                     load(ahead, regs, 2 * (i - 4));
                     load(ahead, regs, 2 * (i - 4) + 1);
                 }
-                if (FK == 4 && i == 3) {
+                if (MORE && FK == 4 && i == 3) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k) load(ahead, regs, k);
                 }
@@ -398,10 +427,8 @@ __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) v
             __syncthreads();
         };
         if (whole_steps) {
-            for (int64_t q = 0; q < steps; q += 2) {
-                step(q, even, f, g);
-                if (q + 1 < steps) step(q + 1, odd, g, f);
-            }
+            in_pairs<NP == 3>(steps, [&](int64_t q, auto more) { step(q, even, f, g, more); },
+                     [&](int64_t q, auto more) { step(q, odd, g, f, more); });
         } else {  // fewer rows than a step
 #pragma unroll
             for (int i = 0; i < FK; ++i)
