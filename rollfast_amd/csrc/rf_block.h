@@ -44,8 +44,6 @@ __host__ __device__ inline int64_t pitch_of(int64_t cols) { return (cols + BLOCK
 template <typename T> struct Raw { u32x4 a; };  // eight 16-bit elements as loaded
 template <> struct Raw<float> { u32x4 a, b; };
 
-template <typename T> __device__ __forceinline__ Raw<T> zero8() { return Raw<T>{}; }
-
 // Loads go in two halves so that a row's loads, and the next row's, are in
 // flight together.  fetch8: eight columns from c of a row of at least eight, as
 // one unconditional load; a chunk that the row ends in, or before, is loaded
@@ -230,9 +228,9 @@ template <bool TAIL = true, typename T> __device__ __forceinline__ void put8(T* 
 }
 
 // Columns of a parameter vector whose type is known at run time (RF_F32 /
-// RF_BF16 / RF_F16), or `fill` for one that is not there; zero past the end.  Loads of several vectors are
-// sent before the first is looked at: `elsewhere` is any eight 16-bit elements
-// that may be read instead of an absent vector's.
+// RF_BF16 / RF_F16), or `fill` for one that is not there; zero past the end.
+// Loads of several vectors are sent before the first is looked at: `elsewhere`
+// is any eight 16-bit elements that may be read instead of an absent vector's.
 struct Vector8 {
     u32x4 a, b;
 

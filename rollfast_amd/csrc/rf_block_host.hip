@@ -77,6 +77,9 @@ template <int ROWS> __device__ __forceinline__ Place place(uint32_t across)
             (int64_t)tile * (blockDim.y * ROWS) + threadIdx.y};
 }
 
+// One walk: a quad of lanes has a block of 32, whose largest magnitude takes two
+// exchanges in the quad.  Bound by memory: 16384 x 11008 bf16 116 us (4.7 TB/s of
+// reads and writes), 3001 x 769 f32 6.1, most of it latency.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void k_checkpoint_store(const T* __restrict__ x, int64_t rows, int64_t cols,
                                                           int64_t stride, int8_t* __restrict__ codes,
@@ -100,6 +103,8 @@ __global__ __launch_bounds__(256) void k_checkpoint_store(const T* __restrict__ 
     }
 }
 
+// Bound by memory: 16384 x 11008 bf16 88 us (6.2 TB/s; the codes, just written,
+// come from the last-level cache in part).
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void k_checkpoint_load(const int8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ exps, int64_t rows, int64_t cols,
@@ -144,6 +149,8 @@ template <int ACT> __device__ __forceinline__ void activation(float x, float& a,
     }
 }
 
+// h = a(gate) up; the checkpoints of gate, up and (rounded) h are written in the
+// same pass.  Bound by memory: 16384 x 11008 bf16 with all three 261 us (5.6 TB/s).
 template <typename T, int ACT, int ROWS>
 __global__ __launch_bounds__(256) void k_gated_forward(const rf_gated a, uint32_t across)
 {
@@ -190,6 +197,8 @@ __global__ __launch_bounds__(256) void k_gated_forward(const rf_gated a, uint32_
     }
 }
 
+// dgate = dh up a'(gate), dup = dh a(gate), a and a' computed again from what was
+// kept.  Bound by memory: 16384 x 11008 bf16 from 8 bits 257 us (5.7 TB/s).
 template <typename T, int ACT, bool SRC8, int ROWS>
 __global__ __launch_bounds__(256) void k_gated_backward(const rf_gated a, uint32_t across)
 {
@@ -314,7 +323,9 @@ constexpr size_t MAX_LDS = 64 * 1024;
 //   16384 x 4096 LayerNorm 298 / 194, 20000 x 1280 76 / 68; backward in f32,
 //   2317 x 1283 LayerNorm 25 / 39 (two chunks spill).
 // - threads a CU: forward 16384 x 4096 157 / 122 / 126 with 512 / 1024 / 2048;
-//   backward 159 / 180 with 512 / 768 (more partial rows to write and add).
+//   backward 158 / 173 with 512 / 768 (more partial rows to write and add);
+//   forward 2317 x 1283 f32 18.3 with 1365 workgroups of 192, which do not fit
+//   at once, 16.6 with 1280, five on every CU.
 NormShape shape_of(const rf_norm& a, int cus, bool back)
 {
     NormShape s{};
@@ -328,7 +339,7 @@ NormShape shape_of(const rf_norm& a, int cus, bool back)
     s.full = a.post == RF_NORM_LAYER || a.next == RF_NORM_LAYER ||
              (back ? a.dbias || a.dnext_bias || (a.bias && a.dgate) : a.bias || a.next_bias);
     s.src8 = a.post == RF_NORM_ABSENT ? a.hidden_codes != nullptr : a.branch_codes != nullptr;
-    s.workers = std::max<int64_t>(1, std::min<int64_t>((a.rows + s.ny - 1) / s.ny, (int64_t)cus * 1024 / (s.tpr * s.ny)));
+    s.workers = std::max<int64_t>(1, std::min<int64_t>((a.rows + s.ny - 1) / s.ny, (int64_t)cus * (1024 / (s.tpr * s.ny))));
     if (s.nv == 0) s.workers = std::max<int64_t>(1, std::min<int64_t>(a.rows, (int64_t)cus * 4));
     return s;
 }
@@ -373,22 +384,40 @@ int64_t workspace_of(const rf_norm& a, const NormShape& s, const NormPlan& p)
     return n * (int64_t)sizeof(float);
 }
 
-// Adds the partial rows: 32 columns a workgroup, 32 lanes a column.  The lanes
-// are dealt to the groups of rows (all of them to one group, or one to each of
-// 32 groups at a time), and within a group to its pieces.  blockIdx.y: 0 the next
-// norm's vectors, 1 the post norm's and the gate (not launched without).
+// Adds the partial rows: 32 columns a workgroup (a cache line of a row), 32 lanes
+// a column.  The lanes are dealt to the groups of rows (all of them to one group,
+// or one to each of 32 groups at a time), and within a group to its pieces.
+// blockIdx.y: 0 the next norm's vectors, 1 the post norm's and the gate (not
+// launched without).
+// Bound by what a CU has on the way to memory, since few take part: 512 partial
+// rows of 4096 columns and two vectors 7.3 us (2.3 TB/s), of 768 columns and one
+// 4.4.  16 columns and 64 lanes, twice the workgroups with half a line each: 14.1 us
+// and 5.0.
 constexpr int FIN_COLS = 32, FIN_LANES = 32;
 
-// Partial rows w0 + i * step below w1, eight loads in flight.
-__device__ __forceinline__ float add_rows(const float* __restrict__ p, int64_t w0, int64_t w1, int64_t step, int64_t pitch)
+// Sums of partial rows w0 + i * step below w1, of vectors p and, not null, q;
+// sixteen rows' loads in flight (512 rows are one round).
+struct Pair {
+    float p, q;
+};
+
+__device__ __forceinline__ Pair add_rows(const float* p, const float* q, int64_t w0, int64_t w1, int64_t step, int64_t pitch)
 {
-    float s = 0.0f;
-    for (int64_t w = w0; w < w1; w += 8 * step) {
-        float v[8];
+    constexpr int N = 16;
+    Pair s = {0.0f, 0.0f};
+    for (int64_t w = w0; w < w1; w += N * step) {
+        float v[N], u[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = w + i * step < w1 ? p[(w + i * step) * pitch] : 0.0f;
+        for (int i = 0; i < N; ++i) {
+            const int64_t at = min(w + i * step, w1 - 1) * pitch;  // (loads without a condition do not wait for another)
+            v[i] = p ? p[at] : 0.0f;
+            u[i] = q ? q[at] : 0.0f;
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[i];
+        for (int i = 0; i < N; ++i) {
+            s.p += w + i * step < w1 ? v[i] : 0.0f;
+            s.q += w + i * step < w1 ? u[i] : 0.0f;
+        }
     }
     return s;
 }
@@ -406,11 +435,11 @@ __global__ __launch_bounds__(FIN_COLS* FIN_LANES) void k_norm_finish(const rf_no
     const int64_t groups = p.pieces > 0 ? p.groups : 1, pieces = p.pieces > 0 ? p.pieces : p.workers;
     const int lanes = (int)max((int64_t)1, FIN_LANES / groups), slots = FIN_LANES / lanes;
     const int slot = ty / lanes, sub = ty % lanes;
-    const float w = a.weight ? scalar_at(a.weight, a.weight_dtype, at) : 1.0f;
-    const float b = a.bias ? scalar_at(a.bias, a.bias_dtype, at) : 0.0f;
     if (blockIdx.y == 0) {  // the next norm's vectors
-        lds[0][ty][tx] = p.i_w2 >= 0 ? add_rows(partial + p.i_w2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
-        lds[1][ty][tx] = p.i_b2 >= 0 ? add_rows(partial + p.i_b2 * cols + at, ty, p.workers, FIN_LANES, pitch) : 0.0f;
+        const Pair v = add_rows(p.i_w2 >= 0 ? partial + p.i_w2 * cols + at : nullptr,
+                                p.i_b2 >= 0 ? partial + p.i_b2 * cols + at : nullptr, ty, p.workers, FIN_LANES, pitch);
+        lds[0][ty][tx] = v.p;
+        lds[1][ty][tx] = v.q;
         __syncthreads();
         void* const out = ty == 0 ? a.dnext_weight : a.dnext_bias;
         if (ty < 2 && in && out) {
@@ -420,28 +449,30 @@ __global__ __launch_bounds__(FIN_COLS* FIN_LANES) void k_norm_finish(const rf_no
         }
         return;
     }
+    const float w = a.weight ? scalar_at(a.weight, a.weight_dtype, at) : 1.0f;
+    const float b = a.bias ? scalar_at(a.bias, a.bias_dtype, at) : 0.0f;
     float dw = 0.0f, db = 0.0f;
-    {
-        for (int64_t first = 0; first < groups; first += slots) {
-            const int64_t g = first + slot, w0 = g * pieces;
-            const bool mine = slot < slots && g < groups;
-            const int64_t w1 = mine ? min(w0 + pieces, (int64_t)p.workers) : 0;
-            lds[2][ty][tx] = add_rows(partial + p.i_p * cols + at, w0 + sub, w1, lanes, pitch);
-            lds[3][ty][tx] = has_q ? add_rows(partial + p.i_q * cols + at, w0 + sub, w1, lanes, pitch) : 0.0f;
-            __syncthreads();
-            if (mine && sub == 0) {
-                float P = 0.0f, Q = 0.0f;
-                for (int i = 0; i < lanes; ++i) {
-                    P += lds[2][ty + i][tx];
-                    Q += lds[3][ty + i][tx];
-                }
-                const float gt = gated ? scalar_at(a.gate, a.gate_dtype, g * cols + at) : 1.0f;
-                if (gated && a.dgate && in) put_scalar(a.dgate, a.gate_dtype, g * cols + c, a.branch_scale * fmaf(w, P, b * Q));
-                dw = fmaf(gt, P, dw);
-                db = fmaf(gt, Q, db);
+    for (int64_t first = 0; first < groups; first += slots) {
+        const int64_t g = first + slot, w0 = g * pieces;
+        const bool mine = slot < slots && g < groups;
+        const int64_t w1 = mine ? min(w0 + pieces, (int64_t)p.workers) : 0;
+        const Pair v = add_rows(partial + p.i_p * cols + at, has_q ? partial + p.i_q * cols + at : nullptr, w0 + sub, w1, lanes,
+                                pitch);
+        lds[2][ty][tx] = v.p;
+        lds[3][ty][tx] = v.q;
+        __syncthreads();
+        if (mine && sub == 0) {
+            float P = 0.0f, Q = 0.0f;
+            for (int i = 0; i < lanes; ++i) {
+                P += lds[2][ty + i][tx];
+                Q += lds[3][ty + i][tx];
             }
-            __syncthreads();
+            const float gt = gated ? scalar_at(a.gate, a.gate_dtype, g * cols + at) : 1.0f;
+            if (gated && a.dgate && in) put_scalar(a.dgate, a.gate_dtype, g * cols + c, a.branch_scale * fmaf(w, P, b * Q));
+            dw = fmaf(gt, P, dw);
+            db = fmaf(gt, Q, db);
         }
+        __syncthreads();
     }
     lds[2][ty][tx] = dw;
     lds[3][ty][tx] = db;

@@ -84,9 +84,15 @@ __device__ __forceinline__ const void* gate_row(const rf_norm& a, int64_t g)
 
 // ------------------------------------------------------------- forward -----
 // blockDim (tpr, ny): tpr lanes a row; ny > 1 only where a wave holds a row.
-// FULL: LayerNorm or a bias somewhere.  The next row's loads are sent before
-// this row's sums.  Past the end of a row the elements and the vectors are
-// zero, and so is what they give.
+// FULL: LayerNorm or a bias somewhere.  TAIL: rows that end inside a chunk.  The
+// next row's loads are sent before this row's sums.  Past the end of a row the
+// elements and the vectors are zero, and so is what they give.
+// Variances are taken around the mean in a second walk of the registers: a sum of
+// squares alone loses the digits that a large mean shares.
+// Bound by memory where there are rows enough: 16384 x 4096 bf16, post and next
+// RMSNorm with both checkpoints, 133 us (5.1 TB/s).  Else by the way of one row
+// through load, sums and barriers: 8192 x 768 11.3 us, 4 x 4096 with one norm 2.8,
+// with both 4.9.
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool TAIL, int NV>
 __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Share share, const uint32_t group_rows)
 {
@@ -166,97 +172,97 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
         rstd = 1.0f / sqrtf(s[0] * inv_cols + eps);
     };
     for (int64_t r = r0; r < r1;) {
-    // the rows of one gate
-    const int64_t g = group_rows ? (uint32_t)r / group_rows : 0, end = group_rows ? min(r1, (g + 1) * group_rows) : r1;
-    float A[EXIT ? NV : 1][8], B[EXIT && FULL ? NV : 1][8];
-    if constexpr (EXIT) {
-        Vector8 w[NV], b[NV], gt[NV];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            w[j].fetch(a.weight, a.weight_dtype, c, cols, some);
-            gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, some);
-            if constexpr (FULL) b[j].fetch(a.bias, a.bias_dtype, c, cols, some);
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            float v[8];
-            w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, A[j]);
-            gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
-            if constexpr (FULL) b[j].template get<TAIL>(a.bias, a.bias_dtype, c, cols, 0.0f, B[j]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                v[k] *= a.branch_scale;
-                A[j][k] *= v[k];
-                if constexpr (FULL) B[j][k] *= v[k];
-            }
-        }
-    }
-    for (; r < end; r += ny) {
-        const Row ahead = load(r + ny < r1 ? r + ny : r);  // the last row again: still cached
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            settle8<TAIL>(now.r[j], c, cols);
-            if constexpr (EXIT) settle8<TAIL>(now.u[j], c, cols);
-        }
+        // the rows of one gate
+        const int64_t g = group_rows ? (uint32_t)r / group_rows : 0, end = group_rows ? min(r1, (g + 1) * group_rows) : r1;
+        float A[EXIT ? NV : 1][8], B[EXIT && FULL ? NV : 1][8];
         if constexpr (EXIT) {
-            float mean = 0.0f, rstd = 1.0f;
-            if (a.post != RF_NORM_NONE) {
-                stats(now.u, FULL && a.post == RF_NORM_LAYER, a.post_eps, mean, rstd);
+            Vector8 w[NV], b[NV], gt[NV];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                w[j].fetch(a.weight, a.weight_dtype, c, cols, some);
+                gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, some);
+                if constexpr (FULL) b[j].fetch(a.bias, a.bias_dtype, c, cols, some);
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                float v[8];
+                w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, A[j]);
+                gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
+                if constexpr (FULL) b[j].template get<TAIL>(a.bias, a.bias_dtype, c, cols, 0.0f, B[j]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    v[k] *= a.branch_scale;
+                    A[j][k] *= v[k];
+                    if constexpr (FULL) B[j][k] *= v[k];
+                }
+            }
+        }
+        for (; r < end; r += ny) {
+            const Row ahead = load(r + ny < r1 ? r + ny : r);  // the last row again: still cached
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                settle8<TAIL>(now.r[j], c, cols);
+                if constexpr (EXIT) settle8<TAIL>(now.u[j], c, cols);
+            }
+            if constexpr (EXIT) {
+                float mean = 0.0f, rstd = 1.0f;
+                if (a.post != RF_NORM_NONE) {
+                    stats(now.u, FULL && a.post == RF_NORM_LAYER, a.post_eps, mean, rstd);
+                    if (tid == 0) {
+                        if (a.post_rstd) a.post_rstd[r] = rstd;
+                        if (a.post_mean) a.post_mean[r] = mean;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                    if (ch < nch) {
+                        float u[8], x[8], o[8];
+                        widen8(now.u[j], u);
+                        widen8(now.r[j], x);
+                        if (a.branch_codes) put_codes(a.branch_codes, a.branch_exponents, r, pitch, ch, encode8(u));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float n = FULL ? fmaf((u[k] - mean) * rstd, A[j][k], B[FULL ? j : 0][k]) : u[k] * rstd * A[j][k];
+                            o[k] = fmaf(a.residual_scale, x[k], n);
+                        }
+                        now.r[j] = narrow8<T>(o);
+                        put8<TAIL>((T*)a.hidden + r * cols + c, now.r[j], cols - c);
+                    }
+                }
+            }
+            if constexpr (NEXT) {
+                float mean, rstd;
+                stats(now.r, FULL && a.next == RF_NORM_LAYER, a.next_eps, mean, rstd);
                 if (tid == 0) {
-                    if (a.post_rstd) a.post_rstd[r] = rstd;
-                    if (a.post_mean) a.post_mean[r] = mean;
+                    if (a.next_rstd) a.next_rstd[r] = rstd;
+                    if (a.next_mean) a.next_mean[r] = mean;
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
-                if (ch < nch) {
-                    float u[8], x[8], o[8];
-                    widen8(now.u[j], u);
-                    widen8(now.r[j], x);
-                    if (a.branch_codes) put_codes(a.branch_codes, a.branch_exponents, r, pitch, ch, encode8(u));
+                for (int j = 0; j < NV; ++j) {
+                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                    if (ch < nch) {
+                        float v[8], y[8];
+                        widen8(now.r[j], v);
+                        if (a.hidden_codes) put_codes(a.hidden_codes, a.hidden_exponents, r, pitch, ch, encode8(v));
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float n = FULL ? fmaf((u[k] - mean) * rstd, A[j][k], B[FULL ? j : 0][k]) : u[k] * rstd * A[j][k];
-                        o[k] = fmaf(a.residual_scale, x[k], n);
+                        for (int k = 0; k < 8; ++k) {
+                            y[k] = FULL ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[FULL ? j : 0][k]) : v[k] * rstd * w2[j][k];
+                        }
+                        const Raw<U> yr = narrow8<U>(y);
+                        put8<TAIL>((U*)a.y + r * cols + c, yr, cols - c);
+                        if (a.y_codes) {
+                            widen8(yr, y);
+                            put_codes(a.y_codes, a.y_exponents, r, pitch, ch, encode8(y));
+                        }
                     }
-                    now.r[j] = narrow8<T>(o);
-                    put8<TAIL>((T*)a.hidden + r * cols + c, now.r[j], cols - c);
                 }
             }
+            now = ahead;
         }
-        if constexpr (NEXT) {
-            float mean, rstd;
-            stats(now.r, FULL && a.next == RF_NORM_LAYER, a.next_eps, mean, rstd);
-            if (tid == 0) {
-                if (a.next_rstd) a.next_rstd[r] = rstd;
-                if (a.next_mean) a.next_mean[r] = mean;
-            }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int64_t ch = tid + j * tpr, c = ch * CHUNK;
-                if (ch < nch) {
-                    float v[8], y[8];
-                    widen8(now.r[j], v);
-                    if (a.hidden_codes) put_codes(a.hidden_codes, a.hidden_exponents, r, pitch, ch, encode8(v));
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        y[k] = FULL ? fmaf((v[k] - mean) * rstd, w2[j][k], b2[FULL ? j : 0][k]) : v[k] * rstd * w2[j][k];
-                    }
-                    const Raw<U> yr = narrow8<U>(y);
-                    put8<TAIL>((U*)a.y + r * cols + c, yr, cols - c);
-                    if (a.y_codes) {
-                        widen8(yr, y);
-                        put_codes(a.y_codes, a.y_exponents, r, pitch, ch, encode8(y));
-                    }
-                }
-            }
-        }
-        now = ahead;
-    }
     }
 }
 
@@ -386,6 +392,9 @@ template <typename T, bool WIDE, bool TAIL> struct Saved<T, true, WIDE, TAIL> {
 // Past the end of a row dy, dhidden and h are zero, so xhat and uhat may be
 // anything finite there.
 // FULL: LayerNorm or a bias somewhere (the sums of g, t and their columns).
+// Bound by memory: 16384 x 4096 bf16, both norms, from 8 bits 157 us (4.3 TB/s; the
+// chip's mix of reads and writes); small calls by the few rows that a lane has to
+// hide its loads behind: 8192 x 768 14.9 us, 2317 x 1283 f32 LayerNorm 23.8.
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL, int NV>
 __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const NormPlan plan, float* __restrict__ partial)
 {
@@ -470,135 +479,135 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
         }
     }
     for (int64_t r = r0; r < r1; ++g) {
-    const int64_t end = whole_groups ? r + plan.group_rows : r1;
-    if constexpr (EXIT) {
-        Vector8 w[NV], gt[NV];
+        const int64_t end = whole_groups ? r + plan.group_rows : r1;
+        if constexpr (EXIT) {
+            Vector8 w[NV], gt[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            w[j].fetch(a.weight, a.weight_dtype, c, cols, a.dbranch);
-            gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, a.dbranch);
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
-            float v[8];
-            w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, h[j]);
-            gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h[j][k] *= a.branch_scale * v[k];
-        }
-    }
-    for (; r < end; r += step) {
-        const Row ahead = load(r + step < r1 ? r + step : r);
-        const float rstd1 = now.rstd1, mean1 = now.mean1, rstd2 = now.rstd2, mean2 = now.mean2;
-        float e[NV][8], x[NEXT ? NV : 1][8], u[EXIT ? NV : 1][8];
-        // g2 xhat, h e uhat, h xhat uhat; FULL: g2, h uhat, h e, h, h xhat
-        float s[FULL ? 8 : 3] = {};
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t ch = tid + j * tpr;
-            settle8<TAIL>(now.dh[j], ch * CHUNK, cols);
-            widen8(now.dh[j], e[j]);
-            if (!a.dhidden) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) e[j][k] = 0.0f;
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                w[j].fetch(a.weight, a.weight_dtype, c, cols, a.dbranch);
+                gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, a.dbranch);
             }
-            if constexpr (NEXT) {
-                float dy[8];
-                settle8<TAIL>(now.dy[j], ch * CHUNK, cols);
-                widen8(now.dy[j], dy);
-                now.h[j].get(x[j], ch, cols);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    x[j][k] = FULL ? (x[j][k] - mean2) * rstd2 : x[j][k] * rstd2;
-                    const float g2 = dy[k] * w2[j][k];
-                    W2[j][k] = fmaf(dy[k], x[j][k], W2[j][k]);
-                    if constexpr (FULL) {
-                        B2[j][k] += dy[k];
-                        s[3] += g2;
-                    }
-                    s[0] = fmaf(g2, x[j][k], s[0]);
-                    e[j][k] = fmaf(rstd2, g2, e[j][k]);
-                }
-            }
-            if constexpr (EXIT) {
-                now.u[j].get(u[j], ch, cols);
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                float v[8];
+                w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, h[j]);
+                gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    u[j][k] = FULL ? (u[j][k] - mean1) * rstd1 : u[j][k] * rstd1;
-                    const float hu = h[j][k] * u[j][k];
-                    s[1] = fmaf(e[j][k], hu, s[1]);
-                    if constexpr (NEXT) s[2] = fmaf(x[j][k], hu, s[2]);
-                    if constexpr (FULL) {
-                        s[4] += hu;
-                        s[5] = fmaf(h[j][k], e[j][k], s[5]);
-                        s[6] += h[j][k];
-                        if constexpr (NEXT) s[7] = fmaf(h[j][k], x[j][k], s[7]);
-                    }
-                }
+                for (int k = 0; k < 8; ++k) h[j][k] *= a.branch_scale * v[k];
             }
         }
-        row_sums(s, red, half);
-        const float k1 = NEXT ? rstd2 * (s[0] * inv_cols) : 0.0f;
-        float k0 = 0.0f, m1 = s[1] - k1 * s[2], m0 = 0.0f;
-        if constexpr (FULL) {
-            k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
-            m1 -= k0 * s[4];
-            m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
-        }
-        m1 = post_norm ? m1 * inv_cols : 0.0f;
+        for (; r < end; r += step) {
+            const Row ahead = load(r + step < r1 ? r + step : r);
+            const float rstd1 = now.rstd1, mean1 = now.mean1, rstd2 = now.rstd2, mean2 = now.mean2;
+            float e[NV][8], x[NEXT ? NV : 1][8], u[EXIT ? NV : 1][8];
+            // g2 xhat, h e uhat, h xhat uhat; FULL: g2, h uhat, h e, h, h xhat
+            float s[FULL ? 8 : 3] = {};
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t ch = tid + j * tpr, c = ch * CHUNK;
-            if (ch < nch) {
-                float o[8];
+            for (int j = 0; j < NV; ++j) {
+                const int64_t ch = tid + j * tpr;
+                settle8<TAIL>(now.dh[j], ch * CHUNK, cols);
+                widen8(now.dh[j], e[j]);
+                if (!a.dhidden) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if constexpr (NEXT) e[j][k] -= fmaf(k1, x[j][k], k0);
-                    o[k] = EXIT ? a.residual_scale * e[j][k] : e[j][k];
+                    for (int k = 0; k < 8; ++k) e[j][k] = 0.0f;
                 }
-                put8<TAIL>((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
-                if constexpr (EXIT) {
+                if constexpr (NEXT) {
+                    float dy[8];
+                    settle8<TAIL>(now.dy[j], ch * CHUNK, cols);
+                    widen8(now.dy[j], dy);
+                    now.h[j].get(x[j], ch, cols);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        P[j][k] = fmaf(u[j][k], e[j][k], P[j][k]);
-                        if constexpr (FULL) Q[j][k] += e[j][k];
-                        o[k] = rstd1 * (FULL ? fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1 : fmaf(h[j][k], e[j][k], -(u[j][k] * m1)));
+                        x[j][k] = FULL ? (x[j][k] - mean2) * rstd2 : x[j][k] * rstd2;
+                        const float g2 = dy[k] * w2[j][k];
+                        W2[j][k] = fmaf(dy[k], x[j][k], W2[j][k]);
+                        if constexpr (FULL) {
+                            B2[j][k] += dy[k];
+                            s[3] += g2;
+                        }
+                        s[0] = fmaf(g2, x[j][k], s[0]);
+                        e[j][k] = fmaf(rstd2, g2, e[j][k]);
                     }
-                    put8<TAIL>((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
+                }
+                if constexpr (EXIT) {
+                    now.u[j].get(u[j], ch, cols);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        u[j][k] = FULL ? (u[j][k] - mean1) * rstd1 : u[j][k] * rstd1;
+                        const float hu = h[j][k] * u[j][k];
+                        s[1] = fmaf(e[j][k], hu, s[1]);
+                        if constexpr (NEXT) s[2] = fmaf(x[j][k], hu, s[2]);
+                        if constexpr (FULL) {
+                            s[4] += hu;
+                            s[5] = fmaf(h[j][k], e[j][k], s[5]);
+                            s[6] += h[j][k];
+                            if constexpr (NEXT) s[7] = fmaf(h[j][k], x[j][k], s[7]);
+                        }
+                    }
                 }
             }
-        }
-        now = ahead;
-    }
-    if constexpr (EXIT) {
-        if (whole_groups) {  // this group is complete: its gate's gradient, and its share of the sums
+            row_sums(s, red, half);
+            const float k1 = NEXT ? rstd2 * (s[0] * inv_cols) : 0.0f;
+            float k0 = 0.0f, m1 = s[1] - k1 * s[2], m0 = 0.0f;
+            if constexpr (FULL) {
+                k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
+                m1 -= k0 * s[4];
+                m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
+            }
+            m1 = post_norm ? m1 * inv_cols : 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int64_t ch = tid + j * tpr, c = ch * CHUNK;
                 if (ch < nch) {
-                    float w[8], b[8], gt[8];
-                    vector8(a.weight, a.weight_dtype, c, cols, 1.0f, w);
-                    vector8(a.bias, a.bias_dtype, c, cols, 0.0f, b);
-                    vector8(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, gt);
+                    float o[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const float q = FULL ? Q[FULL ? j : 0][k] : 0.0f;
-                        if (a.dgate && c + k < cols)
-                            put_scalar(a.dgate, a.gate_dtype, g * cols + c + k,
-                                       a.branch_scale * fmaf(w[k], P[j][k], b[k] * q));
-                        sums_p[c + k] = fmaf(gt[k], P[j][k], sums_p[c + k]);
-                        P[j][k] = 0.0f;
-                        if constexpr (FULL) {
-                            sums_q[c + k] = fmaf(gt[k], q, sums_q[c + k]);
-                            Q[j][k] = 0.0f;
+                        if constexpr (NEXT) e[j][k] -= fmaf(k1, x[j][k], k0);
+                        o[k] = EXIT ? a.residual_scale * e[j][k] : e[j][k];
+                    }
+                    put8<TAIL>((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
+                    if constexpr (EXIT) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            P[j][k] = fmaf(u[j][k], e[j][k], P[j][k]);
+                            if constexpr (FULL) Q[j][k] += e[j][k];
+                            o[k] = rstd1 * (FULL ? fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1 : fmaf(h[j][k], e[j][k], -(u[j][k] * m1)));
+                        }
+                        put8<TAIL>((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
+                    }
+                }
+            }
+            now = ahead;
+        }
+        if constexpr (EXIT) {
+            if (whole_groups) {  // this group is complete: its gate's gradient, and its share of the sums
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                    if (ch < nch) {
+                        float w[8], b[8], gt[8];
+                        vector8(a.weight, a.weight_dtype, c, cols, 1.0f, w);
+                        vector8(a.bias, a.bias_dtype, c, cols, 0.0f, b);
+                        vector8(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, gt);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float q = FULL ? Q[FULL ? j : 0][k] : 0.0f;
+                            if (a.dgate && c + k < cols)
+                                put_scalar(a.dgate, a.gate_dtype, g * cols + c + k,
+                                           a.branch_scale * fmaf(w[k], P[j][k], b[k] * q));
+                            sums_p[c + k] = fmaf(gt[k], P[j][k], sums_p[c + k]);
+                            P[j][k] = 0.0f;
+                            if constexpr (FULL) {
+                                sums_q[c + k] = fmaf(gt[k], q, sums_q[c + k]);
+                                Q[j][k] = 0.0f;
+                            }
                         }
                     }
                 }
             }
         }
-    }
     }
     if constexpr (EXIT) {
         if (whole_groups) {

@@ -207,9 +207,15 @@ struct StagedX { uint32_t c[8], e[2]; };  // codes of the rows, exponents of row
 // The rows past the last whole step are step 0 of the last split, so that the
 // loop's loads need no guard.
 // EDGE: dy's rows are no multiple of four elements.
+//
+// Bound by the matrix cores' instruction slots, which the staging shares: f16 (two
+// pieces) 8192 x 4096 x 4096 668 us (411 TFLOP/s, 823 of products), f32 1235 us (223,
+// 668); short sums by the way through one step: 1001 x 517 x 301 f32 13.6 us.
 template <typename T, int TILE, int WAVES_K, int WAVES_N, bool EDGE>
-__global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) void k_wgrad(const rf_weight_grad a, float* __restrict__ partial,
-                                                                 uint32_t tiles_k, uint32_t tiles, uint32_t splits)
+__global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) void k_wgrad(const rf_weight_grad a,
+                                                                                           float* __restrict__ partial,
+                                                                                           uint32_t tiles_k, uint32_t tiles,
+                                                                                           uint32_t splits)
 {
     constexpr int NP = Pieces<T>::n, HALF = WAVES_K * WAVES_N * WAVE / 2;
     constexpr int WK = TILE / WAVES_K, WN = TILE / WAVES_N, FK = WK / 16, FN = WN / 16;
@@ -469,6 +475,10 @@ __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) v
 // 32-byte units of dy's rows are xored by (t0, t1, t3) so that the sixteen rows
 // of a transposed read lie in different banks.
 //
+// Measured beside k_wgrad (us): 16384 x 11008 x 4096 1389 / 1495, 8192 x 2304 x 768
+// (eight splits) 41 / 42.  At 1389 us, 1.06 PFLOP/s, the matrix cores are busy 43 %
+// of the cycles; 688 tiles on 256 CUs leave the last of three rounds two thirds full.
+//
 // The compiler must not count or order these loads (it would wait for all of
 // them before each LDS read): they are written in assembly, have no results,
 // and the waits for them are explicit.  (m0, which they set, is otherwise unused
@@ -687,7 +697,8 @@ __global__ __launch_bounds__(DIRECT_WAVES* WAVE) void k_wgrad_direct(const rf_we
     store_tile(a, splits == 1 ? nullptr : partial + (int64_t)split * a.outs * a.cols, acc, k0 + wk, n0 + wn);
 }
 
-// Adds the splits' partial sums in their order.
+// Adds the splits' partial sums in their order.  Bound by memory: eight of 2304 x 768
+// 10.1 us (5.6 TB/s read).
 __global__ __launch_bounds__(256) void k_wgrad_join(const rf_weight_grad a, const float* __restrict__ partial,
                                                     uint32_t splits)
 {
