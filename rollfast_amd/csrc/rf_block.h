@@ -188,10 +188,14 @@ template <typename T> __device__ __forceinline__ Raw<T> narrow8(const float (&v)
     return r;
 }
 
-// Stores the first `left` of eight elements.
-template <bool TAIL = true, typename T> __device__ __forceinline__ void put8(T* p, const Raw<T>& r, int64_t left)
+// Stores the first `left` of eight elements.  STREAM: past the caches.
+template <bool TAIL = true, bool STREAM = false, typename T>
+__device__ __forceinline__ void put8(T* p, const Raw<T>& r, int64_t left)
 {
-    if (TAIL ? left >= CHUNK : left > 0) {
+    if (STREAM && left >= CHUNK) {
+        __builtin_nontemporal_store(r.a, (u32x4_at*)p);
+        if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(r.b, (u32x4_at*)(p + 4));
+    } else if (TAIL ? left >= CHUNK : left > 0) {
         *(u32x4_at*)p = r.a;
         if constexpr (sizeof(T) == 4) *(u32x4_at*)(p + 4) = r.b;
     } else if (TAIL && left > 0) {

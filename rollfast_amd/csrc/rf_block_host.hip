@@ -103,9 +103,14 @@ __global__ __launch_bounds__(256) void k_checkpoint_store(const T* __restrict__ 
     }
 }
 
-// Bound by memory: 16384 x 11008 bf16 88 us (6.2 TB/s; the codes, just written,
+// Bound by memory: 16384 x 11008 bf16 89 us (6.1 TB/s; the codes, just written,
 // come from the last-level cache in part).
-template <typename T, int ROWS>
+// STREAM: an output that the last-level cache cannot hold beside the codes is
+// stored past it, so that its lines need not be written back in front of what
+// comes next.  Store and load in turn, us with and without: 16384 x 11008 bf16
+// 184 / 205, 16384 x 8192 122 / 149, 16384 x 11008 f32 376 / 393; smaller ones are
+// left in the cache for their reader.
+template <typename T, int ROWS, bool STREAM>
 __global__ __launch_bounds__(256) void k_checkpoint_load(const int8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ exps, int64_t rows, int64_t cols,
                                                          T* __restrict__ out, uint32_t across)
@@ -121,7 +126,7 @@ __global__ __launch_bounds__(256) void k_checkpoint_load(const int8_t* __restric
         const int64_t r = p.row + i * blockDim.y;
         float f[8];
         decode8(v[i], f);
-        if (r < rows) put8(out + r * cols + p.ch * CHUNK, narrow8<T>(f), cols - p.ch * CHUNK);
+        if (r < rows) put8<true, STREAM>(out + r * cols + p.ch * CHUNK, narrow8<T>(f), cols - p.ch * CHUNK);
     }
 }
 
@@ -150,7 +155,8 @@ template <int ACT> __device__ __forceinline__ void activation(float x, float& a,
 }
 
 // h = a(gate) up; the checkpoints of gate, up and (rounded) h are written in the
-// same pass.  Bound by memory: 16384 x 11008 bf16 with all three 261 us (5.6 TB/s).
+// same pass.  Bound by memory: 16384 x 11008 bf16 with those of gate and up 261 us
+// (5.6 TB/s).
 template <typename T, int ACT, int ROWS>
 __global__ __launch_bounds__(256) void k_gated_forward(const rf_gated a, uint32_t across)
 {
@@ -269,8 +275,11 @@ template <typename T>
 void load(const int8_t* codes, const uint8_t* exps, int64_t rows, int64_t cols, T* out, const Tiles& t, hipStream_t st)
 {
     const dim3 grid((unsigned)t.grid), block(t.bx, t.by);
-    if (t.four) k_checkpoint_load<T, 4><<<grid, block, 0, st>>>(codes, exps, rows, cols, out, t.across);
-    else k_checkpoint_load<T, 1><<<grid, block, 0, st>>>(codes, exps, rows, cols, out, t.across);
+    constexpr int64_t CACHE = 256 << 20;  // the last-level cache
+    if (t.four && rows * (cols * (int64_t)sizeof(T) + pitch_of(cols)) > CACHE)
+        k_checkpoint_load<T, 4, true><<<grid, block, 0, st>>>(codes, exps, rows, cols, out, t.across);
+    else if (t.four) k_checkpoint_load<T, 4, false><<<grid, block, 0, st>>>(codes, exps, rows, cols, out, t.across);
+    else k_checkpoint_load<T, 1, false><<<grid, block, 0, st>>>(codes, exps, rows, cols, out, t.across);
 }
 
 rf_status check_checkpoint(const void* tensor, int32_t dtype, int64_t rows, int64_t cols, const int8_t* codes,

@@ -646,6 +646,20 @@ def test_offsets_past_32_bits():
     assert (whole - parts).abs().max().item() <= 2 * rows ** 0.5 * U * size
 
 
+@pytest.mark.parametrize("rows,cols,dtype", [(9001, 8195, F32), (18003, 8196, BF16), (36001, 4100, F16)])
+def test_restored_outputs_larger_than_the_cache(rows, cols, dtype):
+    """Outputs that are stored past the cache, rows that end inside a chunk:
+    every run of rows is what restoring it alone gives."""
+    x = rand((rows, cols), dtype, 9)
+    x *= torch.linspace(0.1, 4, rows, device="cuda").to(dtype)[:, None]
+    ck = rf().checkpoint_activations(x)
+    y = rf().restore_activations(ck)
+    for at in range(0, rows, 1000):
+        n = min(1000, rows - at)
+        part = rf().ActivationCheckpoint(ck.codes[at: at + n], ck.exponents[at: at + n], (n, cols), dtype)
+        assert torch.equal(y[at: at + n], rf().restore_activations(part)), at
+
+
 # ------------------------------------------------- gradients by differences ---
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 def test_gradients_by_differences(norm):
