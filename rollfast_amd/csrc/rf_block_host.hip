@@ -323,7 +323,7 @@ rf_status gated(const rf_gated* a, bool back, void* stream)
 }
 
 // ----------------------------------------------------------------- norms ---
-constexpr int64_t MAX_REGISTER_COLS = 8192;  // 512 lanes, two chunks each
+constexpr int64_t MAX_REGISTER_COLS = 16384;  // 1024 lanes, two chunks each
 constexpr size_t MAX_LDS = 64 * 1024;
 
 // Lanes and chunks of a row, measured on one GPU (us):
@@ -341,7 +341,7 @@ NormShape shape_of(const rf_norm& a, int cus, bool back)
     const int64_t nch = pitch_of(a.cols) / CHUNK;
     const bool two = nch > 512 || (nch > 64 && (back ? a.dtype != RF_F32 : nch <= 128));
     const int64_t lanes = two ? (nch + 1) / 2 : nch;
-    s.tpr = (int)std::min<int64_t>(512, (lanes + 63) / 64 * 64);
+    s.tpr = (int)std::min<int64_t>(1024, (lanes + 63) / 64 * 64);
     s.nv = a.cols > MAX_REGISTER_COLS || a.cols < CHUNK ? 0 : two ? 2 : 1;
     if (s.nv == 0) s.tpr = 512;
     s.ny = s.tpr == 64 && s.nv ? 4 : 1;
@@ -383,7 +383,8 @@ void plan_of(const rf_norm& a, int cus, NormShape& s, NormPlan& p)
     const int64_t pitch = pitch_of(a.cols);
     s.lds = s.ny > 1 ? pitch * sizeof(float) : 0;
     if (p.pieces == 0) s.lds = (size_t)s.ny * (s.full ? 2 : 1) * pitch * sizeof(float);
-    if (s.lds > MAX_LDS - 1024) s.nv = 0, s.ny = 1, s.tpr = 512, s.lds = 0;
+    // (the broad kernel takes pieces of one group only)
+    if (s.lds > MAX_LDS - 2048 || (p.pieces == 0 && s.tpr > 512)) s.nv = 0, s.ny = 1, s.tpr = 512, s.lds = 0;
 }
 
 int64_t workspace_of(const rf_norm& a, const NormShape& s, const NormPlan& p)

@@ -1,7 +1,7 @@
 // rf_norm.h -- the norms around a block: forward and backward kernels.
 //
-// Rows of up to 8192 columns stay in registers from their one load to their
-// last use (two chunks of eight columns per lane at most, 64 to 512 lanes a
+// Rows of up to 16384 columns stay in registers from their one load to their
+// last use (two chunks of eight columns per lane at most, 64 to 1024 lanes a
 // row); wider rows are walked again by the lanes that loaded them (k_*_wide).
 // The parameter vectors' gradients are sums over rows: a workgroup adds its
 // own rows in registers and writes one partial row, k_norm_finish adds the
@@ -26,7 +26,7 @@
 
 namespace rfb {
 
-constexpr int MAX_WAVES = 8;  // waves of a row in the register kernels
+constexpr int MAX_WAVES = 16;  // waves of a row
 
 // n things dealt to `of` takers in runs; the first `more` get one more than `each`.
 // (Kernels divide nothing: a 64-bit division is 140 instructions.)
@@ -93,8 +93,10 @@ __device__ __forceinline__ const void* gate_row(const rf_norm& a, int64_t g)
 // RMSNorm with both checkpoints, 133 us (5.1 TB/s).  Else by the way of one row
 // through load, sums and barriers: 8192 x 768 11.3 us, 4 x 4096 with one norm 2.8,
 // with both 4.9.
-template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool TAIL, int NV>
-__global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Share share, const uint32_t group_rows)
+// LANES: 1024 for rows of more than 8192 columns.  8192 x 16384 bf16, one norm 112 us,
+// both 200 (k_norm_forward_wide 182, 367).
+template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool TAIL, int NV, int LANES>
+__global__ __launch_bounds__(LANES) void k_norm_forward(const rf_norm a, const Share share, const uint32_t group_rows)
 {
     __shared__ float red[2][MAX_WAVES][8];
     int half = 0;
@@ -103,6 +105,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
     const float inv_cols = 1.0f / (float)cols;
     const int64_t r0 = first_of(share, blockIdx.x) + ty, r1 = first_of(share, blockIdx.x + 1);
     if (r0 >= r1) return;  // a wave of its own (ny > 1): no other waits for it
+    int at = tid;
     struct Row {
         Raw<T> r[NV];
         Raw<U> u[EXIT ? NV : 1];
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
         const T* rp = EXIT ? (const T*)a.residual + r * a.residual_stride : (const T*)a.hidden + r * a.hidden_stride;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
             x.r[j] = fetch8(rp, c, cols);
             if constexpr (EXIT) x.u[j] = fetch8((const U*)a.branch + r * a.branch_stride, c, cols);
         }
@@ -125,13 +128,13 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
         Vector8 w[NV], b[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
             w[j].fetch(a.next_weight, a.next_weight_dtype, c, cols, some);
             if constexpr (FULL) b[j].fetch(a.next_bias, a.next_bias_dtype, c, cols, some);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
             w[j].template get<TAIL>(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, w2[j]);
             if constexpr (FULL) b[j].template get<TAIL>(a.next_bias, a.next_bias_dtype, c, cols, 0.0f, b2[j]);
         }
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
         float s[1] = {0.0f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t left = cols - (int64_t)(tid + j * tpr) * CHUNK;
+            const int64_t left = cols - (int64_t)(at + j * tpr) * CHUNK;
             float v[8], t = 0.0f;
             widen8(x[j], v);
             if (FULL && TAIL) {
@@ -179,14 +182,14 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
             Vector8 w[NV], b[NV], gt[NV];
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
                 w[j].fetch(a.weight, a.weight_dtype, c, cols, some);
                 gt[j].fetch(gate_row(a, g), a.gate_dtype, c, cols, some);
                 if constexpr (FULL) b[j].fetch(a.bias, a.bias_dtype, c, cols, some);
             }
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
                 float v[8];
                 w[j].template get<TAIL>(a.weight, a.weight_dtype, c, cols, 1.0f, A[j]);
                 gt[j].template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
@@ -200,10 +203,11 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
             }
         }
         for (; r < end; r += ny) {
+            if constexpr (LANES > 512) asm volatile("" : "+v"(at));  // 128 registers: no addresses kept from row to row
             const Row ahead = load(r + ny < r1 ? r + ny : r);  // the last row again: still cached
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+                const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
                 settle8<TAIL>(now.r[j], c, cols);
                 if constexpr (EXIT) settle8<TAIL>(now.u[j], c, cols);
             }
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
                 }
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                    const int64_t ch = at + j * tpr, c = ch * CHUNK;
                     if (ch < nch) {
                         float u[8], x[8], o[8];
                         widen8(now.u[j], u);
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(512) void k_norm_forward(const rf_norm a, const Sha
                 }
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    const int64_t ch = tid + j * tpr, c = ch * CHUNK;
+                    const int64_t ch = at + j * tpr, c = ch * CHUNK;
                     if (ch < nch) {
                         float v[8], y[8];
                         widen8(now.r[j], v);
@@ -372,10 +376,12 @@ template <typename T, bool SRC8, bool WIDE, bool TAIL = true> struct Saved {
     {
         t = WIDE ? fetch8(p + r * stride, ch * CHUNK, cols) : fetch8_any(p + r * stride, ch * CHUNK, cols);
     }
+    __device__ __forceinline__ void settle(int64_t ch, int64_t cols) { settle8<TAIL>(t, ch * CHUNK, cols); }
+    __device__ __forceinline__ void values(float (&v)[8]) const { widen8(t, v); }
     __device__ __forceinline__ void get(float (&v)[8], int64_t ch, int64_t cols)
     {
-        settle8<TAIL>(t, ch * CHUNK, cols);
-        widen8(t, v);
+        settle(ch, cols);
+        values(v);
     }
 };
 template <typename T, bool WIDE, bool TAIL> struct Saved<T, true, WIDE, TAIL> {
@@ -386,7 +392,9 @@ template <typename T, bool WIDE, bool TAIL> struct Saved<T, true, WIDE, TAIL> {
         t = get_codes(codes, exps, r, pitch, min(ch, nch - 1));
         if (ch >= nch) t.e = 0;  // reads as zero
     }
-    __device__ __forceinline__ void get(float (&v)[8], int64_t, int64_t) const { decode8(t, v); }
+    __device__ __forceinline__ void settle(int64_t, int64_t) {}
+    __device__ __forceinline__ void values(float (&v)[8]) const { decode8(t, v); }
+    __device__ __forceinline__ void get(float (&v)[8], int64_t, int64_t) const { values(v); }
 };
 
 // Past the end of a row dy, dhidden and h are zero, so xhat and uhat may be
@@ -669,6 +677,230 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
     }
     if constexpr (NEXT) {
         finish(W2, plan.i_w2);
+        if constexpr (FULL) finish(B2, plan.i_b2);
+    }
+}
+
+// Keeps the compiler from seeing that a value is the one from before, and so from
+// keeping in registers what was computed from it.
+__device__ __forceinline__ void forget(Raw<float>& r) { asm volatile("" : "+v"(r.a), "+v"(r.b)); }
+template <typename T> __device__ __forceinline__ void forget(Raw<T>& r) { asm volatile("" : "+v"(r.a)); }
+__device__ __forceinline__ void forget(Codes& r) { asm volatile("" : "+v"(r.c), "+v"(r.e)); }
+
+// Rows of more than 8192 columns and at most 16384, pieces of one group: two
+// chunks a lane, up to 1024 lanes, so 128 registers.  They hold the row as loaded
+// and the column sums; what the row's values give is computed before and after the
+// row's sums, the vectors are read again for each row (they stay in the caches),
+// and the next row is loaded when this one is done: a row is 100 KB and more, few
+// trips to memory for what it takes to stream it.  With both norms two of the
+// column sums lie in LDS: in registers they were spilled, by all CUs together more
+// than the L2 caches hold.
+// Bound by memory for one norm: 8192 x 16384 bf16 from 8 bits 228 us (4.1 TB/s; 775
+// with k_norm_backward_wide); with both norms by the second reading of the values
+// too: 431 (1452 with the wide kernel, 865 with all sums in registers; LDS atomics
+// instead of loads and stores 1476).
+template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL>
+__global__ __launch_bounds__(1024) void k_norm_backward_broad(const rf_norm a, const NormPlan plan,
+                                                              float* __restrict__ partial)
+{
+    constexpr int NV = 2;
+    constexpr bool IN_LDS = EXIT && NEXT;
+    __shared__ float red[2][MAX_WAVES][8];
+    extern __shared__ float cols_lds[];  // IN_LDS: P and W2, [2][NV][8][1024]
+    int half = 0;
+    const int tid = threadIdx.x, tpr = blockDim.x;
+    const int64_t cols = a.cols, pitch = pitch_of(cols), nch = pitch / CHUNK;
+    const float inv_cols = 1.0f / (float)cols;
+    const bool post_layer = FULL && EXIT && a.post == RF_NORM_LAYER, next_layer = FULL && NEXT && a.next == RF_NORM_LAYER;
+    const bool post_norm = EXIT && a.post != RF_NORM_NONE;
+    float P[EXIT && !IN_LDS ? NV : 1][8] = {}, Q[EXIT && FULL ? NV : 1][8] = {};
+    float W2[NEXT && !IN_LDS ? NV : 1][8] = {}, B2[NEXT && FULL ? NV : 1][8] = {};
+    // this lane's place of vector v (0: P, 1: W2), chunk j, column k
+    auto place = [&](int v, int j, int k) { return cols_lds + ((v * NV + j) * 8 + k) * 1024 + tid; };
+    auto add = [&](int v, int j, int k, float x) {
+        *place(v, j, k) += x;
+    };
+    if constexpr (IN_LDS) {
+#pragma unroll
+        for (int i = 0; i < 2 * NV * 8; ++i) cols_lds[i * 1024 + tid] = 0.0f;
+    }
+    const uint32_t piece = blockIdx.x % (uint32_t)plan.pieces;
+    const int64_t g = blockIdx.x / (uint32_t)plan.pieces;
+    const int64_t r0 = g * plan.group_rows + first_of(plan.rows, piece), r1 = g * plan.group_rows + first_of(plan.rows, piece + 1);
+    struct Row {
+        Raw<T> dh[NV];
+        Raw<U> dy[NEXT ? NV : 1];
+        Saved<U, SRC8, true, TAIL> u[EXIT ? NV : 1];
+        Saved<T, SRC8, true, TAIL> h[NEXT ? NV : 1];
+    };
+    for (int64_t r = r0; r < r1; ++r) {
+        // (what is computed from it is not kept from row to row)
+        int at = tid;
+        asm volatile("" : "+v"(at));
+        Row now;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t ch = at + j * tpr, c = ch * CHUNK;
+            // without one: any rows that may be read, cleared below
+            now.dh[j] = fetch8(a.dhidden ? (const T*)a.dhidden + r * a.dhidden_stride : (const T*)a.dresidual + r * cols, c, cols);
+            if constexpr (NEXT) {
+                now.dy[j] = fetch8((const U*)a.dy + r * a.dy_stride, c, cols);
+                now.h[j].fetch((const T*)a.hidden, a.hidden_stride, a.hidden_codes, a.hidden_exponents, r, pitch, ch, nch, cols);
+            }
+            if constexpr (EXIT)
+                now.u[j].fetch((const U*)a.branch, a.branch_stride, a.branch_codes, a.branch_exponents, r, pitch, ch, nch, cols);
+        }
+        const float rstd1 = post_norm ? a.post_rstd[r] : 1.0f, mean1 = post_layer ? a.post_mean[r] : 0.0f;
+        const float rstd2 = NEXT ? a.next_rstd[r] : 0.0f, mean2 = next_layer ? a.next_mean[r] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t ch = at + j * tpr;
+            settle8<TAIL>(now.dh[j], ch * CHUNK, cols);
+            if (!a.dhidden) now.dh[j] = Raw<T>{};
+            if constexpr (NEXT) {
+                settle8<TAIL>(now.dy[j], ch * CHUNK, cols);
+                now.h[j].settle(ch, cols);
+            }
+            if constexpr (EXIT) now.u[j].settle(ch, cols);
+        }
+        // e = dhidden + rstd2 g2, xhat, uhat, h, dy and g2 of a chunk, one after the
+        // other: the registers are full
+        auto expand = [&](int j, float (&e)[8], float (&x)[8], float (&u)[8], float (&h)[8], float (&dy)[8], float (&g2)[8]) {
+            const int64_t c = (int64_t)(at + j * tpr) * CHUNK;
+            if constexpr (EXIT) {
+                Vector8 w, gt;
+                float v[8];
+                w.fetch(a.weight, a.weight_dtype, c, cols, a.dbranch);
+                gt.fetch(gate_row(a, g), a.gate_dtype, c, cols, a.dbranch);
+                w.template get<TAIL>(a.weight, a.weight_dtype, c, cols, a.branch_scale, h);
+                if (a.weight) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) h[k] *= a.branch_scale;
+                }
+                gt.template get<TAIL>(gate_row(a, g), a.gate_dtype, c, cols, 1.0f, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) h[k] *= v[k];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            widen8(now.dh[j], e);
+            if constexpr (NEXT) {
+                Vector8 w2;
+                w2.fetch(a.next_weight, a.next_weight_dtype, c, cols, a.dy);
+                w2.template get<TAIL>(a.next_weight, a.next_weight_dtype, c, cols, 1.0f, g2);
+                now.h[j].values(x);
+                widen8(now.dy[j], dy);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    x[k] = FULL ? (x[k] - mean2) * rstd2 : x[k] * rstd2;
+                    g2[k] *= dy[k];
+                    e[k] = fmaf(rstd2, g2[k], e[k]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (EXIT) {
+                now.u[j].values(u);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) u[k] = FULL ? (u[k] - mean1) * rstd1 : u[k] * rstd1;
+            }
+        };
+        float s[FULL ? 8 : 3] = {};  // as in k_norm_backward
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float e[8], x[8], u[8], h[8], dy[8], g2[8];
+            expand(j, e, x, u, h, dy, g2);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (NEXT) {
+                    s[0] = fmaf(g2[k], x[k], s[0]);
+                    if constexpr (FULL) s[3] += g2[k];
+                }
+                if constexpr (EXIT) {
+                    const float hu = h[k] * u[k];
+                    s[1] = fmaf(e[k], hu, s[1]);
+                    if constexpr (NEXT) s[2] = fmaf(x[k], hu, s[2]);
+                    if constexpr (FULL) {
+                        s[4] += hu;
+                        s[5] = fmaf(h[k], e[k], s[5]);
+                        s[6] += h[k];
+                        if constexpr (NEXT) s[7] = fmaf(h[k], x[k], s[7]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        row_sums(s, red, half);
+        const float k1 = NEXT ? rstd2 * (s[0] * inv_cols) : 0.0f;
+        float k0 = 0.0f, m1 = s[1] - k1 * s[2], m0 = 0.0f;
+        if constexpr (FULL) {
+            k0 = next_layer ? rstd2 * (s[3] * inv_cols) : 0.0f;
+            m1 -= k0 * s[4];
+            m0 = post_layer ? (s[5] - k0 * s[6] - k1 * s[7]) * inv_cols : 0.0f;
+        }
+        m1 = post_norm ? m1 * inv_cols : 0.0f;
+        asm volatile("" : "+v"(at));
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            forget(now.dh[j]);
+            if constexpr (NEXT) {
+                forget(now.dy[j]);
+                forget(now.h[j].t);
+            }
+            if constexpr (EXIT) forget(now.u[j].t);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t ch = at + j * tpr, c = ch * CHUNK;
+            float e[8], x[8], u[8], h[8], dy[8], g2[8], o[8];
+            expand(j, e, x, u, h, dy, g2);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (NEXT) {
+                    if constexpr (IN_LDS) add(1, j, k, dy[k] * x[k]);
+                    else W2[j][k] = fmaf(dy[k], x[k], W2[j][k]);
+                    if constexpr (FULL) B2[j][k] += dy[k];
+                    e[k] -= fmaf(k1, x[k], k0);
+                }
+                o[k] = EXIT ? a.residual_scale * e[k] : e[k];
+            }
+            if (ch < nch) put8<TAIL>((T*)a.dresidual + r * cols + c, narrow8<T>(o), cols - c);
+            if constexpr (EXIT) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (IN_LDS) add(0, j, k, u[k] * e[k]);
+                    else P[j][k] = fmaf(u[k], e[k], P[j][k]);
+                    if constexpr (FULL) Q[j][k] += e[k];
+                    o[k] = rstd1 * (FULL ? fmaf(h[k], e[k], -m0) - u[k] * m1 : fmaf(h[k], e[k], -(u[k] * m1)));
+                }
+                if (ch < nch) put8<TAIL>((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    float* const out = partial + (int64_t)blockIdx.x * plan.vectors * cols;
+    auto finish = [&](auto& acc, int index) {
+        if (index < 0) return;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = (int64_t)(tid + j * tpr) * CHUNK;
+            put8<TAIL>(out + index * cols + c, narrow8<float>(acc[j]), cols - c);
+        }
+    };
+    auto finish_lds = [&](int v, int index) {
+        float acc[NV][8];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[j][k] = *place(v, j, k);
+        finish(acc, index);
+    };
+    if constexpr (EXIT) {
+        if constexpr (IN_LDS) finish_lds(0, plan.i_p);
+        else finish(P, plan.i_p);
+        if constexpr (FULL) finish(Q, plan.i_q);
+    }
+    if constexpr (NEXT) {
+        if constexpr (IN_LDS) finish_lds(1, plan.i_w2);
+        else finish(W2, plan.i_w2);
         if constexpr (FULL) finish(B2, plan.i_b2);
     }
 }

@@ -18,8 +18,9 @@ static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
     const dim3 grid((unsigned)s.workers), block(s.tpr, s.ny);
     const Share rows = share_of(a.rows, s.workers);
     const uint32_t per_gate = a.gates > 1 ? (uint32_t)(a.rows / a.gates) : 0;
-    if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 1><<<grid, block, 0, st>>>(a, rows, per_gate);
-    else k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 2><<<grid, block, 0, st>>>(a, rows, per_gate);
+    if (s.nv == 1) k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 1, 512><<<grid, block, 0, st>>>(a, rows, per_gate);
+    else if (s.tpr <= 512) k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 2, 512><<<grid, block, 0, st>>>(a, rows, per_gate);
+    else k_norm_forward<T, U, EXIT, NEXT, FULL, TAIL, 2, 1024><<<grid, block, 0, st>>>(a, rows, per_gate);
 }
 
 template <bool EXIT, bool NEXT> static void forward(const rf_norm& a, const NormShape& s, hipStream_t st)
@@ -40,7 +41,14 @@ static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, fl
 {
     const dim3 grid((unsigned)p.workers), block(s.tpr, s.ny);
     if (s.nv == 1) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, TAIL, 1><<<grid, block, s.lds, st>>>(a, p, partial);
-    else k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, TAIL, 2><<<grid, block, s.lds, st>>>(a, p, partial);
+    else if (s.tpr <= 512) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, TAIL, 2><<<grid, block, s.lds, st>>>(a, p, partial);
+    else {
+        static std::atomic<uint64_t> done;
+        const auto f = k_norm_backward_broad<T, U, EXIT, NEXT, FULL, SRC8, TAIL>;
+        constexpr size_t lds = EXIT && NEXT ? 1024 * 2 * 2 * 8 * sizeof(float) : 0;
+        if (allow_lds((const void*)f, lds, done) != RF_OK) return;
+        f<<<grid, block, lds, st>>>(a, p, partial);
+    }
 }
 
 template <bool EXIT, bool NEXT, bool SRC8>

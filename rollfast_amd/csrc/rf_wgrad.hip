@@ -769,20 +769,6 @@ Plan plan_of(const rf_weight_grad& a, int cus)
     return best;
 }
 
-// Allows a kernel more than 64 KB of LDS, once on each device.
-rf_status allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done)
-{
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return rf::report_hip(e, "hipGetDevice");
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (bytes <= 64 * 1024 || (done.load(std::memory_order_relaxed) & bit)) return RF_OK;
-    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return RF_OK;
-}
-
 template <typename T, int TILE, int WK, int WN, bool EDGE>
 rf_status launch(const rf_weight_grad& a, const Plan& p, float* partial, hipStream_t st)
 {
@@ -826,6 +812,19 @@ rf_status check(const rf_weight_grad* a)
 }
 
 }  // namespace
+
+rf_status rfb::allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) noexcept
+{
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return rf::report_hip(e, "hipGetDevice");
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bytes <= 64 * 1024 || (done.load(std::memory_order_relaxed) & bit)) return RF_OK;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return rf::report_hip(e, "hipFuncSetAttribute");
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return RF_OK;
+}
 
 extern "C" {
 

@@ -545,6 +545,26 @@ def test_postnorm_gates(shape, vary, norm, bias):
     check_postnorm(shape, BF16, BF16, norm, vary, None, "int8", vectors=BF16, bias=bias)
 
 
+# around the widths at which rows take more lanes, and no longer stay in registers
+BROAD_SHAPES = [(11, 8193), (300, 8704), (21, 12288), (9, 16379), (13, 16384), (5, 16385), (6, 16400)]
+
+
+@pytest.mark.parametrize("r_dtype,u_dtype", PAIRS)
+@pytest.mark.parametrize("rows,cols", BROAD_SHAPES)
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("save", ["int8", "input"])
+def test_broad_rows(rows, cols, r_dtype, u_dtype, norm, save):
+    check_prenorm(rows, cols, r_dtype, u_dtype, norm, F32, save, norm == "layer", True)
+    check_postnorm((rows, cols), r_dtype, u_dtype, norm, "one", norm, save)
+
+
+@pytest.mark.parametrize("shape,vary", [((4, 31, 9000), 1), ((300, 2, 8704), 1), ((7, 1, 16384), 1), ((260, 1, 12290), 1)])
+@pytest.mark.parametrize("norm,follows,bias", [("rms", "rms", False), ("layer", None, True), ("none", "layer", False)])
+def test_broad_rows_gates(shape, vary, norm, follows, bias):
+    check_postnorm(shape, F32, F32, norm, vary, follows, "input", bias=bias)
+    check_postnorm(shape, BF16, BF16, norm, vary, follows, "int8", vectors=F16, bias=bias, dout_given=False)
+
+
 def test_postnorm_without_dout_and_mixed_vectors():
     check_postnorm((30, 200), BF16, BF16, "rms", "one", "rms", "int8", dout_given=False)
     check_postnorm((30, 200), F32, F16, "layer", None, "layer", "input", vectors=F16, dout_given=False)
