@@ -565,6 +565,25 @@ def test_broad_rows_gates(shape, vary, norm, follows, bias):
     check_postnorm(shape, BF16, BF16, norm, vary, follows, "int8", vectors=F16, bias=bias, dout_given=False)
 
 
+@pytest.mark.parametrize("shape", [(16, 9, 70), (17, 9, 70), (32, 200, 96), (33, 40, 130), (66, 41, 391), (382, 5, 99), (255, 8, 64)])
+@pytest.mark.parametrize("gate_dtype", [F32, BF16, F16])
+def test_postnorm_many_gates(shape, gate_dtype):
+    """Numbers of gates around those at which the final sums are dealt out otherwise."""
+    check_postnorm(shape, F32, BF16, "layer", 1, "rms", "input", vectors=gate_dtype, bias=True)
+    check_postnorm(shape, BF16, BF16, "rms", 1, "layer", "int8", vectors=gate_dtype)
+
+
+@pytest.mark.parametrize("gates", [1, 3, 40])
+def test_gates_without_rows(gates):
+    r, u = torch.empty(gates, 0, 50, dtype=BF16, device="cuda"), torch.empty(gates, 0, 50, dtype=BF16, device="cuda")
+    w, gate = rand((50,), F32, 1), rand((gates, 1, 50), F32, 2)
+    out, y, saved = rf().postnorm_residual(r, u, w, w, gate, norm="layer", next_norm="rms", next_weight=w)
+    got = rf().postnorm_residual_grad(out, y, saved)
+    assert got.gate.shape == gate.shape
+    for g in (got.weight, got.bias, got.gate, got.next_weight):
+        assert torch.equal(g, torch.zeros_like(g))
+
+
 def test_postnorm_without_dout_and_mixed_vectors():
     check_postnorm((30, 200), BF16, BF16, "rms", "one", "rms", "int8", dout_given=False)
     check_postnorm((30, 200), F32, F16, "layer", None, "layer", "input", vectors=F16, dout_given=False)
