@@ -205,6 +205,18 @@ struct Call {
         return t;
     }
 
+    // Whether a tensor that the forward pass kept is where and what it was: since then
+    // a parameter's `data` may have been replaced, or a saved-tensor hook have given
+    // back another tensor.
+    bool kept(const at::Tensor& t, at::ScalarType type) const
+    {
+        return t.is_cuda() && t.device() == device && t.scalar_type() == type;
+    }
+    bool kept_bytes(const at::Tensor& t, int64_t n) const
+    {
+        return kept(t, at::kByte) && t.is_contiguous() && t.numel() == n;
+    }
+
     at::TensorOptions options(at::ScalarType t) const { return at::TensorOptions().dtype(t).device(device); }
     at::Tensor empty(at::ScalarType t) const { return at::empty(shape, options(t)); }
     at::Tensor bytes(int64_t n) const { return at::empty({n}, options(at::kByte)); }
@@ -449,7 +461,7 @@ PyObject* py_gated_backward(PyObject*, PyObject* args)
     if (ao != Py_None) {
         keep[0] = THPVariable_Unpack(ao);
         const Arena l(c.rows, c.cols, 2);
-        if (keep[0].numel() != l.size(0)) Py_RETURN_NONE;
+        if (!c.kept_bytes(keep[0], l.size(0))) Py_RETURN_NONE;
         void* const p = keep[0].data_ptr();
         a.gate_codes = l.codes(p, 0);
         a.up_codes = l.codes(p, 1);
@@ -458,6 +470,7 @@ PyObject* py_gated_backward(PyObject*, PyObject* args)
     } else {
         keep[0] = THPVariable_Unpack(go);
         keep[1] = THPVariable_Unpack(uo);
+        if (!c.kept(keep[0], dh.scalar_type()) || !c.kept(keep[1], dh.scalar_type())) Py_RETURN_NONE;
         c.as_rows(keep[0], c.cols, &a.gate, &a.gate_stride);
         c.as_rows(keep[1], c.cols, &a.up, &a.up_stride);
         if (!c.fine) Py_RETURN_NONE;
@@ -611,7 +624,7 @@ PyObject* py_norm_backward(PyObject*, PyObject* args)
     const at::Tensor arena = THPVariable_Unpack(ao);
     const Arena l(c.rows, c.cols, save == 1 ? (post != 0) + (next != 0) : 0);
     const int post_stats = stats_of(post), next_stats = stats_of(next);
-    if (arena.device() != c.device || arena.numel() != l.size(post_stats + next_stats)) Py_RETURN_NONE;
+    if (!c.kept_bytes(arena, l.size(post_stats + next_stats))) Py_RETURN_NONE;
     void* const q = arena.data_ptr();
     at::Tensor branch, hidden;
     if (save == 1) {
@@ -625,8 +638,11 @@ PyObject* py_norm_backward(PyObject*, PyObject* args)
         }
     } else {
         const void* p = nullptr;
-        if (post) branch = c.as_rows(THPVariable_Unpack(bo), c.cols, &a.branch, &a.branch_stride);
-        if (next) hidden = c.as_rows(THPVariable_Unpack(ho), c.cols, &p, &a.hidden_stride);
+        if (post) branch = THPVariable_Unpack(bo);
+        if (next) hidden = THPVariable_Unpack(ho);
+        if ((post && !c.kept(branch, u_type)) || (next && !c.kept(hidden, type))) Py_RETURN_NONE;
+        if (post) c.as_rows(branch, c.cols, &a.branch, &a.branch_stride);
+        if (next) c.as_rows(hidden, c.cols, &p, &a.hidden_stride);
         a.hidden = const_cast<void*>(p);
         if (!c.fine) Py_RETURN_NONE;
     }
@@ -644,6 +660,8 @@ PyObject* py_norm_backward(PyObject*, PyObject* args)
     for (int i = 0; i < 5; ++i) {
         if (v[i] == Py_None) continue;
         const at::Tensor w = THPVariable_Unpack(v[i]);
+        const int64_t size = (i == 2 ? gates : 1) * c.cols;
+        if (!c.kept(w, w.scalar_type()) || !w.is_contiguous() || w.numel() != size) Py_RETURN_NONE;
         g[2 + i] = at::empty(w.sizes(), c.options(w.scalar_type()));
         if (!w.numel()) continue;
         *vectors[i].p = w.data_ptr();
