@@ -37,7 +37,7 @@ typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 
 // Allows a kernel more than 64 KB of LDS, once on each device (rf_wgrad.hip).
-rf_status allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) noexcept;
+[[nodiscard]] rf_status allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) noexcept;
 
 constexpr int CHUNK = 8;   // columns of a lane
 constexpr int BLOCK = 32;  // columns that share a step: a quad of lanes

@@ -582,7 +582,7 @@ rf_status check_backward(const rf_norm* a)
 }
 
 using forward_t = void (*)(const rf_norm&, const NormShape&, hipStream_t);
-using backward_t = void (*)(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
+using backward_t = rf_status (*)(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
 
 forward_t forward_of(const rf_norm& a)
 {
@@ -676,7 +676,7 @@ rf_status rf_norm_backward(const rf_norm* args, void* workspace, int64_t workspa
     if (workspace_bytes < workspace_of(a, s, p) || (workspace_of(a, s, p) && !workspace)) return bad("workspace too small");
     hipStream_t st = (hipStream_t)stream;
     if (a.rows) {
-        backward_of(a)(a, s, p, (float*)workspace, st);
+        if (const rf_status e = backward_of(a)(a, s, p, (float*)workspace, st); e != RF_OK) return e;
     } else {  // sums over no rows: there are no partial rows
         p.workers = 0;
         p.pieces = 1;

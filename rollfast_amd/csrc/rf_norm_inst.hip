@@ -37,7 +37,7 @@ template <bool EXIT, bool NEXT> static void forward(const rf_norm& a, const Norm
 }
 
 template <bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL>
-static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
+static rf_status backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
 {
     const dim3 grid((unsigned)p.workers), block(s.tpr, s.ny);
     if (s.nv == 1) k_norm_backward<T, U, EXIT, NEXT, FULL, SRC8, TAIL, 1><<<grid, block, s.lds, st>>>(a, p, partial);
@@ -46,30 +46,31 @@ static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, fl
         static std::atomic<uint64_t> done;
         const auto f = k_norm_backward_broad<T, U, EXIT, NEXT, FULL, SRC8, TAIL>;
         constexpr size_t lds = EXIT && NEXT ? 1024 * 2 * 2 * 8 * sizeof(float) : 0;
-        if (allow_lds((const void*)f, lds, done) != RF_OK) return;
+        if (const rf_status e = allow_lds((const void*)f, lds, done); e != RF_OK) return e;
         f<<<grid, block, lds, st>>>(a, p, partial);
     }
+    return RF_OK;
 }
 
 template <bool EXIT, bool NEXT, bool SRC8>
-static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
+static rf_status backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
 {
     if (s.nv == 0) {
         k_norm_backward_wide<T, U, EXIT, NEXT, SRC8><<<dim3((unsigned)p.workers), dim3(s.tpr), 0, st>>>(a, p, partial);
-    } else if (a.cols % CHUNK) {
-        if (s.full) backward<EXIT, NEXT, true, SRC8, true>(a, s, p, partial, st);
-        else backward<EXIT, NEXT, false, SRC8, true>(a, s, p, partial, st);
-    } else {
-        if (s.full) backward<EXIT, NEXT, true, SRC8, false>(a, s, p, partial, st);
-        else backward<EXIT, NEXT, false, SRC8, false>(a, s, p, partial, st);
+        return RF_OK;
     }
+    if (a.cols % CHUNK) {
+        return s.full ? backward<EXIT, NEXT, true, SRC8, true>(a, s, p, partial, st)
+                      : backward<EXIT, NEXT, false, SRC8, true>(a, s, p, partial, st);
+    }
+    return s.full ? backward<EXIT, NEXT, true, SRC8, false>(a, s, p, partial, st)
+                  : backward<EXIT, NEXT, false, SRC8, false>(a, s, p, partial, st);
 }
 
 template <bool EXIT, bool NEXT>
-static void backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
+static rf_status backward(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial, hipStream_t st)
 {
-    if (s.src8) backward<EXIT, NEXT, true>(a, s, p, partial, st);
-    else backward<EXIT, NEXT, false>(a, s, p, partial, st);
+    return s.src8 ? backward<EXIT, NEXT, true>(a, s, p, partial, st) : backward<EXIT, NEXT, false>(a, s, p, partial, st);
 }
 
 #define RFI_CAT2(a, b, c) a##b##_##c
@@ -82,12 +83,12 @@ void RFI_CAT(norm_forward_, RFI_T, RFI_U)(const rf_norm& a, const NormShape& s, 
     else forward<true, true>(a, s, st);
 }
 
-void RFI_CAT(norm_backward_, RFI_T, RFI_U)(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial,
-                                           hipStream_t st)
+rf_status RFI_CAT(norm_backward_, RFI_T, RFI_U)(const rf_norm& a, const NormShape& s, const NormPlan& p, float* partial,
+                                                hipStream_t st)
 {
-    if (a.post == RF_NORM_ABSENT) backward<false, true>(a, s, p, partial, st);
-    else if (a.next == RF_NORM_ABSENT) backward<true, false>(a, s, p, partial, st);
-    else backward<true, true>(a, s, p, partial, st);
+    if (a.post == RF_NORM_ABSENT) return backward<false, true>(a, s, p, partial, st);
+    if (a.next == RF_NORM_ABSENT) return backward<true, false>(a, s, p, partial, st);
+    return backward<true, true>(a, s, p, partial, st);
 }
 
 }  // namespace rfb

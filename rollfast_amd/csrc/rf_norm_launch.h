@@ -18,10 +18,11 @@ void norm_forward_1_1(const rf_norm&, const NormShape&, hipStream_t);
 void norm_forward_2_2(const rf_norm&, const NormShape&, hipStream_t);
 void norm_forward_0_1(const rf_norm&, const NormShape&, hipStream_t);
 void norm_forward_0_2(const rf_norm&, const NormShape&, hipStream_t);
-void norm_backward_0_0(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
-void norm_backward_1_1(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
-void norm_backward_2_2(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
-void norm_backward_0_1(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
-void norm_backward_0_2(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
+// A status other than RF_OK: nothing was launched.
+[[nodiscard]] rf_status norm_backward_0_0(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
+[[nodiscard]] rf_status norm_backward_1_1(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
+[[nodiscard]] rf_status norm_backward_2_2(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
+[[nodiscard]] rf_status norm_backward_0_1(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
+[[nodiscard]] rf_status norm_backward_0_2(const rf_norm&, const NormShape&, const NormPlan&, float*, hipStream_t);
 
 }  // namespace rfb
