@@ -150,7 +150,8 @@ template <int ACT> __device__ __forceinline__ void activation(float x, float& a,
         const float x2 = x * x;
         const float s = sigmoid(1.59576912160573071f * x * fmaf(0.044715f, x2, 1.0f));
         a = x * s;
-        slope = fmaf(x * s * (1.0f - s), 1.59576912160573071f * fmaf(0.134145f, x2, 1.0f), s);
+        // from |x| = 100 on s (1 - s) is zero, beside a square that must not be infinite
+        slope = fmaf(x * s * (1.0f - s), 1.59576912160573071f * fmaf(0.134145f, fminf(x2, 1e4f), 1.0f), s);
     }
 }
 
