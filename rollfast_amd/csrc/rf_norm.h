@@ -581,7 +581,8 @@ __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const No
                         for (int k = 0; k < 8; ++k) {
                             P[j][k] = fmaf(u[j][k], e[j][k], P[j][k]);
                             if constexpr (FULL) Q[j][k] += e[j][k];
-                            o[k] = rstd1 * (FULL ? fmaf(h[j][k], e[j][k], -m0) - u[j][k] * m1 : fmaf(h[j][k], e[j][k], -(u[j][k] * m1)));
+                            const float um = post_norm ? u[j][k] * m1 : 0.0f;  // (m1 is zero without one, u perhaps infinite)
+                            o[k] = rstd1 * (FULL ? fmaf(h[j][k], e[j][k], -m0) - um : fmaf(h[j][k], e[j][k], -um));
                         }
                         put8<TAIL>((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
                     }
@@ -869,7 +870,8 @@ __global__ __launch_bounds__(1024) void k_norm_backward_broad(const rf_norm a, c
                     if constexpr (IN_LDS) add(0, j, k, u[k] * e[k]);
                     else P[j][k] = fmaf(u[k], e[k], P[j][k]);
                     if constexpr (FULL) Q[j][k] += e[k];
-                    o[k] = rstd1 * (FULL ? fmaf(h[k], e[k], -m0) - u[k] * m1 : fmaf(h[k], e[k], -(u[k] * m1)));
+                    const float um = post_norm ? u[k] * m1 : 0.0f;
+                    o[k] = rstd1 * (FULL ? fmaf(h[k], e[k], -m0) - um : fmaf(h[k], e[k], -um));
                 }
                 if (ch < nch) put8<TAIL>((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
             }
@@ -1020,7 +1022,7 @@ __global__ __launch_bounds__(512) void k_norm_backward_wide(const rf_norm a, con
                 }
                 if constexpr (EXIT) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) o[k] = rstd1 * (fmaf(h[k], e[k], -m0) - u[k] * m1);
+                    for (int k = 0; k < 8; ++k) o[k] = rstd1 * (fmaf(h[k], e[k], -m0) - (post_norm ? u[k] * m1 : 0.0f));
                     put8((U*)a.dbranch + r * cols + c, narrow8<U>(o), cols - c);
                 }
             }

@@ -35,3 +35,28 @@ def test_activation_slopes_of_large_values(name, dtype):
     dg, du = rf.gated_activation_grad(dh, saved)
     assert torch.equal(dg, on), dg
     assert torch.equal(du, torch.where(x > 0, dh * x, torch.zeros_like(x))), du
+
+
+@pytest.mark.parametrize("shape", [(3, 5), (9, 40), (5, 301), (4, 1283), (6, 4096), (3, 5000), (4, 9000), (3, 16411)])
+@pytest.mark.parametrize("gate", [None, "one", "rows"])
+@pytest.mark.parametrize("save", ["int8", "input"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_branch_that_is_not_finite_without_a_norm(shape, gate, save, dtype):
+    """norm='none': the gradients at the branch and the residual do not depend
+    on the branch's values, so an Inf or NaN in it changes neither; the gate's
+    does, in the columns of its checkpoint's block at most."""
+    rows, cols = shape
+    r, u, dout = (rand(rows, cols, dtype=dtype, seed=i) for i in range(3))
+    g = None if gate is None else rand(cols, seed=3) if gate == "one" else rand(rows, cols, seed=3)
+    u[0, 1], u[1, cols - 1], u[2, cols // 2] = math.inf, -math.inf, math.nan
+    out, _, saved = rf.postnorm_residual(r, u, gate=g, norm="none", branch_scale=0.5, residual_scale=2.0, save=save)
+    got = rf.postnorm_residual_grad(dout, None, saved)
+    assert torch.equal(got.residual, 2 * dout)
+    ref = 0.5 * dout.double() * (1.0 if g is None else g.double())
+    half = U if dtype == F32 else 2.0 ** -8
+    off = (got.branch.double() - ref).abs()
+    assert (off <= 1.01 * (half + U) * ref.abs()).all()  # one product in f32, rounded once
+    if g is not None:
+        block = torch.arange(cols) // 32
+        hit = (block == 0) | (block == (cols - 1) // 32) | (block == cols // 2 // 32)
+        assert torch.isfinite(got.gate[..., ~hit]).all()
