@@ -130,25 +130,31 @@ __global__ __launch_bounds__(256) void k_checkpoint_load(const int8_t* __restric
     }
 }
 
-__device__ __forceinline__ float sigmoid(float x)
+// exp and 1 / (1 + exp(-x)).  FULL (f32 tensors): within an ulp.  Else the native
+// exponential of the rounded product x log2(e), off by |x| 2^-24 of its value, and
+// the native reciprocal: far below the rounding of a 16-bit result.
+template <bool FULL> __device__ __forceinline__ float exponential(float x) { return FULL ? expf(x) : __expf(x); }
+
+template <bool FULL> __device__ __forceinline__ float sigmoid(float x)
 {
-    return __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+    const float d = 1.0f + exponential<FULL>(-x);
+    return FULL ? 1.0f / d : __builtin_amdgcn_rcpf(d);
 }
 
 // a(x) and a'(x).  The tanh form is x sigmoid(2 z), z = sqrt(2 / pi) (x + 0.044715 x^3).
-template <int ACT> __device__ __forceinline__ void activation(float x, float& a, float& slope)
+template <int ACT, bool FULL> __device__ __forceinline__ void activation(float x, float& a, float& slope)
 {
     if constexpr (ACT == RF_ACT_SILU) {
-        const float s = sigmoid(x);
+        const float s = sigmoid<FULL>(x);
         a = x * s;
         slope = s * fmaf(x, 1.0f - s, 1.0f);
     } else if constexpr (ACT == RF_ACT_GELU) {
         const float phi = fmaf(0.5f, erff(x * 0.70710678118654752f), 0.5f);
         a = x * phi;
-        slope = fmaf(x * 0.39894228040143268f, __expf(-0.5f * x * x), phi);
+        slope = fmaf(x * 0.39894228040143268f, exponential<FULL>(-0.5f * x * x), phi);
     } else {
         const float x2 = x * x;
-        const float s = sigmoid(1.59576912160573071f * x * fmaf(0.044715f, x2, 1.0f));
+        const float s = sigmoid<FULL>(1.59576912160573071f * x * fmaf(0.044715f, x2, 1.0f));
         a = x * s;
         // from |x| = 100 on s (1 - s) is zero, beside a square that must not be infinite
         slope = fmaf(x * s * (1.0f - s), 1.59576912160573071f * fmaf(0.134145f, fminf(x2, 1e4f), 1.0f), s);
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(256) void k_gated_forward(const rf_gated a, uint32_
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float s;
-            activation<ACT>(x[k], h[k], s);
+            activation<ACT, sizeof(T) == 4>(x[k], h[k], s);
             h[k] *= y[k];
         }
         const Raw<T> hr = narrow8<T>(h);
@@ -234,7 +240,7 @@ __global__ __launch_bounds__(256) void k_gated_backward(const rf_gated a, uint32
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             float v, s;
-            activation<ACT>(x[k], v, s);
+            activation<ACT, sizeof(T) == 4>(x[k], v, s);
             x[k] = dh[k] * y[k] * s;
             y[k] = dh[k] * v;
         }

@@ -37,6 +37,27 @@ def test_activation_slopes_of_large_values(name, dtype):
     assert torch.equal(du, torch.where(x > 0, dh * x, torch.zeros_like(x))), du
 
 
+def test_silu_keeps_f32s_digits():
+    """f32's SiLU and its slope in relative terms, on the negative tail too.
+    exp is within an ulp (2 U), 1 + e and the quotient within U each, the two
+    products within U each, which is 6 U for h and for dup; the slope adds the
+    difference, the fused product and, by its condition |x| / (|x| - 1) <= 4 / 3
+    for x <= -4, a third of what came before: below 12 U.  16 U for all.  On the
+    positive side the slope's s is off by 1.5 U of 1 and 1 - s by as much, which
+    x (1 - s) multiplies by x, up to the x of about 17 where s is 1: 2 U x more."""
+    x = torch.cat((torch.linspace(-80, -4, 4001), torch.linspace(4, 80, 4001))).cuda()[None]
+    up, dh = rand(1, 8002, seed=1) + 3.0, rand(1, 8002, seed=2) - 4.0
+    h, saved = rf.gated_activation(x, up, save="input")
+    dg, du = rf.gated_activation_grad(dh, saved)
+    x64, u64, d64 = x.double(), up.double(), dh.double()
+    s = 1 / (1 + torch.exp(-x64))
+    for got, ref, what in ((h, x64 * s * u64, "h"), (du, d64 * x64 * s, "dup"),
+                           (dg, d64 * u64 * s * (1 + x64 * (1 - s)), "dgate")):
+        off = ((got.double() - ref) / ref).abs()
+        bound = 16 * U + (2 * U * x64.clamp(0, 18) if what == "dgate" else 0)
+        assert (off <= bound).all(), (what, (off.max() / U).item(), x.flatten()[off.argmax()].item())
+
+
 @pytest.mark.parametrize("shape", [(3, 5), (9, 40), (5, 301), (4, 1283), (6, 4096), (3, 5000), (4, 9000), (3, 16411)])
 @pytest.mark.parametrize("gate", [None, "one", "rows"])
 @pytest.mark.parametrize("save", ["int8", "input"])
