@@ -26,12 +26,17 @@ def _wanted(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _stash(ctx, saved):
+def _stash(ctx, saved, out=None):
     """Moves saved's tensors to save_for_backward (which also notices a write
-    to one of them before the backward pass)."""
+    to one of them before the backward pass).  ``out``: the output whose rows
+    ``hidden_rows`` are.  It is saved itself: a view would hold the output, the
+    output its graph, and the graph the view, so that an output dropped without
+    a backward pass would never be freed."""
     ctx.set_materialize_grads(False)  # no zeros for the checkpoint's buffers
     vectors = getattr(saved, "vectors", ())
     rows = [n for n in saved.__slots__ if n == "arena" or n.endswith("_rows")]
+    if out is not None and saved.hidden_rows is not None:
+        saved.hidden_rows = out
     ctx.save_for_backward(*vectors, *(getattr(saved, n) for n in rows))
     ctx.rest = {n: getattr(saved, n) for n in saved.__slots__ if n not in rows and n not in ("vectors", "output")}
     ctx.rows, ctx.kind = rows, type(saved)
@@ -93,7 +98,7 @@ class _Postnorm(torch.autograd.Function):
     def forward(ctx, residual, branch, weight, bias, gate, next_weight, next_bias, options):
         out, y, saved = blocks.postnorm_residual(residual, branch, weight, bias, gate, next_weight=next_weight,
                                                  next_bias=next_bias, **options)
-        _stash(ctx, saved)
+        _stash(ctx, saved, out)
         return _with_output(ctx, (out, y), saved)
 
     @staticmethod
