@@ -157,6 +157,19 @@ def gated_activation(gate, up=None, *, activation="silu", save="int8", checkpoin
     return (h, _checkpoint(codes, exps, h)) if checkpoint_output else h
 
 
+def _product(x, weight, bias):
+    """torch's linear with autocast's casts, but without its cache: that keeps a
+    weight's for the rest of the region, and one made inside a Function's
+    forward pass has no graph."""
+    device = x.device.type
+    if not torch.is_autocast_enabled(device):
+        return torch.nn.functional.linear(x, weight, bias)
+    dtype = torch.get_autocast_dtype(device)
+    with torch.autocast(device, enabled=False):
+        return torch.nn.functional.linear(*(t if t is None or t.dtype == torch.float64 else t.to(dtype)
+                                            for t in (x, weight, bias)))
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, checkpoint):
@@ -168,7 +181,7 @@ class _Linear(torch.autograd.Function):
             if tuple(kept.shape) != ctx.shape:
                 raise ValueError(f"the checkpoint stands for {tuple(kept.shape)}, x has shape {ctx.shape}")
         ctx.save_for_backward(weight, kept[0], kept[1])
-        return torch.nn.functional.linear(x, weight, bias)
+        return _product(x, weight, bias)
 
     @staticmethod
     @once_differentiable
@@ -176,8 +189,8 @@ class _Linear(torch.autograd.Function):
         weight, codes, exps = ctx.saved_tensors
         dx = dw = db = None
         flat = dy.reshape(-1, dy.shape[-1])
-        if ctx.needs_input_grad[0]:
-            dx = (flat @ weight).view(ctx.shape)
+        if ctx.needs_input_grad[0]:  # in the product's dtype, which autocast may have chosen
+            dx = (flat @ weight.to(dy.dtype)).view(ctx.shape).to(ctx.dtype)
         if ctx.needs_input_grad[1]:
             dw = blocks.linear_weight_grad(dy, ActivationCheckpoint(codes, exps, ctx.shape, ctx.dtype),
                                            dtype=weight.dtype)
@@ -189,5 +202,6 @@ class _Linear(torch.autograd.Function):
 def linear(x, weight, bias=None, *, checkpoint=None):
     """``x @ weight.T + bias`` whose weight gradient reads x from 8 bits:
     from ``checkpoint`` where one was made with x, else from one made here.
-    The products with the weight are the library's."""
+    The products with the weight are the library's, under autocast in its
+    dtype; the weight's gradient has the weight's."""
     return _Linear.apply(x, weight, bias, checkpoint)
