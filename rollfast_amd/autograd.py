@@ -204,4 +204,6 @@ def linear(x, weight, bias=None, *, checkpoint=None):
     from ``checkpoint`` where one was made with x, else from one made here.
     The products with the weight are the library's, under autocast in its
     dtype; the weight's gradient has the weight's."""
+    if not _wanted(x, weight, bias):
+        return torch.nn.functional.linear(x, weight, bias)
     return _Linear.apply(x, weight, bias, checkpoint)

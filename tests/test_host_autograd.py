@@ -29,3 +29,14 @@ def test_linear_under_autocast(dtype):
         grads.append((y, x.grad))
     assert grads[0][1].dtype == torch.float32
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+def test_linear_keeps_nothing_where_no_gradient_is_wanted(monkeypatch):
+    def made(x):
+        raise AssertionError("a checkpoint was made")
+
+    monkeypatch.setattr(blocks, "checkpoint_activations", made)
+    x, w, b = rand(5, 7), torch.nn.Parameter(rand(3, 7, seed=1)), torch.nn.Parameter(rand(3, seed=2))
+    with torch.no_grad():
+        assert torch.equal(ag.linear(x, w, b), torch.nn.functional.linear(x, w, b))
+    assert torch.equal(ag.linear(x, w.detach()), torch.nn.functional.linear(x, w.detach()))
