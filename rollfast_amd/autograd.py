@@ -26,6 +26,11 @@ def _wanted(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _check_save(save):
+    if save not in ("int8", "input"):
+        raise ValueError(f"save must be 'int8' or 'input' where a gradient is wanted, got {save!r}")
+
+
 def _stash(ctx, saved, out=None):
     """Moves saved's tensors to save_for_backward (which also notices a write
     to one of them before the backward pass).  ``out``: the output whose rows
@@ -89,6 +94,7 @@ def prenorm(x, weight=None, bias=None, *, norm="rms", eps=1e-6, dtype=None, save
     if not _wanted(x, weight, bias):
         y = blocks.prenorm(x, weight, bias, save=None, **options)[0]
         return (y, None) if checkpoint_output else y
+    _check_save(save)
     y, codes, exps = _Prenorm.apply(x, weight, bias, {**options, "save": save, "checkpoint_output": checkpoint_output})
     return (y, _checkpoint(codes, exps, y)) if checkpoint_output else y
 
@@ -123,6 +129,7 @@ def postnorm_residual(residual, branch, weight=None, bias=None, gate=None, *, no
                                              next_bias=next_bias, save=None, **options)
         kept = None
     else:
+        _check_save(save)
         options |= {"save": save, "checkpoint_output": checkpoint_output}
         out, y, codes, exps = _Postnorm.apply(residual, branch, weight, bias, gate, next_weight, next_bias, options)
         kept = None if codes is None else _checkpoint(codes, exps, y)
@@ -152,6 +159,7 @@ def gated_activation(gate, up=None, *, activation="silu", save="int8", checkpoin
     if not _wanted(gate, up):
         h = blocks.gated_activation(gate, up, activation=activation, save=None)[0]
         return (h, None) if checkpoint_output else h
+    _check_save(save)
     h, codes, exps = _Gated.apply(gate, up, {"activation": activation, "save": save,
                                              "checkpoint_output": checkpoint_output})
     return (h, _checkpoint(codes, exps, h)) if checkpoint_output else h

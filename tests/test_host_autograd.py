@@ -40,3 +40,11 @@ def test_linear_keeps_nothing_where_no_gradient_is_wanted(monkeypatch):
     with torch.no_grad():
         assert torch.equal(ag.linear(x, w, b), torch.nn.functional.linear(x, w, b))
     assert torch.equal(ag.linear(x, w.detach()), torch.nn.functional.linear(x, w.detach()))
+
+
+def test_gradients_need_something_kept():
+    x = rand(4, 8).requires_grad_(True)
+    for call in (lambda: ag.prenorm(x, save=None), lambda: ag.postnorm_residual(x, x, save=None),
+                 lambda: ag.gated_activation(x, x, save=None)):
+        with pytest.raises(ValueError, match="save must be 'int8' or 'input'"):
+            call()
