@@ -84,6 +84,8 @@ class _Prenorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, *_):
+        if dy is None:  # what used y gave no gradient
+            return (None,) * 4
         return (*blocks.prenorm_grad(dy, _unstash(ctx)), None)
 
 
@@ -110,6 +112,8 @@ class _Postnorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dy, *_):
+        if dout is None and dy is None:
+            return (None,) * 8
         saved = _unstash(ctx)
         if dy is None and saved.meta[2]:  # y was not used
             dy = torch.zeros(saved.shape, dtype=saved.branch_dtype, device=saved.arena.device)
@@ -148,6 +152,8 @@ class _Gated(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, *_):
+        if dh is None:
+            return (None,) * 3
         saved = _unstash(ctx)
         grads = blocks.gated_activation_grad(dh, saved)
         return (grads, None, None) if saved.fused else (*grads, None)

@@ -124,3 +124,26 @@ def test_a_block_under_autocast_trains():
         got = grads()
     for name, a, b in zip(["x", *p], got, ref):
         assert a.dtype == F32 and (a - b).norm() <= 0.05 * b.norm(), (name, ((a - b).norm() / b.norm()).item())
+
+
+class NoGradient(torch.autograd.Function):
+    """Passes its input on, and no gradient back."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x * 1
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def test_outputs_without_a_gradient():
+    """No gradient comes back through an output: none goes on."""
+    x, w = rand(9, 40).requires_grad_(True), rand(40, seed=1).requires_grad_(True)
+    for f in (lambda t: ag.prenorm(t, w), lambda t: ag.gated_activation(t, t),
+              lambda t: ag.postnorm_residual(t, t, w),
+              lambda t: sum(ag.postnorm_residual(t, t, w, next_norm="rms")), lambda t: ag.linear(t, w[None] * 1)):
+        x.grad = w.grad = None
+        (NoGradient.apply(f(x)).sum() + x.sum()).backward()
+        assert torch.equal(x.grad, torch.ones_like(x)) and (w.grad is None or not w.grad.any())
