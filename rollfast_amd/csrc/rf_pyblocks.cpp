@@ -383,6 +383,8 @@ PyObject* py_weight_grad(PyObject*, PyObject* args)
     if (size) space = c.bytes(size);
     call(c, "linear_weight_grad",
          [&](void* s) { return g_lib.weight_grad(&a, size ? space.data_ptr() : nullptr, size, s); });
+    // a write that autograd must notice where it has kept `out` (inference tensors have no version)
+    if (oo != Py_None && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
     return oo != Py_None ? Py_NewRef(oo) : THPVariable_Wrap(out);
     RFB_END
 }

@@ -147,3 +147,22 @@ def test_outputs_without_a_gradient():
         x.grad = w.grad = None
         (NoGradient.apply(f(x)).sum() + x.sum()).backward()
         assert torch.equal(x.grad, torch.ones_like(x)) and (w.grad is None or not w.grad.any())
+
+
+def test_main_gradient_written_is_noticed():
+    """linear_weight_grad writes `out` in place, and says so to autograd."""
+    x, dy = rand(20, 64, dtype=BF16), rand(20, 32, dtype=BF16, seed=1)
+    kept = blocks.checkpoint_activations(x)
+    main = torch.zeros(32, 64, device="cuda")
+    a = rand(32, 64, seed=2).requires_grad_(True)
+    for accumulate in (False, True):
+        y = (a * main).sum()
+        version = main._version
+        assert blocks.linear_weight_grad(dy, kept, out=main, accumulate=accumulate) is main
+        assert main._version > version
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        other = torch.zeros(32, 64, device="cuda")
+    blocks.linear_weight_grad(dy, kept, out=other)
+    assert torch.equal(other, blocks.linear_weight_grad(dy, kept, dtype=F32))
