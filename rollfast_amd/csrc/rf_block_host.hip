@@ -78,8 +78,8 @@ template <int ROWS> __device__ __forceinline__ Place place(uint32_t across)
 }
 
 // One walk: a quad of lanes has a block of 32, whose largest magnitude takes two
-// exchanges in the quad.  Bound by memory: 16384 x 11008 bf16 116 us (4.7 TB/s of
-// reads and writes), 3001 x 769 f32 6.1, most of it latency.
+// exchanges in the quad.  Bound by memory: 16384 x 11008 bf16 96 us (5.7 TB/s of
+// reads and writes), 3001 x 769 f32 6.2, most of it latency.
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void k_checkpoint_store(const T* __restrict__ x, int64_t rows, int64_t cols,
                                                           int64_t stride, int8_t* __restrict__ codes,
@@ -103,8 +103,9 @@ __global__ __launch_bounds__(256) void k_checkpoint_store(const T* __restrict__ 
     }
 }
 
-// Bound by memory: 16384 x 11008 bf16 89 us (6.1 TB/s; the codes, just written,
-// come from the last-level cache in part).
+// Bound by memory: 16384 x 11008 bf16 123 us (4.4 TB/s) where other work lies between
+// store and load, as in a training step; 89 us right after the store, the codes in
+// part from the last-level cache.
 // STREAM: an output that the last-level cache cannot hold beside the codes is
 // stored past it, so that its lines need not be written back in front of what
 // comes next.  Store and load in turn, us with and without: 16384 x 11008 bf16
@@ -162,8 +163,8 @@ template <int ACT, bool FULL> __device__ __forceinline__ void activation(float x
 }
 
 // h = a(gate) up; the checkpoints of gate, up and (rounded) h are written in the
-// same pass.  Bound by memory: 16384 x 11008 bf16 with those of gate and up 261 us
-// (5.6 TB/s).
+// same pass.  Bound by memory: 16384 x 11008 bf16 with those of gate and up 265 us
+// (5.5 TB/s).
 template <typename T, int ACT, int ROWS>
 __global__ __launch_bounds__(256) void k_gated_forward(const rf_gated a, uint32_t across)
 {
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(256) void k_gated_forward(const rf_gated a, uint32_
 }
 
 // dgate = dh up a'(gate), dup = dh a(gate), a and a' computed again from what was
-// kept.  Bound by memory: 16384 x 11008 bf16 from 8 bits 257 us (5.7 TB/s).
+// kept.  Bound by memory: 16384 x 11008 bf16 from 8 bits 260 us (5.6 TB/s).
 template <typename T, int ACT, bool SRC8, int ROWS>
 __global__ __launch_bounds__(256) void k_gated_backward(const rf_gated a, uint32_t across)
 {
@@ -337,7 +338,9 @@ constexpr size_t MAX_LDS = 64 * 1024;
 // - one chunk a lane, or two: forward 16384 x 4096 bf16 122 / 128, 8192 x 768
 //   14.3 / 13.9 (two chunks in one wave need no barrier); backward in 16 bits,
 //   16384 x 4096 LayerNorm 298 / 194, 20000 x 1280 76 / 68; backward in f32,
-//   2317 x 1283 LayerNorm 25 / 39 (two chunks spill).
+//   2317 x 1283 LayerNorm 25 / 39 (two chunks spill).  Rows of more than 4096
+//   columns have more than 512 chunks and so two a lane in every type, f32's
+//   backward with its spills among them (figures in rf_norm.h).
 // - threads a CU: forward 16384 x 4096 157 / 122 / 126 with 512 / 1024 / 2048;
 //   backward 158 / 173 with 512 / 768 (more partial rows to write and add);
 //   forward 2317 x 1283 f32 18.3 with 1365 workgroups of 192, which do not fit

@@ -1,8 +1,15 @@
 // rf_norm.h -- the norms around a block: forward and backward kernels.
 //
-// Rows of up to 16384 columns stay in registers from their one load to their
-// last use (two chunks of eight columns per lane at most, 64 to 1024 lanes a
-// row); wider rows are walked again by the lanes that loaded them (k_*_wide).
+// Rows of up to 16384 columns are loaded once and kept, as loaded, in registers
+// (two chunks of eight columns per lane at most, 64 to 1024 lanes a row); wider
+// rows are walked again by the lanes that loaded them (k_*_wide).  What is computed
+// from a row stays in registers too, except where both norms meet and a lane has
+// two chunks.  There the compiler spills, registers a lane:
+//   k_norm_backward        RMS/RMS   16-bit 0 to 51, f32 14 to 69
+//                          LayerNorm 16-bit 36 to 120, f32 56 to 188
+//   k_norm_backward_broad  RMS/RMS   16-bit 10 to 16, f32 15 to 73
+//                          LayerNorm 16-bit 46 to 84, f32 53 to 179
+//   k_norm_forward of 1024 lanes, LayerNorm 16-bit 37 to 85, f32 97 to 129
 // The parameter vectors' gradients are sums over rows: a workgroup adds its
 // own rows in registers and writes one partial row, k_norm_finish adds the
 // partial rows in their order.  No atomics: the same inputs give the same bits.
@@ -90,11 +97,12 @@ __device__ __forceinline__ const void* gate_row(const rf_norm& a, int64_t g)
 // Variances are taken around the mean in a second walk of the registers: a sum of
 // squares alone loses the digits that a large mean shares.
 // Bound by memory where there are rows enough: 16384 x 4096 bf16, post and next
-// RMSNorm with both checkpoints, 133 us (5.1 TB/s).  Else by the way of one row
-// through load, sums and barriers: 8192 x 768 11.3 us, 4 x 4096 with one norm 2.8,
-// with both 4.9.
-// LANES: 1024 for rows of more than 8192 columns.  8192 x 16384 bf16, one norm 112 us,
-// both 200 (k_norm_forward_wide 182, 367).
+// RMSNorm with both checkpoints, 132 us (5.1 TB/s).  Else by the way of one row
+// through load, sums and barriers: 8192 x 768 11.5 us, 4 x 4096 with one norm 2.8,
+// with both 4.8.
+// LANES: 1024 for rows of more than 8192 columns.  8192 x 16384 bf16 without
+// checkpoints, the next norm alone 105 us, both 212 (k_norm_forward_wide 182, 367);
+// with them 132 and 253.
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool TAIL, int NV, int LANES>
 __global__ __launch_bounds__(LANES) void k_norm_forward(const rf_norm a, const Share share, const uint32_t group_rows)
 {
@@ -400,9 +408,11 @@ template <typename T, bool WIDE, bool TAIL> struct Saved<T, true, WIDE, TAIL> {
 // Past the end of a row dy, dhidden and h are zero, so xhat and uhat may be
 // anything finite there.
 // FULL: LayerNorm or a bias somewhere (the sums of g, t and their columns).
-// Bound by memory: 16384 x 4096 bf16, both norms, from 8 bits 157 us (4.3 TB/s; the
+// Bound by memory: 16384 x 4096 bf16, both norms, from 8 bits 158 us (4.3 TB/s; the
 // chip's mix of reads and writes); small calls by the few rows that a lane has to
-// hide its loads behind: 8192 x 768 14.9 us, 2317 x 1283 f32 LayerNorm 23.8.
+// hide its loads behind: 8192 x 768 15.4 us, 2317 x 1283 f32 LayerNorm 23.6.
+// LayerNorms on both sides, which spill most, take 231 us for 8192 x 8192 bf16
+// (RMSNorms 156) and 90 for 2048 x 5120 f32 (46).
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL, int NV>
 __global__ __launch_bounds__(512) void k_norm_backward(const rf_norm a, const NormPlan plan, float* __restrict__ partial)
 {
@@ -696,10 +706,11 @@ __device__ __forceinline__ void forget(Codes& r) { asm volatile("" : "+v"(r.c), 
 // trips to memory for what it takes to stream it.  With both norms two of the
 // column sums lie in LDS: in registers they were spilled, by all CUs together more
 // than the L2 caches hold.
-// Bound by memory for one norm: 8192 x 16384 bf16 from 8 bits 228 us (4.1 TB/s; 775
-// with k_norm_backward_wide); with both norms by the second reading of the values
-// too: 431 (1452 with the wide kernel, 865 with all sums in registers; LDS atomics
-// instead of loads and stores 1476).
+// Bound by memory for one norm: 8192 x 16384 bf16 from 8 bits 204 us (next norm) and
+// 233 (post norm; 4.1 TB/s; 775 with k_norm_backward_wide); with both norms by the
+// second reading of the values too: 399 (1452 with the wide kernel, 865 with all sums
+// in registers; LDS atomics instead of loads and stores 1476).  LayerNorms on both
+// sides: 8192 x 12288 643 us, RMSNorms 332.
 template <typename T, typename U, bool EXIT, bool NEXT, bool FULL, bool SRC8, bool TAIL>
 __global__ __launch_bounds__(1024) void k_norm_backward_broad(const rf_norm a, const NormPlan plan,
                                                               float* __restrict__ partial)

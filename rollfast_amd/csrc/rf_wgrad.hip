@@ -4,7 +4,8 @@
 // A code times its power-of-two step is exact in bf16, and dy is the sum of
 // bf16 pieces (bf16: itself; f16, 11 bits: two; f32, 24 bits: three of 8 bits
 // each, cut off, not rounded), so every product that the matrix cores form is
-// exact and only the f32 sums round.
+// exact and only the f32 sums round.  (Bits of an f32 gradient below 2^-133, bf16's
+// least, are dropped: gradients under 2^-109, about 1.5e-33, lose their last ones.)
 //
 // Both operands have the summed index t along the rows, while the matrix
 // instructions want each lane to hold eight t of one column.  The transpose is
@@ -149,7 +150,9 @@ template <bool LAST, typename Even, typename Odd> __device__ __forceinline__ voi
 
 // Writes a wave's accumulators, columns from k and outputs from n on: a lane
 // holds four neighbouring columns of an output's row.  `partial`: this split's
-// sums, or null for the result.
+// sums, or null for the result.  f32 sums and plain bf16 results go as one vector;
+// accumulation into 16 bits and f16 results element by element, which costs short
+// sums: 512 x 11008 x 4096 into bf16 213 us, into f32 105.
 template <int FK, int FN>
 __device__ __forceinline__ void store_tile(const rf_weight_grad& a, float* __restrict__ partial, const f32x4 (&acc)[FK][FN],
                                            int64_t k_from, int64_t n_from)
@@ -209,8 +212,8 @@ struct StagedX { uint32_t c[8], e[2]; };  // codes of the rows, exponents of row
 // EDGE: dy's rows are no multiple of four elements.
 //
 // Bound by the matrix cores' instruction slots, which the staging shares: f16 (two
-// pieces) 8192 x 4096 x 4096 668 us (411 TFLOP/s, 823 of products), f32 1235 us (223,
-// 668); short sums by the way through one step: 1001 x 517 x 301 f32 13.6 us.
+// pieces) 8192 x 4096 x 4096 657 us (419 TFLOP/s, 837 of products), f32 1231 us (223,
+// 670); short sums by the way through one step: 1001 x 517 x 301 f32 13.9 us.
 template <typename T, int TILE, int WAVES_K, int WAVES_N, bool EDGE>
 __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) void k_wgrad(const rf_weight_grad a,
                                                                                            float* __restrict__ partial,
@@ -476,7 +479,7 @@ __global__ __launch_bounds__(WAVES_K* WAVES_N* WAVE, Pieces<T>::n < 3 ? 2 : 1) v
 // of a transposed read lie in different banks.
 //
 // Measured beside k_wgrad (us): 16384 x 11008 x 4096 1389 / 1495, 8192 x 2304 x 768
-// (eight splits) 41 / 42.  At 1389 us, 1.06 PFLOP/s, the matrix cores are busy 43 %
+// (eight splits) 41 / 42.  At 1379 us, 1.07 PFLOP/s, the matrix cores are busy 45 %
 // of the cycles; 688 tiles on 256 CUs leave the last of three rounds two thirds full.
 //
 // The compiler must not count or order these loads (it would wait for all of
