@@ -577,6 +577,45 @@ RF_API rf_status rf_linear_weight_grad_workspace(const rf_weight_grad* args, int
 RF_API rf_status rf_linear_weight_grad(const rf_weight_grad* args, void* workspace, int64_t workspace_bytes,
                                        void* stream);
 
+/* Softmax cross entropy over a large vocabulary: the logits of a token are the
+ * products of its row of hidden_rows [tokens, hidden] with the rows of weight
+ * [vocab, hidden], and with lse the log of the sum of their exponentials
+ *   loss[t] = lse - logit[target] + z_loss lse^2      (f32).
+ * A token whose target is ignore_index has a loss of 0 and no part in the
+ * gradients, whatever its row holds; one whose target is another number outside
+ * 0 .. vocab - 1 has a loss of NaN, and makes its gradients NaN.
+ * A reduction writes the sum or the mean of the losses of the tokens that count
+ * to `total` (the mean of none is NaN).  With dhidden [tokens, hidden] and dweight
+ * [vocab, hidden], dense, of `dtype`, the gradients are written too (rows of zeros
+ * for ignored tokens): those of total, or without a reduction of
+ * sum_t dloss[t] loss[t].  Products are of the tensors' own 16-bit values, or of
+ * f32 ones to 22 bits; sums are f32. */
+#define RF_REDUCE_NONE 0
+#define RF_REDUCE_SUM 1
+#define RF_REDUCE_MEAN 2
+typedef struct rf_cross_entropy {
+    int64_t tokens, vocab, hidden;
+    int32_t dtype;             /* hidden_rows, weight and their gradients */
+    int32_t target_bits;       /* 32 or 64 */
+    const void* hidden_rows;
+    const void* weight;
+    int64_t hidden_stride, weight_stride; /* elements between rows */
+    const void* targets;       /* [tokens] */
+    int64_t ignore_index;
+    float* loss;               /* [tokens] */
+    float* total;              /* one value; with a reduction */
+    const float* dloss;        /* [tokens]; gradients without a reduction */
+    void* dhidden;             /* NULL, both: the loss alone */
+    void* dweight;
+    float z_loss;
+    int32_t reduction;         /* RF_REDUCE_* */
+} rf_cross_entropy;
+
+/* Bytes of device workspace (256-byte aligned) on the current device. */
+RF_API rf_status rf_linear_cross_entropy_workspace(const rf_cross_entropy* args, int64_t* bytes);
+RF_API rf_status rf_linear_cross_entropy(const rf_cross_entropy* args, void* workspace, int64_t workspace_bytes,
+                                         void* stream);
+
 /* Host-side: the 256 f32 values of a dynamic codebook (adam8.py:461-503). */
 RF_API rf_status rf_codebook(int32_t quantizer, float* out256);
 

@@ -59,13 +59,18 @@ _BLOCKS = (
     "restore_activations",
 )
 
+# The vocabulary loss (losses.py), likewise.
+_LOSSES = ("LossGrads", "linear_cross_entropy", "linear_cross_entropy_grad")
+
 
 def __getattr__(name):
     import importlib
 
     if name in _BLOCKS:
         value = getattr(importlib.import_module(".blocks", __name__), name)
-    elif name in ("autograd", "blocks"):
+    elif name in _LOSSES:
+        value = getattr(importlib.import_module(".losses", __name__), name)
+    elif name in ("autograd", "blocks", "losses"):
         value = importlib.import_module("." + name, __name__)
     else:
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
@@ -83,6 +88,7 @@ __all__ = (
     "GlobalNormClipState",
     "GradientTransformation",
     "GradientTransformationExtraArgs",
+    "LossGrads",
     "MaskedNode",
     "MaskedState",
     "MultiSteps",
@@ -112,7 +118,10 @@ __all__ = (
     "estimate_quantized_moment_bytes",
     "gated_activation",
     "gated_activation_grad",
+    "linear_cross_entropy",
+    "linear_cross_entropy_grad",
     "linear_weight_grad",
+    "losses",
     "masked",
     "multi_transform",
     "postnorm_residual",

@@ -37,6 +37,7 @@ RF_LEAF_SCALE_F16 = 16
 RF_ACC_SUM, RF_ACC_MEAN, RF_ACC_ZERO = 0, 1, 2
 RF_NOALLOC_SCRATCH_BYTES = 8 << 20
 RF_ACT_SILU, RF_ACT_GELU, RF_ACT_GELU_TANH = 0, 1, 2
+RF_REDUCE_NONE, RF_REDUCE_SUM, RF_REDUCE_MEAN = 0, 1, 2
 RF_NORM_ABSENT, RF_NORM_NONE, RF_NORM_RMS, RF_NORM_LAYER = 0, 1, 2, 3
 
 _p = ctypes.c_void_p
@@ -195,6 +196,20 @@ class WeightGrad(ctypes.Structure):
     ]
 
 
+class CrossEntropy(ctypes.Structure):
+    _fields_ = [
+        *((n, _i64) for n in ("tokens", "vocab", "hidden")),
+        *((n, _i32) for n in ("dtype", "target_bits")),
+        *((n, _p) for n in ("hidden_rows", "weight")),
+        *((n, _i64) for n in ("hidden_stride", "weight_stride")),
+        ("targets", _p),
+        ("ignore_index", _i64),
+        *((n, _p) for n in ("loss", "total", "dloss", "dhidden", "dweight")),
+        ("z_loss", ctypes.c_float),
+        ("reduction", _i32),
+    ]
+
+
 assert ctypes.sizeof(Adam8Leaf) == 120
 assert ctypes.sizeof(Adam8Hparams) == 128
 assert ctypes.sizeof(Adam8Group) == 32
@@ -233,6 +248,8 @@ EXPORTS = (
     "rf_norm_backward",
     "rf_linear_weight_grad_workspace",
     "rf_linear_weight_grad",
+    "rf_linear_cross_entropy_workspace",
+    "rf_linear_cross_entropy",
     "rf_codebook",
     "rf_host_table_codes",
     "rf_host_search_index",
@@ -291,6 +308,8 @@ def lib() -> ctypes.CDLL:
     L.rf_norm_backward.argtypes = [ctypes.POINTER(Norm), _p, i64, _p]
     L.rf_linear_weight_grad_workspace.argtypes = [ctypes.POINTER(WeightGrad), ctypes.POINTER(i64)]
     L.rf_linear_weight_grad.argtypes = [ctypes.POINTER(WeightGrad), _p, i64, _p]
+    L.rf_linear_cross_entropy_workspace.argtypes = [ctypes.POINTER(CrossEntropy), ctypes.POINTER(i64)]
+    L.rf_linear_cross_entropy.argtypes = [ctypes.POINTER(CrossEntropy), _p, i64, _p]
     L.rf_codebook.argtypes = [i32, _p]
     L.rf_host_table_codes.argtypes = [i32, u32, i64, _p]
     L.rf_host_search_index.argtypes = [i32, u32, i64, _p]
@@ -344,7 +363,7 @@ def pyblocks():
 
         L = lib()
         mod = _host_module("_rfblocks")
-        names = [n for n in EXPORTS if n.startswith(("rf_checkpoint_", "rf_gated_", "rf_norm_", "rf_linear_"))]
+        names = [n for n in EXPORTS if n.startswith(("rf_checkpoint_", "rf_gated_", "rf_norm_", "rf_linear_weight_"))]
         mod.set_entries({n: ctypes.cast(getattr(L, n), _p).value for n in (*names, "rf_last_error")},
                         torch._C._cuda_getCurrentRawStream, torch.nn.Parameter)
         _pyblocks = mod

@@ -1,0 +1,284 @@
+// rf_product.h -- the matrix product that the vocabulary loss and the
+// orthogonalisation are made of: a workgroup's tile of
+//   out[q, p] = sum over k of P[p, k] Q[q, k],
+// 16-bit operands, f32 sums.  What becomes of a tile is its caller's: each of
+// them keeps on from the accumulators.
+//
+// An operand lies in memory with k along its rows (KALONG: element (x, k) at
+// x * pitch + k) or with k down its columns (KDOWN: at k * pitch + x).  Both are
+// loaded to LDS as they are, 16 bytes a lane without passing through registers,
+// 64 k at a time.  KALONG fragments are 16-byte reads there, KDOWN ones are
+// transposed by ds_read_b64_tr_b16.
+//
+// Two slots of 64 k suffice without a wait for what was just begun.  A step has
+// two halves, `a` and `b`, of 32 k:
+//   a: products of k 0 .. 31; the fragments of b are read, each into the
+//      registers that its product has just left;
+//   b: after two rows of products the workgroup meets.  By then every wave has
+//      read all it needs of this slot, and its loads of the next step, sent a
+//      whole step before, have landed.  The loads of the step after that are
+//      sent into this slot, and the fragments of the next step's a are read.
+#pragma once
+
+#include "rf_block.h"
+
+namespace rfp {
+
+using namespace rfb;
+
+constexpr int STEP = 64;             // k of a step
+constexpr int ROW = STEP * 2;        // LDS bytes of a KALONG row's step
+
+typedef __attribute__((ext_vector_type(8))) bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) f16 f16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+enum Layout { KALONG, KDOWN };
+
+// One operand.  Up to three planes of the same shape: a split f32 tensor's.
+struct Side {
+    const void* base[3];
+    int64_t pitch;   // bytes, a multiple of 16 below 2^24
+    int64_t extent;  // x that may be read: KDOWN at least 8 and a multiple of 8
+    int64_t depth;   // KDOWN: rows k that may be read, at least 1
+};
+
+template <typename H> struct Eight;
+template <> struct Eight<bf16> { typedef bf16x8 type; };
+template <> struct Eight<f16> { typedef f16x8 type; };
+
+__device__ __forceinline__ f32x4 multiply(bf16x8 x, bf16x8 y, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 multiply(f16x8 x, f16x8 y, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+}
+
+// Loads straight to LDS are written in assembly, so that the compiler neither
+// counts nor orders them (it would wait for all of them before each LDS read);
+// the waits for them are explicit.  m0, which they set, is otherwise unused.
+__device__ __forceinline__ void load_to_lds(uint32_t to, uint32_t off, const char* base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+
+// KDOWN: 32-byte units of a row are xored by this, so that the rows of a
+// transposed read lie in different banks.
+__device__ __forceinline__ int unit(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
+
+// A side of a tile: T of its x, staged by W waves, read by waves that hold F
+// fragments of 16 x each, the first of them at x `mine`.
+template <typename H, Layout L, int T, int W, int F> struct Staged {
+    typedef typename Eight<H>::type h8;
+    static constexpr int BYTES = T * ROW, N = BYTES / 1024 / W;  // loads of a wave
+    static_assert(N * W * 1024 == BYTES, "whole wave loads");
+
+    uint32_t off[N];   // this lane's 16 bytes of each load, from the step's base
+    uint32_t at[2];    // LDS: this lane's part of fragment 0 of either half
+    const char* base;  // the step to be loaded next
+    int64_t pitch;
+    int k0;            // KDOWN: row of this lane in the wave's first load
+
+    __device__ __forceinline__ void set(const Side& s, int64_t x0, int wave, int mine, int lane)
+    {
+        pitch = s.pitch;
+        if constexpr (L == KALONG) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {  // eight rows of 128 bytes; their 16-byte units xored by the row
+                const int64_t row = min(x0 + (wave * N + j) * 8 + lane / 8, s.extent - 1) - x0;
+                off[j] = (uint32_t)(row * s.pitch) + ((lane % 8) ^ (lane / 8)) * 16;
+            }
+            at[0] = (mine + lane % 16) * ROW + ((lane / 16) ^ (lane & 7)) * 16;
+            at[1] = at[0] ^ 64;
+        } else {
+            constexpr int ROWS = 512 / T, LANES = WAVE / ROWS;  // rows of a load, lanes of a row
+            k0 = wave * N * ROWS + lane / LANES;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int k = k0 + j * ROWS;
+                const int64_t from = min(x0 * 2 + ((lane % LANES) ^ (2 * unit(k))) * 16, s.extent * 2 - 16);
+                off[j] = (uint32_t)(k * s.pitch + from);
+            }
+            const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+            at[0] = k * (T * 2) + ((mine / 16) ^ unit(k)) * 32 + (lane & 3) * 8;
+            at[1] = at[0] + 32 * (T * 2);
+        }
+    }
+    // the operand's plane from step `step` on
+    __device__ __forceinline__ void seek(const Side& s, int plane, int64_t x0, int64_t step)
+    {
+        const char* const b = (const char*)s.base[plane];
+        base = L == KALONG ? b + x0 * s.pitch + step * ROW : b + step * STEP * s.pitch;
+    }
+    __device__ __forceinline__ void next() { base += L == KALONG ? (int64_t)ROW : STEP * pitch; }
+    // load j of the step at `base`, of which KDOWN has `left` rows
+    __device__ __forceinline__ void load(uint32_t slot, int wave, int j, int64_t left) const
+    {
+        const uint32_t to = slot + (wave * N + j) * 1024;
+        if constexpr (L == KDOWN) {
+            if (left < STEP) {  // rows behind the last: that one again
+                const int k = k0 + j * (512 / T), over = max(k - (int)left + 1, 0);
+                load_to_lds(to, off[j] - (uint32_t)(over * pitch), base);
+                return;
+            }
+        }
+        load_to_lds(to, off[j], base);
+    }
+    // fragment i of half h
+    __device__ __forceinline__ h8 read(const char* slot, int h, int i) const
+    {
+        if constexpr (L == KALONG) {
+            return *(const h8*)(slot + at[h] + i * 16 * ROW);
+        } else {
+            // (mine / 16 + i) ^ unit: mine / 16 is a multiple of F, i below it
+            const char* const p = slot + (at[h] ^ (uint32_t)(i * 32));
+            union { s16x4 half[2]; h8 v; } u;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)  // rows k + 4: the same unit
+                u.half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)(p + k * 4 * (T * 2)));
+            return u.v;
+        }
+    }
+};
+
+// A tile of TP x TQ by WP x WQ waves.
+template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> struct Product {
+    static constexpr int WAVES = WP * WQ, THREADS = WAVES * WAVE;
+    static constexpr int FP = TP / WP / 16, FQ = TQ / WQ / 16;  // fragments of a wave
+    typedef Staged<H, LP, TP, WAVES, FP> P;
+    typedef Staged<H, LQ, TQ, WAVES, FQ> Q;
+    typedef typename Eight<H>::type h8;
+    static constexpr int SLOT = P::BYTES + Q::BYTES, LDS = 2 * SLOT;
+    static_assert(LDS <= 160 * 1024, "");
+    typedef f32x4 Sums[FP][FQ];
+
+    // acc[i][j][r] = out[q0 + wq() + 16 j + lane % 16, p0 + wp() + 16 i + lane / 16 * 4 + r]
+    static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE); }
+    static __device__ __forceinline__ int wp() { return wave() / WQ * (TP / WP); }
+    static __device__ __forceinline__ int wq() { return wave() % WQ * (TQ / WQ); }
+
+    // The sums over steps s0 .. s1 - 1 of each of the plane pairs (3: high
+    // times high, high times low, low times high).  Ends with no load in flight.
+    static __device__ __forceinline__ void run(char* lds, const Side& sp, const Side& sq, int64_t p0, int64_t q0,
+                                               int64_t s0, int64_t s1, int pairs, Sums& acc)
+    {
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const int64_t steps = (s1 - s0) * pairs;
+        if (steps <= 0) return;
+        const int lane = threadIdx.x % WAVE, w = wave();
+        const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)lds);
+        P p;
+        Q q;
+        p.set(sp, p0, w, wp(), lane);
+        q.set(sq, q0, w, wq(), lane);
+        int pair = 0;
+        int64_t ahead = s0;  // of the step to be loaded next
+        auto seek = [&] {
+            p.seek(sp, pair == 2, p0, ahead);
+            q.seek(sq, pair == 1, q0, ahead);
+        };
+        auto next = [&] {
+            p.next();
+            q.next();
+            if (++ahead == s1 && ++pair < pairs) {
+                ahead = s0;
+                seek();
+            }
+        };
+        auto load = [&](uint32_t slot, int j) {
+            if (j < P::N) p.load(lds0 + slot, w, j, sp.depth - ahead * STEP);
+            else q.load(lds0 + slot + P::BYTES, w, j - P::N, sq.depth - ahead * STEP);
+        };
+        constexpr int LOADS = P::N + Q::N;
+        seek();
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) load(0, j);
+        next();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (steps > 1) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) load(SLOT, j);
+            next();
+        }
+        h8 x[FP], y[2][FQ];
+        {
+#pragma unroll
+            for (int j = 0; j < FQ; ++j) y[0][j] = q.read(lds + P::BYTES, 0, j);
+#pragma unroll
+            for (int i = 0; i < FP; ++i) x[i] = p.read(lds, 0, i);
+        }
+        constexpr int MEET = FP > 4 ? 2 : 1;  // rows of products of b before the workgroup meets
+        uint32_t now = 0;
+        for (int64_t s = 0; s < steps; ++s) {
+            const char* const here = lds + now;
+            const char* const there = lds + (now ^ SLOT);
+#pragma unroll
+            for (int i = 0; i < FP; ++i) {  // a
+#pragma unroll
+                for (int j = i * FQ / FP; j < (i + 1) * FQ / FP; ++j) y[1][j] = q.read(here + P::BYTES, 1, j);
+#pragma unroll
+                for (int j = 0; j < FQ; ++j) acc[i][j] = multiply(x[i], y[0][j], acc[i][j]);
+                x[i] = p.read(here, 1, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const bool more = s + 2 < steps;
+#pragma unroll
+            for (int i = 0; i < FP; ++i) {  // b
+                if (i == MEET) {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    __syncthreads();
+#pragma unroll
+                    for (int j = 0; j < MEET; ++j) x[j] = p.read(there, 0, j);
+                }
+#pragma unroll
+                for (int j = 0; j < FQ; ++j) acc[i][j] = multiply(x[i], y[1][j], acc[i][j]);
+                if (i >= MEET) {
+                    constexpr int ROWS = FP - MEET;
+#pragma unroll
+                    for (int j = (i - MEET) * FQ / ROWS; j < (i - MEET + 1) * FQ / ROWS; ++j)
+                        y[0][j] = q.read(there + P::BYTES, 0, j);
+                    x[i] = p.read(there, 0, i);
+                    if (more) {
+#pragma unroll
+                        for (int j = (i - MEET) * LOADS / ROWS; j < (i - MEET + 1) * LOADS / ROWS; ++j) load(now, j);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (more) next();
+            now ^= SLOT;
+        }
+        static_assert((SLOT & (SLOT - 1)) == 0, "the slots' offsets are 0 and SLOT");
+    }
+};
+
+// Tiles in the order of workgroups.  Workgroups go to the eight XCDs in turn:
+// each XCD takes a run of neighbouring ids, and a run goes through bands of
+// eight q-tiles, q first, so that the workgroups of an XCD share rows of both
+// operands in its L2.
+struct TileAt { uint32_t p, q; };
+
+__device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t all)
+{
+    const uint32_t each = all / 8;
+    return block < each * 8 ? block % 8 * each + block / 8 : block;
+}
+
+__device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t tiles_p, uint32_t tiles_q)
+{
+    constexpr uint32_t BAND = 8;
+    const uint32_t band = id / (BAND * tiles_p), high = min(BAND, tiles_q - band * BAND);
+    const uint32_t in = id - band * BAND * tiles_p;
+    return {in / high, band * BAND + in % high};
+}
+
+}  // namespace rfp

@@ -1,0 +1,123 @@
+"""The loss of a language model over its vocabulary (no reference counterpart).
+
+``linear_cross_entropy`` is the softmax cross entropy of ``hidden @ weight.T``:
+
+    loss = lse - logit[target] + z_loss * lse ** 2,  lse = log(sum(exp(logits)))
+
+for every row of ``hidden``, without a tensor of all logits: each tile of the
+product is reduced to a maximum and a sum as it is computed.
+``linear_cross_entropy_grad`` gives the gradients of ``hidden`` and ``weight`` as
+well, in the same pass: it holds the exponentials of a piece of the tokens in 16
+bits, at most 2 GiB at once, and computes no product twice.
+``rollfast_amd.autograd.linear_cross_entropy`` is differentiable.
+
+A token whose target is ``ignore_index`` has a loss of zero and no part in the
+gradients, whatever its row of ``hidden`` holds (its own gradient is zero).  A
+target that is no row of ``weight`` otherwise makes the loss and the gradients NaN.
+
+``hidden`` and ``weight`` are float32, bfloat16 or float16 on a ROCm device, both
+of one dtype, which is the gradients' too; losses are float32.  Targets are int32
+or int64.  Any row stride is read in place.  Work is enqueued on the current
+stream.  16-bit tensors are multiplied as they are, float32 ones to 22 bits; sums
+are f32 in a fixed order: equal inputs give equal bits.  The gradient of a logit
+is rounded to the tensors' own dtype (float32: to 22 bits) before it is multiplied.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Any, NamedTuple
+
+import torch
+
+from . import _lib
+from .blocks import _code, _rows, _tensor
+
+_REDUCTION = {"none": _lib.RF_REDUCE_NONE, "sum": _lib.RF_REDUCE_SUM, "mean": _lib.RF_REDUCE_MEAN}
+
+
+class LossGrads(NamedTuple):
+    loss: Any
+    hidden: Any
+    weight: Any
+
+
+def _arguments(hidden, weight, targets, ignore_index, z_loss, reduction):
+    """The call's structure and the tensors that it points to."""
+    device = _tensor(hidden, "hidden").device
+    _tensor(weight, "weight", device)
+    _tensor(targets, "targets", device)
+    a = _lib.CrossEntropy()
+    a.dtype = _code(hidden.dtype, "hidden")
+    if weight.dtype != hidden.dtype:
+        raise ValueError(f"weight is {weight.dtype}, hidden is {hidden.dtype}")
+    if hidden.dim() == 0 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
+        raise ValueError(f"hidden [..., n] and weight [vocab, n] do not fit: {tuple(hidden.shape)}, {tuple(weight.shape)}")
+    if weight.shape[0] == 0:
+        raise ValueError("weight needs at least one row")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"targets have shape {tuple(targets.shape)}, expected {tuple(hidden.shape[:-1])}")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"targets must be int64 or int32, got {targets.dtype}")
+    if reduction not in _REDUCTION:
+        raise ValueError(f"reduction must be one of {', '.join(map(repr, _REDUCTION))}, got {reduction!r}")
+    rows, hidden_stride = _rows(hidden, "hidden")
+    table, weight_stride = _rows(weight, "weight")
+    targets = targets.contiguous()
+    a.tokens, a.vocab, a.hidden = targets.numel(), weight.shape[0], weight.shape[1]
+    a.target_bits = 64 if targets.dtype == torch.int64 else 32
+    a.hidden_rows, a.weight, a.targets = rows.data_ptr(), table.data_ptr(), targets.data_ptr()
+    a.hidden_stride, a.weight_stride = hidden_stride, weight_stride
+    a.ignore_index, a.z_loss, a.reduction = int(ignore_index), float(z_loss), _REDUCTION[reduction]
+    return a, (rows, table, targets)
+
+
+def _launch(a, device, what):
+    """Runs the call on the current stream of ``device``, the current one."""
+    need = ctypes.c_int64()
+    _lib.check(_lib.lib().rf_linear_cross_entropy_workspace(a, need), what)
+    workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+    _lib.check(_lib.lib().rf_linear_cross_entropy(a, workspace.data_ptr(), need.value, _lib.stream_ptr()), what)
+
+
+def linear_cross_entropy(hidden, weight, targets, *, ignore_index: int = -100, z_loss: float = 0.0,
+                         reduction: str = "none"):
+    """The loss of every row of ``hidden`` [..., n] with ``targets`` [...] and
+    ``weight`` [vocab, n], in float32: of the targets' shape, or with
+    ``reduction`` 'sum' or 'mean' one value over the targets that count."""
+    a, _held = _arguments(hidden, weight, targets, ignore_index, z_loss, reduction)
+    with torch.cuda.device(hidden.device):
+        loss = torch.empty(targets.shape, dtype=torch.float32, device=hidden.device)
+        a.loss = loss.data_ptr()
+        if a.reduction:
+            total = torch.empty((), dtype=torch.float32, device=hidden.device)
+            a.total = total.data_ptr()
+        _launch(a, hidden.device, "linear_cross_entropy")
+    return total if a.reduction else loss
+
+
+def linear_cross_entropy_grad(hidden, weight, targets, dloss=None, *, ignore_index: int = -100, z_loss: float = 0.0,
+                              reduction: str = "none") -> LossGrads:
+    """The losses, and the gradients of ``sum(dloss * loss)`` with ``dloss``
+    float32 of the targets' shape; or with a ``reduction`` in place of ``dloss``
+    the reduced loss and its gradients."""
+    a, _held = _arguments(hidden, weight, targets, ignore_index, z_loss, reduction)
+    if (dloss is None) == (reduction == "none"):
+        raise ValueError("the gradient needs dloss, or a reduction in its place")
+    device = hidden.device
+    if dloss is not None:
+        _tensor(dloss, "dloss", device)
+        if dloss.shape != targets.shape or dloss.dtype != torch.float32:
+            raise ValueError(f"dloss must be float32 of shape {tuple(targets.shape)}, got {dloss.dtype} {tuple(dloss.shape)}")
+        dloss = dloss.contiguous()
+        a.dloss = dloss.data_ptr()
+    with torch.cuda.device(device):
+        loss = torch.empty(targets.shape, dtype=torch.float32, device=device)
+        dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=device)
+        dweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
+        a.loss, a.dhidden, a.dweight = loss.data_ptr(), dhidden.data_ptr(), dweight.data_ptr()
+        if a.reduction:
+            total = torch.empty((), dtype=torch.float32, device=device)
+            a.total = total.data_ptr()
+        _launch(a, device, "linear_cross_entropy_grad")
+    return LossGrads(total if a.reduction else loss, dhidden, dweight)
