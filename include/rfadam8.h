@@ -616,6 +616,27 @@ RF_API rf_status rf_linear_cross_entropy_workspace(const rf_cross_entropy* args,
 RF_API rf_status rf_linear_cross_entropy(const rf_cross_entropy* args, void* workspace, int64_t workspace_bytes,
                                          void* stream);
 
+/* Newton-Schulz orthogonalisation of matrices: X = in / (|in| + eps) with the
+ * Frobenius norm, then for every step's (a, b, c) A = X X^T (of the shorter side)
+ * and X = a X + (b A + c A^2) X; out = scale X.  Row-major, row strides in
+ * elements; out may be in.  Results in bf16 are worked out in f16 products whose
+ * rounding shows below bf16's, others in split f16 products to about 20 bits. */
+typedef struct rf_orthogonal_matrix {
+    const void* in;
+    void* out;
+    int64_t rows, cols, in_stride, out_stride;
+    int32_t dtype;
+    float scale;
+} rf_orthogonal_matrix;
+
+/* At most 256 matrices in a call, sides up to 2^20 and the shorter to 2^16.  The
+ * workspace is 256-byte aligned.  coefficients [steps, 3] are host memory; those
+ * that let a singular value of at most one grow past 64 are refused. */
+RF_API rf_status rf_orthogonalize_workspace(const rf_orthogonal_matrix* matrices, int32_t count, int64_t* bytes);
+RF_API rf_status rf_orthogonalize(const rf_orthogonal_matrix* matrices, int32_t count, int32_t steps,
+                                  const float* coefficients, float eps, void* workspace, int64_t workspace_bytes,
+                                  void* stream);
+
 /* Host-side: the 256 f32 values of a dynamic codebook (adam8.py:461-503). */
 RF_API rf_status rf_codebook(int32_t quantizer, float* out256);
 

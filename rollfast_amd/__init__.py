@@ -35,6 +35,7 @@ from .optim.adam8 import (
 )
 from .optim.adam import ScaleByAdamState, adamw, adamw_step, scale_by_adam
 from .optim.convert import adam8_state_from_adam, adam_state_from_adam8, dequantize_state_tree, quantize_state_tree
+from .optim.muon import orthogonalize
 from .combine import MultiTransformState, chain, masked, multi_transform
 from .transforms import GlobalNormClipState, apply_if_finite, clip_by_global_norm
 from .multisteps import MultiSteps, MultiStepsState
@@ -124,6 +125,7 @@ __all__ = (
     "losses",
     "masked",
     "multi_transform",
+    "orthogonalize",
     "postnorm_residual",
     "postnorm_residual_grad",
     "prenorm",

@@ -210,6 +210,15 @@ class CrossEntropy(ctypes.Structure):
     ]
 
 
+class OrthogonalMatrix(ctypes.Structure):
+    _fields_ = [
+        *((n, _p) for n in ("in_", "out")),
+        *((n, _i64) for n in ("rows", "cols", "in_stride", "out_stride")),
+        ("dtype", _i32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 assert ctypes.sizeof(Adam8Leaf) == 120
 assert ctypes.sizeof(Adam8Hparams) == 128
 assert ctypes.sizeof(Adam8Group) == 32
@@ -250,6 +259,8 @@ EXPORTS = (
     "rf_linear_weight_grad",
     "rf_linear_cross_entropy_workspace",
     "rf_linear_cross_entropy",
+    "rf_orthogonalize_workspace",
+    "rf_orthogonalize",
     "rf_codebook",
     "rf_host_table_codes",
     "rf_host_search_index",
@@ -310,6 +321,8 @@ def lib() -> ctypes.CDLL:
     L.rf_linear_weight_grad.argtypes = [ctypes.POINTER(WeightGrad), _p, i64, _p]
     L.rf_linear_cross_entropy_workspace.argtypes = [ctypes.POINTER(CrossEntropy), ctypes.POINTER(i64)]
     L.rf_linear_cross_entropy.argtypes = [ctypes.POINTER(CrossEntropy), _p, i64, _p]
+    L.rf_orthogonalize_workspace.argtypes = [ctypes.POINTER(OrthogonalMatrix), i32, ctypes.POINTER(i64)]
+    L.rf_orthogonalize.argtypes = [ctypes.POINTER(OrthogonalMatrix), i32, i32, _p, ctypes.c_float, _p, i64, _p]
     L.rf_codebook.argtypes = [i32, _p]
     L.rf_host_table_codes.argtypes = [i32, u32, i64, _p]
     L.rf_host_search_index.argtypes = [i32, u32, i64, _p]

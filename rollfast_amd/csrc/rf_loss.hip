@@ -64,47 +64,66 @@ __device__ __forceinline__ float inverse(float power_of_two) { return __uint_as_
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 
-constexpr int SELECT = 1024;
+// Raises *top to at least x.  Read first: it seldom has to be raised, and thousands
+// of atomics on one address would take 12 ns each.  (The order does not matter to a
+// maximum.)
+__device__ __forceinline__ void raise(uint32_t* top, uint32_t x)
+{
+    if (x > __hip_atomic_load(top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(top, x);
+}
 
-// order[0 .. count): the tokens that count; behind them the others, whose loss is
-// set.  target[i]: of token order[i], -1 where it is no row of weight.  One
-// workgroup: a thread counts a run of tokens, and writes it behind those before.
+constexpr int SELECT = 1024, RUN = 8;  // threads, tokens of a thread at a time
+
+// order[0 .. count): the tokens that count, in order; the others, whose loss is
+// set, from the end on backwards.  target[i]: of token order[i], -1 where it is no
+// row of weight.  One workgroup: 16384 tokens take 8 us.
 template <typename I>
 __global__ __launch_bounds__(SELECT) void k_select(const I* __restrict__ targets, int64_t tokens, int64_t ignore, int64_t vocab,
                                                   float* __restrict__ loss, int32_t* __restrict__ order,
                                                   int32_t* __restrict__ target, Scalars* sc, int pieces)
 {
-    __shared__ int32_t part[SELECT / WAVE];
-    const int tid = threadIdx.x, lane = tid % WAVE;
-    const int64_t run = (tokens + SELECT - 1) / SELECT, t0 = min(tid * run, tokens), t1 = min(t0 + run, tokens);
-    int32_t mine = 0;
-    for (int64_t t = t0; t < t1; ++t) mine += (int64_t)targets[t] != ignore;
-    int32_t upto = mine;  // inclusive sum over the wave, then the waves before
-    for (int d = 1; d < WAVE; d *= 2) {
-        const int32_t v = __shfl_up(upto, d);
-        if (lane >= d) upto += v;
-    }
-    if (lane == WAVE - 1) part[tid / WAVE] = upto;
-    __syncthreads();
-    int32_t all = 0, before = 0;
-    for (int w = 0; w < SELECT / WAVE; ++w) {
-        if (w < tid / WAVE) before += part[w];
-        all += part[w];
-    }
-    int32_t at = before + upto - mine;      // tokens that count before this run
-    int64_t off = all + (t0 - at);          // and the place of the run's others
-    for (int64_t t = t0; t < t1; ++t) {
-        const int64_t y = (int64_t)targets[t];
-        if (y != ignore) {
-            order[at] = (int32_t)t;
-            target[at++] = y >= 0 && y < vocab ? (int32_t)y : -1;
-        } else {
-            order[off++] = (int32_t)t;
-            loss[t] = 0.0f;
+    __shared__ int32_t part[2][SELECT / WAVE];
+    const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
+    int32_t before = 0;  // tokens that count in the runs before
+    for (int64_t at = 0, turn = 0; at < tokens; at += SELECT * RUN, turn ^= 1) {
+        const int64_t t0 = at + tid * RUN;
+        int64_t y[RUN];
+        int32_t mine = 0;
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) y[k] = t0 + k < tokens ? (int64_t)targets[t0 + k] : ignore;
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) mine += y[k] != ignore;
+        int32_t upto = mine;  // inclusive sum over the wave, then the waves before
+        for (int d = 1; d < WAVE; d *= 2) {
+            const int32_t v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
         }
+        if (lane == WAVE - 1) part[turn][wave] = upto;
+        __syncthreads();  // (the other half of part may still be read)
+        int32_t all = 0, ahead = 0;
+        for (int w = 0; w < SELECT / WAVE; ++w) {
+            const int32_t n = part[turn][w];
+            if (w < wave) ahead += n;
+            all += n;
+        }
+        int32_t on = before + ahead + upto - mine;  // tokens that count before this run
+        int64_t off = tokens - 1 - (t0 - on);       // the next place of the others
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+            const int64_t t = t0 + k;
+            if (t >= tokens) break;
+            if (y[k] != ignore) {
+                order[on] = (int32_t)t;
+                target[on++] = y[k] >= 0 && y[k] < vocab ? (int32_t)y[k] : -1;
+            } else {
+                order[off--] = (int32_t)t;
+                loss[t] = 0.0f;
+            }
+        }
+        before += all;
     }
     if (tid == 0) {
-        sc->count = all;
+        sc->count = before;
         sc->hidden_top = sc->weight_top = 0;
     }
     for (int i = tid; i < pieces; i += SELECT) sc->dz_top[i] = 0;
@@ -124,7 +143,7 @@ __global__ __launch_bounds__(256) void k_top(const float* __restrict__ x, int64_
         }
     }
     for (int d = 1; d < WAVE; d *= 2) best = max(best, (uint32_t)__shfl_xor((int)best, d));
-    if (threadIdx.x % WAVE == 0 && best) atomicMax(top, best);  // (the order does not matter to a maximum)
+    if (threadIdx.x % WAVE == 0) raise(top, best);
 }
 
 // A high and a low part in f16 of scaled values.
@@ -211,39 +230,50 @@ __global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_logits(const Logits a)
     float unscale = 1.0f;
     if (a.pairs > 1) unscale = inverse(scale_of(a.sc->hidden_top)) * inverse(scale_of(a.sc->weight_top));
     const int64_t v0 = p0 + G::wp() + lane / 16 * 4;
-    const bool edge = p0 + G::wp() + TILE / WP > a.vocab;
+    if (a.pairs > 1) {
+#pragma unroll
+        for (int j = 0; j < G::FQ; ++j)
+#pragma unroll
+            for (int i = 0; i < G::FP; ++i) acc[i][j] *= unscale;
+    }
+    if (p0 + G::wp() + TILE / WP > a.vocab) {
+#pragma unroll
+        for (int j = 0; j < G::FQ; ++j)
+#pragma unroll
+            for (int i = 0; i < G::FP; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (v0 + 16 * i + r >= a.vocab) acc[i][j][r] = -__builtin_inff();
+    }
+    constexpr float LOG2E = 1.44269504088896341f;
 #pragma unroll
     for (int j = 0; j < G::FQ; ++j) {
         const int64_t q = q0 + G::wq() + 16 * j + lane % 16;
         const bool mine = q < count;
         const int64_t y = mine ? a.target[a.first + q] - v0 : -1;
-        float m = -__builtin_inff(), zt = 0.0f;
-        bool here = false;
+        if (__any(y >= 0 && y < TILE / WP)) {  // few waves hold a target
 #pragma unroll
-        for (int i = 0; i < G::FP; ++i) {
+            for (int i = 0; i < G::FP; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float z = acc[i][j][r];
-                if (a.pairs > 1) z *= unscale;
-                if (edge && v0 + 16 * i + r >= a.vocab) z = -__builtin_inff();
-                acc[i][j][r] = z;
-                m = fmaxf(m, z);
-                if (y == 16 * i + r) {
-                    zt = z;
-                    here = true;
-                }
-            }
+                for (int r = 0; r < 4; ++r)
+                    if (y == 16 * i + r) a.picked[q] = acc[i][j][r];
         }
+        float m = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < G::FP; ++i)
+            m = fmaxf(fmaxf(fmaxf(m, acc[i][j][0]), acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3]));
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
+        // exp(z - m) = 2^(z log2(e) - m log2(e)), the product in one rounding with the
+        // difference; where nothing is here, exponentials of -inf are 0
+        const float base = m == -__builtin_inff() ? 0.0f : m * -LOG2E;
         float s = 0.0f;
-        const float base = m == -__builtin_inff() ? 0.0f : m;  // nothing here: exponentials of -inf are 0
 #pragma unroll
         for (int i = 0; i < G::FP; ++i) {
             f32x4 e;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                e[r] = exp_of(acc[i][j][r] - base);
+                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], LOG2E, base));
                 s += e[r];
             }
             const int64_t v = v0 + 16 * i;
@@ -265,7 +295,6 @@ __global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_logits(const Logits a)
         if (mine) {
             const int64_t block = (p0 + G::wp()) / (TILE / WP);
             if (lane < 16 && block < a.blocks) a.stats[q * a.blocks + block] = make_float2(m, s);
-            if (here) a.picked[q] = zt;
         }
     }
 }
@@ -316,7 +345,7 @@ __global__ __launch_bounds__(256) void k_rows(const Rows a)
     a.factor[q] = dl * spread / s;
     a.at_target[q] = dl * (expm1f(below) + (spread - 1.0f) * expf(below));
     const uint32_t most = __float_as_uint(fmaxf(fabsf(dl * spread), fabsf(dl)));
-    if (most < 0x7F800000u) atomicMax(a.dz_top + a.piece, most);
+    if (most < 0x7F800000u) raise(a.dz_top + a.piece, most);
 }
 
 // The sum or the mean of the losses that count: one workgroup, in a fixed order, in f64.
@@ -336,7 +365,16 @@ __global__ __launch_bounds__(SELECT) void k_total(const float* __restrict__ loss
     if (tid == 0) *total = (float)(reduction == RF_REDUCE_MEAN ? part[0] / (double)count : part[0]);
 }
 
-// dz of a token from its exponentials, scaled for f16; zeros up to a whole step of
+// dz is held as a fraction of the largest row factor (f16: of 2^14): a mean's
+// dloss is the same for all tokens, and most of their targets' dz are then just
+// below one, where bf16's rounding is least.
+__device__ __forceinline__ float dz_scale(uint32_t top, bool wide)
+{
+    const float t = __uint_as_float(top);
+    return t < 1e-30f ? 1.0f : (wide ? 1.0f : 16384.0f) / t;
+}
+
+// dz of a token from its exponentials; zeros up to a whole step of
 // tokens.  A workgroup a token.  P: dz's type; E: the exponentials'.
 template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogits(const Rows a)
 {
@@ -351,8 +389,7 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
         }
         return;
     }
-    float scale = 1.0f;
-    if constexpr (!__is_same(P, bf16)) scale = scale_of(a.dz_top[a.piece]);
+    const float scale = dz_scale(a.dz_top[a.piece], __is_same(P, bf16));
     const float m = a.top[q], f = a.factor[q] * scale;
     for (int b = threadIdx.x; b < a.blocks; b += 256) {
         const float top = a.stats[q * a.blocks + b].x;
@@ -405,8 +442,7 @@ struct Grad {
 
 __device__ __forceinline__ float unscale_of(const Grad& a)
 {
-    float u = 1.0f;
-    if (a.dtype != RF_BF16) u = inverse(scale_of(a.dz_top[a.piece]));
+    float u = 1.0f / dz_scale(a.dz_top[a.piece], a.dtype == RF_BF16);
     if (a.pairs > 1) u *= inverse(scale_of(a.order ? a.sc->weight_top : a.sc->hidden_top));
     return u;
 }
@@ -675,7 +711,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
     s = launch<k_pack<T>>(all, 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride, p.pad, (const int32_t*)order,
                           (const Scalars*)sc, (const uint32_t*)&sc->hidden_top, hidden, hidden + plane, (T*)a.dhidden, a.tokens);
     if (s != RF_OK) return s;
-    Side w{{a.weight, a.weight, a.weight}, a.weight_stride * 2, a.vocab, a.vocab};
+    Side w{{a.weight, a.weight}, a.weight_stride * 2, a.vocab, a.vocab};
     if (p.own_weight) {
         uint16_t* const own = (uint16_t*)(ws + p.weight);
         s = launch<k_pack<T>>(a.vocab, 256, 0, st, (const T*)a.weight, a.hidden, a.weight_stride, p.pad, none, (const Scalars*)sc,
@@ -689,7 +725,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         const int64_t first = piece * p.rows, rows = std::max<int64_t>(0, std::min(p.rows, a.tokens - first));
         const int64_t held = up(rows, STEP);
         uint16_t* const h = hidden + first * p.pad;
-        Side x{{h, h + (planes - 1) * plane, h}, p.pad * 2, all - first, all - first};
+        Side x{{h, h + (planes - 1) * plane}, p.pad * 2, all - first, all - first};
         Logits l{};
         l.weight = w;
         l.hidden = x;
@@ -742,7 +778,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         s = launch<k_dlogits<H, std::conditional_t<sizeof(T) == 4, float, f16>>>(held, 256, (size_t)p.blocks * 4, st, r);
         if (s != RF_OK) return s;
         Grad g{};
-        Side dz{{r.dz, p.f32 ? (const void*)r.dz_low : r.dz, r.dz}, p.vpad * 2, held, held};
+        Side dz{{r.dz, p.f32 ? (const void*)r.dz_low : r.dz}, p.vpad * 2, held, held};
         g.sc = sc;
         g.dz_top = sc->dz_top;
         g.piece = (int32_t)piece;

@@ -38,9 +38,10 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 enum Layout { KALONG, KDOWN };
 
-// One operand.  Up to three planes of the same shape: a split f32 tensor's.
+// One operand.  Two planes of the same shape, the high and the low part of a split
+// tensor, or one (twice).
 struct Side {
-    const void* base[3];
+    const void* base[2];
     int64_t pitch;   // bytes, a multiple of 16 below 2^24
     int64_t extent;  // x that may be read: KDOWN at least 8 and a multiple of 8
     int64_t depth;   // KDOWN: rows k that may be read, at least 1
