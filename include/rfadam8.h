@@ -637,6 +637,34 @@ RF_API rf_status rf_orthogonalize(const rf_orthogonal_matrix* matrices, int32_t 
                                   const float* coefficients, float eps, void* workspace, int64_t workspace_bytes,
                                   void* stream);
 
+/* Updates of matrices from their gradients, momentum and Newton-Schulz:
+ *   m = momentum m + rest g                       (f32, each operation rounded)
+ *   u = nesterov ? momentum m + rest g : m
+ *   update = scale orthogonalised(u) + decay param
+ * m is kept as rf_blockwise_quantize's dynamic signed codes and f32 scales, rows in
+ * order, padding included, or as f32; u is formed before m is stored.  Matrices are
+ * dense; grad and update have one dtype.  steps, coefficients, eps, workspace and
+ * limits as rf_orthogonalize's. */
+typedef struct rf_muon8_leaf {
+    const void* grad;
+    void* update;
+    const void* param;   /* or NULL: no decay */
+    uint8_t* codes;      /* [ceil(rows cols / block_size), block_size], or NULL */
+    float* scales;
+    float* momentum;     /* [rows, cols], where codes is NULL */
+    int64_t rows, cols;
+    int32_t block_size;
+    int32_t dtype;       /* grad, update */
+    int32_t param_dtype;
+    float scale, decay;
+    int32_t reserved;    /* 0 */
+} rf_muon8_leaf;
+
+RF_API rf_status rf_muon8_update_workspace(const rf_muon8_leaf* leaves, int32_t count, int64_t* bytes);
+RF_API rf_status rf_muon8_update(const rf_muon8_leaf* leaves, int32_t count, float momentum, float rest, int32_t nesterov,
+                                 int32_t steps, const float* coefficients, float eps, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
 /* Host-side: the 256 f32 values of a dynamic codebook (adam8.py:461-503). */
 RF_API rf_status rf_codebook(int32_t quantizer, float* out256);
 

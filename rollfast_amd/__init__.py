@@ -35,7 +35,7 @@ from .optim.adam8 import (
 )
 from .optim.adam import ScaleByAdamState, adamw, adamw_step, scale_by_adam
 from .optim.convert import adam8_state_from_adam, adam_state_from_adam8, dequantize_state_tree, quantize_state_tree
-from .optim.muon import orthogonalize
+from .optim.muon import Muon8State, muon8, orthogonalize
 from .combine import MultiTransformState, chain, masked, multi_transform
 from .transforms import GlobalNormClipState, apply_if_finite, clip_by_global_norm
 from .multisteps import MultiSteps, MultiStepsState
@@ -95,6 +95,7 @@ __all__ = (
     "MultiSteps",
     "MultiStepsState",
     "MultiTransformState",
+    "Muon8State",
     "PostnormGrads",
     "PrenormGrads",
     "QuantizedBlocks",
@@ -125,6 +126,7 @@ __all__ = (
     "losses",
     "masked",
     "multi_transform",
+    "muon8",
     "orthogonalize",
     "postnorm_residual",
     "postnorm_residual_grad",

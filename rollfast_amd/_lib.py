@@ -219,6 +219,16 @@ class OrthogonalMatrix(ctypes.Structure):
     ]
 
 
+class Muon8Leaf(ctypes.Structure):
+    _fields_ = [
+        *((n, _p) for n in ("grad", "update", "param", "codes", "scales", "momentum")),
+        *((n, _i64) for n in ("rows", "cols")),
+        *((n, _i32) for n in ("block_size", "dtype", "param_dtype")),
+        *((n, ctypes.c_float) for n in ("scale", "decay")),
+        ("reserved", _i32),
+    ]
+
+
 assert ctypes.sizeof(Adam8Leaf) == 120
 assert ctypes.sizeof(Adam8Hparams) == 128
 assert ctypes.sizeof(Adam8Group) == 32
@@ -261,6 +271,8 @@ EXPORTS = (
     "rf_linear_cross_entropy",
     "rf_orthogonalize_workspace",
     "rf_orthogonalize",
+    "rf_muon8_update_workspace",
+    "rf_muon8_update",
     "rf_codebook",
     "rf_host_table_codes",
     "rf_host_search_index",
@@ -323,6 +335,9 @@ def lib() -> ctypes.CDLL:
     L.rf_linear_cross_entropy.argtypes = [ctypes.POINTER(CrossEntropy), _p, i64, _p]
     L.rf_orthogonalize_workspace.argtypes = [ctypes.POINTER(OrthogonalMatrix), i32, ctypes.POINTER(i64)]
     L.rf_orthogonalize.argtypes = [ctypes.POINTER(OrthogonalMatrix), i32, i32, _p, ctypes.c_float, _p, i64, _p]
+    L.rf_muon8_update_workspace.argtypes = [ctypes.POINTER(Muon8Leaf), i32, ctypes.POINTER(i64)]
+    L.rf_muon8_update.argtypes = [ctypes.POINTER(Muon8Leaf), i32, ctypes.c_float, ctypes.c_float, i32, i32, _p,
+                                  ctypes.c_float, _p, i64, _p]
     L.rf_codebook.argtypes = [i32, _p]
     L.rf_host_table_codes.argtypes = [i32, u32, i64, _p]
     L.rf_host_search_index.argtypes = [i32, u32, i64, _p]

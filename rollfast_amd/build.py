@@ -40,9 +40,10 @@ VARIANTS = [(a, m, e) for a in (0, 1) for m in (0, 1) for e in (0, 1)]
 BLOCK_SRC = os.path.join(CSRC, "rf_block_host.hip")
 WGRAD_SRC = os.path.join(CSRC, "rf_wgrad.hip")
 NORM_SRC = os.path.join(CSRC, "rf_norm_inst.hip")
-# The vocabulary loss, and the orthogonalisation of matrices.
+# The vocabulary loss, the orthogonalisation of matrices, the updates made with it.
 LOSS_SRC = os.path.join(CSRC, "rf_loss.hip")
 SCHULZ_SRC = os.path.join(CSRC, "rf_schulz.hip")
+MUON_SRC = os.path.join(CSRC, "rf_muon.hip")
 NORM_PAIRS = [(0, 0), (1, 1), (2, 2), (0, 1), (0, 2)]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -78,7 +79,7 @@ def _compile_jobs():
         defs = [f"-DRFI_APPLY={a}", f"-DRFI_MSR={m}", f"-DRFI_EXACT={e}"]
         jobs.append(([HIPCC, *FLAGS, *inc, *defs, "-c", TILE_SRC, "-o", obj], obj))
     for src, name in ((BLOCK_SRC, "rf_block_host.o"), (WGRAD_SRC, "rf_wgrad.o"), (LOSS_SRC, "rf_loss.o"),
-                      (SCHULZ_SRC, "rf_schulz.o")):
+                      (SCHULZ_SRC, "rf_schulz.o"), (MUON_SRC, "rf_muon.o")):
         obj = os.path.join(OBJ_DIR, name)
         jobs.append(([HIPCC, *FLAGS, *inc, "-c", src, "-o", obj], obj))
     for t, u in NORM_PAIRS:
@@ -131,6 +132,8 @@ def _sources_of(obj: str) -> list:
         return [LOSS_SRC, os.path.join(CSRC, "rf_product.h"), *blk, *inc]
     if os.path.basename(obj) == "rf_schulz.o":
         return [SCHULZ_SRC, os.path.join(CSRC, "rf_schulz.h"), os.path.join(CSRC, "rf_product.h"), *blk, *inc]
+    if os.path.basename(obj) == "rf_muon.o":
+        return [MUON_SRC, os.path.join(CSRC, "rf_schulz.h"), *dev, *blk, *inc]
     if os.path.basename(obj).startswith("rf_norm"):
         return [NORM_SRC, *blk, *inc]
     if os.path.basename(obj).startswith("rf_tile"):

@@ -1773,6 +1773,24 @@ rf_status device_state(DevState** out)
 }
 
 inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p % a) == 0; }
+}  // namespace
+
+// This device's lookup tables, for rf_muon.hip.
+namespace rf {
+rf_status lookup_tables_of(const uint4** out) noexcept
+{
+    try {
+        DevState* d = nullptr;
+        const rf_status s = device_state(&d);
+        if (s == RF_OK) *out = d->tables;
+        return s;
+    } catch (...) {
+        return report(RF_ERR_HIP, "no memory for the lookup tables");
+    }
+}
+}  // namespace rf
+
+namespace {
 
 inline bool valid_dtype(int32_t d) { return d == RF_F32 || d == RF_BF16 || d == RF_F16; }
 

@@ -7,8 +7,8 @@
 namespace rfs {
 
 constexpr int PARTS = 128;  // partial sums of squares of a matrix
+constexpr int MAX = 32;     // matrices of a launch
 
-// One matrix.  sums: its partial sums of squares [PARTS], written by the caller; NULL: by the call.
 struct Matrix {
     const void* in;
     void* out;
@@ -16,7 +16,6 @@ struct Matrix {
     int64_t rows, cols, in_stride, out_stride, add_stride;
     int32_t in_dtype, out_dtype, add_dtype;
     float scale, add_scale;
-    const double* sums;
 };
 
 struct Method {
@@ -28,6 +27,13 @@ struct Method {
 // Checks sizes, types and coefficients.
 rf_status check(const Matrix* list, int64_t count, const Method& how) noexcept;
 int64_t workspace(const Matrix* list, int64_t count) noexcept;
-rf_status run(const Matrix* list, int64_t count, const Method& how, char* workspace, hipStream_t stream) noexcept;
+
+// Enqueues what writes the matrices list[which[i]], i < count <= MAX, dense in f32 to
+// u[i], and to sums[i] [PARTS] partial sums of their squares.
+typedef rf_status (*Source)(void* context, const int64_t* which, int count, float* const* u, double* const* sums, hipStream_t stream);
+
+// source: writes the matrices themselves (`in`, its stride and type are not read).
+rf_status run(const Matrix* list, int64_t count, const Method& how, char* workspace, hipStream_t stream, Source source = nullptr,
+              void* context = nullptr) noexcept;
 
 }  // namespace rfs

@@ -36,7 +36,6 @@ using rf::report;
 namespace rfs {
 namespace {
 
-constexpr int MAX = 32;             // matrices of a launch
 constexpr int64_t HELD = 8ll << 30;  // bytes of workspace of matrices worked on together
 
 struct Item {
@@ -99,7 +98,6 @@ __global__ __launch_bounds__(256) void k_squares(const Batch t)
 {
     __shared__ double part[4];
     const Item& it = t.item[blockIdx.x / PARTS];
-    if (it.sums != t.sums + (int64_t)(blockIdx.x / PARTS) * PARTS) return;  // the caller's own
     const int s = blockIdx.x % PARTS, tid = threadIdx.x;
     // a workgroup's threads along a row, or several rows if they are short
     const int across = min(256, max(8, (it.cols + 7) / 8 * 8));
@@ -402,7 +400,6 @@ Item item_of(const Matrix& m)
     it.in = m.in;
     it.out = m.out;
     it.add = m.add;
-    it.sums = m.sums;
     it.in_stride = m.in_stride;
     it.out_stride = m.out_stride;
     it.add_stride = m.add_stride;
@@ -468,7 +465,7 @@ int64_t workspace(const Matrix* list, int64_t count) noexcept
     return most;
 }
 
-rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hipStream_t st) noexcept
+rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hipStream_t st, Source source, void* context) noexcept
 {
     int cus = 0;
     if (const rf_status s = rf::device_cus(&cus); s != RF_OK) return s;
@@ -485,22 +482,30 @@ rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hi
         t.b_scale = scale(most.b);
         t.sums = (double*)ws;
         int64_t used = (end - at) * PARTS * 8;
-        bool own = false;
+        int64_t which[MAX];
+        float* u[MAX];
+        double* sums[MAX];
         for (int64_t i = at; i < end; ++i) {
             const Matrix& m = list[i];
             if (!m.rows || !m.cols) continue;
             Item& it = t.item[t.count];
             it = item_of(m);
-            if (!it.sums) it.sums = t.sums + (int64_t)t.count * PARTS;
-            own |= !m.sums;
+            it.sums = sums[t.count] = t.sums + (int64_t)t.count * PARTS;
             it.buffers = (uint16_t*)(ws + used);
             used += up(it.bytes(split), 256);
+            which[t.count] = i;
+            u[t.count] = (float*)(it.buffers + 2 * it.plane());  // where the next X will lie
+            if (source) {
+                it.in = u[t.count];
+                it.in_dtype = RF_F32;
+                it.in_stride = m.cols;
+            }
             ++t.count;
         }
         at = end;
         if (!t.count) continue;
         rf_status s = RF_OK;
-        if (own) s = launch<k_squares>((int64_t)t.count * PARTS, 256, 0, st, t);
+        s = source ? source(context, which, t.count, u, sums, st) : launch<k_squares>((int64_t)t.count * PARTS, 256, 0, st, t);
         if (s != RF_OK) return s;
         const uint32_t squares = number(t, [](const Item& it) { return (int64_t)it.n / 64 * (it.m / 64); });
         s = launch<k_load>(squares, 256, 0, st, t);
@@ -533,7 +538,7 @@ void convert(const rf_orthogonal_matrix* list, int64_t count, rfs::Matrix* out)
 {
     for (int64_t i = 0; i < count; ++i) {
         const rf_orthogonal_matrix& m = list[i];
-        out[i] = {m.in, m.out, nullptr, m.rows, m.cols, m.in_stride, m.out_stride, 0, m.dtype, m.dtype, m.dtype, m.scale, 0.0f, nullptr};
+        out[i] = {m.in, m.out, nullptr, m.rows, m.cols, m.in_stride, m.out_stride, 0, m.dtype, m.dtype, m.dtype, m.scale, 0.0f};
     }
 }
 

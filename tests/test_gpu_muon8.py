@@ -1,0 +1,78 @@
+"""``muon8`` against its definition: the stored momentum bit for bit (f32 operations
+in order, the CPU oracle's codes), the updates in 64 bits from the momentum as
+computed, within the orthogonalisation's bounds (tests/test_gpu_orthogonalize.py)."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import oracle as orc
+from tests.test_gpu_orthogonalize import BF16, BOUND, F16, F32, exact, gaussian, low_rank
+
+pytestmark = pytest.mark.gpu
+
+
+def rf():
+    import rollfast_amd
+
+    return rollfast_amd
+
+
+def step(m, g, beta, nesterov):
+    """(m, u) in f32, each operation rounded."""
+    beta, rest = np.float32(beta), np.float32(1.0 - beta)
+    m = beta * m + rest * g
+    return m, (beta * m + rest * g if nesterov else m)
+
+
+SHAPES = [(64, 64), (1, 5), (65, 130), (257, 31), (300, 768), (129, 1025)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32, F16])
+@pytest.mark.parametrize("block_size", [2048, 256, 100, 5000])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_steps(nesterov, block_size, dtype):
+    lr, beta, wd = 0.02, 0.95, 0.1
+    tx = rf().muon8(lr, beta, nesterov=nesterov, weight_decay=wd, block_size=block_size, min_size=1000)
+    params = {str(i): gaussian(r, c, dtype, seed=i) for i, (r, c) in enumerate(SHAPES)}
+    state = tx.init(params)
+    host = {k: np.zeros(p.shape, np.float32) for k, p in params.items()}
+    for turn in range(3):
+        grads = {k: low_rank(*p.shape, dtype, seed=10 * turn + int(k), noise=0.3) * 1e-3 for k, p in params.items()}
+        updates, state = tx.update(grads, state, params)
+        assert int(state.count) == turn + 1
+        for k, p in params.items():
+            m, u = step(host[k], grads[k].float().cpu().numpy(), beta, nesterov)
+            if p.numel() >= 1000:
+                codes, scales = orc.quantize(m, block_size)
+                kept = state.mu[k]
+                assert np.array_equal(kept.values.cpu().numpy(), codes), (k, turn)
+                assert np.array_equal(kept.scales.cpu().numpy().view(np.uint32), scales.view(np.uint32))
+                host[k] = orc.dequantize(codes, scales, m.size, block_size).reshape(m.shape)
+            else:
+                assert np.array_equal(state.mu[k].cpu().numpy(), m)
+                host[k] = m
+            r, c = p.shape
+            ref = -lr * (math.sqrt(max(1.0, r / c)) * exact(torch.from_numpy(u).cuda()) + wd * p.double())
+            assert updates[k].dtype == dtype
+            # sums of two terms may cancel: the bound is of the terms' norms
+            size = lr * (math.sqrt(max(1.0, r / c)) * math.sqrt(min(r, c)) * 1.2 + wd * p.double().norm().item())
+            assert (updates[k].double() - ref).norm().item() < BOUND[dtype] * size, (k, turn)
+
+
+def test_adjust_schedule_and_passthrough():
+    g = low_rank(40, 90, F32)
+    for adjust, s in (("spectral", 1.0), ("rms", 0.2 * math.sqrt(90)), (None, 1.0)):
+        tx = rf().muon8(lambda count: 0.5 / (1 + int(count)), adjust=adjust, min_size=0)
+        state = tx.init({"a": g, "b": None, "c": rf().MaskedNode()})
+        for turn in range(2):
+            old = rf().dequantize_blocks(state.mu["a"]).cpu().numpy()
+            updates, state = tx.update({"a": g, "b": None, "c": rf().MaskedNode()}, state)
+            assert updates["b"] is None and updates["c"] == rf().MaskedNode()
+            u = torch.from_numpy(step(old, g.cpu().numpy(), 0.95, True)[1]).cuda()
+            ref = -0.5 / (1 + turn) * s * exact(u)
+            assert ((updates["a"].double() - ref).norm() / ref.norm()).item() < BOUND[F32], (adjust, turn)
