@@ -12,13 +12,13 @@
 //
 //   k_select   the rows that count, in order, behind them the others
 //   k_pack     their hidden vectors, k padded with zeros to whole steps
-//   k_logits   a product's tile of logits becomes, for each token and each block
+//   LogitsJob  a product's tile of logits becomes, for each token and each block
 //              of the vocabulary (a wave's part of the tile: 64 or 128 entries), a
 //              maximum m and a sum s of exp(z - m); for gradients exp(z - m) itself
 //              too, in f16 (f32 tensors: in f32)
 //   k_rows     lse and loss from m and s, factors of the gradient
 //   k_dlogits  exp(z - m) to dz, in place (f32: to two f16 planes)
-//   k_product  dhidden and dweight, two products of the same size
+//   GradJob    dhidden and dweight, two products of the same size
 // Loss alone ends with k_rows and writes no logits.  With gradients a piece of
 // tokens at a time holds at most PIECE bytes of exponentials; the pieces'
 // weight gradients are added in f32.  Three products, none computed twice.
@@ -211,32 +211,60 @@ struct Logits {
     float2* stats;                 // [rows, blocks] m, s
     float* picked;                 // [rows] the target's logit
     void* e;                       // [rows, pitch] exp(z - m)
-    uint32_t tiles_p, tiles_q;
+    uint32_t tiles_p;
+    Stream stream;
+};
+
+// Tiles of equal steps in bands (tile_at), of which a packed piece of tokens has as
+// many as there are tokens that count.
+struct Even {
+    int64_t p0, q0, first, steps;
+};
+
+template <typename H, typename E, int TILE, int WP, int WQ> struct LogitsJob {
+    typedef Logits Args;
+    typedef Even Tile;
+    typedef Product<H, KALONG, KALONG, TILE, TILE, WP, WQ> G;
+    static constexpr int LDS = G::LDS;
+
+    static __device__ int64_t count(const Logits& a) { return max(min((int64_t)a.sc->count - a.first, a.rows), (int64_t)0); }
+    static __device__ uint32_t tiles_q(const Logits& a) { return (uint32_t)((count(a) + TILE - 1) / TILE); }
+    static __device__ Shares shares(const Logits& a)
+    {
+        return rfp::shares(a.tiles_p * tiles_q(a), a.steps, a.stream.room, a.stream.partial != nullptr, TILE, a.pairs);
+    }
+    static __device__ int64_t first(const Logits& a, uint32_t tile) { return tile * a.steps; }
+    static __device__ int64_t units(const Logits& a) { return (int64_t)a.tiles_p * tiles_q(a) * a.steps; }
+    static __device__ Even locate(const Logits& a, int64_t unit)
+    {
+        const uint32_t id = (uint32_t)(unit / a.steps);
+        const TileAt t = tile_at(id, a.tiles_p, tiles_q(a));
+        return {(int64_t)t.p * TILE, (int64_t)t.q * TILE, id * a.steps, a.steps};
+    }
+    static __device__ __forceinline__ void run(const Logits& a, const Even& t, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
+    {
+        G::run(lds, a.weight, a.hidden, t.p0, t.q0, s0, s1, a.pairs, acc);
+    }
+    static __device__ __forceinline__ void finish(const Logits& a, const Even& t, typename G::Sums& acc, int wave, char*);
 };
 
 // E: what is kept of the exponentials: nothing, f16 or f32.
 template <typename H, typename E, int TILE, int WP, int WQ>
-__global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_logits(const Logits a)
+__device__ __forceinline__ void LogitsJob<H, E, TILE, WP, WQ>::finish(const Logits& a, const Even& t, typename G::Sums& acc, int wave, char*)
 {
-    typedef Product<H, KALONG, KALONG, TILE, TILE, WP, WQ> G;
-    extern __shared__ char lds[];
-    const TileAt tile = tile_at(xcd_order(blockIdx.x, a.tiles_p * a.tiles_q), a.tiles_p, a.tiles_q);
-    const int64_t count = min((int64_t)a.sc->count - a.first, a.rows);
-    const int64_t p0 = (int64_t)tile.p * TILE, q0 = (int64_t)tile.q * TILE;
-    if (q0 >= count) return;
-    typename G::Sums acc;
-    G::run(lds, a.weight, a.hidden, p0, q0, 0, a.steps, a.pairs, acc);
-    const int lane = threadIdx.x % WAVE;
+    const int64_t count = LogitsJob::count(a), p0 = t.p0, q0 = t.q0;
+    const int wp = G::wp(wave), wq = G::wq(wave);
+    const int lane = own_lane();
     float unscale = 1.0f;
     if (a.pairs > 1) unscale = inverse(scale_of(a.sc->hidden_top)) * inverse(scale_of(a.sc->weight_top));
-    const int64_t v0 = p0 + G::wp() + lane / 16 * 4;
+    const int64_t v0 = p0 + wp + lane / 16 * 4;
     if (a.pairs > 1) {
 #pragma unroll
         for (int j = 0; j < G::FQ; ++j)
 #pragma unroll
             for (int i = 0; i < G::FP; ++i) acc[i][j] *= unscale;
     }
-    if (p0 + G::wp() + TILE / WP > a.vocab) {
+    if (p0 + wp + TILE / WP > a.vocab) {
 #pragma unroll
         for (int j = 0; j < G::FQ; ++j)
 #pragma unroll
@@ -246,11 +274,14 @@ __global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_logits(const Logits a)
                     if (v0 + 16 * i + r >= a.vocab) acc[i][j][r] = -__builtin_inff();
     }
     constexpr float LOG2E = 1.44269504088896341f;
+    int32_t target[G::FQ];  // loaded together
+#pragma unroll
+    for (int j = 0; j < G::FQ; ++j) target[j] = a.target[a.first + min(q0 + wq + 16 * j + lane % 16, count - 1)];
 #pragma unroll
     for (int j = 0; j < G::FQ; ++j) {
-        const int64_t q = q0 + G::wq() + 16 * j + lane % 16;
+        const int64_t q = q0 + wq + 16 * j + lane % 16;
         const bool mine = q < count;
-        const int64_t y = mine ? a.target[a.first + q] - v0 : -1;
+        const int64_t y = mine ? target[j] - v0 : -1;
         if (__any(y >= 0 && y < TILE / WP)) {  // few waves hold a target
 #pragma unroll
             for (int i = 0; i < G::FP; ++i)
@@ -269,34 +300,43 @@ __global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_logits(const Logits a)
         const float base = m == -__builtin_inff() ? 0.0f : m * -LOG2E;
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < G::FP; ++i) {
-            f32x4 e;
+        for (int i = 0; i < G::FP; i += 2) {
+            f32x4 e[2];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], LOG2E, base));
-                s += e[r];
-            }
-            const int64_t v = v0 + 16 * i;
-            if constexpr (!__is_same(E, void)) {
-                if (mine && v < a.pitch) {
-                    E* const o = (E*)a.e + q * a.pitch + v;
-                    if constexpr (sizeof(E) == 4) {
-                        *(f32x4*)o = e;
-                    } else {
-                        const f16x2 lo = __builtin_convertvector((f32x2{e[0], e[1]}), f16x2);
-                        const f16x2 hi = __builtin_convertvector((f32x2{e[2], e[3]}), f16x2);
-                        *(u32x2*)o = u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
-                    }
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    e[k][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i + k][j][r], LOG2E, base));
+                    s += e[k][r];
                 }
+            if constexpr (__is_same(E, f16)) {
+                const u32x4 c = chunk(narrow4<f16>(e[0]), narrow4<f16>(e[1]));
+                const int64_t v = p0 + wp + 16 * i + chunk_of(lane);
+                if (mine && v < a.pitch) *(u32x4*)((f16*)a.e + q * a.pitch + v) = c;
+            } else if constexpr (__is_same(E, float)) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (mine && v0 + 16 * (i + k) < a.pitch) *(f32x4*)((float*)a.e + q * a.pitch + v0 + 16 * (i + k)) = e[k];
             }
         }
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         if (mine) {
-            const int64_t block = (p0 + G::wp()) / (TILE / WP);
+            const int64_t block = (p0 + wp) / (TILE / WP);
             if (lane < 16 && block < a.blocks) a.stats[q * a.blocks + block] = make_float2(m, s);
         }
     }
+}
+
+template <typename J> __global__ __launch_bounds__(J::G::THREADS, 2) void k_multiply(const typename J::Args)
+{
+    extern __shared__ char lds[];
+    multiply_tiles<J>(argument<typename J::Args>(), lds);
+}
+
+template <typename J> __global__ __launch_bounds__(WAVE, 2) void k_settle(const typename J::Args)
+{
+    settle_tiles<J>(argument<typename J::Args>(), nullptr);
 }
 
 struct Rows {
@@ -315,37 +355,45 @@ struct Rows {
     uint16_t* dz_low;
 };
 
-// A wave a token.
+// A wave a token at a time.  A workgroup's waves raise the largest factor once, so
+// that few atomics meet.
 __global__ __launch_bounds__(256) void k_rows(const Rows a)
 {
-    const int64_t q = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-    if (q >= min((int64_t)a.sc->count - a.first, a.rows)) return;
+    const int64_t count = min((int64_t)a.sc->count - a.first, a.rows);
     const int lane = threadIdx.x % WAVE;
-    const float2* const stats = a.stats + q * a.blocks;
-    float m = -__builtin_inff();
-    for (int b = lane; b < a.blocks; b += WAVE) m = fmaxf(m, stats[b].x);
-    for (int d = 1; d < WAVE; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-    float s = 0.0f;
-    for (int b = lane; b < a.blocks; b += WAVE) {
-        const float2 x = stats[b];
-        s += x.y * exp_of(x.x - m);
+    uint32_t most = 0;
+    for (int64_t q = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE; q < count; q += (int64_t)gridDim.x * 4) {
+        const float2* const stats = a.stats + q * a.blocks;
+        float m = -__builtin_inff();
+        for (int b = lane; b < a.blocks; b += WAVE) m = fmaxf(m, stats[b].x);
+        for (int d = 1; d < WAVE; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        float s = 0.0f;
+        for (int b = lane; b < a.blocks; b += WAVE) {
+            const float2 x = stats[b];
+            s += x.y * exp_of(x.x - m);
+        }
+        s = wave_sum(s);
+        if (lane) continue;
+        const int32_t t = a.order[a.first + q];
+        const bool known = a.target[a.first + q] >= 0;
+        const float logs = logf(s), lse = m + logs, nan = __builtin_nanf("");
+        const float below = known ? a.picked[q] - m - logs : nan;  // the target's log probability
+        a.loss[t] = a.z_loss * lse * lse - below;
+        if (!a.factor) continue;
+        float dl = a.dloss ? a.dloss[t] : a.reduction == RF_REDUCE_MEAN ? 1.0f / (float)a.sc->count : 1.0f;
+        if (!known) dl = nan;
+        const float spread = 1.0f + 2.0f * a.z_loss * lse;
+        a.top[q] = m;
+        a.factor[q] = dl * spread / s;
+        a.at_target[q] = dl * (expm1f(below) + (spread - 1.0f) * expf(below));
+        const uint32_t mine = __float_as_uint(fmaxf(fabsf(dl * spread), fabsf(dl)));
+        if (mine < 0x7F800000u) most = max(most, mine);
     }
-    s = wave_sum(s);
-    if (lane) return;
-    const int32_t t = a.order[a.first + q];
-    const bool known = a.target[a.first + q] >= 0;
-    const float logs = logf(s), lse = m + logs, nan = __builtin_nanf("");
-    const float below = known ? a.picked[q] - m - logs : nan;  // the target's log probability
-    a.loss[t] = a.z_loss * lse * lse - below;
     if (!a.factor) return;
-    float dl = a.dloss ? a.dloss[t] : a.reduction == RF_REDUCE_MEAN ? 1.0f / (float)a.sc->count : 1.0f;
-    if (!known) dl = nan;
-    const float spread = 1.0f + 2.0f * a.z_loss * lse;
-    a.top[q] = m;
-    a.factor[q] = dl * spread / s;
-    a.at_target[q] = dl * (expm1f(below) + (spread - 1.0f) * expf(below));
-    const uint32_t most = __float_as_uint(fmaxf(fabsf(dl * spread), fabsf(dl)));
-    if (most < 0x7F800000u) raise(a.dz_top + a.piece, most);
+    __shared__ uint32_t tops[4];
+    if (lane == 0) tops[threadIdx.x / WAVE] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) raise(a.dz_top + a.piece, max(max(tops[0], tops[1]), max(tops[2], tops[3])));
 }
 
 // The sum or the mean of the losses that count: one workgroup, in a fixed order, in f64.
@@ -429,15 +477,15 @@ struct Grad {
     int64_t cols, rows;            // of the output: p below cols, q below rows
     int64_t first, piece_rows;     // packed tokens of this piece
     int64_t steps;                 // of the sum; 0: the tokens that count
-    int32_t pairs, dtype, splits, piece;
+    int32_t pairs, dtype, piece;
     const Scalars* sc;
     const uint32_t* dz_top;
     const int32_t* order;          // dhidden: the output's row of packed token q; NULL: dweight
     void* out;
     float* sums;                   // dweight, several pieces: f32 sums so far (may be out)
     int32_t begin, end;            // the first piece, the last one
-    float* partial;                // splits > 1: [splits, rows, cols]
-    uint32_t tiles_p, tiles_q;
+    uint32_t tiles_p;
+    Stream stream;
 };
 
 __device__ __forceinline__ float unscale_of(const Grad& a)
@@ -447,131 +495,133 @@ __device__ __forceinline__ float unscale_of(const Grad& a)
     return u;
 }
 
-// Four neighbouring values of an output's row, unscaled sums.
-__device__ __forceinline__ void finish(const Grad& a, int64_t q, int64_t p, f32x4 v, float unscale)
-{
-    const int64_t left = a.cols - p;
-    v *= unscale;
-    int64_t row = q;
-    if (a.order) row = a.order[a.first + q];
-    const int64_t at = row * a.cols + p;
-    float* sums = nullptr;
-    if (!a.order && !(a.begin && a.end)) sums = a.sums + at;
-    if (sums && !a.begin) {
-        if (left >= 4) v += __builtin_bit_cast(f32x4, *(const u32x4_at*)sums);
-        else
-            for (int r = 0; r < 3; ++r)
-                if (r < left) v[r] += sums[r];
+// What becomes of neighbouring sums of an output's row: unscaled, added to the
+// pieces' before, and rounded, or kept for the pieces behind.
+struct Finish {
+    void* out;
+    float* sums;       // NULL: nothing before and nothing behind
+    const int32_t* order;
+    int64_t cols;
+    float unscale;
+    bool add, keep;
+    int32_t dtype;
+
+    __device__ __forceinline__ Finish(const Grad& a)
+        : out(a.out), sums(!a.order && !(a.begin && a.end) ? a.sums : nullptr), order(a.order ? a.order + a.first : nullptr),
+          cols(a.cols), unscale(unscale_of(a)), add(sums && !a.begin), keep(sums && !a.end), dtype(a.dtype)
+    {
     }
-    const int dtype = sums && !a.end ? (int)RF_F32 : a.dtype;
-    void* const out = sums && !a.end ? (void*)a.sums : a.out;
-    if (left < 4) {
-        for (int r = 0; r < 3; ++r)
-            if (r < left) put_scalar(out, dtype, at + r, v[r]);
-    } else if (dtype == RF_F32) {
-        *(u32x4_at*)((float*)out + at) = __builtin_bit_cast(u32x4, v);
-    } else {
-        uint32_t lo, hi;
-        if (dtype == RF_BF16) {
-            lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), bf16x2));
-            hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), bf16x2));
-        } else {
-            lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), f16x2));
-            hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), f16x2));
+    // four of row q from p on, in f32 or element by element
+    __device__ __forceinline__ void put4(int64_t q, int64_t p, f32x4 v) const
+    {
+        v *= unscale;
+        const int64_t left = cols - p, here = q * cols + p, at = (order ? order[q] : q) * cols + p;
+        if (add) {
+            if (left >= 4) v += __builtin_bit_cast(f32x4, *(const u32x4_at*)(sums + here));
+            else
+                for (int r = 0; r < 3; ++r)
+                    if (r < left) v[r] += sums[here + r];
         }
-        *(u32x2_at*)((uint16_t*)out + at) = u32x2{lo, hi};
+        if (left >= 4 && (keep || dtype == RF_F32)) *(u32x4_at*)((float*)(keep ? sums : out) + at) = __builtin_bit_cast(u32x4, v);
+        else
+            for (int r = 0; r < 4; ++r)
+                if (r < left) put_scalar(keep ? sums : out, keep ? (int)RF_F32 : dtype, at + r, v[r]);
     }
-}
+    // the usual case: 16 bits, nothing before and nothing behind
+    __device__ __forceinline__ bool plain() const { return !sums && dtype != RF_F32; }
+};
 
 // dhidden: p the hidden columns of weight (summed down its rows), q the tokens of dz.
 // dweight: p the hidden columns of the packed rows, q the vocabulary, both summed over tokens.
-template <typename H, Layout LQ, int TILE, int WP, int WQ>
-__global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_product(const Grad a)
-{
+template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
+    typedef Grad Args;
+    typedef Even Tile;
     typedef Product<H, KDOWN, LQ, TILE, TILE, WP, WQ> G;
-    extern __shared__ char lds[];
-    const uint32_t tiles = a.tiles_p * a.tiles_q, id = xcd_order(blockIdx.x, tiles * a.splits);
-    const uint32_t split = id / tiles;
-    const TileAt tile = tile_at(id % tiles, a.tiles_p, a.tiles_q);
-    const int64_t count = max(min((int64_t)a.sc->count - a.first, a.piece_rows), (int64_t)0);
-    const int64_t rows = LQ == KALONG ? count : a.rows;
-    const int64_t p0 = (int64_t)tile.p * TILE, q0 = (int64_t)tile.q * TILE;
-    if (q0 >= rows) return;
-    const int64_t steps = LQ == KALONG ? a.steps : (count + STEP - 1) / STEP;
-    if (LQ == KDOWN && !steps && !a.begin && !a.end) return;  // nothing to add
-    typename G::Sums acc;
-    G::run(lds, a.p, a.q, p0, q0, steps * split / a.splits, steps * (split + 1) / a.splits, a.pairs, acc);
-    const int lane = threadIdx.x % WAVE;
-    const float unscale = unscale_of(a);
+    static constexpr int LDS = G::LDS;
+
+    static __device__ int64_t count(const Grad& a) { return max(min((int64_t)a.sc->count - a.first, a.piece_rows), (int64_t)0); }
+    static __device__ int64_t rows(const Grad& a) { return LQ == KALONG ? count(a) : a.rows; }
+    static __device__ int64_t steps(const Grad& a) { return LQ == KALONG ? a.steps : (count(a) + STEP - 1) / STEP; }
+    static __device__ uint32_t tiles_q(const Grad& a) { return (uint32_t)((rows(a) + TILE - 1) / TILE); }
+    static __device__ Shares shares(const Grad& a)
+    {
+        // dweight of a piece without tokens: nothing to add, but what was summed is to be rounded
+        if (LQ == KDOWN && !steps(a)) return {a.begin || a.end ? a.tiles_p * tiles_q(a) : 0, 0};
+        return rfp::shares(a.tiles_p * tiles_q(a), steps(a), a.stream.room, a.stream.partial != nullptr, TILE, a.pairs);
+    }
+    // (a unit a tile where there are no steps)
+    static __device__ int64_t each(const Grad& a) { return max(steps(a), (int64_t)1); }
+    static __device__ int64_t first(const Grad& a, uint32_t tile) { return tile * each(a); }
+    static __device__ int64_t units(const Grad& a) { return (int64_t)a.tiles_p * tiles_q(a) * each(a); }
+    static __device__ Even locate(const Grad& a, int64_t unit)
+    {
+        const uint32_t id = (uint32_t)(unit / each(a));
+        const TileAt t = tile_at(id, a.tiles_p, tiles_q(a));
+        return {(int64_t)t.p * TILE, (int64_t)t.q * TILE, id * each(a), steps(a)};
+    }
+    static __device__ __forceinline__ void run(const Grad& a, const Even& t, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
+    {
+        G::run(lds, a.p, a.q, t.p0, t.q0, s0, s1, a.pairs, acc);
+    }
+    static __device__ __forceinline__ void finish(const Grad& a, const Even& t, typename G::Sums& acc, int wave, char*)
+    {
+        const int64_t rows = GradJob::rows(a);
+        const Finish f(a);
+        const int lane = own_lane();
+        const int64_t p0 = t.p0 + G::wp(wave);
 #pragma unroll
-    for (int j = 0; j < G::FQ; ++j) {
-        const int64_t q = q0 + G::wq() + 16 * j + lane % 16;
-        if (q >= rows) continue;
+        for (int j = 0; j < G::FQ; ++j) {
+            const int64_t q = t.q0 + G::wq(wave) + 16 * j + lane % 16;
+            if (f.plain()) {
+                uint16_t* const row = (uint16_t*)f.out + (f.order ? f.order[min(q, rows - 1)] : q) * f.cols;
 #pragma unroll
-        for (int i = 0; i < G::FP; ++i) {
-            const int64_t p = p0 + G::wp() + 16 * i + lane / 16 * 4;
-            if (p >= a.cols) continue;
-            if (a.splits > 1) {
-                float* const o = a.partial + (split * a.rows + q) * a.cols + p;
-                if (a.cols - p >= 4) *(u32x4_at*)o = __builtin_bit_cast(u32x4, acc[i][j]);
-                else
-                    for (int r = 0; r < 3; ++r)
-                        if (r < a.cols - p) o[r] = acc[i][j][r];
+                for (int i = 0; i < G::FP; i += 2) {
+                    const f32x4 x = acc[i][j] * f.unscale, y = acc[i + 1][j] * f.unscale;
+                    const u32x4 c = __is_same(H, bf16) ? chunk(narrow4<bf16>(x), narrow4<bf16>(y)) : chunk(narrow4<f16>(x), narrow4<f16>(y));
+                    const int64_t from = p0 + 16 * i + chunk_of(lane);
+                    if (q < rows && from < f.cols) put8(row + from, Raw<uint16_t>{c}, f.cols - from);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             } else {
-                finish(a, q, p, acc[i][j], unscale);
+#pragma unroll
+                for (int i = 0; i < G::FP; ++i) {
+                    const int64_t p = p0 + 16 * i + lane / 16 * 4;
+                    if (q < rows && p < f.cols) f.put4(q, p, acc[i][j]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
     }
-}
-
-// Adds the splits' sums in their order.
-__global__ __launch_bounds__(256) void k_join(const Grad a)
-{
-    const int64_t quads = (a.cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t q = i / quads, p = i % quads * 4;
-    const int64_t count = max(min((int64_t)a.sc->count - a.first, a.piece_rows), (int64_t)0);
-    if (q >= (a.order ? count : a.rows)) return;
-    if (!a.order && !count && !a.begin && !a.end) return;
-    const float* o = a.partial + q * a.cols + p;
-    f32x4 v{};
-    for (int s = 0; s < a.splits; ++s, o += a.rows * a.cols) {
-        if (a.cols - p >= 4) v += __builtin_bit_cast(f32x4, *(const u32x4_at*)o);
-        else
-            for (int r = 0; r < 3; ++r)
-                if (r < a.cols - p) v[r] += o[r];
-    }
-    finish(a, q, p, v, unscale_of(a));
-}
+};
 
 // ------------------------------------------------------------------- host ---
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Tile of a product, and splits of its sum: the cheapest by what they take
-// (us, measured): 6 for a round of workgroups and `step` for 64 k; split, 5 and
-// the partial sums at 4 TB/s.  A CU holds one workgroup with tiles of 256, two of 128.
+// Tile of a product: the one that takes less (us, measured): a step of 64 k of the
+// tiles that the GPU holds at a time, 256 wide one a CU or 128 wide two, and 6 or 4 for a
+// tile's start and end.
 struct Shape {
     bool big;
-    uint32_t tiles_p, tiles_q, splits;
-    double us;
+    uint32_t tiles_p, room;
 };
 
-Shape shape_of(int64_t cols, int64_t rows, int64_t steps, bool split, int cus)
+Shape shape_of(int64_t cols, int64_t rows, int64_t steps, int pairs, int cus)
 {
-    Shape best{};
-    best.us = 1e30;
+    double us[2];
     for (int big = 0; big < 2; ++big) {
-        const int64_t tile = big ? 256 : 128, tp = (cols + tile - 1) / tile, tq = (rows + tile - 1) / tile;
-        const int64_t room = (int64_t)cus * (big ? 1 : 2);
-        const double step = big ? 1.65 : 1.15;
-        for (int64_t n = 1; n <= (split ? std::min<int64_t>(std::max<int64_t>(1, steps / 2), 64) : 1); ++n) {
-            const double rounds = (double)((tp * tq * n + room - 1) / room);
-            const double us = rounds * (6 + step * (double)((steps + n - 1) / n)) +
-                              (n > 1 ? 5 + (double)n * (double)rows * (double)cols * 8 / 4e6 : 0);
-            if (us < best.us) best = Shape{big != 0, (uint32_t)tp, (uint32_t)tq, (uint32_t)n, us};
-        }
+        const int64_t tile = big ? 256 : 128, tiles = ((cols + tile - 1) / tile) * ((rows + tile - 1) / tile);
+        const uint32_t room = (uint32_t)cus * (big ? 1 : 2);
+        const double step = (big ? 1.6 : 1.05) * pairs, ends = big ? 6 : 4;
+        const Shares sh = rfp::shares((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, true, (int)tile, pairs);
+        us[big] = (double)((sh.whole + room - 1) / room) * ((double)steps * step + ends);
+        if (sh.workers) us[big] += (double)((tiles - sh.whole) * steps + sh.workers - 1) / sh.workers * step + 2 * ends + 10 + 50.0 * sh.workers / room;
     }
-    return best;
+    const bool big = us[1] < us[0];
+    return {big, (uint32_t)((cols + (big ? 255 : 127)) / (big ? 256 : 128)), (uint32_t)cus * (big ? 1 : 2)};
 }
+
+// Bytes of the parts of split tiles.
+int64_t parts_of(const Shape& s) { return (int64_t)s.room * 2 * (s.big ? 256 * 256 : 128 * 128) * 4; }
 
 struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
@@ -595,7 +645,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     // weight as it is: whole steps of k, 16-byte rows
     p.own_weight = p.f32 || a.hidden % STEP || a.weight_stride % 8 || ((uintptr_t)a.weight & 15) || a.weight_stride * 2 >= (1 << 24);
     const int64_t planes = p.f32 ? 2 : 1, steps = p.pad / STEP;
-    p.logits = shape_of(a.vocab, a.tokens, steps * p.pairs, false, cus);
+    p.logits = shape_of(a.vocab, a.tokens, steps, p.pairs, cus);
     p.shift = p.logits.big ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
     const int64_t each = p.grad ? p.vpad * (p.f32 ? 8 : 2) : p.blocks * 8, most = p.grad ? PIECE : STATS;
@@ -604,7 +654,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.pieces = std::max<int64_t>(1, (a.tokens + fit - 1) / fit);
     p.rows = p.pieces == 1 ? std::max<int64_t>(1, a.tokens) : std::min(fit, up((a.tokens + p.pieces - 1) / p.pieces, 256));
     p.pieces = std::max<int64_t>(1, (a.tokens + p.rows - 1) / p.rows);
-    p.logits = shape_of(a.vocab, p.rows, steps * p.pairs, false, cus);
+    p.logits = shape_of(a.vocab, p.rows, steps, p.pairs, cus);
     p.shift = p.logits.big ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
     int64_t at = 0;
@@ -628,12 +678,12 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.e = take(held * p.vpad * (p.f32 ? 4 : 2));
         p.dz = p.f32 ? take(held * p.vpad * 4) : p.e;
         if (p.pieces > 1 && !p.f32) p.sums = take(a.vocab * a.hidden * 4);
-        p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP * p.pairs, true, cus);
-        p.dweight = shape_of(a.hidden, a.vocab, held / STEP * p.pairs, true, cus);
-        const int64_t h = p.dhidden.splits > 1 ? p.dhidden.splits * p.rows * a.hidden * 4 : 0;
-        const int64_t w = p.dweight.splits > 1 ? p.dweight.splits * a.vocab * a.hidden * 4 : 0;
-        p.partial = take(std::max(h, w));
+        p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, cus);
+        p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, cus);
     }
+    int64_t parts = parts_of(p.logits);
+    if (p.grad) parts = std::max({parts, parts_of(p.dhidden), parts_of(p.dweight)});
+    p.partial = take(parts);
     p.bytes = at;
     return p;
 }
@@ -662,27 +712,27 @@ template <auto K, typename... A> rf_status launch(int64_t grid, int threads, siz
     return RF_OK;
 }
 
-template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
+// A product's launch, and the one that settles split tiles.
+template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, const typename J::Args& a, hipStream_t st)
 {
-    typedef Product<H, KALONG, KALONG, 256, 256, 2, 4> Big;
-    typedef Product<H, KALONG, KALONG, 128, 128, 2, 2> Small;
-    const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
-    return p.logits.big ? launch<k_logits<H, E, 256, 2, 4>>(tiles, Big::THREADS, Big::LDS, st, a)
-                        : launch<k_logits<H, E, 128, 2, 2>>(tiles, Small::THREADS, Small::LDS, st, a);
+    const rf_status s = launch<k_multiply<J>>(tiles + shape.room, J::G::THREADS, J::LDS, st, a);
+    return s != RF_OK ? s : launch<k_settle<J>>((int64_t)shape.room * J::G::WAVES, WAVE, 0, st, a);
 }
 
-template <typename H, Layout LQ> rf_status product(const Shape& shape, Grad& a, hipStream_t st)
+int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles_p * ((rows + (shape.big ? 255 : 127)) / (shape.big ? 256 : 128)); }
+
+template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
 {
-    typedef Product<H, KDOWN, LQ, 256, 256, 2, 4> Big;
-    typedef Product<H, KDOWN, LQ, 128, 128, 2, 2> Small;
+    const int64_t tiles = tiles_of(p.logits, a.rows);
+    return p.logits.big ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st) : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st);
+}
+
+template <typename H, Layout LQ> rf_status product(const Shape& shape, float* partial, Grad& a, hipStream_t st)
+{
     a.tiles_p = shape.tiles_p;
-    a.tiles_q = shape.tiles_q;
-    a.splits = (int32_t)shape.splits;
-    const int64_t grid = (int64_t)a.tiles_p * a.tiles_q * a.splits;
-    const rf_status s = shape.big ? launch<k_product<H, LQ, 256, 2, 4>>(grid, Big::THREADS, Big::LDS, st, a)
-                                  : launch<k_product<H, LQ, 128, 2, 2>>(grid, Small::THREADS, Small::LDS, st, a);
-    if (s != RF_OK || a.splits == 1) return s;
-    return launch<k_join>((a.rows * ((a.cols + 3) / 4) + 255) / 256, 256, 0, st, a);
+    a.stream = {shape.room, partial};
+    const int64_t tiles = tiles_of(shape, a.rows);
+    return shape.big ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st) : multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st);
 }
 
 template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const Plan& p, char* ws, hipStream_t st)
@@ -742,7 +792,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         l.picked = (float*)(ws + p.picked);
         l.e = ws + p.e;
         l.tiles_p = p.logits.tiles_p;
-        l.tiles_q = (uint32_t)((rows + (p.logits.big ? 255 : 127)) / (p.logits.big ? 256 : 128));
+        l.stream = {p.logits.room, (float*)(ws + p.partial)};
         if (!p.grad) s = logits<H, void>(p, l, st);
         else if (p.f32) s = logits<H, float>(p, l, st);
         else s = logits<H, f16>(p, l, st);
@@ -772,7 +822,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         r.e = l.e;
         r.dz = ws + p.dz;
         r.dz_low = (uint16_t*)(ws + p.dz) + up(p.rows, STEP) * p.vpad;
-        s = launch<k_rows>((rows + 3) / 4, 256, 0, st, r);
+        s = launch<k_rows>(std::min<int64_t>((rows + 3) / 4, 2048), 256, 0, st, r);
         if (s != RF_OK) return s;
         if (!p.grad) continue;
         s = launch<k_dlogits<H, std::conditional_t<sizeof(T) == 4, float, f16>>>(held, 256, (size_t)p.blocks * 4, st, r);
@@ -787,7 +837,6 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.pairs = p.pairs;
         g.dtype = a.dtype;
         g.cols = a.hidden;
-        g.partial = (float*)(ws + p.partial);
         g.p = w;
         g.p.extent = p.pad;  // (its columns; as it is, hidden is a multiple of whole steps)
         g.q = dz;
@@ -796,9 +845,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.order = order;
         g.out = a.dhidden;
         if (rows) {
-            Shape shape = p.dhidden;
-            shape.tiles_q = (uint32_t)((rows + (shape.big ? 255 : 127)) / (shape.big ? 256 : 128));
-            s = product<H, KALONG>(shape, g, st);
+            s = product<H, KALONG>(p.dhidden, (float*)(ws + p.partial), g, st);
             if (s != RF_OK) return s;
         }
         g.p = x;
@@ -810,7 +857,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.sums = p.f32 ? (float*)a.dweight : (float*)(ws + p.sums);
         g.begin = piece == 0;
         g.end = piece + 1 == p.pieces;
-        s = product<H, KDOWN>(p.dweight, g, st);
+        s = product<H, KDOWN>(p.dweight, (float*)(ws + p.partial), g, st);
         if (s != RF_OK) return s;
     }
     if (a.reduction != RF_REDUCE_NONE)

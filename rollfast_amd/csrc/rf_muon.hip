@@ -222,8 +222,7 @@ rf_status rf_muon8_update_workspace(const rf_muon8_leaf* leaves, int32_t count, 
     rfs::Matrix list[256];
     convert(leaves, count, list);
     if (const rf_status s = rfs::check(list, count, {0, nullptr, 0.0f}); s != RF_OK) return s;
-    *bytes = rfs::workspace(list, count);
-    return RF_OK;
+    return rfs::workspace(list, count, bytes);
 }
 
 rf_status rf_muon8_update(const rf_muon8_leaf* leaves, int32_t count, float momentum, float rest, int32_t nesterov, int32_t steps,
@@ -234,7 +233,8 @@ rf_status rf_muon8_update(const rf_muon8_leaf* leaves, int32_t count, float mome
     convert(leaves, count, list);
     const rfs::Method how{steps, coefficients, eps};
     if (const rf_status s = rfs::check(list, count, how); s != RF_OK) return s;
-    const int64_t need = rfs::workspace(list, count);
+    int64_t need = 0;
+    if (const rf_status s = rfs::workspace(list, count, &need); s != RF_OK) return s;
     if (need && (!workspace || need > workspace_bytes)) return report(RF_ERR_INVALID, "workspace too small");
     if ((uintptr_t)workspace & 255) return report(RF_ERR_INVALID, "workspace must be 256-byte aligned");
     Call call{leaves, momentum, rest, nesterov != 0, nullptr};

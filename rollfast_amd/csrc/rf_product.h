@@ -20,6 +20,8 @@
 //      sent into this slot, and the fragments of the next step's a are read.
 #pragma once
 
+#include <type_traits>
+
 #include "rf_block.h"
 
 namespace rfp {
@@ -60,12 +62,36 @@ __device__ __forceinline__ f32x4 multiply(f16x8 x, f16x8 y, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
 }
 
+// A value that all lanes hold, to scalar registers (divisions leave it in vector ones).
+__device__ __forceinline__ int64_t uniform(int64_t v)
+{
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // Loads straight to LDS are written in assembly, so that the compiler neither
 // counts nor orders them (it would wait for all of them before each LDS read);
 // the waits for them are explicit.  m0, which they set, is otherwise unused.
 __device__ __forceinline__ void load_to_lds(uint32_t to, uint32_t off, const char* base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+    const uint32_t at = __builtin_amdgcn_readfirstlane(to);
+    const char* const from = (const char*)uniform((int64_t)base);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(from) : "memory");
+}
+
+// A kernel's only argument where it lies.  Through the parameter, of which parts are
+// picked at run time, the compiler would copy all of it to scratch memory and read it
+// back into vector registers.
+template <typename A> __device__ __forceinline__ const A& argument() { return *(const A*)__builtin_amdgcn_kernarg_segment_ptr(); }
+
+// This lane's number, of which the compiler does not know that it never changes: it
+// would work out all that follows from it ahead of a loop over tiles, and keep it in
+// registers that the sums need.
+__device__ __forceinline__ int own_lane()
+{
+    int lane = threadIdx.x % WAVE;
+    asm volatile("" : "+v"(lane));
+    return lane;
 }
 
 // KDOWN: 32-byte units of a row are xored by this, so that the rows of a
@@ -156,12 +182,19 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
     typedef typename Eight<H>::type h8;
     static constexpr int SLOT = P::BYTES + Q::BYTES, LDS = 2 * SLOT;
     static_assert(LDS <= 160 * 1024, "");
+    // Small tiles: the last fragment of P is read where its half begins and Q's as
+    // soon as they may be, so that nothing read late in a half is waited for at the
+    // next one's start, and the last two steps are copies of the loop's body without
+    // loads (4096 cubed, tiles of 128: 146 -> 139 us with both operands KALONG, 172 ->
+    // 139 with both KDOWN).  Large tiles have no registers for it (4 % slower).
+    static constexpr int LATE = FP <= 4 ? 1 : 0;
     typedef f32x4 Sums[FP][FQ];
 
-    // acc[i][j][r] = out[q0 + wq() + 16 j + lane % 16, p0 + wp() + 16 i + lane / 16 * 4 + r]
+    // A wave's place in the tile:
+    // acc[i][j][r] = out[q0 + wq + 16 j + lane % 16, p0 + wp + 16 i + lane / 16 * 4 + r]
     static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE); }
-    static __device__ __forceinline__ int wp() { return wave() / WQ * (TP / WP); }
-    static __device__ __forceinline__ int wq() { return wave() % WQ * (TQ / WQ); }
+    static __device__ __forceinline__ int wp(int w) { return w / WQ * (TP / WP); }
+    static __device__ __forceinline__ int wq(int w) { return w % WQ * (TQ / WQ); }
 
     // The sums over steps s0 .. s1 - 1 of each of the plane pairs (3: high
     // times high, high times low, low times high).  Ends with no load in flight.
@@ -172,14 +205,18 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
         for (int i = 0; i < FP; ++i)
 #pragma unroll
             for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        p0 = uniform(p0);
+        q0 = uniform(q0);
+        s0 = uniform(s0);
+        s1 = uniform(s1);
         const int64_t steps = (s1 - s0) * pairs;
         if (steps <= 0) return;
-        const int lane = threadIdx.x % WAVE, w = wave();
+        const int lane = own_lane(), w = wave();
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)lds);
         P p;
         Q q;
-        p.set(sp, p0, w, wp(), lane);
-        q.set(sq, q0, w, wq(), lane);
+        p.set(sp, p0, w, wp(w), lane);
+        q.set(sq, q0, w, wq(w), lane);
         int pair = 0;
         int64_t ahead = s0;  // of the step to be loaded next
         auto seek = [&] {
@@ -204,34 +241,39 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
         for (int j = 0; j < LOADS; ++j) load(0, j);
         next();
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+        __syncthreads();  // (also: a tile before this one may be read no more)
         if (steps > 1) {
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) load(SLOT, j);
             next();
         }
         h8 x[FP], y[2][FQ];
-        {
 #pragma unroll
-            for (int j = 0; j < FQ; ++j) y[0][j] = q.read(lds + P::BYTES, 0, j);
+        for (int j = 0; j < FQ; ++j) y[0][j] = q.read(lds + P::BYTES, 0, j);
 #pragma unroll
-            for (int i = 0; i < FP; ++i) x[i] = p.read(lds, 0, i);
-        }
+        for (int i = 0; i < FP - LATE; ++i) x[i] = p.read(lds, 0, i);
         constexpr int MEET = FP > 4 ? 2 : 1;  // rows of products of b before the workgroup meets
         uint32_t now = 0;
-        for (int64_t s = 0; s < steps; ++s) {
+        // one of Q's fragments for each of the first rows, or two as soon as they may be read
+        auto fill = [&](const char* slot, int half, int row, int rows) {
+            const int from = LATE ? min(2 * row, FQ) : row * FQ / rows, to = LATE ? min(2 * row + 2, FQ) : (row + 1) * FQ / rows;
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+                if (j >= from && j < to) y[half][j] = q.read(slot + P::BYTES, half, j);
+        };
+        auto step = [&](auto more) {
             const char* const here = lds + now;
             const char* const there = lds + (now ^ SLOT);
+            if (LATE) x[FP - 1] = p.read(here, 0, FP - 1);
 #pragma unroll
             for (int i = 0; i < FP; ++i) {  // a
-#pragma unroll
-                for (int j = i * FQ / FP; j < (i + 1) * FQ / FP; ++j) y[1][j] = q.read(here + P::BYTES, 1, j);
+                fill(here, 1, i, FP);
 #pragma unroll
                 for (int j = 0; j < FQ; ++j) acc[i][j] = multiply(x[i], y[0][j], acc[i][j]);
-                x[i] = p.read(here, 1, i);
+                if (i < FP - LATE) x[i] = p.read(here, 1, i);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const bool more = s + 2 < steps;
+            if (LATE) x[FP - 1] = p.read(here, 1, FP - 1);
 #pragma unroll
             for (int i = 0; i < FP; ++i) {  // b
                 if (i == MEET) {
@@ -240,14 +282,12 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
 #pragma unroll
                     for (int j = 0; j < MEET; ++j) x[j] = p.read(there, 0, j);
                 }
+                if (i >= MEET) fill(there, 0, i - MEET, FP - MEET);
 #pragma unroll
                 for (int j = 0; j < FQ; ++j) acc[i][j] = multiply(x[i], y[1][j], acc[i][j]);
                 if (i >= MEET) {
                     constexpr int ROWS = FP - MEET;
-#pragma unroll
-                    for (int j = (i - MEET) * FQ / ROWS; j < (i - MEET + 1) * FQ / ROWS; ++j)
-                        y[0][j] = q.read(there + P::BYTES, 0, j);
-                    x[i] = p.read(there, 0, i);
+                    if (i < FP - LATE) x[i] = p.read(there, 0, i);
                     if (more) {
 #pragma unroll
                         for (int j = (i - MEET) * LOADS / ROWS; j < (i - MEET + 1) * LOADS / ROWS; ++j) load(now, j);
@@ -257,10 +297,60 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
             }
             if (more) next();
             now ^= SLOT;
+        };
+        if constexpr (LATE) {
+            for (int64_t s = 2; s < steps; ++s) step(std::true_type{});
+            if (steps > 1) step(std::false_type{});
+            step(std::false_type{});
+        } else {
+            for (int64_t s = 0; s < steps; ++s) step(s + 2 < steps);
         }
         static_assert((SLOT & (SLOT - 1)) == 0, "the slots' offsets are 0 and SLOT");
     }
 };
+
+// Of a tile's sums a lane holds four neighbours of a row (acc[i][j]), and its row's
+// other three quads of those 16 lie 16, 32 and 48 lanes on.  In 16 bits two
+// fragments' quads become eight neighbours of one of them: lanes of an even sixteen
+// take fragment i's, those of an odd one fragment i + 1's, so that the four lanes of
+// a row hold 64 bytes in order.  chunk_of() is the place of the first of them
+// behind fragment i's first column; quads() takes them apart again.
+typedef uint32_t u32x4_16 __attribute__((ext_vector_type(4), aligned(16)));
+
+__device__ __forceinline__ int chunk_of(int lane) { return (lane >> 4 & 1) * 16 + (lane >> 5) * 8; }
+
+__device__ __forceinline__ u32x4 chunk(u32x2 first, u32x2 second)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(first[0], second[0], false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(first[1], second[1], false, false);
+    return u32x4{a[0], b[0], a[1], b[1]};
+}
+
+__device__ __forceinline__ void quads(u32x4 chunk, u32x2& first, u32x2& second)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(chunk[0], chunk[2], false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(chunk[1], chunk[3], false, false);
+    first = u32x2{a[0], b[0]};
+    second = u32x2{a[1], b[1]};
+}
+
+template <typename T> __device__ __forceinline__ u32x2 narrow4(f32x4 v)
+{
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const t2 lo = __builtin_convertvector((f32x2{v[0], v[1]}), t2), hi = __builtin_convertvector((f32x2{v[2], v[3]}), t2);
+    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+template <typename T> __device__ __forceinline__ f32x4 widen4(u32x2 w)
+{
+    const uint32_t a = w[0], b = w[1];  // (a vector's element has no address of its own for the casts)
+    if constexpr (__is_same(T, bf16)) {
+        return f32x4{__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)};
+    } else {
+        const f16x2 lo = __builtin_bit_cast(f16x2, a), hi = __builtin_bit_cast(f16x2, b);
+        return f32x4{(float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]};
+    }
+}
 
 // Tiles in the order of workgroups.  Workgroups go to the eight XCDs in turn:
 // each XCD takes a run of neighbouring ids, and a run goes through bands of
@@ -280,6 +370,126 @@ __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t tiles_p, uint32_
     const uint32_t band = id / (BAND * tiles_p), high = min(BAND, tiles_q - band * BAND);
     const uint32_t in = id - band * BAND * tiles_p;
     return {in / high, band * BAND + in % high};
+}
+
+// How a launch deals with its tiles.  Whole rounds of tiles go to workgroups of their
+// own; where the last round would leave much of the GPU idle, the tiles of the last two
+// are shared out evenly among `workers`, by their steps, in order: a tile that a
+// worker's share begins or ends in is split, its sums go to memory, and a second launch
+// (settle) adds the parts in their order and does what the first does with a whole
+// tile's sums.  A job J has
+//   Args               with `stream` and the tiles' description
+//   Tile               where a tile lies: its id, steps, first unit
+//   units, locate      all units (a step of a tile), the tile that holds a unit
+//   run                the tile's sums over some of its steps
+//   finish             what becomes of a wave's sums
+struct Stream {
+    uint32_t room;    // workgroups that the GPU holds at a time
+    float* partial;   // [room, 2] tiles of sums, or NULL: no tile is split
+};
+
+// Tiles with workgroups of their own, and the workers of the others.
+struct Shares {
+    uint32_t whole, workers;
+};
+
+constexpr int LEAST = 4;  // steps of a worker's share at least
+
+__host__ __device__ inline Shares shares(uint32_t tiles, int64_t steps, uint32_t room, bool split, int tile, int pairs)
+{
+    const uint32_t last = tiles % room;
+    if (!split || last == 0) return {tiles, 0};
+    // ns: a step of as many tiles as there is room for; the parts' way through memory
+    // and the second launch
+    const int64_t step = (tile > 128 ? 1600 : 1050) * pairs, parts = tile > 128 ? 55000 : 35000;
+    if (tiles < room) {
+        const int64_t units = (int64_t)tiles * steps, most = (units + LEAST - 1) / LEAST;
+        const uint32_t workers = (uint32_t)(most < room ? most : room);
+        const int64_t less = step * (steps - (units + workers - 1) / (workers ? workers : 1));
+        return less > 10000 + parts * workers / room ? Shares{0, workers} : Shares{tiles, 0};
+    }
+    return (room - last) * step * steps > parts * room ? Shares{tiles - last - room, room} : Shares{tiles, 0};
+}
+
+template <typename J> __device__ __forceinline__ float* part_of(const typename J::Args& a, uint32_t worker, int slot)
+{
+    typedef typename J::G G;
+    return a.stream.partial + ((int64_t)worker * 2 + slot) * (G::THREADS * G::FP * G::FQ * 4);
+}
+
+template <typename J> __device__ __forceinline__ void multiply_tiles(const typename J::Args& a, char* lds)
+{
+    typedef typename J::G G;
+    Shares sh = J::shares(a);
+    sh = {(uint32_t)__builtin_amdgcn_readfirstlane(sh.whole), (uint32_t)__builtin_amdgcn_readfirstlane(sh.workers)};
+    int64_t u0, u1;
+    uint32_t worker = 0;
+    if (blockIdx.x < sh.whole) {
+        u0 = J::first(a, xcd_order(blockIdx.x, sh.whole));
+        u1 = u0 + 1;  // to the tile's end
+    } else {
+        worker = blockIdx.x - sh.whole;
+        if (worker >= sh.workers) return;
+        worker = xcd_order(worker, sh.workers);
+        const int64_t from = J::first(a, sh.whole), all = J::units(a) - from;
+        u0 = from + all * worker / sh.workers;
+        u1 = from + all * (worker + 1) / sh.workers;
+    }
+    u0 = uniform(u0);
+    u1 = uniform(u1);
+    while (u0 < u1) {
+        typename J::Tile t = J::locate(a, u0);
+        t.first = uniform(t.first);
+        t.steps = uniform(t.steps);
+        if (blockIdx.x < sh.whole) u1 = uniform(t.first + max(t.steps, (int64_t)1));
+        const int64_t s0 = uniform(u0 - t.first), s1 = uniform(min(t.steps, u1 - t.first));
+        typename G::Sums acc;
+        J::run(a, t, lds, s0, s1, acc);
+        if (s0 == 0 && s1 == t.steps) {
+            J::finish(a, t, acc, G::wave(), lds);
+        } else {
+            float* const o = part_of<J>(a, worker, s0 == 0);
+            const int thread = G::wave() * WAVE + own_lane();
+#pragma unroll
+            for (int i = 0; i < G::FP; ++i)
+#pragma unroll
+                for (int j = 0; j < G::FQ; ++j) *(f32x4*)(o + ((i * G::FQ + j) * G::THREADS + thread) * 4) = acc[i][j];
+        }
+        u0 = uniform(t.first + max(s1, (int64_t)1));
+        if (u0 < u1) __syncthreads();  // LDS may have been used by finish
+    }
+}
+
+// A wave of a split tile to each workgroup.  Its number: the worker whose share begins
+// in the tile, the first of them; the one before it holds the tile's first part.
+template <typename J> __device__ __forceinline__ void settle_tiles(const typename J::Args& a, char* lds)
+{
+    typedef typename J::G G;
+    Shares sh = J::shares(a);
+    sh = {(uint32_t)__builtin_amdgcn_readfirstlane(sh.whole), (uint32_t)__builtin_amdgcn_readfirstlane(sh.workers)};
+    const uint32_t worker = blockIdx.x / G::WAVES + 1;
+    const int wave = blockIdx.x % G::WAVES;
+    if (worker >= sh.workers) return;
+    const int64_t from = J::first(a, sh.whole), all = J::units(a) - from;
+    auto begin = [&](uint32_t w) { return from + all * w / sh.workers; };
+    const int64_t u = begin(worker);
+    if (u >= begin(worker + 1) || u >= from + all) return;  // (an empty share: none, with LEAST)
+    const typename J::Tile t = J::locate(a, u);
+    if (u == t.first || begin(worker - 1) > t.first) return;
+    typename G::Sums acc;
+    auto add = [&](uint32_t w, int slot, bool whole) {
+        const float* const o = part_of<J>(a, w, slot);
+#pragma unroll
+        for (int i = 0; i < G::FP; ++i)
+#pragma unroll
+            for (int j = 0; j < G::FQ; ++j) {
+                const f32x4 v = *(const f32x4*)(o + ((i * G::FQ + j) * G::THREADS + wave * WAVE + threadIdx.x) * 4);
+                acc[i][j] = whole ? v : acc[i][j] + v;
+            }
+    };
+    add(worker - 1, 1, true);
+    for (uint32_t w = worker; w < sh.workers && begin(w) < t.first + t.steps; ++w) add(w, 0, false);
+    J::finish(a, t, acc, wave, lds);
 }
 
 }  // namespace rfp

@@ -6,7 +6,7 @@
 
 namespace rfs {
 
-constexpr int PARTS = 128;  // partial sums of squares of a matrix
+constexpr int PARTS = 512;  // partial sums of squares of a matrix
 constexpr int MAX = 32;     // matrices of a launch
 
 struct Matrix {
@@ -26,7 +26,7 @@ struct Method {
 
 // Checks sizes, types and coefficients.
 rf_status check(const Matrix* list, int64_t count, const Method& how) noexcept;
-int64_t workspace(const Matrix* list, int64_t count) noexcept;
+rf_status workspace(const Matrix* list, int64_t count, int64_t* bytes) noexcept;
 
 // Enqueues what writes the matrices list[which[i]], i < count <= MAX, dense in f32 to
 // u[i], and to sums[i] [PARTS] partial sums of their squares.

@@ -42,13 +42,14 @@ struct Item {
     const void* in;
     void* out;
     const void* add;
-    const double* sums;
+    double* sums;
     uint16_t* buffers;
     int64_t in_stride, out_stride, add_stride;
     int32_t n, m;      // padded to whole steps
     int32_t rows, cols;
     float scale, add_scale;
     uint32_t first;    // its first tile
+    int64_t unit;      // its first unit (a step of a tile)
     uint8_t tall, in_dtype, out_dtype, add_dtype;
 
     // X and the next X: [n, m] high parts, then low parts.  A and B: [n, n] high
@@ -67,7 +68,9 @@ struct Batch {
     float a, b, c;        // the step's coefficients
     float eps, x_scale, a_scale, b_scale;
     uint32_t tiles;
-    double* sums;         // [count, PARTS]
+    int64_t units;
+    Shares share;         // what becomes of the tiles (rf_product.h)
+    Stream stream;
     Item item[MAX];
 };
 static_assert(sizeof(Batch) <= 4096, "kernel arguments");
@@ -79,40 +82,46 @@ __device__ __forceinline__ int find(const Batch& t, uint32_t id)
     return i;
 }
 
-__device__ __forceinline__ u32x2 narrow4(f32x4 v)
+// The item of tile or unit `at`.
+template <typename F> __device__ __forceinline__ int find_by(const Batch& t, F before)
 {
-    const f16x2 lo = __builtin_convertvector((f32x2{v[0], v[1]}), f16x2);
-    const f16x2 hi = __builtin_convertvector((f32x2{v[2], v[3]}), f16x2);
-    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    int i = 0;
+    while (i + 1 < t.count && before(t.item[i + 1])) ++i;
+    return i;
 }
 
-__device__ __forceinline__ f32x4 widen4(u32x2 w)
+// Partial sums of squares, in f64 (a square of an f32 may have no f32): part s of a
+// matrix takes every PARTS-th group of rows, as many as its lanes cover with eight
+// columns each.
+template <typename T> __device__ __forceinline__ double squares(const Item& it, int part)
 {
-    const uint32_t first = w[0], second = w[1];  // (a vector's element has no address of its own for the cast)
-    const f16x2 lo = __builtin_bit_cast(f16x2, first), hi = __builtin_bit_cast(f16x2, second);
-    return f32x4{(float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]};
+    const int64_t chunks = (it.cols + 7) / 8;
+    int lanes = 256;
+    while (lanes > 1 && lanes / 2 >= chunks) lanes /= 2;
+    const int rows = 256 / lanes;
+    double sum = 0;
+    for (int64_t r = (int64_t)part * rows + threadIdx.x / lanes; r < it.rows; r += (int64_t)PARTS * rows) {
+        const T* const row = (const T*)it.in + r * it.in_stride;
+        for (int64_t c = threadIdx.x % lanes; c < chunks; c += lanes) {
+            float v[8];
+            widen8(load8(row, c * 8, it.cols), v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum += (double)v[k] * (double)v[k];
+        }
+    }
+    return sum;
 }
 
-// Partial sums of squares: part s of a matrix takes every PARTS-th group of rows.
 __global__ __launch_bounds__(256) void k_squares(const Batch t)
 {
     __shared__ double part[4];
     const Item& it = t.item[blockIdx.x / PARTS];
     const int s = blockIdx.x % PARTS, tid = threadIdx.x;
-    // a workgroup's threads along a row, or several rows if they are short
-    const int across = min(256, max(8, (it.cols + 7) / 8 * 8));
-    const int lanes = across >= 256 ? 256 : across >= 128 ? 128 : across >= 64 ? 64 : across >= 32 ? 32 : across >= 16 ? 16 : 8;
-    const int rows = 256 / lanes;
-    double sum = 0;
-    for (int64_t r = s * rows + tid / lanes; r < it.rows; r += PARTS * rows)
-        for (int64_t c = tid % lanes; c < it.cols; c += lanes) {
-            const double v = scalar_at(it.in, it.in_dtype, r * it.in_stride + c);
-            sum += v * v;
-        }
+    double sum = it.in_dtype == RF_F32 ? squares<float>(it, s) : it.in_dtype == RF_BF16 ? squares<bf16>(it, s) : squares<f16>(it, s);
     for (int d = 1; d < WAVE; d *= 2) sum += __shfl_xor(sum, d);
     if (tid % WAVE == 0) part[tid / WAVE] = sum;
     __syncthreads();
-    if (tid == 0) t.sums[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+    if (tid == 0) it.sums[s] = part[0] + part[1] + part[2] + part[3];
 }
 
 // G into X's layout, a tile of 64 x 64 of X a workgroup.
@@ -127,26 +136,39 @@ __global__ __launch_bounds__(256) void k_load(const Batch t)
     for (int i = lane; i < PARTS; i += WAVE) norm += it.sums[i];
     for (int d = 1; d < WAVE; d *= 2) norm += __shfl_xor(norm, d);
     const double s = (double)t.x_scale / (sqrt(norm) + (double)t.eps);
-    // G's rows along the wave: X's columns, or its rows if G is tall
     const int64_t r0 = it.tall ? p0 : q0, c0 = it.tall ? q0 : p0;
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-        const int64_t r = r0 + tid / WAVE * 16 + i, c = c0 + lane;
-        float v = 0.0f;
-        if (r < it.rows && c < it.cols) v = (float)((double)scalar_at(it.in, it.in_dtype, r * it.in_stride + c) * s);
-        if (it.tall) tile[lane][tid / WAVE * 16 + i] = v;
-        else tile[tid / WAVE * 16 + i][lane] = v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = i * 32 + tid / 8, c = tid % 8 * 8;
+        float v[8] = {};
+        if (r0 + r < it.rows) {
+            const int64_t at = (r0 + r) * it.in_stride;
+            if (it.in_dtype == RF_F32) widen8(load8((const float*)it.in + at, c0 + c, it.cols), v);
+            else if (it.in_dtype == RF_BF16) widen8(load8((const bf16*)it.in + at, c0 + c, it.cols), v);
+            else widen8(load8((const f16*)it.in + at, c0 + c, it.cols), v);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float w = (float)((double)v[k] * s);
+            if (it.tall) tile[c + k][r] = w;
+            else tile[r][c + k] = w;
+        }
     }
     __syncthreads();
     const int64_t plane = (int64_t)it.n * it.m;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int q = i * 16 + tid / 16, p = tid % 16 * 4;
-        const f32x4 v = {tile[q][p], tile[q][p + 1], tile[q][p + 2], tile[q][p + 3]};
-        const u32x2 hi = narrow4(v);
+    for (int i = 0; i < 2; ++i) {
+        const int q = i * 32 + tid / 8, p = tid % 8 * 8;
+        float v[8], back[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = tile[q][p + k];
+        const Raw<f16> hi = narrow8<f16>(v);
+        widen8(hi, back);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] -= back[k];
         uint16_t* const o = it.x(0) + (q0 + q) * it.m + p0 + p;
-        *(u32x2*)o = hi;
-        *(u32x2*)(o + plane) = narrow4(v - widen4(hi));
+        *(u32x4*)o = hi.a;
+        *(u32x4*)(o + plane) = narrow8<f16>(v).a;
     }
 }
 
@@ -159,137 +181,306 @@ __device__ __forceinline__ TileAt lower(uint32_t id)
     return {id - q * (q + 1) / 2, q};
 }
 
-// Four neighbouring values of a row of a symmetric matrix, and where the tile is
-// not on the diagonal the same values down a column.
-template <bool SPLIT>
-__device__ __forceinline__ void put_symmetric(uint16_t* o, int64_t n, int64_t q, int64_t p, f32x4 v, bool mirror)
+// A wave's tile of a symmetric matrix, in f16: its rows, and where the tile is not
+// on the diagonal its columns as rows, transposed through LDS (`room`: the wave's
+// own, rows of PITCH bytes, so that neither writes nor reads of a column meet in a
+// bank).  With `low` the low parts go to `o + low`.
+template <typename G, int PITCH, bool LOW>
+__device__ __forceinline__ void put_symmetric(uint16_t* o, int64_t low, int64_t n, int64_t q0, int64_t p0,
+                                              const typename G::Sums& v, bool mirror, char* room)
 {
-    const u32x2 hi = narrow4(v), lo = narrow4(v - widen4(hi));
-    *(u32x2*)(o + q * n + p) = hi;
-    if (SPLIT) *(u32x2*)(o + n * n + q * n + p) = lo;
-    if (mirror) {
+    const int lane = own_lane();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            o[(p + r) * n + q] = (uint16_t)(hi[r / 2] >> (16 * (r & 1)));
-            if (SPLIT) o[n * n + (p + r) * n + q] = (uint16_t)(lo[r / 2] >> (16 * (r & 1)));
+    for (int part = 0; part < (LOW ? 2 : 1); ++part) {
+#pragma unroll
+        for (int j = 0; j < G::FQ; ++j) {
+            const int64_t q = q0 + 16 * j + lane % 16;
+#pragma unroll
+            for (int i = 0; i < G::FP; i += 2) {
+                u32x2 w[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f32x4 x = v[i + k][j];
+                    w[k] = narrow4<f16>(x);
+                    if (part) w[k] = narrow4<f16>(x - widen4<f16>(w[k]));
+                }
+                const u32x4 c = chunk(w[0], w[1]);
+                const int64_t p = p0 + 16 * i + chunk_of(lane);
+                if (q < n && p < n) *(u32x4*)(o + part * low + q * n + p) = c;
+                if (mirror) *(u32x4*)(room + (16 * j + lane % 16) * PITCH + (16 * i + chunk_of(lane)) * 2) = c;
+            }
         }
+        if (!mirror) continue;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        // lane l: column l % 16 of a fragment, rows 8 (l / 16) .. + 7 of 32
+#pragma unroll
+        for (int h = 0; h < G::FQ / 2; ++h)
+#pragma unroll
+            for (int i = 0; i < G::FP; ++i) {
+                union { s16x4 half[2]; u32x4 v; } u;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    u.half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(lds_char*)(room + (32 * h + 8 * (lane >> 4) + ((lane & 15) >> 2) + 4 * k) * PITCH + i * 32 + (lane & 3) * 8));
+                const int64_t p = p0 + 16 * i + lane % 16, q = q0 + 32 * h + lane / 16 * 8;
+                if (p < n && q < n) *(u32x4*)(o + part * low + p * n + q) = u.v;
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
+
+// A tile of one of the batch's matrices; they differ in their number of steps.
+struct Place {
+    int item;
+    int64_t p0, q0, first, steps;
+};
+
+// What the jobs of a batch share.  J: steps(item), place(item, tile) of TILE.
+template <typename J> struct Batched {
+    typedef Batch Args;
+    typedef Place Tile;
+
+    static __device__ Shares shares(const Batch& t) { return t.share; }
+    static __device__ int64_t units(const Batch& t) { return t.units; }
+    static __device__ int64_t first(const Batch& t, uint32_t tile)
+    {
+        const Item& it = t.item[find_by(t, [&](const Item& next) { return tile >= next.first; })];
+        return tile < t.tiles ? it.unit + (int64_t)(tile - it.first) * J::steps(it) : t.units;
+    }
+    static __device__ Place locate(const Batch& t, int64_t unit)
+    {
+        const int i = find_by(t, [&](const Item& next) { return unit >= next.unit; });
+        const Item& it = t.item[i];
+        const int64_t steps = J::steps(it);
+        const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(unit - it.unit) / (uint32_t)steps);
+        const TileAt at = J::place(it, id);
+        return {i, (int64_t)at.p * J::TILE, (int64_t)at.q * J::TILE, it.unit + (int64_t)id * steps, steps};
+    }
+};
 
 // SQUARE: B from A; else A from X.
-template <bool SQUARE, bool SPLIT, int TILE, int WP, int WQ>
-__global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_symmetric(const Batch t)
-{
+template <bool SQUARE, bool SPLIT, int TILE_, int WP, int WQ> struct Symmetric : Batched<Symmetric<SQUARE, SPLIT, TILE_, WP, WQ>> {
+    static constexpr int TILE = TILE_;
     typedef Product<f16, KALONG, KALONG, TILE, TILE, WP, WQ> G;
-    extern __shared__ char lds[];
-    const uint32_t id = xcd_order(blockIdx.x, t.tiles);
-    const Item& it = t.item[find(t, id)];
-    const TileAt tile = lower(id - it.first);
-    const int64_t n = it.n, p0 = (int64_t)tile.p * TILE, q0 = (int64_t)tile.q * TILE;
-    const uint16_t* const from = SQUARE ? it.a() : it.x(t.turn);
-    const int64_t depth = SQUARE ? n : it.m, plane = n * depth;
-    const Side s{{from, from + (SPLIT ? plane : 0)}, depth * 2, n, n};
-    typename G::Sums acc;
-    G::run(lds, s, s, p0, q0, 0, depth / STEP, SPLIT ? 3 : 1, acc);
-    const int lane = threadIdx.x % WAVE;
-    const bool mirror = tile.p != tile.q;
-    // stored A = a_scale A, X = x_scale X
-    const float of_a = t.a_scale / (t.x_scale * t.x_scale);
-    const float b_of = t.b * t.b_scale / t.a_scale, c_of = t.c * t.b_scale / (t.a_scale * t.a_scale);
+    static constexpr int PITCH = TILE / WP * 2 + 16, ROOM = TILE / WQ * PITCH;
+    static constexpr int LDS = std::max(G::LDS, G::WAVES * ROOM), SETTLE_LDS = ROOM;
+
+    static __host__ __device__ int64_t steps(const Item& it) { return (SQUARE ? it.n : it.m) / STEP; }
+    static __host__ int64_t tiles(const Item& it)
+    {
+        const int64_t n = (it.n + TILE - 1) / TILE;
+        return n * (n + 1) / 2;
+    }
+    static __device__ TileAt place(const Item&, uint32_t id) { return lower(id); }
+
+    static __device__ __forceinline__ void run(const Batch& t, const Place& at, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
+    {
+        const Item& it = t.item[at.item];
+        const uint16_t* const from = SQUARE ? it.a() : it.x(t.turn);
+        const int64_t depth = SQUARE ? it.n : it.m;
+        const Side s{{from, from + (SPLIT ? it.n * depth : 0)}, depth * 2, it.n, it.n};
+        G::run(lds, s, s, at.p0, at.q0, s0, s1, SPLIT ? 3 : 1, acc);
+    }
+    static __device__ __forceinline__ void finish(const Batch& t, const Place& at, typename G::Sums& acc, int wave, char* lds)
+    {
+        const Item& it = t.item[at.item];
+        const int64_t n = it.n, plane = n * n;
+        const int lane = own_lane();
+        const bool mirror = at.p0 != at.q0;
+        const int64_t wp = at.p0 + G::wp(wave), wq = at.q0 + G::wq(wave);
+        // stored A = a_scale A, X = x_scale X
+        const float of_a = t.a_scale / (t.x_scale * t.x_scale);
+        const float b_of = t.b * t.b_scale / t.a_scale, c_of = t.c * t.b_scale / (t.a_scale * t.a_scale);
 #pragma unroll
-    for (int j = 0; j < G::FQ; ++j) {
-        const int64_t q = q0 + G::wq() + 16 * j + lane % 16;
-        if (q >= n) continue;
+        for (int j = 0; j < G::FQ; ++j) {
+            const int64_t q = wq + 16 * j + lane % 16;
+            if constexpr (!SQUARE) {
 #pragma unroll
-        for (int i = 0; i < G::FP; ++i) {
-            const int64_t p = p0 + G::wp() + 16 * i + lane / 16 * 4;
-            if (p >= n) continue;
-            f32x4 v = acc[i][j];
-            if constexpr (SQUARE) {
-                f32x4 a = widen4(*(const u32x2*)(it.a() + q * n + p));
-                if (SPLIT) a += widen4(*(const u32x2*)(it.a() + n * n + q * n + p));
-                v = b_of * a + c_of * v;
-                if (!mirror) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (p + r == q) {
-                            it.d(SPLIT)[q] = v[r] / t.b_scale;
-                            v[r] = 0.0f;
-                        }
-                }
-                put_symmetric<SPLIT>(it.b(SPLIT), n, q, p, v, mirror);
+                for (int i = 0; i < G::FP; ++i) acc[i][j] *= of_a;
             } else {
-                put_symmetric<SPLIT>(it.a(), n, q, p, v * of_a, mirror);
+                u32x4 old[SPLIT ? 1 : G::FP / 2];  // A here; of one part all loads in flight together
+                auto load = [&](int part, int i) {
+                    return *(const u32x4*)(it.a() + part * plane + min(q, n - 1) * n + min(wp + 16 * i + chunk_of(lane), n - 8));
+                };
+                if (!SPLIT) {
+#pragma unroll
+                    for (int i = 0; i < G::FP; i += 2) old[SPLIT ? 0 : i / 2] = load(0, i);
+                }
+#pragma unroll
+                for (int i = 0; i < G::FP; i += 2) {
+                    f32x4 a[2] = {};
+#pragma unroll
+                    for (int part = 0; part < (SPLIT ? 2 : 1); ++part) {
+                        u32x2 x, y;
+                        quads(SPLIT ? load(part, i) : old[SPLIT ? 0 : i / 2], x, y);
+                        a[0] += widen4<f16>(x);
+                        a[1] += widen4<f16>(y);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        f32x4 v = b_of * a[k] + c_of * acc[i + k][j];
+                        const int64_t p = wp + 16 * (i + k) + lane / 16 * 4;
+                        if (!mirror && q < n) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (p + r == q) {
+                                    it.d(SPLIT)[q] = v[r] / t.b_scale;
+                                    v[r] = 0.0f;
+                                }
+                        }
+                        acc[i + k][j] = v;
+                    }
+                }
             }
         }
+        // a wave's own room in LDS: its part of the workgroup's, or all of a settling wave's
+        char* const room = lds + (blockDim.x > WAVE ? wave * ROOM : 0);
+        put_symmetric<G, PITCH, SPLIT>(SQUARE ? it.b(SPLIT) : it.a(), plane, n, wq, wp, acc, mirror, room);
     }
+};
+
+// scale times eight neighbours of an output's row, and add_scale times what is to be
+// added, from column c on.
+__device__ __forceinline__ void put_out8(const Item& it, int64_t r, int64_t c, float (&v)[8])
+{
+    const int64_t left = it.cols - c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= it.scale;
+    if (it.add) {
+        float w[8];
+        if (it.add_dtype == RF_F32) widen8(load8((const float*)it.add + r * it.add_stride, c, it.cols), w);
+        else if (it.add_dtype == RF_BF16) widen8(load8((const bf16*)it.add + r * it.add_stride, c, it.cols), w);
+        else widen8(load8((const f16*)it.add + r * it.add_stride, c, it.cols), w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += it.add_scale * w[k];
+    }
+    const int64_t at = r * it.out_stride + c;
+    if (it.out_dtype == RF_F32) put8((float*)it.out + at, narrow8<float>(v), left);
+    else if (it.out_dtype == RF_BF16) put8((bf16*)it.out + at, narrow8<bf16>(v), left);
+    else put8((f16*)it.out + at, narrow8<f16>(v), left);
 }
 
-__device__ __forceinline__ void put_out(const Item& it, int64_t r, int64_t c, float v)
-{
-    v *= it.scale;
-    if (it.add) v += it.add_scale * scalar_at(it.add, it.add_dtype, r * it.add_stride + c);
-    put_scalar(it.out, it.out_dtype, r * it.out_stride + c, v);
-}
-
-// X = (a + B_ii) X + (the rest of B) X.  LAST: to the output.
-template <bool LAST, bool SPLIT, int TILE, int WP, int WQ>
-__global__ __launch_bounds__(WP* WQ* WAVE, 2) void k_apply(const Batch t)
-{
+// X = (a + B_ii) X + (the rest of B) X.
+template <bool SPLIT, int TILE_, int WP, int WQ> struct Apply : Batched<Apply<SPLIT, TILE_, WP, WQ>> {
+    static constexpr int TILE = TILE_;
     typedef Product<f16, KDOWN, KALONG, TILE, TILE, WP, WQ> G;
-    extern __shared__ char lds[];
-    const uint32_t id = xcd_order(blockIdx.x, t.tiles);
-    const Item& it = t.item[find(t, id)];
+    static constexpr int LDS = G::LDS, SETTLE_LDS = 0;
+
+    static __host__ __device__ int64_t steps(const Item& it) { return it.n / STEP; }
+    static __host__ int64_t tiles(const Item& it) { return (int64_t)((it.n + TILE - 1) / TILE) * ((it.m + TILE - 1) / TILE); }
+    static __device__ TileAt place(const Item& it, uint32_t id)
+    {
+        return tile_at(id, (uint32_t)((it.m + TILE - 1) / TILE), (uint32_t)((it.n + TILE - 1) / TILE));
+    }
+    static __device__ __forceinline__ void run(const Batch& t, const Place& at, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
+    {
+        const Item& it = t.item[at.item];
+        const int64_t n = it.n, m = it.m;
+        const uint16_t *const x = it.x(t.turn), *const b = it.b(SPLIT);
+        const Side sx{{x, x + (SPLIT ? it.plane() : 0)}, m * 2, m, n};
+        const Side sb{{b, b + (SPLIT ? n * n : 0)}, n * 2, n, n};
+        G::run(lds, sx, sb, at.p0, at.q0, s0, s1, SPLIT ? 3 : 1, acc);
+    }
+    static __device__ __forceinline__ void finish(const Batch& t, const Place& at, typename G::Sums& acc, int wave, char*);
+};
+
+template <bool SPLIT, int TILE, int WP, int WQ>
+__device__ __forceinline__ void Apply<SPLIT, TILE, WP, WQ>::finish(const Batch& t, const Place& at, typename G::Sums& acc, int wave, char*)
+{
+    const Item& it = t.item[at.item];
     const int64_t n = it.n, m = it.m, plane = n * m;
-    const TileAt tile = tile_at(id - it.first, (uint32_t)((m + TILE - 1) / TILE), (uint32_t)((n + TILE - 1) / TILE));
-    const int64_t p0 = (int64_t)tile.p * TILE, q0 = (int64_t)tile.q * TILE;
     const uint16_t* const x = it.x(t.turn);
     uint16_t* const y = it.x(!t.turn);
-    const Side sx{{x, x + (SPLIT ? plane : 0)}, m * 2, m, n};
-    const uint16_t* const b = it.b(SPLIT);
-    const Side sb{{b, b + (SPLIT ? n * n : 0)}, n * 2, n, n};
-    typename G::Sums acc;
-    G::run(lds, sx, sb, p0, q0, 0, n / STEP, SPLIT ? 3 : 1, acc);
-    const int lane = threadIdx.x % WAVE;
-    const float of_product = 1.0f / t.b_scale, last = 1.0f / t.x_scale;
+    const int lane = own_lane();
+    const float of_product = 1.0f / t.b_scale;
+    const int64_t wp = at.p0 + G::wp(wave), wq = at.q0 + G::wq(wave);
+    // X here, a row of fragments ahead: all of its loads in flight together
+    struct Row { u32x4 hi[G::FP / 2], lo[G::FP / 2]; float d; } row[2];
+    auto fetch = [&](int j, Row& r) {
+        const int64_t q = min(wq + 16 * j + lane % 16, n - 1);
+        r.d = it.d(SPLIT)[q];
+#pragma unroll
+        for (int i = 0; i < G::FP; i += 2) {
+            const uint16_t* const o = x + q * m + min(wp + 16 * i + chunk_of(lane), m - 8);
+            r.hi[i / 2] = *(const u32x4*)o;
+            r.lo[i / 2] = *(const u32x4*)(o + plane);
+        }
+    };
+    fetch(0, row[0]);
 #pragma unroll
     for (int j = 0; j < G::FQ; ++j) {
-        const int64_t q = q0 + G::wq() + 16 * j + lane % 16;
-        if (q >= n) continue;
-        const float diagonal = t.a + it.d(SPLIT)[q];
+        if (j + 1 < G::FQ) fetch(j + 1, row[(j + 1) & 1]);
+        const Row& old = row[j & 1];
+        const int64_t q = wq + 16 * j + lane % 16;
+        const float diagonal = t.a + old.d;
 #pragma unroll
-        for (int i = 0; i < G::FP; ++i) {
-            const int64_t p = p0 + G::wp() + 16 * i + lane / 16 * 4;
-            if (p >= m) continue;
-            const int64_t at = q * m + p;
-            const f32x4 old = widen4(*(const u32x2*)(x + at)) + widen4(*(const u32x2*)(x + plane + at));
-            const f32x4 v = diagonal * old + of_product * acc[i][j];
-            if constexpr (LAST) {
+        for (int i = 0; i < G::FP; i += 2) {
+            f32x4 v[2];
+            u32x2 h[2], l[2];
+            quads(old.hi[i / 2], h[0], h[1]);
+            quads(old.lo[i / 2], l[0], l[1]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int64_t row = it.tall ? p + r : q, col = it.tall ? q : p + r;
-                    if (row < it.rows && col < it.cols) put_out(it, row, col, v[r] * last);
-                }
-            } else {
-                const u32x2 hi = narrow4(v);
-                *(u32x2*)(y + at) = hi;
-                *(u32x2*)(y + plane + at) = narrow4(v - widen4(hi));
+            for (int k = 0; k < 2; ++k) {
+                v[k] = diagonal * (widen4<f16>(h[k]) + widen4<f16>(l[k])) + of_product * acc[i + k][j];
+                h[k] = narrow4<f16>(v[k]);
+                l[k] = narrow4<f16>(v[k] - widen4<f16>(h[k]));
+            }
+            const int64_t p = wp + 16 * i + chunk_of(lane), to = q * m + p;
+            const u32x4 hi = chunk(h[0], h[1]), lo = chunk(l[0], l[1]);
+            if (q < n && p < m) {
+                *(u32x4*)(y + to) = hi;
+                *(u32x4*)(y + plane + to) = lo;
             }
         }
     }
 }
 
-// Without steps: X itself.
-__global__ __launch_bounds__(256) void k_copy(const Batch t)
+template <typename J> __global__ __launch_bounds__(J::G::THREADS, 2) void k_multiply(const Batch)
 {
+    extern __shared__ char lds[];
+    multiply_tiles<J>(argument<Batch>(), lds);
+}
+
+template <typename J> __global__ __launch_bounds__(WAVE, 2) void k_settle(const Batch)
+{
+    extern __shared__ char lds[];
+    settle_tiles<J>(argument<Batch>(), lds);
+}
+
+// Outputs from X, a tile of 64 x 64 a workgroup; tall matrices' are transposed.  (In the
+// last product's epilogue they would need registers that its sums take: with tiles of 256
+// it spilled 340 and took 942 us where this and the product take 560.)
+__global__ __launch_bounds__(256) void k_store(const Batch t)
+{
+    __shared__ float tile[64][65];
     const Item& it = t.item[find(t, blockIdx.x)];
     const uint32_t id = blockIdx.x - it.first, across = it.m / 64;
-    const int64_t plane = (int64_t)it.n * it.m;
-    for (int i = 0; i < 16; ++i) {
-        const int64_t q = id / across * 64 + threadIdx.x / 64 * 16 + i, p = id % across * 64 + threadIdx.x % 64, at = q * it.m + p;
-        const int64_t row = it.tall ? p : q, col = it.tall ? q : p;
-        const f16 hi = __builtin_bit_cast(f16, it.x(0)[at]), lo = __builtin_bit_cast(f16, it.x(0)[plane + at]);
-        if (row < it.rows && col < it.cols) put_out(it, row, col, ((float)hi + (float)lo) / t.x_scale);
+    const int64_t p0 = id % across * 64, q0 = id / across * 64, plane = it.plane();
+    const int tid = threadIdx.x;
+    const float last = 1.0f / t.x_scale;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int q = i * 32 + tid / 8, p = tid % 8 * 8;
+        const uint16_t* const o = it.x(t.turn) + (q0 + q) * it.m + p0 + p;
+        float w[8], w2[8];
+        widen8(Raw<f16>{*(const u32x4*)o}, w);
+        widen8(Raw<f16>{*(const u32x4*)(o + plane)}, w2);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float v = (w[k] + w2[k]) * last;
+            if (it.tall) tile[p + k][q] = v;
+            else tile[q][p + k] = v;
+        }
+    }
+    __syncthreads();
+    const int64_t r0 = it.tall ? p0 : q0, c0 = it.tall ? q0 : p0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = i * 32 + tid / 8, c = tid % 8 * 8;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = tile[r][c + k];
+        if (r0 + r < it.rows && c0 + c < it.cols) put_out8(it, r0 + r, c0 + c, v);
     }
 }
 
@@ -317,49 +508,61 @@ template <typename F> uint32_t number(Batch& t, F tiles)
     return t.tiles = all;
 }
 
-int64_t triangle(int64_t n, int tile) { const int64_t t = (n + tile - 1) / tile; return t * (t + 1) / 2; }
-
-// Whether tiles of 256 (a workgroup a CU, 1.65 us for 64 k) or of 128 (two, 1.15 us)
-// take less, 6 us for a round of workgroups.
-template <typename F> bool large(const Batch& t, int cus, bool split, F work)
+// A product of all matrices of the batch: numbers its tiles and units, longest sums
+// first as the list is (see run), and shares them out.  us: what it takes.
+template <typename J> double lay_out(Batch& t, int cus, int pairs)
 {
-    double us[2];
-    for (int big = 0; big < 2; ++big) {
-        const int64_t room = cus * (big ? 1 : 2);
-        int64_t tiles = 0, steps = 0, longest = 0;
-        for (int i = 0; i < t.count; ++i) {
-            const auto [n, k] = work(t.item[i], big ? 256 : 128);
-            tiles += n;
-            steps += n * k;
-            longest = std::max<int64_t>(longest, k);
-        }
-        const double rounds = (double)((tiles + room - 1) / room), each = (big ? 1.65 : 1.15) * (split ? 3 : 1);
-        us[big] = rounds * 6 + each * std::max((double)longest, (double)steps / (double)std::max<int64_t>(tiles, 1) * rounds);
+    const bool big = J::TILE > 128;
+    const uint32_t room = (uint32_t)cus * (big ? 1 : 2);
+    t.tiles = 0;
+    t.units = 0;
+    int64_t longest = 0;
+    for (int i = 0; i < t.count; ++i) {
+        t.item[i].first = t.tiles;
+        t.item[i].unit = t.units;
+        t.tiles += (uint32_t)J::tiles(t.item[i]);
+        t.units += J::tiles(t.item[i]) * J::steps(t.item[i]);
+        longest = std::max(longest, J::steps(t.item[i]));
     }
-    return us[1] < us[0];
+    const double step = (big ? 1.6 : 1.05) * pairs, ends = big ? 8 : 5, parts = 12 + (big ? 45 : 25);
+    // tiles of their own: as the GPU takes them, longest first; or all shared out
+    const double even = (double)t.units / t.tiles;
+    const double rounds = (double)((t.tiles + room - 1) / room);
+    const double whole = std::max((double)longest, std::max(rounds * even, (double)t.units / std::min(room, t.tiles))) * step + rounds * ends;
+    const uint32_t workers = (uint32_t)std::min<int64_t>(room, (t.units + LEAST - 1) / LEAST);
+    const double each = (double)(t.units + workers - 1) / workers;
+    const double shared = each * step + (2 + t.tiles / room) * ends + 10 + parts * workers / room;
+    if (shared < whole && t.stream.partial) {
+        t.share = {0, workers};
+        return shared;
+    }
+    t.share = {t.tiles, 0};
+    return whole;
 }
 
-template <bool SQUARE, bool SPLIT> rf_status symmetric(Batch& t, int cus, hipStream_t st)
+template <typename J> rf_status multiply(Batch& t, hipStream_t st)
 {
-    typedef Product<f16, KALONG, KALONG, 256, 256, 2, 4> Big;
-    typedef Product<f16, KALONG, KALONG, 128, 128, 2, 2> Small;
-    struct Work { int64_t tiles, steps; };
-    const bool big = large(t, cus, SPLIT, [](const Item& it, int tile) { return Work{triangle(it.n, tile), (SQUARE ? it.n : it.m) / STEP}; });
-    const uint32_t grid = number(t, [&](const Item& it) { return triangle(it.n, big ? 256 : 128); });
-    return big ? launch<k_symmetric<SQUARE, SPLIT, 256, 2, 4>>(grid, Big::THREADS, Big::LDS, st, t)
-               : launch<k_symmetric<SQUARE, SPLIT, 128, 2, 2>>(grid, Small::THREADS, Small::LDS, st, t);
+    const rf_status s = launch<k_multiply<J>>((int64_t)t.share.whole + t.share.workers, J::G::THREADS, J::LDS, st, t);
+    if (s != RF_OK || t.share.workers < 2) return s;
+    return launch<k_settle<J>>((int64_t)(t.share.workers - 1) * J::G::WAVES, WAVE, J::SETTLE_LDS, st, t);
 }
 
-template <bool LAST, bool SPLIT> rf_status apply(Batch& t, int cus, hipStream_t st)
+// With the tiles that take less.
+template <typename Big, typename Small> rf_status product(Batch& t, int cus, int pairs, hipStream_t st)
 {
-    typedef Product<f16, KDOWN, KALONG, 256, 256, 2, 4> Big;
-    typedef Product<f16, KDOWN, KALONG, 128, 128, 2, 2> Small;
-    struct Work { int64_t tiles, steps; };
-    auto tiles = [](const Item& it, int tile) { return (int64_t)((it.n + tile - 1) / tile) * ((it.m + tile - 1) / tile); };
-    const bool big = large(t, cus, SPLIT, [&](const Item& it, int tile) { return Work{tiles(it, tile), it.n / STEP}; });
-    const uint32_t grid = number(t, [&](const Item& it) { return tiles(it, big ? 256 : 128); });
-    return big ? launch<k_apply<LAST, SPLIT, 256, 2, 4>>(grid, Big::THREADS, Big::LDS, st, t)
-               : launch<k_apply<LAST, SPLIT, 128, 2, 2>>(grid, Small::THREADS, Small::LDS, st, t);
+    const double big = lay_out<Big>(t, cus, pairs);
+    if (lay_out<Small>(t, cus, pairs) <= big) return multiply<Small>(t, st);
+    lay_out<Big>(t, cus, pairs);
+    return multiply<Big>(t, st);
+}
+
+template <bool SPLIT> rf_status step(Batch& t, int cus, hipStream_t st)
+{
+    constexpr int PAIRS = SPLIT ? 3 : 1;
+    rf_status s = product<Symmetric<false, SPLIT, 256, 2, 4>, Symmetric<false, SPLIT, 128, 2, 2>>(t, cus, PAIRS, st);
+    if (s == RF_OK) s = product<Symmetric<true, SPLIT, 256, 2, 4>, Symmetric<true, SPLIT, 128, 2, 2>>(t, cus, PAIRS, st);
+    if (s != RF_OK) return s;
+    return product<Apply<SPLIT, 256, 2, 4>, Apply<SPLIT, 128, 2, 2>>(t, cus, PAIRS, st);
 }
 
 // The largest singular value, and the largest |b s^2 + c s^4|, that the steps can
@@ -416,19 +619,39 @@ Item item_of(const Matrix& m)
     return it;
 }
 
-int64_t bytes_of(const Matrix& m) { return up(item_of(m).bytes(split_of(m)), 256) + PARTS * 8; }
+int64_t bytes_of(const Matrix& m) { return up(item_of(m).bytes(split_of(m)), 256); }
 
-// The matrices from `at` on that are worked on together.
-int64_t batch_end(const Matrix* list, int64_t count, int64_t at, int64_t& bytes)
+// The matrices from `at` on that are worked on together, and what they need: sums of
+// squares, the parts of split tiles, their buffers.
+struct Needs {
+    int64_t end, sums, parts, buffers;
+    int64_t all() const { return sums + parts + buffers; }
+};
+
+Needs needs_of(const Matrix* list, int64_t count, int64_t at, int cus)
 {
-    int64_t end = at;
-    bytes = 0;
-    for (; end < count && end - at < MAX; ++end) {
-        const int64_t more = list[end].rows && list[end].cols ? bytes_of(list[end]) : PARTS * 8;
-        if (end > at && (bytes + more > HELD || split_of(list[end]) != split_of(list[at]))) break;
-        bytes += more;
+    Needs need{at, 0, 0, 0};
+    int64_t units[2][3] = {};  // of tiles of 128 and 256; of the three products
+    for (; need.end < count && need.end - at < MAX; ++need.end) {
+        const Matrix& m = list[need.end];
+        const bool some = m.rows && m.cols;
+        const int64_t more = some ? bytes_of(m) : 0;
+        if (need.end > at && (need.buffers + more > HELD || split_of(m) != split_of(list[at]))) break;
+        need.buffers += more;
+        if (!some) continue;
+        const Item it = item_of(m);
+        for (int big = 0; big < 2; ++big) {
+            const int64_t tile = big ? 256 : 128, n = (it.n + tile - 1) / tile, w = (it.m + tile - 1) / tile;
+            units[big][0] += n * (n + 1) / 2 * (it.m / STEP);
+            units[big][1] += n * (n + 1) / 2 * (it.n / STEP);
+            units[big][2] += n * w * (it.n / STEP);
+        }
     }
-    return end;
+    for (int big = 0; big < 2; ++big)
+        for (int64_t u : units[big])
+            need.parts = std::max(need.parts, std::min<int64_t>(cus * (big ? 1 : 2), (u + LEAST - 1) / LEAST) * 2 * (big ? 256 * 256 : 128 * 128) * 4);
+    need.sums = (need.end - at) * PARTS * 8;
+    return need;
 }
 
 }  // namespace
@@ -454,15 +677,17 @@ rf_status check(const Matrix* list, int64_t count, const Method& how) noexcept
     return RF_OK;
 }
 
-int64_t workspace(const Matrix* list, int64_t count) noexcept
+rf_status workspace(const Matrix* list, int64_t count, int64_t* bytes) noexcept
 {
-    int64_t most = 0;
+    int cus = 0;
+    if (const rf_status s = rf::device_cus(&cus); s != RF_OK) return s;
+    *bytes = 0;
     for (int64_t at = 0; at < count;) {
-        int64_t bytes;
-        at = batch_end(list, count, at, bytes);
-        most = std::max(most, bytes);
+        const Needs need = needs_of(list, count, at, cus);
+        at = need.end;
+        *bytes = std::max(*bytes, need.all());
     }
-    return most;
+    return RF_OK;
 }
 
 rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hipStream_t st, Source source, void* context) noexcept
@@ -472,16 +697,16 @@ rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hi
     const Bounds most = bounds_of(how);
     auto scale = [](double bound) { return (float)std::exp2(std::min(15.0, std::floor(std::log2(60000.0 / std::max(bound, 1e-3))))); };
     for (int64_t at = 0; at < count;) {
-        int64_t bytes;
-        const int64_t end = batch_end(list, count, at, bytes);
+        const Needs need = needs_of(list, count, at, cus);
+        const int64_t end = need.end;
         const bool split = split_of(list[at]);
         Batch t{};
         t.eps = how.eps;
         t.x_scale = scale(most.x);
         t.a_scale = scale(most.x * most.x);
         t.b_scale = scale(most.b);
-        t.sums = (double*)ws;
-        int64_t used = (end - at) * PARTS * 8;
+        t.stream.partial = (float*)(ws + need.sums);
+        int64_t used = need.sums + need.parts;
         int64_t which[MAX];
         float* u[MAX];
         double* sums[MAX];
@@ -490,7 +715,7 @@ rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hi
             if (!m.rows || !m.cols) continue;
             Item& it = t.item[t.count];
             it = item_of(m);
-            it.sums = sums[t.count] = t.sums + (int64_t)t.count * PARTS;
+            it.sums = sums[t.count] = (double*)ws + (int64_t)t.count * PARTS;
             it.buffers = (uint16_t*)(ws + used);
             used += up(it.bytes(split), 256);
             which[t.count] = i;
@@ -504,25 +729,24 @@ rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hi
         }
         at = end;
         if (!t.count) continue;
+        // those with the longest sums first: what is left at a launch's end is short
+        std::stable_sort(t.item, t.item + t.count, [](const Item& x, const Item& y) { return x.m > y.m; });
         rf_status s = RF_OK;
         s = source ? source(context, which, t.count, u, sums, st) : launch<k_squares>((int64_t)t.count * PARTS, 256, 0, st, t);
         if (s != RF_OK) return s;
         const uint32_t squares = number(t, [](const Item& it) { return (int64_t)it.n / 64 * (it.m / 64); });
         s = launch<k_load>(squares, 256, 0, st, t);
         if (s != RF_OK) return s;
-        if (!how.steps) s = launch<k_copy>(squares, 256, 0, st, t);
         for (int i = 0; i < how.steps && s == RF_OK; ++i) {
             t.a = how.coefficients[3 * i];
             t.b = how.coefficients[3 * i + 1];
             t.c = how.coefficients[3 * i + 2];
             t.turn = i & 1;
-            const bool last = i + 1 == how.steps;
-            s = split ? symmetric<false, true>(t, cus, st) : symmetric<false, false>(t, cus, st);
-            if (s == RF_OK) s = split ? symmetric<true, true>(t, cus, st) : symmetric<true, false>(t, cus, st);
-            if (s != RF_OK) break;
-            if (split) s = last ? apply<true, true>(t, cus, st) : apply<false, true>(t, cus, st);
-            else s = last ? apply<true, false>(t, cus, st) : apply<false, false>(t, cus, st);
+            s = split ? step<true>(t, cus, st) : step<false>(t, cus, st);
         }
+        t.turn = how.steps & 1;
+        number(t, [](const Item& it) { return (int64_t)it.n / 64 * (it.m / 64); });
+        if (s == RF_OK) s = launch<k_store>(squares, 256, 0, st, t);
         if (s != RF_OK) return s;
     }
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return rf::report_hip(e, "orthogonalisation");
@@ -553,8 +777,7 @@ rf_status rf_orthogonalize_workspace(const rf_orthogonal_matrix* matrices, int32
     rfs::Matrix list[256];
     convert(matrices, count, list);
     if (const rf_status s = rfs::check(list, count, {0, nullptr, 0.0f}); s != RF_OK) return s;
-    *bytes = rfs::workspace(list, count);
-    return RF_OK;
+    return rfs::workspace(list, count, bytes);
 }
 
 rf_status rf_orthogonalize(const rf_orthogonal_matrix* matrices, int32_t count, int32_t steps, const float* coefficients, float eps,
@@ -565,7 +788,8 @@ rf_status rf_orthogonalize(const rf_orthogonal_matrix* matrices, int32_t count, 
     convert(matrices, count, list);
     const rfs::Method how{steps, coefficients, eps};
     if (const rf_status s = rfs::check(list, count, how); s != RF_OK) return s;
-    const int64_t need = rfs::workspace(list, count);
+    int64_t need = 0;
+    if (const rf_status s = rfs::workspace(list, count, &need); s != RF_OK) return s;
     if (need && (!workspace || need > workspace_bytes)) return report(RF_ERR_INVALID, "workspace too small");
     if ((uintptr_t)workspace & 255) return report(RF_ERR_INVALID, "workspace must be 256-byte aligned");
     return rfs::run(list, count, how, (char*)workspace, (hipStream_t)stream);
