@@ -49,8 +49,39 @@ struct Scalars {
     int32_t count, pad[3];
     uint32_t hidden_top, weight_top;  // f32: bits of the largest finite magnitudes
     uint32_t pad2[2];
-    uint32_t dz_top[1];               // of each piece: bits of the largest row factor
 };
+
+// Of each piece of tokens: its products' shares, which depend on how many tokens count,
+// and bits of the largest row factor.
+struct Piece {
+    Share logits, dhidden, dweight;
+    uint32_t dz_top;
+    uint32_t pad[2];
+};
+
+// The products of a piece, for k_select.
+struct Products {
+    int64_t rows, vocab, hidden, logits_steps, dhidden_steps;
+    int32_t pieces, pairs, grad, cus;
+    int32_t logits_tile, dhidden_tile, dweight_tile;
+};
+
+__device__ __forceinline__ Piece piece_of(const Products& p, int64_t count, int64_t piece)
+{
+    const int64_t rows = max(min(count - piece * p.rows, p.rows), (int64_t)0), steps = (rows + STEP - 1) / STEP;
+    auto tiles = [](int64_t x, int64_t y, int tile) { return (uint32_t)(((x + tile - 1) / tile) * ((y + tile - 1) / tile)); };
+    auto room = [&](int tile) { return (uint32_t)(p.cus * (tile > 128 ? 1 : 2)); };
+    auto share = [&](int64_t x, int64_t y, int64_t n, int tile) { return share_of(tiles(x, y, tile), n, room(tile), tile, p.pairs); };
+    Piece out{};
+    out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile);
+    if (!p.grad) return out;
+    out.dhidden = share(p.hidden, rows, p.dhidden_steps, p.dhidden_tile);
+    // without tokens there is nothing to add, but what the pieces have summed is to be
+    // written by the first and rounded by the last
+    if (steps) out.dweight = share(p.hidden, p.vocab, steps, p.dweight_tile);
+    else if (piece == 0 || piece + 1 == p.pieces) out.dweight = {tiles(p.hidden, p.vocab, p.dweight_tile), 0, 1};
+    return out;
+}
 
 // The power of two that brings magnitudes up to `top` below 2^15 (1: nothing finite, or zero).
 __device__ __forceinline__ float scale_of(uint32_t top)
@@ -80,7 +111,7 @@ constexpr int SELECT = 1024, RUN = 8;  // threads, tokens of a thread at a time
 template <typename I>
 __global__ __launch_bounds__(SELECT) void k_select(const I* __restrict__ targets, int64_t tokens, int64_t ignore, int64_t vocab,
                                                   float* __restrict__ loss, int32_t* __restrict__ order,
-                                                  int32_t* __restrict__ target, Scalars* sc, int pieces)
+                                                  int32_t* __restrict__ target, Scalars* sc, Piece* pieces, Products products)
 {
     __shared__ int32_t part[2][SELECT / WAVE];
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
@@ -126,7 +157,7 @@ __global__ __launch_bounds__(SELECT) void k_select(const I* __restrict__ targets
         sc->count = before;
         sc->hidden_top = sc->weight_top = 0;
     }
-    for (int i = tid; i < pieces; i += SELECT) sc->dz_top[i] = 0;
+    for (int i = tid; i < products.pieces; i += SELECT) pieces[i] = piece_of(products, before, i);
 }
 
 // Largest finite magnitude of rows (of those that count, where order is given).
@@ -211,14 +242,15 @@ struct Logits {
     float2* stats;                 // [rows, blocks] m, s
     float* picked;                 // [rows] the target's logit
     void* e;                       // [rows, pitch] exp(z - m)
-    uint32_t tiles_p;
-    Stream stream;
+    uint32_t tiles_p, room;
+    float* partial;
+    const Piece* piece;
 };
 
 // Tiles of equal steps in bands (tile_at), of which a packed piece of tokens has as
 // many as there are tokens that count.
 struct Even {
-    int64_t p0, q0, first, steps;
+    int64_t p0, q0, steps;
 };
 
 template <typename H, typename E, int TILE, int WP, int WQ> struct LogitsJob {
@@ -226,20 +258,18 @@ template <typename H, typename E, int TILE, int WP, int WQ> struct LogitsJob {
     typedef Even Tile;
     typedef Product<H, KALONG, KALONG, TILE, TILE, WP, WQ> G;
     static constexpr int LDS = G::LDS;
+    // The argument in registers: read where it lies it takes scalar ones past their end
+    // here (8192 x 50257 x 768 with exponentials 741 us, so 857), while the gradients'
+    // kernels need it there.
+    static constexpr bool FEW_SCALARS = true;
 
     static __device__ int64_t count(const Logits& a) { return max(min((int64_t)a.sc->count - a.first, a.rows), (int64_t)0); }
     static __device__ uint32_t tiles_q(const Logits& a) { return (uint32_t)((count(a) + TILE - 1) / TILE); }
-    static __device__ Shares shares(const Logits& a)
+    static __device__ Share share(const Logits& a) { return a.piece->logits; }
+    static __device__ Even tile(const Logits& a, uint32_t id)
     {
-        return rfp::shares(a.tiles_p * tiles_q(a), a.steps, a.stream.room, a.stream.partial != nullptr, TILE, a.pairs);
-    }
-    static __device__ int64_t first(const Logits& a, uint32_t tile) { return tile * a.steps; }
-    static __device__ int64_t units(const Logits& a) { return (int64_t)a.tiles_p * tiles_q(a) * a.steps; }
-    static __device__ Even locate(const Logits& a, int64_t unit)
-    {
-        const uint32_t id = (uint32_t)(unit / a.steps);
         const TileAt t = tile_at(id, a.tiles_p, tiles_q(a));
-        return {(int64_t)t.p * TILE, (int64_t)t.q * TILE, id * a.steps, a.steps};
+        return {(int64_t)t.p * TILE, (int64_t)t.q * TILE, a.steps};
     }
     static __device__ __forceinline__ void run(const Logits& a, const Even& t, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
     {
@@ -266,12 +296,15 @@ __device__ __forceinline__ void LogitsJob<H, E, TILE, WP, WQ>::finish(const Logi
     }
     if (p0 + wp + TILE / WP > a.vocab) {
 #pragma unroll
-        for (int j = 0; j < G::FQ; ++j)
+        for (int j = 0; j < G::FQ; ++j) {
+            int left = (int)max(min(a.vocab - v0, (int64_t)TILE), (int64_t)0);
+            asm volatile("" : "+v"(left));  // (no masks of 32 comparisons to be kept from one j to the next)
 #pragma unroll
             for (int i = 0; i < G::FP; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (v0 + 16 * i + r >= a.vocab) acc[i][j][r] = -__builtin_inff();
+                    if (16 * i + r >= left) acc[i][j][r] = -__builtin_inff();
+        }
     }
     constexpr float LOG2E = 1.44269504088896341f;
     int32_t target[G::FQ];  // loaded together
@@ -328,24 +361,26 @@ __device__ __forceinline__ void LogitsJob<H, E, TILE, WP, WQ>::finish(const Logi
     }
 }
 
-template <typename J> __global__ __launch_bounds__(J::G::THREADS, 2) void k_multiply(const typename J::Args)
+template <typename J> __global__ __launch_bounds__(J::G::THREADS, 2) void k_multiply(const typename J::Args a)
 {
     extern __shared__ char lds[];
-    multiply_tiles<J>(argument<typename J::Args>(), lds);
+    if constexpr (J::FEW_SCALARS) multiply_tiles<J>(a, lds);
+    else multiply_tiles<J>(argument<typename J::Args>(), lds);
 }
 
-template <typename J> __global__ __launch_bounds__(WAVE, 2) void k_settle(const typename J::Args)
+template <typename J> __global__ __launch_bounds__(WAVE, 2) void k_settle(const typename J::Args a)
 {
-    settle_tiles<J>(argument<typename J::Args>(), nullptr);
+    if constexpr (J::FEW_SCALARS) settle_tiles<J>(a, nullptr);
+    else settle_tiles<J>(argument<typename J::Args>(), nullptr);
 }
 
 struct Rows {
     int64_t first, rows, pitch;
     int32_t blocks, shift;  // entries of a block: 1 << shift
-    int32_t piece, reduction;
+    int32_t reduction;
     float z_loss;
     const Scalars* sc;
-    uint32_t* dz_top;
+    Piece* piece;
     const int32_t *order, *target;
     const float2* stats;
     const float *picked, *dloss;
@@ -393,7 +428,7 @@ __global__ __launch_bounds__(256) void k_rows(const Rows a)
     __shared__ uint32_t tops[4];
     if (lane == 0) tops[threadIdx.x / WAVE] = most;
     __syncthreads();
-    if (threadIdx.x == 0) raise(a.dz_top + a.piece, max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+    if (threadIdx.x == 0) raise(&a.piece->dz_top, max(max(tops[0], tops[1]), max(tops[2], tops[3])));
 }
 
 // The sum or the mean of the losses that count: one workgroup, in a fixed order, in f64.
@@ -437,7 +472,7 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
         }
         return;
     }
-    const float scale = dz_scale(a.dz_top[a.piece], __is_same(P, bf16));
+    const float scale = dz_scale(a.piece->dz_top, __is_same(P, bf16));
     const float m = a.top[q], f = a.factor[q] * scale;
     for (int b = threadIdx.x; b < a.blocks; b += 256) {
         const float top = a.stats[q * a.blocks + b].x;
@@ -477,20 +512,20 @@ struct Grad {
     int64_t cols, rows;            // of the output: p below cols, q below rows
     int64_t first, piece_rows;     // packed tokens of this piece
     int64_t steps;                 // of the sum; 0: the tokens that count
-    int32_t pairs, dtype, piece;
+    int32_t pairs, dtype;
     const Scalars* sc;
-    const uint32_t* dz_top;
+    const Piece* piece;
     const int32_t* order;          // dhidden: the output's row of packed token q; NULL: dweight
     void* out;
     float* sums;                   // dweight, several pieces: f32 sums so far (may be out)
     int32_t begin, end;            // the first piece, the last one
-    uint32_t tiles_p;
-    Stream stream;
+    uint32_t tiles_p, room;
+    float* partial;
 };
 
 __device__ __forceinline__ float unscale_of(const Grad& a)
 {
-    float u = 1.0f / dz_scale(a.dz_top[a.piece], a.dtype == RF_BF16);
+    float u = 1.0f / dz_scale(a.piece->dz_top, a.dtype == RF_BF16);
     if (a.pairs > 1) u *= inverse(scale_of(a.order ? a.sc->weight_top : a.sc->hidden_top));
     return u;
 }
@@ -536,28 +571,19 @@ struct Finish {
 template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
     typedef Grad Args;
     typedef Even Tile;
-    typedef Product<H, KDOWN, LQ, TILE, TILE, WP, WQ> G;
+    typedef Product<H, KDOWN, LQ, TILE, TILE, WP, WQ, LQ == KALONG> G;
     static constexpr int LDS = G::LDS;
+    static constexpr bool FEW_SCALARS = false;
 
     static __device__ int64_t count(const Grad& a) { return max(min((int64_t)a.sc->count - a.first, a.piece_rows), (int64_t)0); }
     static __device__ int64_t rows(const Grad& a) { return LQ == KALONG ? count(a) : a.rows; }
     static __device__ int64_t steps(const Grad& a) { return LQ == KALONG ? a.steps : (count(a) + STEP - 1) / STEP; }
     static __device__ uint32_t tiles_q(const Grad& a) { return (uint32_t)((rows(a) + TILE - 1) / TILE); }
-    static __device__ Shares shares(const Grad& a)
+    static __device__ Share share(const Grad& a) { return LQ == KALONG ? a.piece->dhidden : a.piece->dweight; }
+    static __device__ Even tile(const Grad& a, uint32_t id)
     {
-        // dweight of a piece without tokens: nothing to add, but what was summed is to be rounded
-        if (LQ == KDOWN && !steps(a)) return {a.begin || a.end ? a.tiles_p * tiles_q(a) : 0, 0};
-        return rfp::shares(a.tiles_p * tiles_q(a), steps(a), a.stream.room, a.stream.partial != nullptr, TILE, a.pairs);
-    }
-    // (a unit a tile where there are no steps)
-    static __device__ int64_t each(const Grad& a) { return max(steps(a), (int64_t)1); }
-    static __device__ int64_t first(const Grad& a, uint32_t tile) { return tile * each(a); }
-    static __device__ int64_t units(const Grad& a) { return (int64_t)a.tiles_p * tiles_q(a) * each(a); }
-    static __device__ Even locate(const Grad& a, int64_t unit)
-    {
-        const uint32_t id = (uint32_t)(unit / each(a));
         const TileAt t = tile_at(id, a.tiles_p, tiles_q(a));
-        return {(int64_t)t.p * TILE, (int64_t)t.q * TILE, id * each(a), steps(a)};
+        return {(int64_t)t.p * TILE, (int64_t)t.q * TILE, steps(a)};
     }
     static __device__ __forceinline__ void run(const Grad& a, const Even& t, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
     {
@@ -601,35 +627,32 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 // tiles that the GPU holds at a time, 256 wide one a CU or 128 wide two, and 6 or 4 for a
 // tile's start and end.
 struct Shape {
-    bool big;
+    int tile;
     uint32_t tiles_p, room;
 };
 
 Shape shape_of(int64_t cols, int64_t rows, int64_t steps, int pairs, int cus)
 {
-    double us[2];
+    double ns[2];
     for (int big = 0; big < 2; ++big) {
         const int64_t tile = big ? 256 : 128, tiles = ((cols + tile - 1) / tile) * ((rows + tile - 1) / tile);
         const uint32_t room = (uint32_t)cus * (big ? 1 : 2);
-        const double step = (big ? 1.6 : 1.05) * pairs, ends = big ? 6 : 4;
-        const Shares sh = rfp::shares((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, true, (int)tile, pairs);
-        us[big] = (double)((sh.whole + room - 1) / room) * ((double)steps * step + ends);
-        if (sh.workers) us[big] += (double)((tiles - sh.whole) * steps + sh.workers - 1) / sh.workers * step + 2 * ends + 10 + 50.0 * sh.workers / room;
+        ns[big] = ns_of(share_of((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, (int)tile, pairs), steps, room, (int)tile, pairs);
     }
-    const bool big = us[1] < us[0];
-    return {big, (uint32_t)((cols + (big ? 255 : 127)) / (big ? 256 : 128)), (uint32_t)cus * (big ? 1 : 2)};
+    const int tile = ns[1] < ns[0] ? 256 : 128;
+    return {tile, (uint32_t)((cols + tile - 1) / tile), (uint32_t)cus * (tile > 128 ? 1 : 2)};
 }
 
 // Bytes of the parts of split tiles.
-int64_t parts_of(const Shape& s) { return (int64_t)s.room * 2 * (s.big ? 256 * 256 : 128 * 128) * 4; }
+int64_t parts_of(const Shape& s) { return (int64_t)s.room * PARTS_ROOM * s.tile * s.tile * 4; }
 
 struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
     bool own_weight, f32, grad;
-    int32_t blocks, shift, pairs;
+    int32_t blocks, shift, pairs, cus;
     Shape logits, dhidden, dweight;
     // offsets in the workspace
-    int64_t scalars, order, target, stats, picked, top, factor, at_target, hidden, weight, e, dz, sums, partial, bytes;
+    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, hidden, weight, e, dz, sums, partial, bytes;
 };
 
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
@@ -637,6 +660,7 @@ bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype 
 Plan plan_of(const rf_cross_entropy& a, int cus)
 {
     Plan p{};
+    p.cus = cus;
     p.f32 = a.dtype == RF_F32;
     p.grad = a.dweight != nullptr;
     p.pairs = p.f32 ? 3 : 1;
@@ -646,7 +670,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.own_weight = p.f32 || a.hidden % STEP || a.weight_stride % 8 || ((uintptr_t)a.weight & 15) || a.weight_stride * 2 >= (1 << 24);
     const int64_t planes = p.f32 ? 2 : 1, steps = p.pad / STEP;
     p.logits = shape_of(a.vocab, a.tokens, steps, p.pairs, cus);
-    p.shift = p.logits.big ? 7 : 6;
+    p.shift = p.logits.tile > 128 ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
     const int64_t each = p.grad ? p.vpad * (p.f32 ? 8 : 2) : p.blocks * 8, most = p.grad ? PIECE : STATS;
     // pieces of equal numbers of whole tiles
@@ -655,7 +679,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.rows = p.pieces == 1 ? std::max<int64_t>(1, a.tokens) : std::min(fit, up((a.tokens + p.pieces - 1) / p.pieces, 256));
     p.pieces = std::max<int64_t>(1, (a.tokens + p.rows - 1) / p.rows);
     p.logits = shape_of(a.vocab, p.rows, steps, p.pairs, cus);
-    p.shift = p.logits.big ? 7 : 6;
+    p.shift = p.logits.tile > 128 ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -664,7 +688,8 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         return from;
     };
     const int64_t held = up(p.rows, STEP);
-    p.scalars = take(sizeof(Scalars) + p.pieces * 4);
+    p.scalars = take(sizeof(Scalars));
+    p.piece = take(sizeof(Piece) * p.pieces);
     p.order = take(a.tokens * 4);
     p.target = take(a.tokens * 4);
     p.stats = take(p.rows * p.blocks * 8);
@@ -712,27 +737,29 @@ template <auto K, typename... A> rf_status launch(int64_t grid, int threads, siz
     return RF_OK;
 }
 
-// A product's launch, and the one that settles split tiles.
+// A product's launch, and the one that settles split tiles (which of them are is known on
+// the device alone).
 template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, const typename J::Args& a, hipStream_t st)
 {
-    const rf_status s = launch<k_multiply<J>>(tiles + shape.room, J::G::THREADS, J::LDS, st, a);
-    return s != RF_OK ? s : launch<k_settle<J>>((int64_t)shape.room * J::G::WAVES, WAVE, 0, st, a);
+    const rf_status s = launch<k_multiply<J>>(tiles + PARTS_ROOM * shape.room, J::G::THREADS, J::LDS, st, a);
+    return s != RF_OK ? s : launch<k_settle<J>>((int64_t)std::min<int64_t>(tiles, shape.room) * J::G::WAVES, WAVE, 0, st, a);
 }
 
-int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles_p * ((rows + (shape.big ? 255 : 127)) / (shape.big ? 256 : 128)); }
+int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles_p * ((rows + shape.tile - 1) / shape.tile); }
 
 template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
 {
     const int64_t tiles = tiles_of(p.logits, a.rows);
-    return p.logits.big ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st) : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st);
+    return p.logits.tile > 128 ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st) : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st);
 }
 
 template <typename H, Layout LQ> rf_status product(const Shape& shape, float* partial, Grad& a, hipStream_t st)
 {
     a.tiles_p = shape.tiles_p;
-    a.stream = {shape.room, partial};
+    a.room = shape.room;
+    a.partial = partial;
     const int64_t tiles = tiles_of(shape, a.rows);
-    return shape.big ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st) : multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st);
+    return shape.tile > 128 ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st) : multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st);
 }
 
 template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const Plan& p, char* ws, hipStream_t st)
@@ -743,11 +770,13 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
     int32_t* const target = (int32_t*)(ws + p.target);
     uint16_t* const hidden = (uint16_t*)(ws + p.hidden);
     const int64_t all = up(a.tokens, STEP), plane = all * p.pad;
+    const Products products{p.rows, a.vocab, a.hidden, p.pad / STEP, p.vpad / STEP, (int32_t)p.pieces, p.pairs, p.grad, p.cus,
+                            p.logits.tile, p.dhidden.tile, p.dweight.tile};
     rf_status s = a.target_bits == 64
         ? launch<k_select<int64_t>>(1, SELECT, 0, st, (const int64_t*)a.targets, a.tokens, a.ignore_index, a.vocab, a.loss, order,
-                                    target, sc, (int)p.pieces)
+                                    target, sc, (Piece*)(ws + p.piece), products)
         : launch<k_select<int32_t>>(1, SELECT, 0, st, (const int32_t*)a.targets, a.tokens, a.ignore_index, a.vocab, a.loss, order,
-                                    target, sc, (int)p.pieces);
+                                    target, sc, (Piece*)(ws + p.piece), products);
     if (s != RF_OK) return s;
     const int32_t* const none = nullptr;
     if constexpr (sizeof(T) == 4) {
@@ -775,6 +804,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         const int64_t first = piece * p.rows, rows = std::max<int64_t>(0, std::min(p.rows, a.tokens - first));
         const int64_t held = up(rows, STEP);
         uint16_t* const h = hidden + first * p.pad;
+        Piece* const piece_info = (Piece*)(ws + p.piece) + piece;
         Side x{{h, h + (planes - 1) * plane}, p.pad * 2, all - first, all - first};
         Logits l{};
         l.weight = w;
@@ -792,7 +822,9 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         l.picked = (float*)(ws + p.picked);
         l.e = ws + p.e;
         l.tiles_p = p.logits.tiles_p;
-        l.stream = {p.logits.room, (float*)(ws + p.partial)};
+        l.room = p.logits.room;
+        l.partial = (float*)(ws + p.partial);
+        l.piece = piece_info;
         if (!p.grad) s = logits<H, void>(p, l, st);
         else if (p.f32) s = logits<H, float>(p, l, st);
         else s = logits<H, f16>(p, l, st);
@@ -803,10 +835,9 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         r.pitch = p.vpad;
         r.blocks = p.blocks;
         r.shift = p.shift;
-        r.piece = (int32_t)piece;
+        r.piece = piece_info;
         r.z_loss = a.z_loss;
         r.sc = sc;
-        r.dz_top = sc->dz_top;
         r.order = order;
         r.target = target;
         r.stats = l.stats;
@@ -830,8 +861,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         Grad g{};
         Side dz{{r.dz, p.f32 ? (const void*)r.dz_low : r.dz}, p.vpad * 2, held, held};
         g.sc = sc;
-        g.dz_top = sc->dz_top;
-        g.piece = (int32_t)piece;
+        g.piece = piece_info;
         g.first = first;
         g.piece_rows = rows;
         g.pairs = p.pairs;

@@ -46,7 +46,7 @@ struct Side {
     const void* base[2];
     int64_t pitch;   // bytes, a multiple of 16 below 2^24
     int64_t extent;  // x that may be read: KDOWN at least 8 and a multiple of 8
-    int64_t depth;   // KDOWN: rows k that may be read, at least 1
+    int64_t depth;   // KDOWN, where a product ends in half a step: rows k that may be read, at least 1
 };
 
 template <typename H> struct Eight;
@@ -100,7 +100,9 @@ __device__ __forceinline__ int unit(int k) { return (k & 3) | ((k >> 3) & 1) << 
 
 // A side of a tile: T of its x, staged by W waves, read by waves that hold F
 // fragments of 16 x each, the first of them at x `mine`.
-template <typename H, Layout L, int T, int W, int F> struct Staged {
+// RAGGED: the last step may have fewer rows k than 64 (KDOWN); its last one stands for those behind
+// it, which meet zeros of the other side.
+template <typename H, Layout L, int T, int W, int F, bool RAGGED> struct Staged {
     typedef typename Eight<H>::type h8;
     static constexpr int BYTES = T * ROW, N = BYTES / 1024 / W;  // loads of a wave
     static_assert(N * W * 1024 == BYTES, "whole wave loads");
@@ -110,6 +112,7 @@ template <typename H, Layout L, int T, int W, int F> struct Staged {
     const char* base;  // the step to be loaded next
     int64_t pitch;
     int k0;            // KDOWN: row of this lane in the wave's first load
+    int left;          // RAGGED: rows from the step on, or 64
 
     __device__ __forceinline__ void set(const Side& s, int64_t x0, int wave, int mine, int lane)
     {
@@ -141,15 +144,24 @@ template <typename H, Layout L, int T, int W, int F> struct Staged {
     {
         const char* const b = (const char*)s.base[plane];
         base = L == KALONG ? b + x0 * s.pitch + step * ROW : b + step * STEP * s.pitch;
+        if (RAGGED) rows(s, step);
     }
-    __device__ __forceinline__ void next() { base += L == KALONG ? (int64_t)ROW : STEP * pitch; }
-    // load j of the step at `base`, of which KDOWN has `left` rows
-    __device__ __forceinline__ void load(uint32_t slot, int wave, int j, int64_t left) const
+    __device__ __forceinline__ void next(const Side& s, int64_t step)
+    {
+        base += L == KALONG ? (int64_t)ROW : STEP * pitch;
+        if (RAGGED) rows(s, step);
+    }
+    __device__ __forceinline__ void rows(const Side& s, int64_t step)
+    {
+        left = __builtin_amdgcn_readfirstlane((int)min(s.depth - step * STEP, (int64_t)STEP));
+    }
+    // load j of the step at `base`
+    __device__ __forceinline__ void load(uint32_t slot, int wave, int j) const
     {
         const uint32_t to = slot + (wave * N + j) * 1024;
-        if constexpr (L == KDOWN) {
+        if constexpr (RAGGED) {
             if (left < STEP) {  // rows behind the last: that one again
-                const int k = k0 + j * (512 / T), over = max(k - (int)left + 1, 0);
+                const int k = k0 + j * (512 / T), over = max(k - left + 1, 0);
                 load_to_lds(to, off[j] - (uint32_t)(over * pitch), base);
                 return;
             }
@@ -174,11 +186,11 @@ template <typename H, Layout L, int T, int W, int F> struct Staged {
 };
 
 // A tile of TP x TQ by WP x WQ waves.
-template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> struct Product {
+template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ, bool RAGGED = false> struct Product {
     static constexpr int WAVES = WP * WQ, THREADS = WAVES * WAVE;
     static constexpr int FP = TP / WP / 16, FQ = TQ / WQ / 16;  // fragments of a wave
-    typedef Staged<H, LP, TP, WAVES, FP> P;
-    typedef Staged<H, LQ, TQ, WAVES, FQ> Q;
+    typedef Staged<H, LP, TP, WAVES, FP, RAGGED && LP == KDOWN> P;  // (Q's rows are whole steps)
+    typedef Staged<H, LQ, TQ, WAVES, FQ, false> Q;
     typedef typename Eight<H>::type h8;
     static constexpr int SLOT = P::BYTES + Q::BYTES, LDS = 2 * SLOT;
     static_assert(LDS <= 160 * 1024, "");
@@ -207,9 +219,8 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
             for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         p0 = uniform(p0);
         q0 = uniform(q0);
-        s0 = uniform(s0);
-        s1 = uniform(s1);
-        const int64_t steps = (s1 - s0) * pairs;
+        const int from = __builtin_amdgcn_readfirstlane((int)s0), to = __builtin_amdgcn_readfirstlane((int)s1);
+        const int steps = (to - from) * __builtin_amdgcn_readfirstlane(pairs);
         if (steps <= 0) return;
         const int lane = own_lane(), w = wave();
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)lds);
@@ -217,23 +228,25 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
         Q q;
         p.set(sp, p0, w, wp(w), lane);
         q.set(sq, q0, w, wq(w), lane);
-        int pair = 0;
-        int64_t ahead = s0;  // of the step to be loaded next
+        int pair = 0, ahead = from;  // of the step to be loaded next
         auto seek = [&] {
             p.seek(sp, pair == 2, p0, ahead);
             q.seek(sq, pair == 1, q0, ahead);
         };
         auto next = [&] {
-            p.next();
-            q.next();
-            if (++ahead == s1 && ++pair < pairs) {
-                ahead = s0;
-                seek();
+            ++ahead;
+            if (ahead == to) {
+                ahead = from;
+                ++pair;
+                if (pair < pairs) seek();
+            } else {
+                p.next(sp, ahead);
+                q.next(sq, ahead);
             }
         };
         auto load = [&](uint32_t slot, int j) {
-            if (j < P::N) p.load(lds0 + slot, w, j, sp.depth - ahead * STEP);
-            else q.load(lds0 + slot + P::BYTES, w, j - P::N, sq.depth - ahead * STEP);
+            if (j < P::N) p.load(lds0 + slot, w, j);
+            else q.load(lds0 + slot + P::BYTES, w, j - P::N);
         };
         constexpr int LOADS = P::N + Q::N;
         seek();
@@ -299,11 +312,11 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ> stru
             now ^= SLOT;
         };
         if constexpr (LATE) {
-            for (int64_t s = 2; s < steps; ++s) step(std::true_type{});
+            for (int s = 2; s < steps; ++s) step(std::true_type{});
             if (steps > 1) step(std::false_type{});
             step(std::false_type{});
         } else {
-            for (int64_t s = 0; s < steps; ++s) step(s + 2 < steps);
+            for (int s = 0; s < steps; ++s) step(s + 2 < steps);
         }
         static_assert((SLOT & (SLOT - 1)) == 0, "the slots' offsets are 0 and SLOT");
     }
@@ -352,17 +365,16 @@ template <typename T> __device__ __forceinline__ f32x4 widen4(u32x2 w)
     }
 }
 
-// Tiles in the order of workgroups.  Workgroups go to the eight XCDs in turn:
-// each XCD takes a run of neighbouring ids, and a run goes through bands of
-// eight q-tiles, q first, so that the workgroups of an XCD share rows of both
-// operands in its L2.
-struct TileAt { uint32_t p, q; };
-
-__device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t all)
+// Workgroups go to the eight XCDs in turn.  Of every `room` of them, as many as the
+// GPU holds at a time, an XCD takes neighbouring ids, which go through bands of eight
+// q-tiles, q first: its workgroups share rows of both operands in its L2.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t block, uint32_t all, uint32_t room)
 {
-    const uint32_t each = all / 8;
-    return block < each * 8 ? block % 8 * each + block / 8 : block;
+    const uint32_t from = block / room * room, in = block - from, here = min(room, all - from), each = here / 8;
+    return from + (in < each * 8 ? in % 8 * each + in / 8 : in);
 }
+
+struct TileAt { uint32_t p, q; };
 
 __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t tiles_p, uint32_t tiles_q)
 {
@@ -372,123 +384,105 @@ __device__ __forceinline__ TileAt tile_at(uint32_t id, uint32_t tiles_p, uint32_
     return {in / high, band * BAND + in % high};
 }
 
-// How a launch deals with its tiles.  Whole rounds of tiles go to workgroups of their
-// own; where the last round would leave much of the GPU idle, the tiles of the last two
-// are shared out evenly among `workers`, by their steps, in order: a tile that a
-// worker's share begins or ends in is split, its sums go to memory, and a second launch
-// (settle) adds the parts in their order and does what the first does with a whole
-// tile's sums.  A job J has
-//   Args               with `stream` and the tiles' description
-//   Tile               where a tile lies: its id, steps, first unit
-//   units, locate      all units (a step of a tile), the tile that holds a unit
-//   run                the tile's sums over some of its steps
-//   finish             what becomes of a wave's sums
-struct Stream {
-    uint32_t room;    // workgroups that the GPU holds at a time
-    float* partial;   // [room, 2] tiles of sums, or NULL: no tile is split
+// How a launch deals with its tiles.  Each has a workgroup; but where the last round
+// of them would leave much of the GPU idle, or there is less than a round, the sums of
+// its tiles are split into parts along k.  Parts go to memory, and a second launch
+// (settle) adds those of a tile in their order and does what the first does with a
+// whole tile's sums.  Parts are in the order of k: those that run at a time read the
+// same k of both operands.
+struct Share {
+    uint32_t whole, rest, parts;  // tiles with a workgroup of their own, the others, parts of each of these
 };
 
-// Tiles with workgroups of their own, and the workers of the others.
-struct Shares {
-    uint32_t whole, workers;
-};
+constexpr uint32_t PARTS_ROOM = 2;  // parts of a launch, in rooms of workgroups
 
-constexpr int LEAST = 4;  // steps of a worker's share at least
-
-__host__ __device__ inline Shares shares(uint32_t tiles, int64_t steps, uint32_t room, bool split, int tile, int pairs)
+// ns, measured: a step of as many tiles as the GPU holds at a time (256 wide: one a CU,
+// 128 wide: two), a part's way through memory and back, the second launch.
+__host__ __device__ inline Share share_of(uint32_t tiles, int64_t steps, uint32_t room, int tile, int pairs)
 {
-    const uint32_t last = tiles % room;
-    if (!split || last == 0) return {tiles, 0};
-    // ns: a step of as many tiles as there is room for; the parts' way through memory
-    // and the second launch
-    const int64_t step = (tile > 128 ? 1600 : 1050) * pairs, parts = tile > 128 ? 55000 : 35000;
-    if (tiles < room) {
-        const int64_t units = (int64_t)tiles * steps, most = (units + LEAST - 1) / LEAST;
-        const uint32_t workers = (uint32_t)(most < room ? most : room);
-        const int64_t less = step * (steps - (units + workers - 1) / (workers ? workers : 1));
-        return less > 10000 + parts * workers / room ? Shares{0, workers} : Shares{tiles, 0};
+    const uint32_t rest = tiles % room;
+    Share best{tiles, 0, 1};
+    if (rest == 0) return best;
+    const int64_t step = (tile > 128 ? 1600 : 1050) * pairs, part = tile > 128 ? 110 : 28, again = 10000;
+    const int64_t ends = tile > 128 ? 6000 : 4000;
+    int64_t least = steps * step + ends;
+    for (uint32_t n = 2; n <= 64 && n * rest <= PARTS_ROOM * room && 2 * n <= steps; ++n) {
+        const int64_t rounds = (n * rest + room - 1) / room;
+        const int64_t ns = rounds * ((steps + n - 1) / n * step + ends) + again + part * n * rest;
+        if (ns < least) {
+            least = ns;
+            best = {tiles - rest, rest, n};
+        }
     }
-    return (room - last) * step * steps > parts * room ? Shares{tiles - last - room, room} : Shares{tiles, 0};
+    return best;
 }
 
-template <typename J> __device__ __forceinline__ float* part_of(const typename J::Args& a, uint32_t worker, int slot)
+// What a launch takes by the same figures.
+inline double ns_of(const Share& s, int64_t steps, uint32_t room, int tile, int pairs)
+{
+    const double step = (tile > 128 ? 1600 : 1050) * pairs, ends = tile > 128 ? 6000 : 4000;
+    double ns = (double)((s.whole + room - 1) / room) * (steps * step + ends);
+    if (s.rest) ns += (double)((s.rest * s.parts + room - 1) / room) * ((double)((steps + s.parts - 1) / s.parts) * step + ends) + 10000 + (tile > 128 ? 110.0 : 28.0) * s.rest * s.parts;
+    return ns;
+}
+
+// A job J has
+//   G                  its Product
+//   Args               the launch's arguments, with `room` and `partial`
+//   Tile               where a tile lies, with its `steps`
+//   share, tile        a batch's Share of tiles; tile number i
+//   run                the tile's sums over some of its steps
+//   finish             what becomes of a wave's sums
+template <typename J> __device__ __forceinline__ float* part_of(const typename J::Args& a, uint32_t part)
 {
     typedef typename J::G G;
-    return a.stream.partial + ((int64_t)worker * 2 + slot) * (G::THREADS * G::FP * G::FQ * 4);
+    return a.partial + (int64_t)part * (G::THREADS * G::FP * G::FQ * 4);
 }
 
 template <typename J> __device__ __forceinline__ void multiply_tiles(const typename J::Args& a, char* lds)
 {
     typedef typename J::G G;
-    Shares sh = J::shares(a);
-    sh = {(uint32_t)__builtin_amdgcn_readfirstlane(sh.whole), (uint32_t)__builtin_amdgcn_readfirstlane(sh.workers)};
-    int64_t u0, u1;
-    uint32_t worker = 0;
+    const Share sh = J::share(a);
+    typename G::Sums acc;
     if (blockIdx.x < sh.whole) {
-        u0 = J::first(a, xcd_order(blockIdx.x, sh.whole));
-        u1 = u0 + 1;  // to the tile's end
-    } else {
-        worker = blockIdx.x - sh.whole;
-        if (worker >= sh.workers) return;
-        worker = xcd_order(worker, sh.workers);
-        const int64_t from = J::first(a, sh.whole), all = J::units(a) - from;
-        u0 = from + all * worker / sh.workers;
-        u1 = from + all * (worker + 1) / sh.workers;
+        const typename J::Tile t = J::tile(a, xcd_order(blockIdx.x, sh.whole, a.room));
+        J::run(a, t, lds, 0, t.steps, acc);
+        J::finish(a, t, acc, G::wave(), lds);
+        return;
     }
-    u0 = uniform(u0);
-    u1 = uniform(u1);
-    while (u0 < u1) {
-        typename J::Tile t = J::locate(a, u0);
-        t.first = uniform(t.first);
-        t.steps = uniform(t.steps);
-        if (blockIdx.x < sh.whole) u1 = uniform(t.first + max(t.steps, (int64_t)1));
-        const int64_t s0 = uniform(u0 - t.first), s1 = uniform(min(t.steps, u1 - t.first));
-        typename G::Sums acc;
-        J::run(a, t, lds, s0, s1, acc);
-        if (s0 == 0 && s1 == t.steps) {
-            J::finish(a, t, acc, G::wave(), lds);
-        } else {
-            float* const o = part_of<J>(a, worker, s0 == 0);
-            const int thread = G::wave() * WAVE + own_lane();
+    const uint32_t block = blockIdx.x - sh.whole, all = sh.rest * sh.parts;
+    if (block >= all) return;
+    const uint32_t part = xcd_order(block, all, a.room), number = part / sh.rest;
+    const typename J::Tile t = J::tile(a, sh.whole + part % sh.rest);
+    J::run(a, t, lds, t.steps * number / sh.parts, t.steps * (number + 1) / sh.parts, acc);
+    float* const o = part_of<J>(a, part);
 #pragma unroll
-            for (int i = 0; i < G::FP; ++i)
+    for (int i = 0; i < G::FP; ++i)
 #pragma unroll
-                for (int j = 0; j < G::FQ; ++j) *(f32x4*)(o + ((i * G::FQ + j) * G::THREADS + thread) * 4) = acc[i][j];
-        }
-        u0 = uniform(t.first + max(s1, (int64_t)1));
-        if (u0 < u1) __syncthreads();  // LDS may have been used by finish
-    }
+        for (int j = 0; j < G::FQ; ++j) *(f32x4*)(o + ((i * G::FQ + j) * G::THREADS + threadIdx.x) * 4) = acc[i][j];
 }
 
-// A wave of a split tile to each workgroup.  Its number: the worker whose share begins
-// in the tile, the first of them; the one before it holds the tile's first part.
+// A wave of a split tile to each workgroup.
 template <typename J> __device__ __forceinline__ void settle_tiles(const typename J::Args& a, char* lds)
 {
     typedef typename J::G G;
-    Shares sh = J::shares(a);
-    sh = {(uint32_t)__builtin_amdgcn_readfirstlane(sh.whole), (uint32_t)__builtin_amdgcn_readfirstlane(sh.workers)};
-    const uint32_t worker = blockIdx.x / G::WAVES + 1;
+    const Share sh = J::share(a);
+    const uint32_t which = blockIdx.x / G::WAVES;
     const int wave = blockIdx.x % G::WAVES;
-    if (worker >= sh.workers) return;
-    const int64_t from = J::first(a, sh.whole), all = J::units(a) - from;
-    auto begin = [&](uint32_t w) { return from + all * w / sh.workers; };
-    const int64_t u = begin(worker);
-    if (u >= begin(worker + 1) || u >= from + all) return;  // (an empty share: none, with LEAST)
-    const typename J::Tile t = J::locate(a, u);
-    if (u == t.first || begin(worker - 1) > t.first) return;
+    if (which >= sh.rest) return;
+    const typename J::Tile t = J::tile(a, sh.whole + which);
     typename G::Sums acc;
-    auto add = [&](uint32_t w, int slot, bool whole) {
-        const float* const o = part_of<J>(a, w, slot);
+#pragma unroll
+    for (int i = 0; i < G::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < G::FQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t n = 0; n < sh.parts; ++n) {
+        const float* const o = part_of<J>(a, n * sh.rest + which);
 #pragma unroll
         for (int i = 0; i < G::FP; ++i)
 #pragma unroll
-            for (int j = 0; j < G::FQ; ++j) {
-                const f32x4 v = *(const f32x4*)(o + ((i * G::FQ + j) * G::THREADS + wave * WAVE + threadIdx.x) * 4);
-                acc[i][j] = whole ? v : acc[i][j] + v;
-            }
-    };
-    add(worker - 1, 1, true);
-    for (uint32_t w = worker; w < sh.workers && begin(w) < t.first + t.steps; ++w) add(w, 0, false);
+            for (int j = 0; j < G::FQ; ++j) acc[i][j] += *(const f32x4*)(o + ((i * G::FQ + j) * G::THREADS + wave * WAVE + threadIdx.x) * 4);
+    }
     J::finish(a, t, acc, wave, lds);
 }
 

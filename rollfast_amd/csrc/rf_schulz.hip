@@ -49,7 +49,6 @@ struct Item {
     int32_t rows, cols;
     float scale, add_scale;
     uint32_t first;    // its first tile
-    int64_t unit;      // its first unit (a step of a tile)
     uint8_t tall, in_dtype, out_dtype, add_dtype;
 
     // X and the next X: [n, m] high parts, then low parts.  A and B: [n, n] high
@@ -68,9 +67,9 @@ struct Batch {
     float a, b, c;        // the step's coefficients
     float eps, x_scale, a_scale, b_scale;
     uint32_t tiles;
-    int64_t units;
-    Shares share;         // what becomes of the tiles (rf_product.h)
-    Stream stream;
+    Share share;          // what becomes of the tiles (rf_product.h)
+    uint32_t room;
+    float* partial;
     Item item[MAX];
 };
 static_assert(sizeof(Batch) <= 4096, "kernel arguments");
@@ -79,14 +78,6 @@ __device__ __forceinline__ int find(const Batch& t, uint32_t id)
 {
     int i = 0;
     while (i + 1 < t.count && id >= t.item[i + 1].first) ++i;
-    return i;
-}
-
-// The item of tile or unit `at`.
-template <typename F> __device__ __forceinline__ int find_by(const Batch& t, F before)
-{
-    int i = 0;
-    while (i + 1 < t.count && before(t.item[i + 1])) ++i;
     return i;
 }
 
@@ -232,7 +223,7 @@ __device__ __forceinline__ void put_symmetric(uint16_t* o, int64_t low, int64_t 
 // A tile of one of the batch's matrices; they differ in their number of steps.
 struct Place {
     int item;
-    int64_t p0, q0, first, steps;
+    int64_t p0, q0, steps;
 };
 
 // What the jobs of a batch share.  J: steps(item), place(item, tile) of TILE.
@@ -240,21 +231,12 @@ template <typename J> struct Batched {
     typedef Batch Args;
     typedef Place Tile;
 
-    static __device__ Shares shares(const Batch& t) { return t.share; }
-    static __device__ int64_t units(const Batch& t) { return t.units; }
-    static __device__ int64_t first(const Batch& t, uint32_t tile)
+    static __device__ Share share(const Batch& t) { return t.share; }
+    static __device__ Place tile(const Batch& t, uint32_t id)
     {
-        const Item& it = t.item[find_by(t, [&](const Item& next) { return tile >= next.first; })];
-        return tile < t.tiles ? it.unit + (int64_t)(tile - it.first) * J::steps(it) : t.units;
-    }
-    static __device__ Place locate(const Batch& t, int64_t unit)
-    {
-        const int i = find_by(t, [&](const Item& next) { return unit >= next.unit; });
-        const Item& it = t.item[i];
-        const int64_t steps = J::steps(it);
-        const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(unit - it.unit) / (uint32_t)steps);
-        const TileAt at = J::place(it, id);
-        return {i, (int64_t)at.p * J::TILE, (int64_t)at.q * J::TILE, it.unit + (int64_t)id * steps, steps};
+        const int i = find(t, id);
+        const TileAt at = J::place(t.item[i], id - t.item[i].first);
+        return {i, (int64_t)at.p * J::TILE, (int64_t)at.q * J::TILE, J::steps(t.item[i])};
     }
 };
 
@@ -508,43 +490,35 @@ template <typename F> uint32_t number(Batch& t, F tiles)
     return t.tiles = all;
 }
 
-// A product of all matrices of the batch: numbers its tiles and units, longest sums
-// first as the list is (see run), and shares them out.  us: what it takes.
+// A product of all matrices of the batch: numbers its tiles, those with the longest
+// sums first as the list is (see run), and shares them out.  ns: what it takes.
 template <typename J> double lay_out(Batch& t, int cus, int pairs)
 {
-    const bool big = J::TILE > 128;
-    const uint32_t room = (uint32_t)cus * (big ? 1 : 2);
+    t.room = (uint32_t)cus * (J::TILE > 128 ? 1 : 2);
     t.tiles = 0;
-    t.units = 0;
-    int64_t longest = 0;
+    int64_t units = 0, longest = 0, shortest = 1ll << 40;
     for (int i = 0; i < t.count; ++i) {
+        const int64_t tiles = J::tiles(t.item[i]), steps = J::steps(t.item[i]);
         t.item[i].first = t.tiles;
-        t.item[i].unit = t.units;
-        t.tiles += (uint32_t)J::tiles(t.item[i]);
-        t.units += J::tiles(t.item[i]) * J::steps(t.item[i]);
-        longest = std::max(longest, J::steps(t.item[i]));
+        t.tiles += (uint32_t)tiles;
+        units += tiles * steps;
+        longest = std::max(longest, steps);
+        shortest = std::min(shortest, steps);
     }
-    const double step = (big ? 1.6 : 1.05) * pairs, ends = big ? 8 : 5, parts = 12 + (big ? 45 : 25);
-    // tiles of their own: as the GPU takes them, longest first; or all shared out
-    const double even = (double)t.units / t.tiles;
-    const double rounds = (double)((t.tiles + room - 1) / room);
-    const double whole = std::max((double)longest, std::max(rounds * even, (double)t.units / std::min(room, t.tiles))) * step + rounds * ends;
-    const uint32_t workers = (uint32_t)std::min<int64_t>(room, (t.units + LEAST - 1) / LEAST);
-    const double each = (double)(t.units + workers - 1) / workers;
-    const double shared = each * step + (2 + t.tiles / room) * ends + 10 + parts * workers / room;
-    if (shared < whole && t.stream.partial) {
-        t.share = {0, workers};
-        return shared;
-    }
-    t.share = {t.tiles, 0};
-    return whole;
+    // sums of unlike length are split where there are few of them alone, all alike: the last
+    // round is of the shortest
+    const double step = (J::TILE > 128 ? 1600.0 : 1050.0) * pairs, ends = J::TILE > 128 ? 6000 : 4000;
+    t.share = {t.tiles, 0, 1};
+    if (longest == shortest || t.tiles < t.room) t.share = share_of(t.tiles, longest, t.room, J::TILE, pairs);
+    if (longest == shortest || t.share.rest) return ns_of(t.share, longest, t.room, J::TILE, pairs);
+    return std::max((double)longest, (double)units / std::min(t.room, t.tiles) + (double)shortest / 2) * step +
+           (double)((t.tiles + t.room - 1) / t.room) * ends;
 }
 
 template <typename J> rf_status multiply(Batch& t, hipStream_t st)
 {
-    const rf_status s = launch<k_multiply<J>>((int64_t)t.share.whole + t.share.workers, J::G::THREADS, J::LDS, st, t);
-    if (s != RF_OK || t.share.workers < 2) return s;
-    return launch<k_settle<J>>((int64_t)(t.share.workers - 1) * J::G::WAVES, WAVE, J::SETTLE_LDS, st, t);
+    const rf_status s = launch<k_multiply<J>>((int64_t)t.share.whole + (int64_t)t.share.rest * t.share.parts, J::G::THREADS, J::LDS, st, t);
+    return s != RF_OK ? s : launch<k_settle<J>>((int64_t)t.share.rest * J::G::WAVES, WAVE, J::SETTLE_LDS, st, t);
 }
 
 // With the tiles that take less.
@@ -631,7 +605,7 @@ struct Needs {
 Needs needs_of(const Matrix* list, int64_t count, int64_t at, int cus)
 {
     Needs need{at, 0, 0, 0};
-    int64_t units[2][3] = {};  // of tiles of 128 and 256; of the three products
+    int64_t tiles[2] = {};  // of the product with the most
     for (; need.end < count && need.end - at < MAX; ++need.end) {
         const Matrix& m = list[need.end];
         const bool some = m.rows && m.cols;
@@ -640,16 +614,11 @@ Needs needs_of(const Matrix* list, int64_t count, int64_t at, int cus)
         need.buffers += more;
         if (!some) continue;
         const Item it = item_of(m);
-        for (int big = 0; big < 2; ++big) {
-            const int64_t tile = big ? 256 : 128, n = (it.n + tile - 1) / tile, w = (it.m + tile - 1) / tile;
-            units[big][0] += n * (n + 1) / 2 * (it.m / STEP);
-            units[big][1] += n * (n + 1) / 2 * (it.n / STEP);
-            units[big][2] += n * w * (it.n / STEP);
-        }
+        for (int big = 0; big < 2; ++big) tiles[big] += up(it.n, big ? 256 : 128) * up(it.m, big ? 256 : 128) / (big ? 65536 : 16384);
     }
+    // at most 64 parts of a tile
     for (int big = 0; big < 2; ++big)
-        for (int64_t u : units[big])
-            need.parts = std::max(need.parts, std::min<int64_t>(cus * (big ? 1 : 2), (u + LEAST - 1) / LEAST) * 2 * (big ? 256 * 256 : 128 * 128) * 4);
+        need.parts = std::max(need.parts, std::min<int64_t>(cus * (big ? 1 : 2) * PARTS_ROOM, tiles[big] * 64) * (big ? 65536 : 16384) * 4);
     need.sums = (need.end - at) * PARTS * 8;
     return need;
 }
@@ -705,7 +674,7 @@ rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hi
         t.x_scale = scale(most.x);
         t.a_scale = scale(most.x * most.x);
         t.b_scale = scale(most.b);
-        t.stream.partial = (float*)(ws + need.sums);
+        t.partial = (float*)(ws + need.sums);
         int64_t used = need.sums + need.parts;
         int64_t which[MAX];
         float* u[MAX];
