@@ -384,14 +384,14 @@ def pyhost():
 
 def pyblocks():
     """The native host module ``_rfblocks`` of the residual-block operators
-    (built with the library by ``rollfast_amd.build``)."""
+    and the vocabulary loss (built with the library by ``rollfast_amd.build``)."""
     global _pyblocks
     if _pyblocks is None:
         import torch
 
         L = lib()
         mod = _host_module("_rfblocks")
-        names = [n for n in EXPORTS if n.startswith(("rf_checkpoint_", "rf_gated_", "rf_norm_", "rf_linear_weight_"))]
+        names = [n for n in EXPORTS if n.startswith(("rf_checkpoint_", "rf_gated_", "rf_norm_", "rf_linear_"))]
         mod.set_entries({n: ctypes.cast(getattr(L, n), _p).value for n in (*names, "rf_last_error")},
                         torch._C._cuda_getCurrentRawStream, torch.nn.Parameter)
         _pyblocks = mod

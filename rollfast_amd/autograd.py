@@ -1,5 +1,5 @@
-"""The residual-block operators (``rollfast_amd.blocks``) as differentiable
-torch functions.  What the backward pass needs is kept as 8-bit checkpoints
+"""The residual-block operators (``rollfast_amd.blocks``) and the vocabulary loss
+(``rollfast_amd.losses``) as differentiable torch functions.  What the backward pass needs is kept as 8-bit checkpoints
 (``save="int8"``, the default) or as the tensors themselves
 (``save="input"``); under ``torch.no_grad`` nothing is kept.
 
@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import blocks
+from . import blocks, losses
 from .blocks import ActivationCheckpoint
 
 
@@ -221,3 +221,38 @@ def linear(x, weight, bias=None, *, checkpoint=None):
     if not _wanted(x, weight, bias):
         return torch.nn.functional.linear(x, weight, bias)
     return _Linear.apply(x, weight, bias, checkpoint)
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, z_loss, reduction):
+        got = losses.linear_cross_entropy_grad(hidden, weight, targets, ignore_index=ignore_index, z_loss=z_loss,
+                                               reduction=reduction)
+        ctx.save_for_backward(got.hidden if ctx.needs_input_grad[0] else None,
+                              got.weight if ctx.needs_input_grad[1] else None)
+        return got.loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        dhidden, dweight = ctx.saved_tensors  # of a dloss of one
+        return (None if dhidden is None else dhidden * dloss, None if dweight is None else dweight * dloss,
+                None, None, None, None)
+
+
+def linear_cross_entropy(hidden, weight, targets, *, ignore_index=-100, z_loss=0.0, reduction="mean"):
+    """``losses.linear_cross_entropy`` summed ('sum') or averaged ('mean') over
+    the targets that count, differentiable.  The forward pass computes both
+    gradients in the same pass as the loss and keeps them; the backward pass
+    multiplies them by the loss' own.  Under autocast both tensors go to its
+    dtype.  A mean over no targets is NaN with gradients of zero."""
+    if reduction not in ("sum", "mean"):
+        raise ValueError(f"reduction must be 'sum' or 'mean', got {reduction!r}")
+    device = hidden.device.type
+    if torch.is_autocast_enabled(device):
+        dtype = torch.get_autocast_dtype(device)
+        hidden, weight = hidden.to(dtype), weight.to(dtype)
+    if not _wanted(hidden, weight):
+        return losses.linear_cross_entropy(hidden, weight, targets, ignore_index=ignore_index, z_loss=z_loss,
+                                           reduction=reduction)
+    return _CrossEntropy.apply(hidden, weight, targets, ignore_index, z_loss, reduction)

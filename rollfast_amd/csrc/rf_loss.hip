@@ -66,12 +66,13 @@ struct Products {
     int32_t logits_tile, dhidden_tile, dweight_tile;
 };
 
+// By a whole wave.
 __device__ __forceinline__ Piece piece_of(const Products& p, int64_t count, int64_t piece)
 {
     const int64_t rows = max(min(count - piece * p.rows, p.rows), (int64_t)0), steps = (rows + STEP - 1) / STEP;
     auto tiles = [](int64_t x, int64_t y, int tile) { return (uint32_t)(((x + tile - 1) / tile) * ((y + tile - 1) / tile)); };
     auto room = [&](int tile) { return (uint32_t)(p.cus * (tile > 128 ? 1 : 2)); };
-    auto share = [&](int64_t x, int64_t y, int64_t n, int tile) { return share_of(tiles(x, y, tile), n, room(tile), tile, p.pairs); };
+    auto share = [&](int64_t x, int64_t y, int64_t n, int tile) { return share_by_wave(tiles(x, y, tile), n, room(tile), cost_of(tile, p.pairs)); };
     Piece out{};
     out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile);
     if (!p.grad) return out;
@@ -157,7 +158,10 @@ __global__ __launch_bounds__(SELECT) void k_select(const I* __restrict__ targets
         sc->count = before;
         sc->hidden_top = sc->weight_top = 0;
     }
-    for (int i = tid; i < products.pieces; i += SELECT) pieces[i] = piece_of(products, before, i);
+    for (int i = wave; i < products.pieces; i += SELECT / WAVE) {
+        const Piece piece = piece_of(products, before, i);
+        if (lane == 0) pieces[i] = piece;
+    }
 }
 
 // Largest finite magnitude of rows (of those that count, where order is given).
@@ -637,7 +641,8 @@ Shape shape_of(int64_t cols, int64_t rows, int64_t steps, int pairs, int cus)
     for (int big = 0; big < 2; ++big) {
         const int64_t tile = big ? 256 : 128, tiles = ((cols + tile - 1) / tile) * ((rows + tile - 1) / tile);
         const uint32_t room = (uint32_t)cus * (big ? 1 : 2);
-        ns[big] = ns_of(share_of((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, (int)tile, pairs), steps, room, (int)tile, pairs);
+        const Cost c = cost_of((int)tile, pairs);
+        ns[big] = ns_of(share_of((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, c), steps, room, c);
     }
     const int tile = ns[1] < ns[0] ? 256 : 128;
     return {tile, (uint32_t)((cols + tile - 1) / tile), (uint32_t)cus * (tile > 128 ? 1 : 2)};
@@ -739,10 +744,11 @@ template <auto K, typename... A> rf_status launch(int64_t grid, int threads, siz
 
 // A product's launch, and the one that settles split tiles (which of them are is known on
 // the device alone).
-template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, const typename J::Args& a, hipStream_t st)
+template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, const typename J::Args& a, hipStream_t st, bool never_split = false)
 {
     const rf_status s = launch<k_multiply<J>>(tiles + PARTS_ROOM * shape.room, J::G::THREADS, J::LDS, st, a);
-    return s != RF_OK ? s : launch<k_settle<J>>((int64_t)std::min<int64_t>(tiles, shape.room) * J::G::WAVES, WAVE, 0, st, a);
+    if (s != RF_OK || never_split) return s;
+    return launch<k_settle<J>>((int64_t)std::min<int64_t>(tiles, shape.room) * J::G::WAVES, WAVE, 0, st, a);
 }
 
 int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles_p * ((rows + shape.tile - 1) / shape.tile); }
@@ -750,7 +756,10 @@ int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles
 template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
 {
     const int64_t tiles = tiles_of(p.logits, a.rows);
-    return p.logits.tile > 128 ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st) : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st);
+    // one row of tiles, or none: the share is known here
+    const bool whole = a.rows <= p.logits.tile && share_of(p.logits.tiles_p, a.steps, p.logits.room, cost_of(p.logits.tile, a.pairs)).rest == 0;
+    return p.logits.tile > 128 ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
+                               : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole);
 }
 
 template <typename H, Layout LQ> rf_status product(const Shape& shape, float* partial, Grad& a, hipStream_t st)

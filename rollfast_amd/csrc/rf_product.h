@@ -394,36 +394,65 @@ struct Share {
     uint32_t whole, rest, parts;  // tiles with a workgroup of their own, the others, parts of each of these
 };
 
-constexpr uint32_t PARTS_ROOM = 2;  // parts of a launch, in rooms of workgroups
+constexpr uint32_t PARTS_ROOM = 2, MOST_PARTS = 64;  // parts of a launch, in rooms of workgroups; of a tile
 
-// ns, measured: a step of as many tiles as the GPU holds at a time (256 wide: one a CU,
-// 128 wide: two), a part's way through memory and back, the second launch.
-__host__ __device__ inline Share share_of(uint32_t tiles, int64_t steps, uint32_t room, int tile, int pairs)
+// What a launch takes, in ns, measured: `step` a step of as many tiles as the GPU holds
+// at a time (256 wide: one a CU, 128 wide: two), `ends` a tile's start and end, a part's
+// way through memory and back, the second launch.
+struct Cost {
+    int32_t step, ends, part, again;
+};
+
+__host__ __device__ inline Cost cost_of(int tile, int pairs, int ends = 0)
 {
-    const uint32_t rest = tiles % room;
-    Share best{tiles, 0, 1};
-    if (rest == 0) return best;
-    const int64_t step = (tile > 128 ? 1600 : 1050) * pairs, part = tile > 128 ? 110 : 28, again = 10000;
-    const int64_t ends = tile > 128 ? 6000 : 4000;
-    int64_t least = steps * step + ends;
-    for (uint32_t n = 2; n <= 64 && n * rest <= PARTS_ROOM * room && 2 * n <= steps; ++n) {
-        const int64_t rounds = (n * rest + room - 1) / room;
-        const int64_t ns = rounds * ((steps + n - 1) / n * step + ends) + again + part * n * rest;
-        if (ns < least) {
-            least = ns;
-            best = {tiles - rest, rest, n};
-        }
-    }
-    return best;
+    if (tile > 128) return {1600 * pairs, ends ? ends : 6000, 110, 10000};
+    return {1050 * pairs, ends ? ends : 4000, 28, 10000};
 }
 
-// What a launch takes by the same figures.
-inline double ns_of(const Share& s, int64_t steps, uint32_t room, int tile, int pairs)
+// The last, incomplete round of `rest` tiles in n parts each; -1 where that is not done.
+__host__ __device__ inline int64_t ns_of_rest(uint32_t rest, int64_t steps, uint32_t room, uint32_t n, const Cost& c)
 {
-    const double step = (tile > 128 ? 1600 : 1050) * pairs, ends = tile > 128 ? 6000 : 4000;
-    double ns = (double)((s.whole + room - 1) / room) * (steps * step + ends);
-    if (s.rest) ns += (double)((s.rest * s.parts + room - 1) / room) * ((double)((steps + s.parts - 1) / s.parts) * step + ends) + 10000 + (tile > 128 ? 110.0 : 28.0) * s.rest * s.parts;
-    return ns;
+    if (n == 1) return steps * c.step + c.ends;
+    if (n * rest > PARTS_ROOM * room || 2 * n > steps) return -1;
+    return (n * rest + room - 1) / room * ((steps + n - 1) / n * c.step + c.ends) + c.again + (int64_t)c.part * n * rest;
+}
+
+inline Share share_of(uint32_t tiles, int64_t steps, uint32_t room, const Cost& c)
+{
+    const uint32_t rest = tiles % room;
+    uint32_t best = 1;
+    int64_t least = ns_of_rest(rest, steps, room, 1, c);
+    for (uint32_t n = 2; rest && n <= MOST_PARTS; ++n)
+        if (const int64_t ns = ns_of_rest(rest, steps, room, n, c); ns >= 0 && ns < least) {
+            least = ns;
+            best = n;
+        }
+    return best == 1 ? Share{tiles, 0, 1} : Share{tiles - rest, rest, best};
+}
+
+// The same by a whole wave, a number of parts to each lane.
+__device__ __forceinline__ Share share_by_wave(uint32_t tiles, int64_t steps, uint32_t room, const Cost& c)
+{
+    static_assert(MOST_PARTS == WAVE, "");
+    const uint32_t rest = tiles % room, n = threadIdx.x % WAVE + 1;
+    int64_t least = rest ? ns_of_rest(rest, steps, room, n, c) : -1;
+    if (least < 0) least = 1ll << 62;
+    uint32_t best = n;
+    for (int d = 1; d < WAVE; d *= 2) {
+        const int64_t ns = __shfl_xor(least, d);
+        const uint32_t other = (uint32_t)__shfl_xor((int)best, d);
+        if (ns < least || (ns == least && other < best)) {
+            least = ns;
+            best = other;
+        }
+    }
+    return rest == 0 || best == 1 ? Share{tiles, 0, 1} : Share{tiles - rest, rest, best};
+}
+
+inline double ns_of(const Share& s, int64_t steps, uint32_t room, const Cost& c)
+{
+    return (double)((s.whole + room - 1) / room) * (double)(steps * c.step + c.ends) +
+           (s.rest ? (double)ns_of_rest(s.rest, steps, room, s.parts, c) : 0.0);
 }
 
 // A job J has

@@ -1,11 +1,11 @@
-// rf_pyblocks.cpp -- native host path of the residual-block operators
-// (CPython module rollfast_amd._lib._rfblocks).
+// rf_pyblocks.cpp -- native host path of the residual-block operators and of the
+// vocabulary loss (CPython module rollfast_amd._lib._rfblocks).
 //
 // Each function checks its tensors, allocates the outputs and calls the C
 // entry (include/rfadam8.h), in one to two microseconds where the same steps
 // from Python take eight to fifteen.  What is not the plain case (another
 // device than the current one, a layout to copy, an argument to refuse) makes
-// a function return None; rollfast_amd.blocks then checks and lays out the
+// a function return None; rollfast_amd.blocks (or losses) then checks and lays out the
 // arguments and calls again with `shape`, the outputs' shape, which says that
 // every tensor is rows [rows, cols] in order.
 //
@@ -41,6 +41,8 @@ struct Entries {
     decltype(&rf_norm_backward) norm_backward;
     decltype(&rf_linear_weight_grad_workspace) weight_grad_workspace;
     decltype(&rf_linear_weight_grad) weight_grad;
+    decltype(&rf_linear_cross_entropy_workspace) cross_entropy_workspace;
+    decltype(&rf_linear_cross_entropy) cross_entropy;
     decltype(&rf_last_error) last_error;
 };
 Entries g_lib{};
@@ -69,6 +71,8 @@ PyObject* py_set_entries(PyObject*, PyObject* args)
         {"rf_norm_backward", (void**)&g_lib.norm_backward},
         {"rf_linear_weight_grad_workspace", (void**)&g_lib.weight_grad_workspace},
         {"rf_linear_weight_grad", (void**)&g_lib.weight_grad},
+        {"rf_linear_cross_entropy_workspace", (void**)&g_lib.cross_entropy_workspace},
+        {"rf_linear_cross_entropy", (void**)&g_lib.cross_entropy},
         {"rf_last_error", (void**)&g_lib.last_error},
     };
     for (const auto& e : all) {
@@ -389,6 +393,72 @@ PyObject* py_weight_grad(PyObject*, PyObject* args)
     RFB_END
 }
 
+// cross_entropy(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, grad)
+//   -> (loss, or with a reduction the reduced one; dhidden; dweight) or None
+PyObject* py_cross_entropy(PyObject*, PyObject* args)
+{
+    PyObject *ho, *wo, *to, *dlo;
+    long long ignore_index;
+    float z_loss;
+    int reduction, grad;
+    if (!PyArg_ParseTuple(args, "OOOOLfip", &ho, &wo, &to, &dlo, &ignore_index, &z_loss, &reduction, &grad)) return nullptr;
+    RFB_BEGIN
+    Call c;
+    const at::Tensor hidden = c.first(ho, Py_None);
+    rf_cross_entropy a{};
+    if (c.fine) c.as_rows(hidden, c.cols, &a.hidden_rows, &a.hidden_stride);
+    // another plain tensor of the call's device, contiguous, of the targets' shape
+    auto per_token = [&](PyObject* o) -> at::Tensor {
+        if (!c.fine || !THPVariable_Check(o) || !Call::plain(o)) return c.no();
+        const at::Tensor t = THPVariable_Unpack(o);
+        if (t.device() != c.device || t.dim() + 1 != (int64_t)c.shape.size() || !t.is_contiguous()) return c.no();
+        for (int64_t i = 0; i < t.dim(); ++i)
+            if (t.size(i) != c.shape[(size_t)i]) return c.no();
+        return t;
+    };
+    const at::Tensor targets = per_token(to);
+    if (!c.fine || (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt)) Py_RETURN_NONE;
+    if (dlo != Py_None) {
+        const at::Tensor dloss = per_token(dlo);
+        if (!c.fine || dloss.scalar_type() != at::kFloat) Py_RETURN_NONE;
+        a.dloss = (const float*)dloss.data_ptr();
+    }
+    if (!THPVariable_Check(wo) || !Call::plain(wo)) Py_RETURN_NONE;
+    const at::Tensor weight = THPVariable_Unpack(wo);
+    if (weight.device() != c.device || weight.scalar_type() != hidden.scalar_type() || weight.dim() != 2 || weight.size(1) != c.cols ||
+        weight.size(0) < 1 || (weight.stride(1) != 1 && c.cols > 1))
+        Py_RETURN_NONE;
+    a.tokens = c.rows;
+    a.vocab = weight.size(0);
+    a.hidden = c.cols;
+    a.dtype = code_of(hidden.scalar_type());
+    a.target_bits = targets.scalar_type() == at::kLong ? 64 : 32;
+    a.weight = weight.data_ptr();
+    a.weight_stride = weight.stride(0);
+    a.targets = targets.data_ptr();
+    a.ignore_index = ignore_index;
+    a.z_loss = z_loss;
+    a.reduction = reduction;
+    std::array<at::Tensor, 3> out;
+    const at::Tensor loss = at::empty(targets.sizes(), c.options(at::kFloat));
+    a.loss = (float*)loss.data_ptr();
+    out[0] = reduction ? at::empty({}, c.options(at::kFloat)) : loss;
+    if (reduction) a.total = (float*)out[0].data_ptr();
+    if (grad) {
+        out[1] = c.empty(hidden.scalar_type());
+        out[2] = at::empty(weight.sizes(), c.options(hidden.scalar_type()));
+        a.dhidden = out[1].data_ptr();
+        a.dweight = out[2].data_ptr();
+    }
+    const char* const what = grad ? "linear_cross_entropy_grad" : "linear_cross_entropy";
+    int64_t size = 0;
+    check(g_lib.cross_entropy_workspace(&a, &size), what);
+    const at::Tensor space = c.bytes(size);  // memory of the current stream: reused only behind this call's work
+    call(c, what, [&](void* s) { return g_lib.cross_entropy(&a, space.data_ptr(), size, s); });
+    return pack<3>(out);
+    RFB_END
+}
+
 // gated_forward(gate, up, shape, activation, save, output) -> (h, arena, codes, exponents) or None
 //   up None: gate holds both halves.  save: 0 nothing, 1 8-bit, 2 the inputs.
 PyObject* py_gated_forward(PyObject*, PyObject* args)
@@ -691,6 +761,7 @@ PyMethodDef methods[] = {
     {"checkpoint_store", py_checkpoint_store, METH_VARARGS, "(codes, exponents), or None"},
     {"checkpoint_load", py_checkpoint_load, METH_VARARGS, "the values, or None"},
     {"weight_grad", py_weight_grad, METH_VARARGS, "out, or None"},
+    {"cross_entropy", py_cross_entropy, METH_VARARGS, "(loss, dhidden, dweight), or None"},
     {"gated_forward", py_gated_forward, METH_VARARGS, "(h, arena, codes, exponents), or None"},
     {"gated_backward", py_gated_backward, METH_VARARGS, "(dgate, dup) or one tensor, or None"},
     {"norm_forward", py_norm_forward, METH_VARARGS, "(out, y, arena, gates, codes, exponents), or None"},

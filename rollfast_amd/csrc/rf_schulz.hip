@@ -245,7 +245,7 @@ template <bool SQUARE, bool SPLIT, int TILE_, int WP, int WQ> struct Symmetric :
     static constexpr int TILE = TILE_;
     typedef Product<f16, KALONG, KALONG, TILE, TILE, WP, WQ> G;
     static constexpr int PITCH = TILE / WP * 2 + 16, ROOM = TILE / WQ * PITCH;
-    static constexpr int LDS = std::max(G::LDS, G::WAVES * ROOM), SETTLE_LDS = ROOM;
+    static constexpr int LDS = std::max(G::LDS, G::WAVES * ROOM), SETTLE_LDS = ROOM, ENDS = TILE > 128 ? 8000 : 5000;
 
     static __host__ __device__ int64_t steps(const Item& it) { return (SQUARE ? it.n : it.m) / STEP; }
     static __host__ int64_t tiles(const Item& it)
@@ -346,7 +346,7 @@ __device__ __forceinline__ void put_out8(const Item& it, int64_t r, int64_t c, f
 template <bool SPLIT, int TILE_, int WP, int WQ> struct Apply : Batched<Apply<SPLIT, TILE_, WP, WQ>> {
     static constexpr int TILE = TILE_;
     typedef Product<f16, KDOWN, KALONG, TILE, TILE, WP, WQ> G;
-    static constexpr int LDS = G::LDS, SETTLE_LDS = 0;
+    static constexpr int LDS = G::LDS, SETTLE_LDS = 0, ENDS = TILE > 128 ? 24000 : 8500;  // (X read and written)
 
     static __host__ __device__ int64_t steps(const Item& it) { return it.n / STEP; }
     static __host__ int64_t tiles(const Item& it) { return (int64_t)((it.n + TILE - 1) / TILE) * ((it.m + TILE - 1) / TILE); }
@@ -505,14 +505,14 @@ template <typename J> double lay_out(Batch& t, int cus, int pairs)
         longest = std::max(longest, steps);
         shortest = std::min(shortest, steps);
     }
-    // sums of unlike length are split where there are few of them alone, all alike: the last
-    // round is of the shortest
-    const double step = (J::TILE > 128 ? 1600.0 : 1050.0) * pairs, ends = J::TILE > 128 ? 6000 : 4000;
+    // sums of unlike length are split, all alike, only where there is less than a round of
+    // them: a last round is of the shortest
+    const Cost c = cost_of(J::TILE, pairs, J::ENDS);
     t.share = {t.tiles, 0, 1};
-    if (longest == shortest || t.tiles < t.room) t.share = share_of(t.tiles, longest, t.room, J::TILE, pairs);
-    if (longest == shortest || t.share.rest) return ns_of(t.share, longest, t.room, J::TILE, pairs);
-    return std::max((double)longest, (double)units / std::min(t.room, t.tiles) + (double)shortest / 2) * step +
-           (double)((t.tiles + t.room - 1) / t.room) * ends;
+    if (longest == shortest || t.tiles < t.room) t.share = share_of(t.tiles, longest, t.room, c);
+    if (longest == shortest || t.share.rest) return ns_of(t.share, longest, t.room, c);
+    return std::max((double)longest, (double)units / std::min(t.room, t.tiles) + (double)shortest / 2) * c.step +
+           (double)((t.tiles + t.room - 1) / t.room) * c.ends;
 }
 
 template <typename J> rf_status multiply(Batch& t, hipStream_t st)

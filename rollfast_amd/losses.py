@@ -14,6 +14,8 @@ bits, at most 2 GiB at once, and computes no product twice.
 A token whose target is ``ignore_index`` has a loss of zero and no part in the
 gradients, whatever its row of ``hidden`` holds (its own gradient is zero).  A
 target that is no row of ``weight`` otherwise makes the loss and the gradients NaN.
+In float32 an Inf in ``weight`` makes every loss NaN, and one in a row of ``hidden``
+its own, since split numbers have no infinities of one sign.
 
 ``hidden`` and ``weight`` are float32, bfloat16 or float16 on a ROCm device, both
 of one dtype, which is the gradients' too; losses are float32.  Targets are int32
@@ -72,38 +74,15 @@ def _arguments(hidden, weight, targets, ignore_index, z_loss, reduction):
     return a, (rows, table, targets)
 
 
-def _launch(a, device, what):
-    """Runs the call on the current stream of ``device``, the current one."""
-    need = ctypes.c_int64()
-    _lib.check(_lib.lib().rf_linear_cross_entropy_workspace(a, need), what)
-    workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
-    _lib.check(_lib.lib().rf_linear_cross_entropy(a, workspace.data_ptr(), need.value, _lib.stream_ptr()), what)
-
-
-def linear_cross_entropy(hidden, weight, targets, *, ignore_index: int = -100, z_loss: float = 0.0,
-                         reduction: str = "none"):
-    """The loss of every row of ``hidden`` [..., n] with ``targets`` [...] and
-    ``weight`` [vocab, n], in float32: of the targets' shape, or with
-    ``reduction`` 'sum' or 'mean' one value over the targets that count."""
+def _call(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, grad):
+    """(loss, dhidden, dweight): the native host path where the tensors are as
+    they may be, on the current device; else laid out here."""
+    code = _REDUCTION.get(reduction)
+    if code is not None:
+        got = _lib.pyblocks().cross_entropy(hidden, weight, targets, dloss, int(ignore_index), float(z_loss), code, grad)
+        if got is not None:
+            return got
     a, _held = _arguments(hidden, weight, targets, ignore_index, z_loss, reduction)
-    with torch.cuda.device(hidden.device):
-        loss = torch.empty(targets.shape, dtype=torch.float32, device=hidden.device)
-        a.loss = loss.data_ptr()
-        if a.reduction:
-            total = torch.empty((), dtype=torch.float32, device=hidden.device)
-            a.total = total.data_ptr()
-        _launch(a, hidden.device, "linear_cross_entropy")
-    return total if a.reduction else loss
-
-
-def linear_cross_entropy_grad(hidden, weight, targets, dloss=None, *, ignore_index: int = -100, z_loss: float = 0.0,
-                              reduction: str = "none") -> LossGrads:
-    """The losses, and the gradients of ``sum(dloss * loss)`` with ``dloss``
-    float32 of the targets' shape; or with a ``reduction`` in place of ``dloss``
-    the reduced loss and its gradients."""
-    a, _held = _arguments(hidden, weight, targets, ignore_index, z_loss, reduction)
-    if (dloss is None) == (reduction == "none"):
-        raise ValueError("the gradient needs dloss, or a reduction in its place")
     device = hidden.device
     if dloss is not None:
         _tensor(dloss, "dloss", device)
@@ -111,13 +90,37 @@ def linear_cross_entropy_grad(hidden, weight, targets, dloss=None, *, ignore_ind
             raise ValueError(f"dloss must be float32 of shape {tuple(targets.shape)}, got {dloss.dtype} {tuple(dloss.shape)}")
         dloss = dloss.contiguous()
         a.dloss = dloss.data_ptr()
+    total = dhidden = dweight = None
     with torch.cuda.device(device):
         loss = torch.empty(targets.shape, dtype=torch.float32, device=device)
-        dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=device)
-        dweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
-        a.loss, a.dhidden, a.dweight = loss.data_ptr(), dhidden.data_ptr(), dweight.data_ptr()
+        a.loss = loss.data_ptr()
         if a.reduction:
             total = torch.empty((), dtype=torch.float32, device=device)
             a.total = total.data_ptr()
-        _launch(a, device, "linear_cross_entropy_grad")
-    return LossGrads(total if a.reduction else loss, dhidden, dweight)
+        if grad:
+            dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=device)
+            dweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
+            a.dhidden, a.dweight = dhidden.data_ptr(), dweight.data_ptr()
+        need, what = ctypes.c_int64(), "linear_cross_entropy_grad" if grad else "linear_cross_entropy"
+        _lib.check(_lib.lib().rf_linear_cross_entropy_workspace(a, need), what)
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
+        _lib.check(_lib.lib().rf_linear_cross_entropy(a, workspace.data_ptr(), need.value, _lib.stream_ptr()), what)
+    return total if a.reduction else loss, dhidden, dweight
+
+
+def linear_cross_entropy(hidden, weight, targets, *, ignore_index: int = -100, z_loss: float = 0.0,
+                         reduction: str = "none"):
+    """The loss of every row of ``hidden`` [..., n] with ``targets`` [...] and
+    ``weight`` [vocab, n], in float32: of the targets' shape, or with
+    ``reduction`` 'sum' or 'mean' one value over the targets that count."""
+    return _call(hidden, weight, targets, None, ignore_index, z_loss, reduction, False)[0]
+
+
+def linear_cross_entropy_grad(hidden, weight, targets, dloss=None, *, ignore_index: int = -100, z_loss: float = 0.0,
+                              reduction: str = "none") -> LossGrads:
+    """The losses, and the gradients of ``sum(dloss * loss)`` with ``dloss``
+    float32 of the targets' shape; or with a ``reduction`` in place of ``dloss``
+    the reduced loss and its gradients."""
+    if (dloss is None) == (reduction == "none"):
+        raise ValueError("the gradient needs dloss, or a reduction in its place")
+    return LossGrads(*_call(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, True))

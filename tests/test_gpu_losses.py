@@ -147,3 +147,217 @@ def test_sizes(size, dtype):
 @pytest.mark.parametrize("masked", [0.3, 0.97])
 def test_masked_and_z_loss(masked, kind, dtype):
     check(*make(201, 777, 160, dtype, seed=3, masked=masked, ignore=7, kind=kind), z_loss=0.01, ignore=7)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_what_lies_in_ignored_rows_reaches_nothing(dtype):
+    hidden, weight, targets, dloss = make(70, 300, 72, dtype, seed=5, masked=0.4)
+    clean = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    for junk in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max):
+        bad, bad_dloss = hidden.clone(), dloss.clone()
+        bad[targets == -100] = junk
+        bad_dloss[targets == -100] = junk
+        got = rf().linear_cross_entropy_grad(bad, weight, targets, bad_dloss)
+        for x, y in zip(got, clean):
+            assert torch.equal(x, y)
+        assert torch.equal(rf().linear_cross_entropy(bad, weight, targets), clean.loss)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_no_tokens(dtype):
+    hidden, weight, _, _ = make(9, 130, 40, dtype)
+    for rows, targets in ((hidden, torch.full((9,), -100, device="cuda")),
+                          (hidden[:0], torch.zeros(0, dtype=torch.int64, device="cuda"))):
+        got = rf().linear_cross_entropy_grad(rows, weight, targets, torch.ones(len(rows), device="cuda"))
+        assert got.hidden.shape == rows.shape
+        assert not got.loss.any() and not got.hidden.any() and not got.weight.any()
+        assert not rf().linear_cross_entropy(rows, weight, targets).any()
+        assert rf().linear_cross_entropy(rows, weight, targets, reduction="mean").isnan()
+        assert rf().linear_cross_entropy(rows, weight, targets, reduction="sum").item() == 0.0
+        got = rf().linear_cross_entropy_grad(rows, weight, targets, reduction="mean")
+        assert got.loss.isnan() and not got.hidden.any() and not got.weight.any()
+
+
+def test_targets_out_of_range_are_nan():
+    hidden, weight, targets, dloss = make(40, 150, 64, BF16, seed=9)
+    fine = rf().linear_cross_entropy(hidden, weight, targets)
+    for wrong in (150, -1, 2 ** 31, -2 ** 40, 2 ** 62):
+        bad = targets.clone()
+        bad[7] = wrong
+        loss = rf().linear_cross_entropy(hidden, weight, bad)
+        assert loss[7].isnan()
+        loss[7] = fine[7]
+        assert torch.equal(loss, fine)
+        got = rf().linear_cross_entropy_grad(hidden, weight, bad, dloss)
+        assert got.loss[7].isnan() and got.hidden[7].isnan().all() and got.weight.isnan().all()
+        assert got.hidden[torch.arange(40, device="cuda") != 7].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_layouts(dtype):
+    hidden, weight, targets, dloss = make(66, 203, 80, dtype, seed=11, masked=0.2)
+    ref = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+
+    def same(h, w, t, d):
+        got = rf().linear_cross_entropy_grad(h, w, t, d)
+        assert torch.equal(got.loss.reshape(-1), ref.loss)
+        assert torch.equal(got.hidden.reshape(66, 80), ref.hidden)
+        assert torch.equal(got.weight, ref.weight)
+
+    wide = torch.full((66, 97), math.nan, dtype=dtype, device="cuda")
+    wide[:, 5:85] = hidden
+    same(wide[:, 5:85], weight, targets, dloss)
+    tall = torch.full((203, 91), math.nan, dtype=dtype, device="cuda")
+    tall[:, 3:83] = weight
+    same(hidden, tall[:, 3:83], targets, dloss)
+    same(hidden.t().contiguous().t(), weight.t().contiguous().t(), targets, dloss)
+    same(hidden.view(6, 11, 80), weight, targets.view(6, 11), dloss.view(6, 11))
+    twice = torch.stack((targets, targets), 1)
+    same(hidden, torch.nn.Parameter(weight), twice[:, 0], torch.stack((dloss, dloss), 1)[:, 1])
+    buffer = torch.empty(66 * 80 + 1, dtype=dtype, device="cuda")
+    buffer[1:] = hidden.reshape(-1)
+    same(buffer[1:].view(66, 80), weight, targets, dloss)
+    # one row for all tokens
+    one = rf().linear_cross_entropy_grad(hidden[:1].expand(66, 80), weight, targets, dloss)
+    check(hidden[:1].expand(66, 80).contiguous(), weight, targets, dloss)
+    assert one.hidden.shape == (66, 80)
+    # one token, no dimension of tokens
+    got = rf().linear_cross_entropy(hidden[3], weight, targets[3])
+    assert got.shape == () and got == ref.loss[3]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("logit", [1e-3, 30.0, 1000.0])
+def test_small_and_large_logits(logit, dtype):
+    check(*make(50, 400, 64, dtype, seed=13, logit=logit))
+
+
+def test_confident_tokens_keep_their_gradients():
+    """Probabilities next to one: dz at the target is a difference of nearly equal numbers."""
+    hidden, weight, targets, dloss = make(64, 500, 64, F32, seed=17)
+    hidden = (hidden + 12.0 * weight[targets] / weight[targets].square().sum(1, keepdim=True)).contiguous()
+    got = check(hidden, weight, targets, dloss)
+    assert got.loss.min() < 0.02
+    hidden, weight = hidden.to(BF16), weight.to(BF16)
+    check(hidden, weight, targets, dloss)
+
+
+def test_infinite_logits():
+    hidden, weight, targets, dloss = make(6, 90, 8, F32, seed=19)
+    weight[11] = 0.0
+    weight[11, 0] = -math.inf
+    hidden[:, 0] = hidden[:, 0].abs() + 0.1
+    hidden[2, 0] = -1.0  # its logit 11 is +inf
+    targets[:] = 3
+    loss = rf().linear_cross_entropy(hidden, weight, targets)
+    keep = torch.arange(90, device="cuda") != 11
+    ref = rf().linear_cross_entropy(hidden, weight[keep].contiguous(), targets)
+    assert loss[2].isnan()
+    other = torch.arange(6, device="cuda") != 2
+    # f32's split parts: 0 times an infinity is NaN in its low part, as the logit itself is in a product of halves
+    assert (loss[other].isnan() | torch.isclose(loss[other], ref[other], rtol=1e-5)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_reductions(dtype):
+    hidden, weight, targets, _ = make(1500, 333, 48, dtype, seed=23, masked=0.3)
+    loss = rf().linear_cross_entropy(hidden, weight, targets, z_loss=1e-3)
+    count = int((targets != -100).sum())
+    for reduction, ref, each in (("sum", loss.double().sum(), 1.0), ("mean", loss.double().sum() / count, 1.0 / count)):
+        got = rf().linear_cross_entropy(hidden, weight, targets, z_loss=1e-3, reduction=reduction)
+        assert got.shape == () and abs(got.item() - ref.item()) <= 2 * U * abs(ref.item())
+        a = rf().linear_cross_entropy_grad(hidden, weight, targets, z_loss=1e-3, reduction=reduction)
+        b = rf().linear_cross_entropy_grad(hidden, weight, targets, torch.full_like(loss, each), z_loss=1e-3)
+        assert torch.equal(a.loss, got)
+        for x, y in ((a.hidden, b.hidden), (a.weight, b.weight)):  # 1 / count may differ by an ulp
+            assert ((x.double() - y.double()).abs() <= 2 * HALF_ULP[dtype] * y.double().abs() + TINY[dtype] + 4 * U * y.abs().max()).all()
+
+
+@pytest.mark.parametrize("dtype,tokens,hidden", [(BF16, 1537, 16), (F32, 600, 9)])
+def test_several_pieces_of_tokens(dtype, tokens, hidden):
+    """A vocabulary of 2^20: 1024 tokens' exponentials at a time in 16 bits, 256 in f32."""
+    h, w, targets, dloss = make(tokens, 1 << 20, hidden, dtype, seed=29, masked=0.1)
+    got = rf().linear_cross_entropy_grad(h, w, targets, dloss, z_loss=1e-4)
+    on = targets != -100
+    rows = torch.nonzero(on)[:, 0]
+    loss, dh, dw = torch.zeros(tokens, dtype=torch.float64, device="cuda"), torch.zeros_like(h, dtype=torch.float64), torch.zeros_like(w, dtype=torch.float64)
+    for at in rows.split(256):
+        z = product(h[at].double(), w.double())
+        lse = torch.logsumexp(z, 1, keepdim=True)
+        mine = torch.arange(len(at), device="cuda")
+        loss[at] = (lse[:, 0] - z[mine, targets[at]]) + 1e-4 * lse[:, 0] ** 2
+        p = torch.exp(z - lse) * (1 + 2e-4 * lse)
+        p[mine, targets[at]] -= 1
+        p *= dloss[at].double()[:, None]
+        dh[at] = torch.matmul(p, w.double())
+        dw += torch.matmul(p.t().contiguous(), h[at].double())
+    tol = 2 * HALF_ULP[dtype] if dtype == BF16 else 2e-5  # dz and the result are rounded once each
+    for x, y, bound in ((got.loss, loss, 1e-5), (got.hidden, dh, tol), (got.weight, dw, tol)):
+        assert ((x.double() - y).norm() / y.norm()).item() < bound
+    assert torch.equal(got.loss, rf().linear_cross_entropy(h, w, targets, z_loss=1e-4))
+
+
+def test_offsets_past_32_bits():
+    """weight has more than 2^31 elements."""
+    vocab, n = 1 << 20, 2112
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(31)
+    weight = torch.empty(vocab, n, dtype=BF16, device="cuda")
+    for part in weight.split(1 << 17):
+        part.copy_(torch.randn(part.shape, generator=gen, device="cuda") * 0.02)
+    hidden = torch.randn(3, n, generator=gen, device="cuda").to(BF16)
+    targets = torch.tensor([vocab - 1, 5, vocab - 70000], device="cuda")
+    dloss = torch.ones(3, device="cuda")
+    z = torch.cat([product(hidden.double(), part.double()) for part in weight.split(1 << 17)], 1)
+    lse = torch.logsumexp(z, 1)
+    loss = lse - z[torch.arange(3, device="cuda"), targets]
+    got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    assert torch.allclose(got.loss.double(), loss, rtol=1e-5)
+    p = torch.exp(z - lse[:, None])
+    p[torch.arange(3, device="cuda"), targets] -= 1
+    for at in (0, 5, vocab // 2, vocab - 70000, vocab - 1):
+        ref = p[:, at] @ hidden.double()
+        assert ((got.weight[at].double() - ref).norm() / ref.norm()).item() < 2.0 ** -7
+    dh = sum(torch.matmul(p[:, i: i + (1 << 17)].contiguous(), weight[i: i + (1 << 17)].double()) for i in range(0, vocab, 1 << 17))
+    assert ((got.hidden.double() - dh).norm() / dh.norm()).item() < 2.0 ** -7
+
+
+def test_equal_inputs_give_equal_bits():
+    for args in (make(300, 5000, 136, BF16, seed=37), make(3, 9000, 512, F32, seed=38)):
+        a = rf().linear_cross_entropy_grad(*args)
+        for _ in range(3):
+            for x, y in zip(rf().linear_cross_entropy_grad(*args), a):
+                assert torch.equal(x, y)
+
+
+def test_another_stream():
+    args = make(257, 1000, 72, BF16, seed=41)
+    ref = rf().linear_cross_entropy_grad(*args)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = rf().linear_cross_entropy_grad(*args)
+    stream.synchronize()
+    for x, y in zip(got, ref):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_captured_and_replayed(dtype):
+    hidden, weight, targets, dloss = make(130, 700, 64, dtype, seed=43, masked=0.2)
+    rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+        mean = rf().linear_cross_entropy(hidden, weight, targets, reduction="mean")
+    for turn in range(4):
+        h2, w2, t2, d2 = make(130, 700, 64, dtype, seed=100 + turn, masked=0.1 * turn)
+        for x, y in ((hidden, h2), (weight, w2), (targets, t2), (dloss, d2)):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = rf().linear_cross_entropy_grad(h2, w2, t2, d2)
+        for x, y in zip(got, ref):
+            assert torch.equal(x, y), turn
+        assert torch.equal(mean, rf().linear_cross_entropy(h2, w2, t2, reduction="mean"))

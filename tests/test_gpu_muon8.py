@@ -76,3 +76,77 @@ def test_adjust_schedule_and_passthrough():
             u = torch.from_numpy(step(old, g.cpu().numpy(), 0.95, True)[1]).cuda()
             ref = -0.5 / (1 + turn) * s * exact(u)
             assert ((updates["a"].double() - ref).norm() / ref.norm()).item() < BOUND[F32], (adjust, turn)
+
+
+def test_layouts_and_shared_memory():
+    p = gaussian(70, 140, BF16, seed=1)
+    g = low_rank(70, 140, BF16, seed=2)
+    tx = rf().muon8(0.1, weight_decay=0.01, min_size=0, block_size=256)
+    ref, state = tx.update([g], tx.init([p]), [p])
+    wide = torch.empty(70, 150, dtype=BF16, device="cuda")
+    wide[:, 3:143] = g
+    got, other = tx.update([wide[:, 3:143]], tx.init([p]), [p.t().contiguous().t()])
+    assert torch.equal(got[0], ref[0]) and torch.equal(other.mu[0].values, state.mu[0].values)
+    # the state is updated in place
+    before = state.mu[0].values.data_ptr()
+    _, state = tx.update([g], state, [p])
+    assert state.mu[0].values.data_ptr() == before
+
+
+def test_empty_matrices_and_none():
+    p = {"a": torch.zeros(0, 4, device="cuda"), "b": None}
+    tx = rf().muon8(0.1)
+    updates, _ = tx.update(p, tx.init(p))
+    assert updates["a"].shape == (0, 4) and updates["b"] is None
+
+
+def test_a_gradient_that_is_not_finite_stays_in_its_matrix():
+    grads = [low_rank(80, 64, F32, seed=i) for i in range(3)]
+    tx = rf().muon8(0.1, min_size=0)
+    ref, _ = tx.update(grads, tx.init(grads))
+    bad = [g.clone() for g in grads]
+    bad[1][5, 5] = math.nan
+    got, _ = tx.update(bad, tx.init(bad))
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[2], ref[2]) and got[1].isnan().all()
+
+
+def test_captured_and_replayed():
+    """The momentum goes on from replay to replay as it does from call to call."""
+    g, p = low_rank(130, 200, BF16, seed=1), gaussian(130, 200, BF16, seed=2)
+    tx = rf().muon8(0.1, weight_decay=0.1)
+    eager = tx.init([p])
+    tx.update([g], tx.init([p]), [p])
+    state = tx.init([p])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, _ = tx.update([g], state, [p])
+    state.mu[0].values.copy_(eager.mu[0].values)
+    state.mu[0].scales.copy_(eager.mu[0].scales)
+    for turn in range(4):
+        g.copy_(low_rank(130, 200, BF16, seed=20 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, eager = tx.update([g], eager, [p])
+        assert torch.equal(got[0], ref[0]) and torch.equal(state.mu[0].values, eager.mu[0].values), turn
+
+
+def test_with_adamw8_for_the_other_leaves():
+    """Matrices to muon8, vectors and the embedding to adamw8, in one transformation."""
+    params = {"embed": gaussian(500, 64, BF16, seed=1), "norm": torch.ones(64, dtype=BF16, device="cuda"),
+              "up": gaussian(256, 64, BF16, seed=2), "down": gaussian(64, 256, BF16, seed=3)}
+    labels = {"embed": "rest", "norm": "rest", "up": "matrix", "down": "matrix"}
+    tx = rf().multi_transform({"matrix": rf().muon8(0.02, weight_decay=0.1), "rest": rf().adamw8(1e-3)}, labels)
+    state = tx.init(params)
+    single = rf().muon8(0.02, weight_decay=0.1)
+    alone = single.init({k: params[k] for k in ("up", "down")})
+    adam = rf().adamw8(1e-3)
+    rest = adam.init({k: params[k] for k in ("embed", "norm")})
+    for turn in range(3):
+        grads = {k: (low_rank(*p.shape, BF16, seed=turn) if p.dim() == 2 else gaussian(1, 64, BF16, seed=turn)[0]) for k, p in params.items()}
+        updates, state = tx.update(grads, state, params)
+        a, alone = single.update({k: grads[k] for k in alone.mu}, alone, {k: params[k] for k in alone.mu})
+        b, rest = adam.update({k: grads[k] for k in ("embed", "norm")}, rest, {k: params[k] for k in ("embed", "norm")})
+        for k in params:
+            assert torch.equal(updates[k], (a if k in a else b)[k]), (k, turn)
+        params = rf().apply_updates(params, updates, stochastic=False) if turn == 0 else params

@@ -99,3 +99,109 @@ def test_steps_coefficients_and_scale():
     assert off(rf().orthogonalize(g, steps=3, coefficients=rows), exact(g, 3, rows)) < BOUND[F32]
     assert off(rf().orthogonalize(g, scale=-2.5), -2.5 * exact(g)) < BOUND[F32]
     assert off(rf().orthogonalize(g, eps=100.0), exact(g, eps=100.0)) < BOUND[F32]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_layouts(dtype):
+    g = gaussian(70, 130, dtype, seed=3)
+    ref = rf().orthogonalize(g)
+    wide = torch.full((70, 150), math.nan, dtype=dtype, device="cuda")
+    wide[:, 7:137] = g
+    assert torch.equal(rf().orthogonalize(wide[:, 7:137]), ref)
+    assert torch.equal(rf().orthogonalize(g.t().contiguous().t()), ref)
+    assert torch.equal(rf().orthogonalize(torch.nn.Parameter(g)), ref)
+    buffer = torch.empty(70 * 130 + 1, dtype=dtype, device="cuda")
+    buffer[1:] = g.reshape(-1)
+    assert torch.equal(rf().orthogonalize(buffer[1:].view(70, 130)), ref)
+    # the transposed matrix: the same products, read and written the other way round
+    assert torch.equal(rf().orthogonalize(g.t()), ref.t())
+    # stacked matrices
+    other = gaussian(70, 130, dtype, seed=4)
+    both = rf().orthogonalize(torch.stack((g, other)).view(1, 2, 70, 130))
+    assert both.shape == (1, 2, 70, 130) and torch.equal(both[0, 0], ref)
+    assert off(both[0, 1], exact(other)) < BOUND[dtype]
+    one = rf().orthogonalize(g[:1].expand(70, 130))
+    assert off(one, exact(g[:1].expand(70, 130))) < BOUND[dtype]
+
+
+def test_nothing_and_zeros():
+    assert rf().orthogonalize([]) == []
+    for shape in ((0, 5), (5, 0), (0, 3, 4)):
+        assert rf().orthogonalize(torch.empty(shape, device="cuda")).shape == shape
+    zero = torch.zeros(30, 50, device="cuda")
+    assert not rf().orthogonalize(zero).any()
+    assert not rf().orthogonalize(zero.to(BF16)).any()
+    assert rf().orthogonalize(zero, eps=0.0).isnan().all()
+
+
+@pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
+def test_what_is_not_finite_stays_in_its_matrix(junk):
+    a, b, c = (gaussian(90, 200, BF16, seed=i) for i in range(3))
+    bad = b.clone()
+    bad[3, 4] = junk
+    x, y, z = rf().orthogonalize([a, bad, c])
+    assert torch.equal(x, rf().orthogonalize([a, b, c])[0]) and torch.equal(z, rf().orthogonalize([a, b, c])[2])
+    assert y.isnan().all()
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e25])
+def test_small_and_large_values(scale):
+    g = gaussian(65, 100, F32, seed=5) * scale
+    assert off(rf().orthogonalize(g, eps=0.0), exact(g, eps=0.0)) < BOUND[F32]
+
+
+def test_near_rank_one():
+    """What float16 rounds away from X must not be lost: it grows 485 times."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(6)
+    for noise in (1e-2, 1e-3, 1e-4):
+        g = torch.randn(512, 1, generator=gen, device="cuda") @ torch.randn(1, 700, generator=gen, device="cuda")
+        g = (g + noise * torch.randn(512, 700, generator=gen, device="cuda")).to(BF16)
+        assert off(rf().orthogonalize(g), exact(g)) < BOUND[BF16]
+
+
+def test_long_thin_and_many():
+    for shape in ((3, 100000), (200000, 2)):
+        g = gaussian(*shape, BF16, seed=8)
+        assert off(rf().orthogonalize(g), exact(g)) < BOUND[BF16]
+    many = [gaussian(1 + i % 70, 3 + i % 45, (BF16, F32, F16)[i % 3], seed=i) for i in range(301)]
+    for g, x in zip(many, rf().orthogonalize(many)):
+        assert off(x, exact(g)) < BOUND[g.dtype]
+
+
+def test_tiles_of_256_and_split_sums():
+    """Large enough for whole rounds, a last round in parts, and both kinds of tiles."""
+    for dtype in (BF16, F32):
+        matrices = [gaussian(1100, 3000, dtype, seed=1), gaussian(2100, 2100, dtype, seed=2), gaussian(3001, 700, dtype, seed=3)]
+        for g, x in zip(matrices, rf().orthogonalize(matrices)):
+            assert off(x, exact(g)) < BOUND[dtype]
+        for g in matrices:
+            assert off(rf().orthogonalize(g), exact(g)) < BOUND[dtype]
+
+
+def test_equal_inputs_give_equal_bits():
+    g = [gaussian(700, 900, BF16, seed=1), gaussian(300, 200, BF16, seed=2)]
+    first = rf().orthogonalize(g)
+    for _ in range(3):
+        for x, y in zip(rf().orthogonalize(g), first):
+            assert torch.equal(x, y)
+
+
+def test_another_stream_and_a_graph():
+    g = gaussian(200, 333, BF16, seed=1)
+    ref = rf().orthogonalize(g)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = rf().orthogonalize(g)
+    stream.synchronize()
+    assert torch.equal(got, ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = rf().orthogonalize(g)
+    for turn in range(4):
+        other = gaussian(200, 333, BF16, seed=50 + turn)
+        g.copy_(other)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, rf().orthogonalize(other)), turn
