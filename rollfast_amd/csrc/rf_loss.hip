@@ -71,8 +71,11 @@ __device__ __forceinline__ Piece piece_of(const Products& p, int64_t count, int6
 {
     const int64_t rows = max(min(count - piece * p.rows, p.rows), (int64_t)0), steps = (rows + STEP - 1) / STEP;
     auto tiles = [](int64_t x, int64_t y, int tile) { return (uint32_t)(((x + tile - 1) / tile) * ((y + tile - 1) / tile)); };
-    auto room = [&](int tile) { return (uint32_t)(p.cus * (tile > 128 ? 1 : 2)); };
-    auto share = [&](int64_t x, int64_t y, int64_t n, int tile) { return share_by_wave(tiles(x, y, tile), n, room(tile), cost_of(tile, p.pairs)); };
+    // each product reads weight, or writes a gradient as large
+    const int64_t bytes = p.vocab * p.hidden * (p.pairs > 1 ? 4 : 2);
+    auto share = [&](int64_t x, int64_t y, int64_t n, int tile) {
+        return share_by_wave(tiles(x, y, tile), n, room_of(tile, p.cus), cost_of(tile, p.pairs, 0, bytes));
+    };
     Piece out{};
     out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile);
     if (!p.grad) return out;
@@ -178,7 +181,10 @@ __global__ __launch_bounds__(256) void k_top(const float* __restrict__ x, int64_
         }
     }
     for (int d = 1; d < WAVE; d *= 2) best = max(best, (uint32_t)__shfl_xor((int)best, d));
-    if (threadIdx.x % WAVE == 0) raise(top, best);
+    __shared__ uint32_t tops[4];
+    if (threadIdx.x % WAVE == 0) tops[threadIdx.x / WAVE] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) raise(top, max(max(tops[0], tops[1]), max(tops[2], tops[3])));
 }
 
 // A high and a low part in f16 of scaled values.
@@ -635,25 +641,31 @@ struct Shape {
     uint32_t tiles_p, room;
 };
 
-Shape shape_of(int64_t cols, int64_t rows, int64_t steps, int pairs, int cus)
+Shape shape_of(int64_t cols, int64_t rows, int64_t steps, int pairs, int64_t bytes, int cus)
 {
     double ns[2];
     for (int big = 0; big < 2; ++big) {
-        const int64_t tile = big ? 256 : 128, tiles = ((cols + tile - 1) / tile) * ((rows + tile - 1) / tile);
-        const uint32_t room = (uint32_t)cus * (big ? 1 : 2);
-        const Cost c = cost_of((int)tile, pairs);
+        const int tile = big ? 256 : 128;
+        const int64_t tiles = ((cols + tile - 1) / tile) * ((rows + tile - 1) / tile);
+        const uint32_t room = room_of(tile, cus);
+        const Cost c = cost_of(tile, pairs, 0, bytes);
         ns[big] = ns_of(share_of((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, c), steps, room, c);
     }
     const int tile = ns[1] < ns[0] ? 256 : 128;
-    return {tile, (uint32_t)((cols + tile - 1) / tile), (uint32_t)cus * (tile > 128 ? 1 : 2)};
+    return {tile, (uint32_t)((cols + tile - 1) / tile), room_of(tile, cus)};
 }
 
-// Bytes of the parts of split tiles.
-int64_t parts_of(const Shape& s) { return (int64_t)s.room * PARTS_ROOM * s.tile * s.tile * 4; }
+// Bytes of the parts of split tiles: of `tiles` at most, with sums of `steps`.
+int64_t parts_of(const Shape& s, int64_t tiles, int64_t steps)
+{
+    const int64_t most = std::min<int64_t>({(int64_t)s.room * PARTS_ROOM, tiles * MOST_PARTS, tiles * std::max<int64_t>(1, steps / 2)});
+    return most * s.tile * s.tile * 4;
+}
 
 struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
     bool own_weight, f32, grad;
+    int64_t bytes_of_weight;
     int32_t blocks, shift, pairs, cus;
     Shape logits, dhidden, dweight;
     // offsets in the workspace
@@ -674,7 +686,8 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     // weight as it is: whole steps of k, 16-byte rows
     p.own_weight = p.f32 || a.hidden % STEP || a.weight_stride % 8 || ((uintptr_t)a.weight & 15) || a.weight_stride * 2 >= (1 << 24);
     const int64_t planes = p.f32 ? 2 : 1, steps = p.pad / STEP;
-    p.logits = shape_of(a.vocab, a.tokens, steps, p.pairs, cus);
+    const int64_t bytes = a.vocab * a.hidden * (p.f32 ? 4 : 2);
+    p.logits = shape_of(a.vocab, a.tokens, steps, p.pairs, bytes, cus);
     p.shift = p.logits.tile > 128 ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
     const int64_t each = p.grad ? p.vpad * (p.f32 ? 8 : 2) : p.blocks * 8, most = p.grad ? PIECE : STATS;
@@ -683,9 +696,10 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.pieces = std::max<int64_t>(1, (a.tokens + fit - 1) / fit);
     p.rows = p.pieces == 1 ? std::max<int64_t>(1, a.tokens) : std::min(fit, up((a.tokens + p.pieces - 1) / p.pieces, 256));
     p.pieces = std::max<int64_t>(1, (a.tokens + p.rows - 1) / p.rows);
-    p.logits = shape_of(a.vocab, p.rows, steps, p.pairs, cus);
+    p.logits = shape_of(a.vocab, p.rows, steps, p.pairs, bytes, cus);
     p.shift = p.logits.tile > 128 ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
+    p.bytes_of_weight = bytes;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t from = at;
@@ -708,11 +722,13 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.e = take(held * p.vpad * (p.f32 ? 4 : 2));
         p.dz = p.f32 ? take(held * p.vpad * 4) : p.e;
         if (p.pieces > 1 && !p.f32) p.sums = take(a.vocab * a.hidden * 4);
-        p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, cus);
-        p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, cus);
+        p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, bytes, cus);
+        p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, bytes, cus);
     }
-    int64_t parts = parts_of(p.logits);
-    if (p.grad) parts = std::max({parts, parts_of(p.dhidden), parts_of(p.dweight)});
+    auto tiles = [](const Shape& s, int64_t rows) { return (int64_t)s.tiles_p * ((rows + s.tile - 1) / s.tile); };
+    int64_t parts = parts_of(p.logits, tiles(p.logits, p.rows), steps);
+    if (p.grad)
+        parts = std::max({parts, parts_of(p.dhidden, tiles(p.dhidden, p.rows), p.vpad / STEP), parts_of(p.dweight, tiles(p.dweight, a.vocab), held / STEP)});
     p.partial = take(parts);
     p.bytes = at;
     return p;
@@ -757,7 +773,7 @@ template <typename H, typename E> rf_status logits(const Plan& p, const Logits& 
 {
     const int64_t tiles = tiles_of(p.logits, a.rows);
     // one row of tiles, or none: the share is known here
-    const bool whole = a.rows <= p.logits.tile && share_of(p.logits.tiles_p, a.steps, p.logits.room, cost_of(p.logits.tile, a.pairs)).rest == 0;
+    const bool whole = a.rows <= p.logits.tile && share_of(p.logits.tiles_p, a.steps, p.logits.room, cost_of(p.logits.tile, a.pairs, 0, p.bytes_of_weight)).rest == 0;
     return p.logits.tile > 128 ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
                                : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole);
 }
@@ -789,10 +805,10 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
     if (s != RF_OK) return s;
     const int32_t* const none = nullptr;
     if constexpr (sizeof(T) == 4) {
-        s = launch<k_top>(std::min<int64_t>(a.tokens, 2048), 256, 0, st, (const float*)a.hidden_rows, a.tokens, a.hidden, a.hidden_stride,
+        s = launch<k_top>(std::min<int64_t>(a.tokens, 1024), 256, 0, st, (const float*)a.hidden_rows, a.tokens, a.hidden, a.hidden_stride,
                           (const int32_t*)order, (const Scalars*)sc, &sc->hidden_top);
         if (s != RF_OK) return s;
-        s = launch<k_top>(std::min<int64_t>(a.vocab, 4096), 256, 0, st, (const float*)a.weight, a.vocab, a.hidden, a.weight_stride, none,
+        s = launch<k_top>(std::min<int64_t>(a.vocab, 1024), 256, 0, st, (const float*)a.weight, a.vocab, a.hidden, a.weight_stride, none,
                           (const Scalars*)sc, &sc->weight_top);
         if (s != RF_OK) return s;
     }

@@ -95,8 +95,13 @@ __device__ __forceinline__ int own_lane()
 }
 
 // KDOWN: 32-byte units of a row are xored by this, so that the rows of a
-// transposed read lie in different banks.
-__device__ __forceinline__ int unit(int k) { return (k & 3) | ((k >> 3) & 1) << 2; }
+// transposed read lie in different banks.  (Tiles of 64: two rows fill the banks, four
+// units a row.)
+template <int T> __device__ __forceinline__ int unit(int k)
+{
+    static_assert(T >= 64, "");
+    return T > 64 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+}
 
 // A side of a tile: T of its x, staged by W waves, read by waves that hold F
 // fragments of 16 x each, the first of them at x `mine`.
@@ -131,11 +136,11 @@ template <typename H, Layout L, int T, int W, int F, bool RAGGED> struct Staged 
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const int k = k0 + j * ROWS;
-                const int64_t from = min(x0 * 2 + ((lane % LANES) ^ (2 * unit(k))) * 16, s.extent * 2 - 16);
+                const int64_t from = min(x0 * 2 + ((lane % LANES) ^ (2 * unit<T>(k))) * 16, s.extent * 2 - 16);
                 off[j] = (uint32_t)(k * s.pitch + from);
             }
             const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
-            at[0] = k * (T * 2) + ((mine / 16) ^ unit(k)) * 32 + (lane & 3) * 8;
+            at[0] = k * (T * 2) + ((mine / 16) ^ unit<T>(k)) * 32 + (lane & 3) * 8;
             at[1] = at[0] + 32 * (T * 2);
         }
     }
@@ -394,27 +399,34 @@ struct Share {
     uint32_t whole, rest, parts;  // tiles with a workgroup of their own, the others, parts of each of these
 };
 
-constexpr uint32_t PARTS_ROOM = 2, MOST_PARTS = 64;  // parts of a launch, in rooms of workgroups; of a tile
+constexpr uint32_t PARTS_ROOM = 4, MOST_PARTS = 64;  // parts of a launch, in rooms of workgroups; of a tile
 
 // What a launch takes, in ns, measured: `step` a step of as many tiles as the GPU holds
-// at a time (256 wide: one a CU, 128 wide: two), `ends` a tile's start and end, a part's
-// way through memory and back, the second launch.
+// at a time (256 wide: one a CU, 128 wide: two, 64 wide: four), `alone` of at most one a
+// CU, `ends` a tile's start and end, a part's way through memory and back, the second
+// launch, and `least` what all of its operands' way from memory takes.
 struct Cost {
-    int32_t step, ends, part, again;
+    int32_t step, alone, ends, part, again;
+    int64_t least;
 };
 
-__host__ __device__ inline Cost cost_of(int tile, int pairs, int ends = 0)
+__host__ __device__ inline uint32_t room_of(int tile, int cus) { return (uint32_t)cus * (tile > 128 ? 1 : tile > 64 ? 2 : 4); }
+
+__host__ __device__ inline Cost cost_of(int tile, int pairs, int ends = 0, int64_t bytes = 0)
 {
-    if (tile > 128) return {1600 * pairs, ends ? ends : 6000, 110, 10000};
-    return {1050 * pairs, ends ? ends : 4000, 28, 10000};
+    const int64_t least = bytes / 4900;  // at 4.9 TB/s
+    if (tile > 128) return {1600 * pairs, 1600 * pairs, ends ? ends : 6000, 110, 10000, least};
+    if (tile > 64) return {1050 * pairs, 630 * pairs, ends ? ends : 4000, 28, 10000, least};
+    return {900 * pairs, 400 * pairs, ends ? ends : 3000, 7, 10000, least};
 }
 
 // The last, incomplete round of `rest` tiles in n parts each; -1 where that is not done.
 __host__ __device__ inline int64_t ns_of_rest(uint32_t rest, int64_t steps, uint32_t room, uint32_t n, const Cost& c)
 {
-    if (n == 1) return steps * c.step + c.ends;
-    if (n * rest > PARTS_ROOM * room || 2 * n > steps) return -1;
-    return (n * rest + room - 1) / room * ((steps + n - 1) / n * c.step + c.ends) + c.again + (int64_t)c.part * n * rest;
+    if (n > 1 && (n * rest > PARTS_ROOM * room || 2 * n > steps)) return -1;
+    const uint32_t all = n * rest;
+    const int64_t ns = (all + room - 1) / room * ((steps + n - 1) / n * (all <= room / 4 || (all <= room / 2 && c.part > 7) ? c.alone : c.step) + c.ends);
+    return (ns > c.least ? ns : c.least) + (n > 1 ? c.again + (int64_t)c.part * all : 0);
 }
 
 inline Share share_of(uint32_t tiles, int64_t steps, uint32_t room, const Cost& c)
@@ -505,6 +517,8 @@ template <typename J> __device__ __forceinline__ void settle_tiles(const typenam
     for (int i = 0; i < G::FP; ++i)
 #pragma unroll
         for (int j = 0; j < G::FQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // small tiles: two parts on their way at a time
+#pragma unroll(G::FP <= 4 ? 2 : 1)
     for (uint32_t n = 0; n < sh.parts; ++n) {
         const float* const o = part_of<J>(a, n * sh.rest + which);
 #pragma unroll

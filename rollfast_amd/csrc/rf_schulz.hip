@@ -245,7 +245,7 @@ template <bool SQUARE, bool SPLIT, int TILE_, int WP, int WQ> struct Symmetric :
     static constexpr int TILE = TILE_;
     typedef Product<f16, KALONG, KALONG, TILE, TILE, WP, WQ> G;
     static constexpr int PITCH = TILE / WP * 2 + 16, ROOM = TILE / WQ * PITCH;
-    static constexpr int LDS = std::max(G::LDS, G::WAVES * ROOM), SETTLE_LDS = ROOM, ENDS = TILE > 128 ? 8000 : 5000;
+    static constexpr int LDS = std::max(G::LDS, G::WAVES * ROOM), SETTLE_LDS = ROOM, ENDS = TILE > 128 ? 8000 : TILE > 64 ? 5000 : 3000;
 
     static __host__ __device__ int64_t steps(const Item& it) { return (SQUARE ? it.n : it.m) / STEP; }
     static __host__ int64_t tiles(const Item& it)
@@ -346,7 +346,7 @@ __device__ __forceinline__ void put_out8(const Item& it, int64_t r, int64_t c, f
 template <bool SPLIT, int TILE_, int WP, int WQ> struct Apply : Batched<Apply<SPLIT, TILE_, WP, WQ>> {
     static constexpr int TILE = TILE_;
     typedef Product<f16, KDOWN, KALONG, TILE, TILE, WP, WQ> G;
-    static constexpr int LDS = G::LDS, SETTLE_LDS = 0, ENDS = TILE > 128 ? 24000 : 8500;  // (X read and written)
+    static constexpr int LDS = G::LDS, SETTLE_LDS = 0, ENDS = TILE > 128 ? 24000 : TILE > 64 ? 8500 : 5000;  // (X read and written)
 
     static __host__ __device__ int64_t steps(const Item& it) { return it.n / STEP; }
     static __host__ int64_t tiles(const Item& it) { return (int64_t)((it.n + TILE - 1) / TILE) * ((it.m + TILE - 1) / TILE); }
@@ -494,7 +494,7 @@ template <typename F> uint32_t number(Batch& t, F tiles)
 // sums first as the list is (see run), and shares them out.  ns: what it takes.
 template <typename J> double lay_out(Batch& t, int cus, int pairs)
 {
-    t.room = (uint32_t)cus * (J::TILE > 128 ? 1 : 2);
+    t.room = room_of(J::TILE, cus);
     t.tiles = 0;
     int64_t units = 0, longest = 0, shortest = 1ll << 40;
     for (int i = 0; i < t.count; ++i) {
@@ -521,11 +521,15 @@ template <typename J> rf_status multiply(Batch& t, hipStream_t st)
     return s != RF_OK ? s : launch<k_settle<J>>((int64_t)t.share.rest * J::G::WAVES, WAVE, J::SETTLE_LDS, st, t);
 }
 
-// With the tiles that take less.
-template <typename Big, typename Small> rf_status product(Batch& t, int cus, int pairs, hipStream_t st)
+// With the tiles that take least.
+template <typename Big, typename Middle, typename Small> rf_status product(Batch& t, int cus, int pairs, hipStream_t st)
 {
-    const double big = lay_out<Big>(t, cus, pairs);
-    if (lay_out<Small>(t, cus, pairs) <= big) return multiply<Small>(t, st);
+    const double big = lay_out<Big>(t, cus, pairs), middle = lay_out<Middle>(t, cus, pairs);
+    if (lay_out<Small>(t, cus, pairs) <= std::min(big, middle)) return multiply<Small>(t, st);
+    if (middle <= big) {
+        lay_out<Middle>(t, cus, pairs);
+        return multiply<Middle>(t, st);
+    }
     lay_out<Big>(t, cus, pairs);
     return multiply<Big>(t, st);
 }
@@ -533,10 +537,10 @@ template <typename Big, typename Small> rf_status product(Batch& t, int cus, int
 template <bool SPLIT> rf_status step(Batch& t, int cus, hipStream_t st)
 {
     constexpr int PAIRS = SPLIT ? 3 : 1;
-    rf_status s = product<Symmetric<false, SPLIT, 256, 2, 4>, Symmetric<false, SPLIT, 128, 2, 2>>(t, cus, PAIRS, st);
-    if (s == RF_OK) s = product<Symmetric<true, SPLIT, 256, 2, 4>, Symmetric<true, SPLIT, 128, 2, 2>>(t, cus, PAIRS, st);
+    rf_status s = product<Symmetric<false, SPLIT, 256, 2, 4>, Symmetric<false, SPLIT, 128, 2, 2>, Symmetric<false, SPLIT, 64, 2, 2>>(t, cus, PAIRS, st);
+    if (s == RF_OK) s = product<Symmetric<true, SPLIT, 256, 2, 4>, Symmetric<true, SPLIT, 128, 2, 2>, Symmetric<true, SPLIT, 64, 2, 2>>(t, cus, PAIRS, st);
     if (s != RF_OK) return s;
-    return product<Apply<SPLIT, 256, 2, 4>, Apply<SPLIT, 128, 2, 2>>(t, cus, PAIRS, st);
+    return product<Apply<SPLIT, 256, 2, 4>, Apply<SPLIT, 128, 2, 2>, Apply<SPLIT, 64, 2, 2>>(t, cus, PAIRS, st);
 }
 
 // The largest singular value, and the largest |b s^2 + c s^4|, that the steps can
@@ -605,7 +609,8 @@ struct Needs {
 Needs needs_of(const Matrix* list, int64_t count, int64_t at, int cus)
 {
     Needs need{at, 0, 0, 0};
-    int64_t tiles[2] = {};  // of the product with the most
+    constexpr int64_t TILES[3] = {64, 128, 256};
+    int64_t tiles[3] = {};  // of the product with the most
     for (; need.end < count && need.end - at < MAX; ++need.end) {
         const Matrix& m = list[need.end];
         const bool some = m.rows && m.cols;
@@ -614,11 +619,10 @@ Needs needs_of(const Matrix* list, int64_t count, int64_t at, int cus)
         need.buffers += more;
         if (!some) continue;
         const Item it = item_of(m);
-        for (int big = 0; big < 2; ++big) tiles[big] += up(it.n, big ? 256 : 128) * up(it.m, big ? 256 : 128) / (big ? 65536 : 16384);
+        for (int k = 0; k < 3; ++k) tiles[k] += ((it.n + TILES[k] - 1) / TILES[k]) * ((it.m + TILES[k] - 1) / TILES[k]);
     }
-    // at most 64 parts of a tile
-    for (int big = 0; big < 2; ++big)
-        need.parts = std::max(need.parts, std::min<int64_t>(cus * (big ? 1 : 2) * PARTS_ROOM, tiles[big] * 64) * (big ? 65536 : 16384) * 4);
+    for (int k = 0; k < 3; ++k)
+        need.parts = std::max(need.parts, std::min<int64_t>((int64_t)room_of((int)TILES[k], cus) * PARTS_ROOM, tiles[k] * MOST_PARTS) * TILES[k] * TILES[k] * 4);
     need.sums = (need.end - at) * PARTS * 8;
     return need;
 }
