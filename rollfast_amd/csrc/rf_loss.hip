@@ -643,15 +643,18 @@ struct Shape {
 
 Shape shape_of(int64_t cols, int64_t rows, int64_t steps, int pairs, int64_t bytes, int cus)
 {
-    double ns[2];
-    for (int big = 0; big < 2; ++big) {
-        const int tile = big ? 256 : 128;
-        const int64_t tiles = ((cols + tile - 1) / tile) * ((rows + tile - 1) / tile);
-        const uint32_t room = room_of(tile, cus);
-        const Cost c = cost_of(tile, pairs, 0, bytes);
-        ns[big] = ns_of(share_of((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, c), steps, room, c);
+    int tile = 0;
+    double least = 0;
+    for (const int of : {64, 128, 256}) {
+        const int64_t tiles = ((cols + of - 1) / of) * ((rows + of - 1) / of);
+        const uint32_t room = room_of(of, cus);
+        const Cost c = cost_of(of, pairs, 0, bytes);
+        const double ns = ns_of(share_of((uint32_t)std::min<int64_t>(tiles, 1u << 30), steps, room, c), steps, room, c);
+        if (!tile || ns < least) {
+            tile = of;
+            least = ns;
+        }
     }
-    const int tile = ns[1] < ns[0] ? 256 : 128;
     return {tile, (uint32_t)((cols + tile - 1) / tile), room_of(tile, cus)};
 }
 
@@ -774,8 +777,9 @@ template <typename H, typename E> rf_status logits(const Plan& p, const Logits& 
     const int64_t tiles = tiles_of(p.logits, a.rows);
     // one row of tiles, or none: the share is known here
     const bool whole = a.rows <= p.logits.tile && share_of(p.logits.tiles_p, a.steps, p.logits.room, cost_of(p.logits.tile, a.pairs, 0, p.bytes_of_weight)).rest == 0;
-    return p.logits.tile > 128 ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
-                               : multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole);
+    return p.logits.tile > 128  ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
+           : p.logits.tile > 64 ? multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole)
+                                : multiply<LogitsJob<H, E, 64, 1, 4>>(p.logits, tiles, a, st, whole);
 }
 
 template <typename H, Layout LQ> rf_status product(const Shape& shape, float* partial, Grad& a, hipStream_t st)
@@ -784,7 +788,9 @@ template <typename H, Layout LQ> rf_status product(const Shape& shape, float* pa
     a.room = shape.room;
     a.partial = partial;
     const int64_t tiles = tiles_of(shape, a.rows);
-    return shape.tile > 128 ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st) : multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st);
+    return shape.tile > 128  ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st)
+           : shape.tile > 64 ? multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st)
+                             : multiply<GradJob<H, LQ, 64, 2, 2>>(shape, tiles, a, st);
 }
 
 template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const Plan& p, char* ws, hipStream_t st)

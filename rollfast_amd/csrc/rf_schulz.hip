@@ -14,12 +14,13 @@
 // bring them near f16's largest, and entries 2^-29 of the bound are still exact to
 // their last bits.  What f16 rounds away from X would be lost to small singular
 // values, which grow by a factor of a in every step: X is kept in two parts, high
-// and low, 22 bits, and the term (a + B_ii) X takes both; only the product with the
-// rest of B takes the high part alone, B's diagonal being kept in f32 apart.  In
-// 64-bit simulation that leaves an error of 3e-4 to 9e-4 of the result's norm for
-// matrices of 256 x 256 to 768 x 2304, Gaussian or close to low rank (both parts left
-// out: 1.5e-2 for the latter, 1.2e-1 near rank one), beside bf16's rounding of the
-// result, 1.7e-3.  Results in f32 or f16 take both parts of X, A and B everywhere, in
+// and low, the low one a byte, 19 bits together, and the term (a + B_ii) X takes both;
+// only the product with the rest of B takes the high part alone, B's diagonal being
+// kept in f32 apart.  In 64-bit simulation that leaves an error of 3e-4 to 9e-4 of the
+// result's norm for matrices of 256 x 256 to 768 x 2304, Gaussian or close to low rank
+// (without low parts and diagonal: 1.5e-2 for the latter), and up to 1.2e-3 near rank
+// one (low parts of 22 bits 1.1e-3, none 1.5e-1), beside bf16's rounding of the result,
+// 1.7e-3.  Results in f32 or f16 take both parts of X, A and B everywhere, in
 // three products: high high, high low, low high.
 #include "rf_schulz.h"
 
@@ -51,8 +52,9 @@ struct Item {
     uint32_t first;    // its first tile
     uint8_t tall, in_dtype, out_dtype, add_dtype;
 
-    // X and the next X: [n, m] high parts, then low parts.  A and B: [n, n] high
-    // parts; split: then low parts.  B's diagonal [n].
+    // X and the next X: [n, m] high parts, then low parts (a byte each, or f16 where they
+    // are operands: split).  A and B: [n, n] high parts; split: then low parts.  B's
+    // diagonal [n].
     __host__ __device__ int64_t plane() const { return (int64_t)n * m; }
     __host__ __device__ int64_t square(bool split) const { return (int64_t)n * n * (split ? 2 : 1); }
     __device__ uint16_t* x(int turn) const { return buffers + (turn ? 2 * plane() : 0); }
@@ -64,6 +66,7 @@ struct Item {
 
 struct Batch {
     int32_t count, turn;  // turn: x and y change places
+    int32_t last;         // the last step: X's low parts are read no more
     float a, b, c;        // the step's coefficients
     float eps, x_scale, a_scale, b_scale;
     uint32_t tiles;
@@ -79,6 +82,33 @@ __device__ __forceinline__ int find(const Batch& t, uint32_t id)
     int i = 0;
     while (i + 1 < t.count && id >= t.item[i + 1].first) ++i;
     return i;
+}
+
+// What f16 rounded away of a value, in a byte: the difference of the two as f32 have
+// it in their last bits, 13 of them, to 8 (so 19 bits of X's 24 are kept).  Where hi
+// is below f16's normal numbers it may not fit, and is off by less than 2^-25.
+__device__ __forceinline__ uint32_t low_byte(float v, float hi)
+{
+    const int d = (int)__float_as_uint(v) - (int)__float_as_uint(hi);
+    return (uint32_t)min(max((d + 16) >> 5, -128), 127) & 255u;
+}
+
+__device__ __forceinline__ uint32_t low_bytes(f32x4 v, f32x4 hi)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w |= low_byte(v[k], hi[k]) << (8 * k);
+    return w;
+}
+
+__device__ __forceinline__ f32x4 with_low_bytes(f32x4 hi, uint32_t low)
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int d = (int)(low << (24 - 8 * k)) >> 24;
+        hi[k] = __uint_as_float(__float_as_uint(hi[k]) + (uint32_t)(d * 32));
+    }
+    return hi;
 }
 
 // Partial sums of squares, in f64 (a square of an f32 may have no f32): part s of a
@@ -116,7 +146,7 @@ __global__ __launch_bounds__(256) void k_squares(const Batch t)
 }
 
 // G into X's layout, a tile of 64 x 64 of X a workgroup.
-__global__ __launch_bounds__(256) void k_load(const Batch t)
+template <bool SPLIT> __global__ __launch_bounds__(256) void k_load(const Batch t)
 {
     __shared__ float tile[64][65];
     const Item& it = t.item[find(t, blockIdx.x)];
@@ -155,11 +185,17 @@ __global__ __launch_bounds__(256) void k_load(const Batch t)
         for (int k = 0; k < 8; ++k) v[k] = tile[q][p + k];
         const Raw<f16> hi = narrow8<f16>(v);
         widen8(hi, back);
+        const int64_t at = (q0 + q) * it.m + p0 + p;
+        *(u32x4*)(it.x(0) + at) = hi.a;
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] -= back[k];
-        uint16_t* const o = it.x(0) + (q0 + q) * it.m + p0 + p;
-        *(u32x4*)o = hi.a;
-        *(u32x4*)(o + plane) = narrow8<f16>(v).a;
+            for (int k = 0; k < 8; ++k) v[k] -= back[k];
+            *(u32x4*)(it.x(0) + plane + at) = narrow8<f16>(v).a;
+        } else {
+            const u32x2 low = {low_bytes(f32x4{v[0], v[1], v[2], v[3]}, f32x4{back[0], back[1], back[2], back[3]}),
+                               low_bytes(f32x4{v[4], v[5], v[6], v[7]}, f32x4{back[4], back[5], back[6], back[7]})};
+            *(u32x2*)((uint8_t*)(it.x(0) + plane) + at) = low;
+        }
     }
 }
 
@@ -377,15 +413,17 @@ __device__ __forceinline__ void Apply<SPLIT, TILE, WP, WQ>::finish(const Batch& 
     const float of_product = 1.0f / t.b_scale;
     const int64_t wp = at.p0 + G::wp(wave), wq = at.q0 + G::wq(wave);
     // X here, a row of fragments ahead: all of its loads in flight together
-    struct Row { u32x4 hi[G::FP / 2], lo[G::FP / 2]; float d; } row[2];
+    typedef std::conditional_t<SPLIT, u32x4, u32x2> Low;
+    struct Row { u32x4 hi[G::FP / 2]; Low lo[G::FP / 2]; float d; } row[2];
     auto fetch = [&](int j, Row& r) {
         const int64_t q = min(wq + 16 * j + lane % 16, n - 1);
         r.d = it.d(SPLIT)[q];
 #pragma unroll
         for (int i = 0; i < G::FP; i += 2) {
-            const uint16_t* const o = x + q * m + min(wp + 16 * i + chunk_of(lane), m - 8);
-            r.hi[i / 2] = *(const u32x4*)o;
-            r.lo[i / 2] = *(const u32x4*)(o + plane);
+            const int64_t from = q * m + min(wp + 16 * i + chunk_of(lane), m - 8);
+            r.hi[i / 2] = *(const u32x4*)(x + from);
+            if constexpr (SPLIT) r.lo[i / 2] = *(const u32x4*)(x + plane + from);
+            else r.lo[i / 2] = *(const u32x2*)((const uint8_t*)(x + plane) + from);
         }
     };
     fetch(0, row[0]);
@@ -399,19 +437,37 @@ __device__ __forceinline__ void Apply<SPLIT, TILE, WP, WQ>::finish(const Batch& 
         for (int i = 0; i < G::FP; i += 2) {
             f32x4 v[2];
             u32x2 h[2], l[2];
+            uint32_t bytes[2];
             quads(old.hi[i / 2], h[0], h[1]);
-            quads(old.lo[i / 2], l[0], l[1]);
+            if constexpr (SPLIT) {
+                quads(old.lo[i / 2], l[0], l[1]);
+            } else {
+                const auto b = __builtin_amdgcn_permlane16_swap(old.lo[i / 2][0], old.lo[i / 2][1], false, false);
+                bytes[0] = b[0];
+                bytes[1] = b[1];
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                v[k] = diagonal * (widen4<f16>(h[k]) + widen4<f16>(l[k])) + of_product * acc[i + k][j];
+                const f32x4 was = SPLIT ? widen4<f16>(h[k]) + widen4<f16>(l[k]) : with_low_bytes(widen4<f16>(h[k]), bytes[k]);
+                v[k] = diagonal * was + of_product * acc[i + k][j];
                 h[k] = narrow4<f16>(v[k]);
-                l[k] = narrow4<f16>(v[k] - widen4<f16>(h[k]));
+                if (SPLIT) l[k] = narrow4<f16>(v[k] - widen4<f16>(h[k]));
+                else bytes[k] = low_bytes(v[k], widen4<f16>(h[k]));
             }
             const int64_t p = wp + 16 * i + chunk_of(lane), to = q * m + p;
-            const u32x4 hi = chunk(h[0], h[1]), lo = chunk(l[0], l[1]);
-            if (q < n && p < m) {
-                *(u32x4*)(y + to) = hi;
-                *(u32x4*)(y + plane + to) = lo;
+            const u32x4 hi = chunk(h[0], h[1]);
+            if constexpr (SPLIT) {
+                const u32x4 lo = chunk(l[0], l[1]);
+                if (q < n && p < m) {
+                    *(u32x4*)(y + to) = hi;
+                    *(u32x4*)(y + plane + to) = lo;
+                }
+            } else {
+                const auto lo = __builtin_amdgcn_permlane16_swap(bytes[0], bytes[1], false, false);
+                if (q < n && p < m) {
+                    *(u32x4*)(y + to) = hi;
+                    if (!t.last) *(u32x2*)((uint8_t*)(y + plane) + to) = u32x2{lo[0], lo[1]};
+                }
             }
         }
     }
@@ -431,8 +487,9 @@ template <typename J> __global__ __launch_bounds__(WAVE, 2) void k_settle(const 
 
 // Outputs from X, a tile of 64 x 64 a workgroup; tall matrices' are transposed.  (In the
 // last product's epilogue they would need registers that its sums take: with tiles of 256
-// it spilled 340 and took 942 us where this and the product take 560.)
-__global__ __launch_bounds__(256) void k_store(const Batch t)
+// it spilled 340 and took 942 us where this and the product take 560.)  bf16 results are
+// rounded from X's high part, whose 11 bits add an eighth to their worst half step.
+template <bool SPLIT> __global__ __launch_bounds__(256) void k_store(const Batch t)
 {
     __shared__ float tile[64][65];
     const Item& it = t.item[find(t, blockIdx.x)];
@@ -444,9 +501,9 @@ __global__ __launch_bounds__(256) void k_store(const Batch t)
     for (int i = 0; i < 2; ++i) {
         const int q = i * 32 + tid / 8, p = tid % 8 * 8;
         const uint16_t* const o = it.x(t.turn) + (q0 + q) * it.m + p0 + p;
-        float w[8], w2[8];
+        float w[8], w2[8] = {};
         widen8(Raw<f16>{*(const u32x4*)o}, w);
-        widen8(Raw<f16>{*(const u32x4*)(o + plane)}, w2);
+        if (SPLIT) widen8(Raw<f16>{*(const u32x4*)(o + plane)}, w2);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float v = (w[k] + w2[k]) * last;
@@ -708,18 +765,19 @@ rf_status run(const Matrix* list, int64_t count, const Method& how, char* ws, hi
         s = source ? source(context, which, t.count, u, sums, st) : launch<k_squares>((int64_t)t.count * PARTS, 256, 0, st, t);
         if (s != RF_OK) return s;
         const uint32_t squares = number(t, [](const Item& it) { return (int64_t)it.n / 64 * (it.m / 64); });
-        s = launch<k_load>(squares, 256, 0, st, t);
+        s = split ? launch<k_load<true>>(squares, 256, 0, st, t) : launch<k_load<false>>(squares, 256, 0, st, t);
         if (s != RF_OK) return s;
         for (int i = 0; i < how.steps && s == RF_OK; ++i) {
             t.a = how.coefficients[3 * i];
             t.b = how.coefficients[3 * i + 1];
             t.c = how.coefficients[3 * i + 2];
             t.turn = i & 1;
+            t.last = i + 1 == how.steps;
             s = split ? step<true>(t, cus, st) : step<false>(t, cus, st);
         }
         t.turn = how.steps & 1;
         number(t, [](const Item& it) { return (int64_t)it.n / 64 * (it.m / 64); });
-        if (s == RF_OK) s = launch<k_store>(squares, 256, 0, st, t);
+        if (s == RF_OK) s = split ? launch<k_store<true>>(squares, 256, 0, st, t) : launch<k_store<false>>(squares, 256, 0, st, t);
         if (s != RF_OK) return s;
     }
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return rf::report_hip(e, "orthogonalisation");
