@@ -213,8 +213,9 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ, bool
     static __device__ __forceinline__ int wp(int w) { return w / WQ * (TP / WP); }
     static __device__ __forceinline__ int wq(int w) { return w % WQ * (TQ / WQ); }
 
-    // The sums over steps s0 .. s1 - 1 of each of the plane pairs (3: high
-    // times high, high times low, low times high).  Ends with no load in flight.
+    // The sums over steps s0 .. s1 - 1 of each of the plane pairs (3: high times low, low
+    // times high, high times high: the small ones first, that fewer sums are rounded at
+    // full size).  Ends with no load in flight.
     static __device__ __forceinline__ void run(char* lds, const Side& sp, const Side& sq, int64_t p0, int64_t q0,
                                                int64_t s0, int64_t s1, int pairs, Sums& acc)
     {
@@ -235,8 +236,8 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ, bool
         q.set(sq, q0, w, wq(w), lane);
         int pair = 0, ahead = from;  // of the step to be loaded next
         auto seek = [&] {
-            p.seek(sp, pair == 2, p0, ahead);
-            q.seek(sq, pair == 1, q0, ahead);
+            p.seek(sp, pair == 1, p0, ahead);
+            q.seek(sq, pairs > 1 && pair == 0, q0, ahead);
         };
         auto next = [&] {
             ++ahead;
