@@ -765,9 +765,21 @@ template <auto K, typename... A> rf_status launch(int64_t grid, int threads, siz
 // the device alone).
 template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, const typename J::Args& a, hipStream_t st, bool never_split = false)
 {
-    const rf_status s = launch<k_multiply<J>>(tiles + PARTS_ROOM * shape.room, J::G::THREADS, J::LDS, st, a);
+    const rf_status s = launch<k_multiply<J>>(tiles + (never_split ? 0 : PARTS_ROOM * shape.room), J::G::THREADS, J::LDS, st, a);
     if (s != RF_OK || never_split) return s;
     return launch<k_settle<J>>((int64_t)std::min<int64_t>(tiles, shape.room) * J::G::WAVES, WAVE, 0, st, a);
+}
+
+// Whether no number of tokens that count splits a tile, where that is soon found: a
+// launch with nothing to settle takes 4.5 us.
+bool never_splits(const Shape& shape, const Plan& p, int64_t tiles_q, int64_t steps)
+{
+    if (steps < 4) return true;  // (no part of fewer than two)
+    if (tiles_q > 4) return false;
+    const Cost c = cost_of(shape.tile, p.pairs, 0, p.bytes_of_weight);
+    for (int64_t q = 1; q <= tiles_q; ++q)
+        if (share_of((uint32_t)(shape.tiles_p * q), steps, shape.room, c).rest) return false;
+    return true;
 }
 
 int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles_p * ((rows + shape.tile - 1) / shape.tile); }
@@ -775,22 +787,23 @@ int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles
 template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
 {
     const int64_t tiles = tiles_of(p.logits, a.rows);
-    // one row of tiles, or none: the share is known here
-    const bool whole = a.rows <= p.logits.tile && share_of(p.logits.tiles_p, a.steps, p.logits.room, cost_of(p.logits.tile, a.pairs, 0, p.bytes_of_weight)).rest == 0;
+    const bool whole = never_splits(p.logits, p, (a.rows + p.logits.tile - 1) / p.logits.tile, a.steps);
     return p.logits.tile > 128  ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
            : p.logits.tile > 64 ? multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole)
                                 : multiply<LogitsJob<H, E, 64, 1, 4>>(p.logits, tiles, a, st, whole);
 }
 
-template <typename H, Layout LQ> rf_status product(const Shape& shape, float* partial, Grad& a, hipStream_t st)
+template <typename H, Layout LQ> rf_status product(const Plan& p, const Shape& shape, float* partial, Grad& a, hipStream_t st)
 {
     a.tiles_p = shape.tiles_p;
     a.room = shape.room;
     a.partial = partial;
     const int64_t tiles = tiles_of(shape, a.rows);
-    return shape.tile > 128  ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st)
-           : shape.tile > 64 ? multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st)
-                             : multiply<GradJob<H, LQ, 64, 2, 2>>(shape, tiles, a, st);
+    // dhidden: the sums' steps are known, of dweight the tiles
+    const bool whole = LQ == KALONG ? never_splits(shape, p, (a.rows + shape.tile - 1) / shape.tile, a.steps) : (a.piece_rows + STEP - 1) / STEP < 4;
+    return shape.tile > 128  ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st, whole)
+           : shape.tile > 64 ? multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st, whole)
+                             : multiply<GradJob<H, LQ, 64, 2, 2>>(shape, tiles, a, st, whole);
 }
 
 template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const Plan& p, char* ws, hipStream_t st)
@@ -906,7 +919,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.order = order;
         g.out = a.dhidden;
         if (rows) {
-            s = product<H, KALONG>(p.dhidden, (float*)(ws + p.partial), g, st);
+            s = product<H, KALONG>(p, p.dhidden, (float*)(ws + p.partial), g, st);
             if (s != RF_OK) return s;
         }
         g.p = x;
@@ -918,7 +931,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.sums = p.f32 ? (float*)a.dweight : (float*)(ws + p.sums);
         g.begin = piece == 0;
         g.end = piece + 1 == p.pieces;
-        s = product<H, KDOWN>(p.dweight, (float*)(ws + p.partial), g, st);
+        s = product<H, KDOWN>(p, p.dweight, (float*)(ws + p.partial), g, st);
         if (s != RF_OK) return s;
     }
     if (a.reduction != RF_REDUCE_NONE)

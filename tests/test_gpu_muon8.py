@@ -150,3 +150,26 @@ def test_with_adamw8_for_the_other_leaves():
         for k in params:
             assert torch.equal(updates[k], (a if k in a else b)[k]), (k, turn)
         params = rf().apply_updates(params, updates, stochastic=False) if turn == 0 else params
+
+
+@pytest.mark.parametrize("block_size", [1, 4, 8, 16, 64, 512, 1024, 4096])
+@pytest.mark.parametrize("count", [1, 5])
+def test_block_sizes(count, block_size):
+    """Blocks that a wave takes several of, and others; in one list or many."""
+    tx = rf().muon8(0.02, block_size=block_size, min_size=0)
+    params = [gaussian(r, c, F32, seed=i) for i, (r, c) in enumerate([(257, 31), (1, 5), (64, 64), (130, 515), (9, 57)][:count])]
+    state = tx.init(params)
+    host = [np.zeros(p.shape, np.float32) for p in params]
+    for turn in range(2):
+        grads = [low_rank(*p.shape, F32, seed=10 * turn + i, noise=0.3) for i, p in enumerate(params)]
+        grads[0][3] = 0.0  # a row of nothing: blocks with a scale of their own
+        updates, state = tx.update(grads, state, params)
+        for i, p in enumerate(params):
+            m, u = step(host[i], grads[i].cpu().numpy(), 0.95, True)
+            codes, scales = orc.quantize(m, block_size)
+            assert np.array_equal(state.mu[i].values.cpu().numpy(), codes), (i, turn)
+            assert np.array_equal(state.mu[i].scales.cpu().numpy().view(np.uint32), scales.view(np.uint32)), (i, turn)
+            host[i] = orc.dequantize(codes, scales, m.size, block_size).reshape(m.shape)
+            r, c = p.shape
+            ref = -0.02 * math.sqrt(max(1.0, r / c)) * exact(torch.from_numpy(u).cuda())
+            assert (updates[i].double() - ref).norm().item() < BOUND[F32] * ref.norm().item() * 1.2, (i, turn)
