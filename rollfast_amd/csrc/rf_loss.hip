@@ -494,7 +494,7 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
     const E* const in = (const E*)a.e + q * a.pitch;
     for (int64_t v = (int64_t)threadIdx.x * 8; v < a.pitch; v += 2048) {
         Raw<E> raw;
-        raw.a = *(const u32x4*)(in + v);
+        raw.a = __builtin_nontemporal_load((const u32x4*)(in + v));
         if constexpr (sizeof(E) == 4) raw.b = *(const u32x4*)(in + v + 4);
         float x[8];
         widen8(raw, x);
@@ -511,7 +511,7 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
             *(u32x4*)(out + v) = h.a;
             *(u32x4*)(a.dz_low + q * a.pitch + v) = l.a;
         } else {
-            *(u32x4*)(out + v) = narrow8<P>(x).a;
+            __builtin_nontemporal_store(narrow8<P>(x).a, (u32x4*)(out + v));
         }
     }
 }
