@@ -615,7 +615,7 @@ template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
                     const f32x4 x = acc[i][j] * f.unscale, y = acc[i + 1][j] * f.unscale;
                     const u32x4 c = __is_same(H, bf16) ? chunk(narrow4<bf16>(x), narrow4<bf16>(y)) : chunk(narrow4<f16>(x), narrow4<f16>(y));
                     const int64_t from = p0 + 16 * i + chunk_of(lane);
-                    if (q < rows && from < f.cols) put8(row + from, Raw<uint16_t>{c}, f.cols - from);
+                    if (q < rows && from < f.cols) put8<true, LQ == KDOWN>(row + from, Raw<uint16_t>{c}, f.cols - from);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
