@@ -361,3 +361,26 @@ def test_captured_and_replayed(dtype):
         for x, y in zip(got, ref):
             assert torch.equal(x, y), turn
         assert torch.equal(mean, rf().linear_cross_entropy(h2, w2, t2, reduction="mean"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens,vocab,n", [(60, 16000, 576), (65, 8200, 1024), (150, 20011, 256), (193, 4100, 2048),
+                                            (520, 3000, 70), (300, 33000, 128)])
+@pytest.mark.parametrize("masked", [0.0, 0.6, 0.98])
+def test_few_tokens_of_larger_tables(masked, tokens, vocab, n, dtype):
+    """Tiles of every width, whole and split, with as many tokens as the call has or far fewer."""
+    check(*make(tokens, vocab, n, dtype, seed=vocab, masked=masked))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_rows_that_share_memory(dtype):
+    """Expanded rows are read in place; the gradients are those of rows apart."""
+    hidden, weight, targets, dloss = make(70, 300, 128, dtype, seed=9, masked=0.2)
+    one = hidden[3:4].expand(70, 128)
+    check(one, weight, targets, dloss)
+    same = weight[5:6].expand(300, 128)
+    check(hidden, same, targets, dloss)
+    rows = weight.as_strided((200, 128), (64, 1))  # each row begins in the middle of the one before
+    check(hidden, rows, targets % 200, dloss)
+    # one tensor as both: a table of 64 rows against itself
+    check(weight[:64], weight[:64], targets[:64].clamp(min=0) % 64, dloss[:64])

@@ -205,3 +205,24 @@ def test_another_stream_and_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, rf().orthogonalize(other)), turn
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32, F16])
+def test_rows_that_share_memory(dtype):
+    g = gaussian(1, 96, dtype)
+    wide = g.expand(40, 96)
+    # rank one: its only singular value is the norm
+    assert off(rf().orthogonalize(wide), exact(wide.contiguous())) < BOUND[dtype]
+    table = gaussian(300, 64, dtype, seed=1)
+    rows = table.as_strided((120, 64), (16, 1))
+    assert off(rf().orthogonalize(rows), exact(rows.contiguous())) < BOUND[dtype]
+    got = rf().orthogonalize([table, table])
+    assert torch.equal(got[0], got[1]) and got[0].data_ptr() != got[1].data_ptr()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_matrix_of_each_tile(dtype):
+    """From sides that tiles of 64 share out to ones that fill the GPU with tiles of 256."""
+    for r, c in ((200, 330), (390, 1300), (1000, 1100), (1700, 2600)):
+        g = low_rank(r, c, dtype, seed=r, noise=0.2)
+        assert off(rf().orthogonalize(g), exact(g)) < BOUND[dtype], (r, c)
