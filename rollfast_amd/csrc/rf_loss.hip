@@ -633,9 +633,9 @@ template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
 // ------------------------------------------------------------------- host ---
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Tile of a product: the one that takes less (us, measured): a step of 64 k of the
-// tiles that the GPU holds at a time, 256 wide one a CU or 128 wide two, and 6 or 4 for a
-// tile's start and end.
+// Tile of a product: the one that takes least by the measured costs in rf_product.h.
+// Logits of 1 x 32000 x 4096: tiles of 64 40 us, of 128 53; both gradients of 6001 x
+// 131101 x 2048: tiles of 256, dhidden's 192 in four parts, 2.5 ms, tiles of 128 3.4.
 struct Shape {
     int tile;
     uint32_t tiles_p, room;

@@ -400,7 +400,9 @@ struct Share {
     uint32_t whole, rest, parts;  // tiles with a workgroup of their own, the others, parts of each of these
 };
 
-constexpr uint32_t PARTS_ROOM = 4, MOST_PARTS = 64;  // parts of a launch, in rooms of workgroups; of a tile
+// Parts of a launch, in rooms of workgroups (with two in place of four a product of 192
+// tiles of 256 stayed whole, or took tiles of 128: 3.4 ms, so 2.5); parts of a tile.
+constexpr uint32_t PARTS_ROOM = 4, MOST_PARTS = 64;
 
 // What a launch takes, in ns, measured: `step` a step of as many tiles as the GPU holds
 // at a time (256 wide: one a CU, 128 wide: two, 64 wide: four), `alone` of at most one a
