@@ -6,6 +6,11 @@ Drop-in for the reference's adam8 hot path (rollfast ``adamw8``,
 ``scale_by_adam``): same names, arguments, state pytree and errors, with
 torch tensors on a ROCm device in place of jax arrays.  ``adamw8_step`` /
 ``adamw_step`` fuse ``tx.update`` and ``apply_updates`` into one HBM pass.
+
+Beside it, without reference counterparts: the operators of a residual block with
+8-bit saved activations (``blocks``), the loss over the vocabulary with its
+gradients (``losses``), their differentiable forms (``autograd``), and
+``orthogonalize`` with ``muon8``, the optimizer made of it.
 """
 
 from . import prng

@@ -11,6 +11,8 @@ singular values that are still small, whose part of the norm is as small.
   most each, reach the result through (b A + c A^2) X with a factor of at most
   |B| = 4.8 in one of 5 steps and 2.8 in the others, and average out over n terms:
   2 * 2^-11 * (4.8 + 4 * 2.8) / sqrt(3) / 4 = 2.3e-3 together.  2^-8 + 2.3e-3 = 6.2e-3.
+  (The result is rounded to float16 before it is rounded to bfloat16, up to 2^-11
+  more: not added, the bound stays.)
 - float32 results: split numbers of 22 bits and sums of f32 in every product: an
   error of 2^-22 + sqrt(k) U of each entry, times 485 at worst for what is small
   and about 10 for what is not: 2e-5 covers k up to 4096.
