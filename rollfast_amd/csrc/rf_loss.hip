@@ -17,7 +17,8 @@
 //              maximum m and a sum s of exp(z - m); for gradients exp(z - m) itself
 //              too, in f16 (f32 tensors: in f32)
 //   k_rows     lse and loss from m and s, factors of the gradient
-//   k_dlogits  exp(z - m) to dz, in place (f32: to two f16 planes)
+//   k_dlogits  exp(z - m) to dz, in place (f32: to two f16 planes; where few tokens
+//              count to two planes of the tensors' type)
 //   GradJob    dhidden and dweight, two products of the same size
 // Loss alone ends with k_rows and writes no logits.  With gradients a piece of
 // tokens at a time holds at most PIECE bytes of exponentials; the pieces'
@@ -43,6 +44,12 @@ namespace {
 
 constexpr int64_t PIECE = 2ll << 30;        // bytes of exponentials held at once
 constexpr int64_t STATS = 256ll << 20;      // bytes of m and s held at once
+// Where so few 16-bit tokens count, dz goes to its products in two parts, high and low:
+// with few terms its rounding does not average out (bf16, 1 x 896 x 225: gradients off by
+// up to 2.8e-3 of their norm, so 1.7e-3, the rounding of the result; 16 tokens: 2.1e-3).
+// For all of 67 f16 tokens with 32000 x 4096 it would take 327 us in place of 261.
+constexpr int64_t FEW = 16;
+constexpr int64_t HALF = 128;               // tokens of a call that has a place for the low parts
 
 // Written by the kernels, read by later ones.
 struct Scalars {
@@ -56,13 +63,14 @@ struct Scalars {
 struct Piece {
     Share logits, dhidden, dweight;
     uint32_t dz_top;
-    uint32_t pad[2];
+    int32_t pairs;   // plane pairs of the gradients' products
+    uint32_t pad;
 };
 
 // The products of a piece, for k_select.
 struct Products {
     int64_t rows, vocab, hidden, logits_steps, dhidden_steps;
-    int32_t pieces, pairs, grad, cus;
+    int32_t pieces, pairs, grad, few, cus;  // few: dz may go in two parts
     int32_t logits_tile, dhidden_tile, dweight_tile;
 };
 
@@ -73,16 +81,17 @@ __device__ __forceinline__ Piece piece_of(const Products& p, int64_t count, int6
     auto tiles = [](int64_t x, int64_t y, int tile) { return (uint32_t)(((x + tile - 1) / tile) * ((y + tile - 1) / tile)); };
     // each product reads weight, or writes a gradient as large
     const int64_t bytes = p.vocab * p.hidden * (p.pairs > 1 ? 4 : 2);
-    auto share = [&](int64_t x, int64_t y, int64_t n, int tile) {
-        return share_by_wave(tiles(x, y, tile), n, room_of(tile, p.cus), cost_of(tile, p.pairs, 0, bytes));
+    auto share = [&](int64_t x, int64_t y, int64_t n, int tile, int pairs) {
+        return share_by_wave(tiles(x, y, tile), n, room_of(tile, p.cus), cost_of(tile, pairs, 0, bytes));
     };
     Piece out{};
-    out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile);
+    out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile, p.pairs);
     if (!p.grad) return out;
-    out.dhidden = share(p.hidden, rows, p.dhidden_steps, p.dhidden_tile);
+    out.pairs = p.few && count <= FEW ? 2 : p.pairs;
+    out.dhidden = share(p.hidden, rows, p.dhidden_steps, p.dhidden_tile, out.pairs);
     // without tokens there is nothing to add, but what the pieces have summed is to be
     // written by the first and rounded by the last
-    if (steps) out.dweight = share(p.hidden, p.vocab, steps, p.dweight_tile);
+    if (steps) out.dweight = share(p.hidden, p.vocab, steps, p.dweight_tile, out.pairs);
     else if (piece == 0 || piece + 1 == p.pieces) out.dweight = {tiles(p.hidden, p.vocab, p.dweight_tile), 0, 1};
     return out;
 }
@@ -482,10 +491,11 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
     const int64_t q = blockIdx.x, count = min((int64_t)a.sc->count - a.first, a.rows);
     if (q >= (count + STEP - 1) / STEP * STEP) return;
     P* const out = (P*)a.dz + q * a.pitch;
+    uint16_t* const low = a.piece->pairs > 1 ? a.dz_low : nullptr;
     if (q >= count) {
         for (int64_t v = (int64_t)threadIdx.x * 8; v < a.pitch; v += 2048) {
             *(u32x4*)(out + v) = u32x4{};
-            if (sizeof(E) == 4) *(u32x4*)(a.dz_low + q * a.pitch + v) = u32x4{};
+            if (low) *(u32x4*)(low + q * a.pitch + v) = u32x4{};
         }
         return;
     }
@@ -516,9 +526,17 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
             Raw<f16> h, l;
             split8(x, 1.0f, h, l);
             *(u32x4*)(out + v) = h.a;
-            *(u32x4*)(a.dz_low + q * a.pitch + v) = l.a;
+            *(u32x4*)(low + q * a.pitch + v) = l.a;
         } else {
-            __builtin_nontemporal_store(narrow8<P>(x).a, (u32x4*)(out + v));
+            const Raw<P> h = narrow8<P>(x);
+            __builtin_nontemporal_store(h.a, (u32x4*)(out + v));
+            if (low) {
+                float back[8];
+                widen8(h, back);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] -= back[k];
+                *(u32x4*)(low + q * a.pitch + v) = narrow8<P>(x).a;
+            }
         }
     }
 }
@@ -529,7 +547,7 @@ struct Grad {
     int64_t cols, rows;            // of the output: p below cols, q below rows
     int64_t first, piece_rows;     // packed tokens of this piece
     int64_t steps;                 // of the sum; 0: the tokens that count
-    int32_t pairs, dtype;
+    int32_t pairs, dtype;          // pairs: as hidden and weight have them
     const Scalars* sc;
     const Piece* piece;
     const int32_t* order;          // dhidden: the output's row of packed token q; NULL: dweight
@@ -607,7 +625,7 @@ template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
     }
     static __device__ __forceinline__ void run(const Grad& a, const Even& t, char* lds, int64_t s0, int64_t s1, typename G::Sums& acc)
     {
-        G::run(lds, a.p, a.q, t.p0, t.q0, s0, s1, a.pairs, acc);
+        G::run(lds, a.p, a.q, t.p0, t.q0, s0, s1, a.piece->pairs, acc);
     }
     static __device__ __forceinline__ void finish(const Grad& a, const Even& t, typename G::Sums& acc, int wave, char*)
     {
@@ -677,12 +695,12 @@ int64_t parts_of(const Shape& s, int64_t tiles, int64_t steps)
 
 struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
-    bool own_weight, f32, grad;
+    bool own_weight, f32, grad, few;
     int64_t bytes_of_weight;
     int32_t blocks, shift, pairs, cus;
     Shape logits, dhidden, dweight;
     // offsets in the workspace
-    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, hidden, weight, e, dz, sums, partial, bytes;
+    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, hidden, weight, e, dz, low, sums, partial, bytes;
 };
 
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
@@ -694,6 +712,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.f32 = a.dtype == RF_F32;
     p.grad = a.dweight != nullptr;
     p.pairs = p.f32 ? 3 : 1;
+    p.few = p.grad && !p.f32 && a.tokens <= HALF;
     p.pad = up(a.hidden, STEP);
     p.vpad = up(a.vocab, STEP);
     // weight as it is: whole steps of k, 16-byte rows
@@ -734,6 +753,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.at_target = take(p.rows * 4);
         p.e = take(held * p.vpad * (p.f32 ? 4 : 2));
         p.dz = p.f32 ? take(held * p.vpad * 4) : p.e;
+        if (p.few) p.low = take(held * p.vpad * 2);
         if (p.pieces > 1 && !p.f32) p.sums = take(a.vocab * a.hidden * 4);
         p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, bytes, cus);
         p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, bytes, cus);
@@ -782,13 +802,15 @@ template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, cons
 
 // Whether no number of tokens that count splits a tile, where that is soon found: a
 // launch with nothing to settle takes 4.5 us.
-bool never_splits(const Shape& shape, const Plan& p, int64_t tiles_q, int64_t steps)
+bool never_splits(const Shape& shape, const Plan& p, bool few, int64_t tiles_q, int64_t steps)
 {
     if (steps < 4) return true;  // (no part of fewer than two)
     if (tiles_q > 4) return false;
-    const Cost c = cost_of(shape.tile, p.pairs, 0, p.bytes_of_weight);
-    for (int64_t q = 1; q <= tiles_q; ++q)
-        if (share_of((uint32_t)(shape.tiles_p * q), steps, shape.room, c).rest) return false;
+    for (int pairs = p.pairs; pairs <= (few ? 2 : p.pairs); ++pairs) {
+        const Cost c = cost_of(shape.tile, pairs, 0, p.bytes_of_weight);
+        for (int64_t q = 1; q <= tiles_q; ++q)
+            if (share_of((uint32_t)(shape.tiles_p * q), steps, shape.room, c).rest) return false;
+    }
     return true;
 }
 
@@ -797,7 +819,7 @@ int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles
 template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
 {
     const int64_t tiles = tiles_of(p.logits, a.rows);
-    const bool whole = never_splits(p.logits, p, (a.rows + p.logits.tile - 1) / p.logits.tile, a.steps);
+    const bool whole = never_splits(p.logits, p, false, (a.rows + p.logits.tile - 1) / p.logits.tile, a.steps);
     return p.logits.tile > 128  ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
            : p.logits.tile > 64 ? multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole)
                                 : multiply<LogitsJob<H, E, 64, 1, 4>>(p.logits, tiles, a, st, whole);
@@ -810,7 +832,7 @@ template <typename H, Layout LQ> rf_status product(const Plan& p, const Shape& s
     a.partial = partial;
     const int64_t tiles = tiles_of(shape, a.rows);
     // dhidden: the sums' steps are known, of dweight the tiles
-    const bool whole = LQ == KALONG ? never_splits(shape, p, (a.rows + shape.tile - 1) / shape.tile, a.steps) : (a.piece_rows + STEP - 1) / STEP < 4;
+    const bool whole = LQ == KALONG ? never_splits(shape, p, p.few, (a.rows + shape.tile - 1) / shape.tile, a.steps) : (a.piece_rows + STEP - 1) / STEP < 4;
     return shape.tile > 128  ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st, whole)
            : shape.tile > 64 ? multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st, whole)
                              : multiply<GradJob<H, LQ, 64, 2, 2>>(shape, tiles, a, st, whole);
@@ -824,7 +846,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
     int32_t* const target = (int32_t*)(ws + p.target);
     uint16_t* const hidden = (uint16_t*)(ws + p.hidden);
     const int64_t all = up(a.tokens, STEP), plane = all * p.pad;
-    const Products products{p.rows, a.vocab, a.hidden, p.pad / STEP, p.vpad / STEP, (int32_t)p.pieces, p.pairs, p.grad, p.cus,
+    const Products products{p.rows, a.vocab, a.hidden, p.pad / STEP, p.vpad / STEP, (int32_t)p.pieces, p.pairs, p.grad, p.few, p.cus,
                             p.logits.tile, p.dhidden.tile, p.dweight.tile};
     rf_status s = a.target_bits == 64
         ? launch<k_select<int64_t>>(1, SELECT, 0, st, (const int64_t*)a.targets, a.tokens, a.ignore_index, a.vocab, a.loss, order,
@@ -906,14 +928,15 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         }
         r.e = l.e;
         r.dz = ws + p.dz;
-        r.dz_low = (uint16_t*)(ws + p.dz) + up(p.rows, STEP) * p.vpad;
+        if (p.f32) r.dz_low = (uint16_t*)(ws + p.dz) + up(p.rows, STEP) * p.vpad;
+        else if (p.few) r.dz_low = (uint16_t*)(ws + p.low);
         s = launch<k_rows>(std::min<int64_t>((rows + 3) / 4, 2048), 256, 0, st, r);
         if (s != RF_OK) return s;
         if (!p.grad) continue;
         s = launch<k_dlogits<H, std::conditional_t<sizeof(T) == 4, float, f16>>>(held, 256, (size_t)p.blocks * 4, st, r);
         if (s != RF_OK) return s;
         Grad g{};
-        Side dz{{r.dz, p.f32 ? (const void*)r.dz_low : r.dz}, p.vpad * 2, held, held};
+        Side dz{{r.dz, r.dz_low ? (const void*)r.dz_low : r.dz}, p.vpad * 2, held, held};
         g.sc = sc;
         g.piece = piece_info;
         g.first = first;

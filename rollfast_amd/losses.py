@@ -22,7 +22,8 @@ of one dtype, which is the gradients' too; losses are float32.  Targets are int3
 or int64.  Any row stride is read in place.  Work is enqueued on the current
 stream.  16-bit tensors are multiplied as they are, float32 ones to 22 bits; sums
 are f32 in a fixed order: equal inputs give equal bits.  The gradient of a logit
-is rounded to the tensors' own dtype (float32: to 22 bits) before it is multiplied.
+is rounded to the tensors' own dtype (float32: to 22 bits; 16-bit ones where at
+most 16 tokens count: to twice its bits) before it is multiplied.
 """
 
 from __future__ import annotations
