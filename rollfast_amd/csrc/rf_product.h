@@ -407,7 +407,9 @@ constexpr uint32_t PARTS_ROOM = 4, MOST_PARTS = 64;
 // What a launch takes, in ns, measured: `step` a step of as many tiles as the GPU holds
 // at a time (256 wide: one a CU, 128 wide: two, 64 wide: four), `alone` of at most one a
 // CU, `ends` a tile's start and end, a part's way through memory and back, the second
-// launch, and `least` what all of its operands' way from memory takes.
+// launch, and `least` what all of its operands' way from memory takes.  (With 900 and
+// 10000 for the tiles of 64 and 10000 for the second launch of those of 128 lists of
+// small matrices took 9 to 21 % longer, with 650 for 780 some 5 % less, others 2 % more.)
 struct Cost {
     int32_t step, alone, ends, part, again;
     int64_t least;
@@ -419,8 +421,8 @@ __host__ __device__ inline Cost cost_of(int tile, int pairs, int ends = 0, int64
 {
     const int64_t least = bytes / 4900;  // at 4.9 TB/s
     if (tile > 128) return {1600 * pairs, 1600 * pairs, ends ? ends : 6000, 110, 10000, least};
-    if (tile > 64) return {1050 * pairs, 630 * pairs, ends ? ends : 4000, 28, 10000, least};
-    return {900 * pairs, 400 * pairs, ends ? ends : 3000, 7, 10000, least};
+    if (tile > 64) return {1050 * pairs, 630 * pairs, ends ? ends : 4000, 28, 14000, least};
+    return {780 * pairs, 400 * pairs, ends ? ends : 3000, 7, 6000, least};
 }
 
 // The last, incomplete round of `rest` tiles in n parts each; -1 where that is not done.
