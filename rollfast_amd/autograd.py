@@ -235,8 +235,11 @@ class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        dhidden, dweight = ctx.saved_tensors  # of a dloss of one
-        return (None if dhidden is None else dhidden * dloss, None if dweight is None else dweight * dloss,
+        # the kept ones are of a dloss of one.  It goes in as a tensor of one dimension, so that
+        # the product is f32 (one of none would go to the gradients' type first: 2^16 is no
+        # f16, a third off by 2^-9 in bf16) and rounded once
+        dloss = dloss.reshape(1)
+        return (*(None if g is None else torch.mul(g, dloss, out=torch.empty_like(g)) for g in ctx.saved_tensors),
                 None, None, None, None)
 
 
