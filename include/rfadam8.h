@@ -593,6 +593,9 @@ RF_API rf_status rf_linear_weight_grad(const rf_weight_grad* args, void* workspa
 #define RF_REDUCE_NONE 0
 #define RF_REDUCE_SUM 1
 #define RF_REDUCE_MEAN 2
+/* Added to a reduction: dhidden and dweight are f32, whatever dtype is.  (f16 ones of
+ * a mean over many tokens are subnormal: a loss scale has to reach them first.) */
+#define RF_GRADS_F32 256
 typedef struct rf_cross_entropy {
     int64_t tokens, vocab, hidden;
     int32_t dtype;             /* hidden_rows, weight and their gradients */
@@ -608,7 +611,7 @@ typedef struct rf_cross_entropy {
     void* dhidden;             /* NULL, both: the loss alone */
     void* dweight;
     float z_loss;
-    int32_t reduction;         /* RF_REDUCE_* */
+    int32_t reduction;         /* RF_REDUCE_*, + RF_GRADS_F32 */
 } rf_cross_entropy;
 
 /* Bytes of device workspace (256-byte aligned) on the current device. */

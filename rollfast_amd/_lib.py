@@ -38,6 +38,7 @@ RF_ACC_SUM, RF_ACC_MEAN, RF_ACC_ZERO = 0, 1, 2
 RF_NOALLOC_SCRATCH_BYTES = 8 << 20
 RF_ACT_SILU, RF_ACT_GELU, RF_ACT_GELU_TANH = 0, 1, 2
 RF_REDUCE_NONE, RF_REDUCE_SUM, RF_REDUCE_MEAN = 0, 1, 2
+RF_GRADS_F32 = 256
 RF_NORM_ABSENT, RF_NORM_NONE, RF_NORM_RMS, RF_NORM_LAYER = 0, 1, 2, 3
 
 _p = ctypes.c_void_p

@@ -224,30 +224,34 @@ def linear(x, weight, bias=None, *, checkpoint=None):
 
 
 class _CrossEntropy(torch.autograd.Function):
+    """Keeps the gradients of a loss' gradient of one, which the backward pass
+    multiplies: of float16 tensors in float32, since those of a mean over many
+    tokens are below float16's normal numbers until a loss scale has reached them."""
+
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, z_loss, reduction):
-        got = losses.linear_cross_entropy_grad(hidden, weight, targets, ignore_index=ignore_index, z_loss=z_loss,
-                                               reduction=reduction)
-        ctx.save_for_backward(got.hidden if ctx.needs_input_grad[0] else None,
-                              got.weight if ctx.needs_input_grad[1] else None)
-        return got.loss
+        loss, dhidden, dweight = losses._call(hidden, weight, targets, None, ignore_index, z_loss, reduction, True,
+                                              wide=hidden.dtype == torch.float16)
+        ctx.dtype = hidden.dtype
+        ctx.save_for_backward(*(g if wanted else None for g, wanted in zip((dhidden, dweight), ctx.needs_input_grad)))
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        # the kept ones are of a dloss of one.  It goes in as a tensor of one dimension, so that
-        # the product is f32 (one of none would go to the gradients' type first: 2^16 is no
-        # f16, a third off by 2^-9 in bf16) and rounded once
+        # a tensor of one dimension, so that the product is f32 (one of none would go to g's
+        # type first: 2^16 is no f16, a third off by 2^-9 in bf16) and rounded once
         dloss = dloss.reshape(1)
-        return (*(None if g is None else torch.mul(g, dloss, out=torch.empty_like(g)) for g in ctx.saved_tensors),
-                None, None, None, None)
+        return (*(None if g is None else torch.mul(g, dloss, out=torch.empty_like(g, dtype=ctx.dtype))
+                  for g in ctx.saved_tensors), None, None, None, None)
 
 
 def linear_cross_entropy(hidden, weight, targets, *, ignore_index=-100, z_loss=0.0, reduction="mean"):
     """``losses.linear_cross_entropy`` summed ('sum') or averaged ('mean') over
     the targets that count, differentiable.  The forward pass computes both
-    gradients in the same pass as the loss and keeps them; the backward pass
-    multiplies them by the loss' own.  Under autocast both tensors go to its
+    gradients in the same pass as the loss and keeps them, float16 tensors' in
+    float32 and others in their own dtype; the backward pass multiplies them by
+    the loss' own, a loss scale included.  Under autocast both tensors go to its
     dtype.  A mean over no targets is NaN with gradients of zero."""
     if reduction not in ("sum", "mean"):
         raise ValueError(f"reduction must be 'sum' or 'mean', got {reduction!r}")

@@ -221,8 +221,8 @@ __device__ __forceinline__ void split8(const float (&v)[8], float scale, Raw<f16
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t cols, int64_t stride, int64_t pitch,
                                              const int32_t* __restrict__ order, const Scalars* sc, const uint32_t* top,
-                                             uint16_t* __restrict__ hi, uint16_t* __restrict__ lo, T* __restrict__ clear,
-                                             int64_t rows)
+                                             uint16_t* __restrict__ hi, uint16_t* __restrict__ lo, void* __restrict__ clear,
+                                             int wide, int64_t rows)
 {
     const int64_t r = blockIdx.x;
     int64_t from = r;
@@ -232,7 +232,10 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t c
         zero = r >= count;
         if (r < rows) from = order[r];
         if (zero && r < rows && clear)
-            for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += 2048) put8(clear + from * cols + c, Raw<T>{}, cols - c);
+            for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += 2048) {
+                if (wide) put8((float*)clear + from * cols + c, Raw<float>{}, cols - c);
+                else put8((T*)clear + from * cols + c, Raw<T>{}, cols - c);
+            }
         if (r >= (count + STEP - 1) / STEP * STEP) return;
     }
     const T* const row = x + from * stride;
@@ -552,7 +555,7 @@ struct Grad {
     int64_t cols, rows;            // of the output: p below cols, q below rows
     int64_t first, piece_rows;     // packed tokens of this piece
     int64_t steps;                 // of the sum; 0: the tokens that count
-    int32_t pairs, dtype;          // pairs: as hidden and weight have them
+    int32_t pairs, dtype;          // pairs: as hidden and weight have them; dtype: of the output
     const Scalars* sc;
     const Piece* piece;
     const int32_t* order;          // dhidden: the output's row of packed token q; NULL: dweight
@@ -563,9 +566,9 @@ struct Grad {
     float* partial;
 };
 
-__device__ __forceinline__ float unscale_of(const Grad& a)
+__device__ __forceinline__ float unscale_of(const Grad& a, bool wide)
 {
-    float u = 1.0f / dz_scale(a.piece->dz_top, a.dtype == RF_BF16);
+    float u = 1.0f / dz_scale(a.piece->dz_top, wide);
     if (a.pairs > 1) u *= inverse(scale_of(a.order ? a.sc->weight_top : a.sc->hidden_top));
     return u;
 }
@@ -581,9 +584,9 @@ struct Finish {
     bool add, keep;
     int32_t dtype;
 
-    __device__ __forceinline__ Finish(const Grad& a)
+    __device__ __forceinline__ Finish(const Grad& a, bool wide)
         : out(a.out), sums(!a.order && !(a.begin && a.end) ? a.sums : nullptr), order(a.order ? a.order + a.first : nullptr),
-          cols(a.cols), unscale(unscale_of(a)), add(sums && !a.begin), keep(sums && !a.end), dtype(a.dtype)
+          cols(a.cols), unscale(unscale_of(a, wide)), add(sums && !a.begin), keep(sums && !a.end), dtype(a.dtype)
     {
     }
     // four of row q from p on, in f32 or element by element
@@ -635,7 +638,7 @@ template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
     static __device__ __forceinline__ void finish(const Grad& a, const Even& t, typename G::Sums& acc, int wave, char*)
     {
         const int64_t rows = GradJob::rows(a);
-        const Finish f(a);
+        const Finish f(a, __is_same(H, bf16));
         const int lane = own_lane();
         const int64_t p0 = t.p0 + G::wp(wave);
 #pragma unroll
@@ -700,7 +703,7 @@ int64_t parts_of(const Shape& s, int64_t tiles, int64_t steps)
 
 struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
-    bool own_weight, f32, grad, few;
+    bool own_weight, f32, grad, few, wide;  // wide: gradients in f32
     int64_t bytes_of_weight;
     int32_t blocks, shift, pairs, cus;
     Shape logits, dhidden, dweight;
@@ -710,12 +713,15 @@ struct Plan {
 
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
 
+int32_t reduction_of(const rf_cross_entropy& a) { return a.reduction & ~RF_GRADS_F32; }
+
 Plan plan_of(const rf_cross_entropy& a, int cus)
 {
     Plan p{};
     p.cus = cus;
     p.f32 = a.dtype == RF_F32;
     p.grad = a.dweight != nullptr;
+    p.wide = p.f32 || (a.reduction & RF_GRADS_F32);
     p.pairs = p.f32 ? 3 : 1;
     p.few = p.grad && !p.f32 && a.tokens <= HALF;
     p.pad = up(a.hidden, STEP);
@@ -759,7 +765,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.e = take(held * p.vpad * (p.f32 ? 4 : 2));
         p.dz = p.f32 ? take(held * p.vpad * 4) : p.e;
         if (p.few) p.low = take(held * p.vpad * 2);
-        if (p.pieces > 1 && !p.f32) p.sums = take(a.vocab * a.hidden * 4);
+        if (p.pieces > 1 && !p.wide) p.sums = take(a.vocab * a.hidden * 4);
         p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, bytes, cus, true);
         p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, bytes, cus);
     }
@@ -780,7 +786,7 @@ rf_status check(const rf_cross_entropy* a)
         return report(RF_ERR_INVALID, "tokens, vocab or hidden out of range");
     if (!known(a->dtype)) return report(RF_ERR_UNSUPPORTED, "dtype must be f32, bf16 or f16");
     if (a->target_bits != 32 && a->target_bits != 64) return report(RF_ERR_UNSUPPORTED, "targets must be int32 or int64");
-    if (a->reduction < RF_REDUCE_NONE || a->reduction > RF_REDUCE_MEAN) return report(RF_ERR_INVALID, "unknown reduction");
+    if (reduction_of(*a) < RF_REDUCE_NONE || reduction_of(*a) > RF_REDUCE_MEAN) return report(RF_ERR_INVALID, "unknown reduction");
     if (!(a->z_loss >= 0.0f) || a->z_loss > 3e38f) return report(RF_ERR_INVALID, "z_loss must be finite and not negative");
     if (a->hidden_stride < 0 || a->weight_stride < 0) return report(RF_ERR_INVALID, "negative stride");
     return RF_OK;
@@ -869,13 +875,13 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         if (s != RF_OK) return s;
     }
     s = launch<k_pack<T>>(all, 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride, p.pad, (const int32_t*)order,
-                          (const Scalars*)sc, (const uint32_t*)&sc->hidden_top, hidden, hidden + plane, (T*)a.dhidden, a.tokens);
+                          (const Scalars*)sc, (const uint32_t*)&sc->hidden_top, hidden, hidden + plane, a.dhidden, (int)p.wide, a.tokens);
     if (s != RF_OK) return s;
     Side w{{a.weight, a.weight}, a.weight_stride * 2, a.vocab, a.vocab};
     if (p.own_weight) {
         uint16_t* const own = (uint16_t*)(ws + p.weight);
         s = launch<k_pack<T>>(a.vocab, 256, 0, st, (const T*)a.weight, a.hidden, a.weight_stride, p.pad, none, (const Scalars*)sc,
-                              (const uint32_t*)&sc->weight_top, own, own + a.vocab * p.pad, (T*)nullptr, a.vocab);
+                              (const uint32_t*)&sc->weight_top, own, own + a.vocab * p.pad, (void*)nullptr, 0, a.vocab);
         if (s != RF_OK) return s;
         w.base[0] = own;
         w.base[1] = own + (planes - 1) * a.vocab * p.pad;
@@ -925,7 +931,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         r.picked = l.picked;
         r.dloss = a.dloss;
         r.loss = a.loss;
-        r.reduction = a.reduction;
+        r.reduction = reduction_of(a);
         if (p.grad) {
             r.top = (float*)(ws + p.top);
             r.factor = (float*)(ws + p.factor);
@@ -947,7 +953,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.first = first;
         g.piece_rows = rows;
         g.pairs = p.pairs;
-        g.dtype = a.dtype;
+        g.dtype = p.wide ? RF_F32 : a.dtype;
         g.cols = a.hidden;
         g.p = w;
         g.p.extent = p.pad;  // (its columns; as it is, hidden is a multiple of whole steps)
@@ -966,14 +972,14 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.rows = a.vocab;
         g.order = nullptr;
         g.out = a.dweight;
-        g.sums = p.f32 ? (float*)a.dweight : (float*)(ws + p.sums);
+        g.sums = p.wide ? (float*)a.dweight : (float*)(ws + p.sums);
         g.begin = piece == 0;
         g.end = piece + 1 == p.pieces;
         s = product<H, KDOWN>(p, p.dweight, (float*)(ws + p.partial), g, st);
         if (s != RF_OK) return s;
     }
-    if (a.reduction != RF_REDUCE_NONE)
-        return launch<k_total>(1, SELECT, 0, st, (const float*)a.loss, (const int32_t*)order, (const Scalars*)sc, (int)a.reduction, a.total);
+    if (reduction_of(a) != RF_REDUCE_NONE)
+        return launch<k_total>(1, SELECT, 0, st, (const float*)a.loss, (const int32_t*)order, (const Scalars*)sc, (int)reduction_of(a), a.total);
     return RF_OK;
 }
 
@@ -996,10 +1002,10 @@ rf_status rf_linear_cross_entropy(const rf_cross_entropy* args, void* workspace,
     if (const rf_status s = check(args); s != RF_OK) return s;
     const rf_cross_entropy& a = *args;
     if (!a.weight || (a.tokens && (!a.hidden_rows || !a.targets || !a.loss))) return report(RF_ERR_INVALID, "null buffer");
-    if (a.reduction != RF_REDUCE_NONE && !a.total) return report(RF_ERR_INVALID, "a reduction needs total");
-    if (a.reduction != RF_REDUCE_NONE && a.dloss) return report(RF_ERR_INVALID, "dloss and a reduction exclude each other");
+    if (reduction_of(a) != RF_REDUCE_NONE && !a.total) return report(RF_ERR_INVALID, "a reduction needs total");
+    if (reduction_of(a) != RF_REDUCE_NONE && a.dloss) return report(RF_ERR_INVALID, "dloss and a reduction exclude each other");
     if (a.dloss || a.dhidden || a.dweight) {
-        if (!a.dweight || (a.tokens && (!a.dhidden || (!a.dloss && a.reduction == RF_REDUCE_NONE))))
+        if (!a.dweight || (a.tokens && (!a.dhidden || (!a.dloss && reduction_of(a) == RF_REDUCE_NONE))))
             return report(RF_ERR_INVALID, "gradients need dhidden, dweight and dloss or a reduction");
     }
     int cus = 0;

@@ -395,6 +395,7 @@ PyObject* py_weight_grad(PyObject*, PyObject* args)
 
 // cross_entropy(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, grad)
 //   -> (loss, or with a reduction the reduced one; dhidden; dweight) or None
+//   reduction: RF_REDUCE_*, + RF_GRADS_F32 for gradients in f32
 PyObject* py_cross_entropy(PyObject*, PyObject* args)
 {
     PyObject *ho, *wo, *to, *dlo;
@@ -442,11 +443,13 @@ PyObject* py_cross_entropy(PyObject*, PyObject* args)
     std::array<at::Tensor, 3> out;
     const at::Tensor loss = at::empty(targets.sizes(), c.options(at::kFloat));
     a.loss = (float*)loss.data_ptr();
-    out[0] = reduction ? at::empty({}, c.options(at::kFloat)) : loss;
-    if (reduction) a.total = (float*)out[0].data_ptr();
+    const bool reduced = (reduction & ~RF_GRADS_F32) != RF_REDUCE_NONE;
+    out[0] = reduced ? at::empty({}, c.options(at::kFloat)) : loss;
+    if (reduced) a.total = (float*)out[0].data_ptr();
     if (grad) {
-        out[1] = c.empty(hidden.scalar_type());
-        out[2] = at::empty(weight.sizes(), c.options(hidden.scalar_type()));
+        const at::ScalarType type = reduction & RF_GRADS_F32 ? at::kFloat : hidden.scalar_type();
+        out[1] = c.empty(type);
+        out[2] = at::empty(weight.sizes(), c.options(type));
         a.dhidden = out[1].data_ptr();
         a.dweight = out[2].data_ptr();
     }

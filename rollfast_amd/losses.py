@@ -75,11 +75,13 @@ def _arguments(hidden, weight, targets, ignore_index, z_loss, reduction):
     return a, (rows, table, targets)
 
 
-def _call(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, grad):
+def _call(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, grad, wide=False):
     """(loss, dhidden, dweight): the native host path where the tensors are as
-    they may be, on the current device; else laid out here."""
+    they may be, on the current device; else laid out here.  ``wide``: the
+    gradients in float32, whatever the tensors are."""
     code = _REDUCTION.get(reduction)
     if code is not None:
+        code |= _lib.RF_GRADS_F32 if wide else 0
         got = _lib.pyblocks().cross_entropy(hidden, weight, targets, dloss, int(ignore_index), float(z_loss), code, grad)
         if got is not None:
             return got
@@ -95,18 +97,20 @@ def _call(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, grad)
     with torch.cuda.device(device):
         loss = torch.empty(targets.shape, dtype=torch.float32, device=device)
         a.loss = loss.data_ptr()
-        if a.reduction:
+        if reduction != "none":
             total = torch.empty((), dtype=torch.float32, device=device)
             a.total = total.data_ptr()
         if grad:
-            dhidden = torch.empty(hidden.shape, dtype=hidden.dtype, device=device)
-            dweight = torch.empty(weight.shape, dtype=weight.dtype, device=device)
+            dtype = torch.float32 if wide else hidden.dtype
+            dhidden = torch.empty(hidden.shape, dtype=dtype, device=device)
+            dweight = torch.empty(weight.shape, dtype=dtype, device=device)
+            a.reduction |= _lib.RF_GRADS_F32 if wide else 0
             a.dhidden, a.dweight = dhidden.data_ptr(), dweight.data_ptr()
         need, what = ctypes.c_int64(), "linear_cross_entropy_grad" if grad else "linear_cross_entropy"
         _lib.check(_lib.lib().rf_linear_cross_entropy_workspace(a, need), what)
         workspace = torch.empty(need.value, dtype=torch.uint8, device=device)
         _lib.check(_lib.lib().rf_linear_cross_entropy(a, workspace.data_ptr(), need.value, _lib.stream_ptr()), what)
-    return total if a.reduction else loss, dhidden, dweight
+    return loss if reduction == "none" else total, dhidden, dweight
 
 
 def linear_cross_entropy(hidden, weight, targets, *, ignore_index: int = -100, z_loss: float = 0.0,

@@ -126,3 +126,14 @@ def test_python_refusals():
             rf.linear_cross_entropy_grad(h, w, t, bad)
     with pytest.raises(ValueError, match="z_loss"):
         rf.linear_cross_entropy(h, w, t, z_loss=-1.0)
+
+
+def test_f32_gradients_are_added_to_a_reduction():
+    L, size = _lib.lib(), ctypes.c_int64()
+    for bad in (_lib.RF_GRADS_F32 | 3, _lib.RF_GRADS_F32 * 2, _lib.RF_GRADS_F32 * 2 + 1):
+        refused(L.rf_linear_cross_entropy_workspace(args(reduction=bad), size), "unknown reduction")
+    wide = {"dhidden": P, "dweight": P, "reduction": _lib.RF_GRADS_F32}
+    refused(L.rf_linear_cross_entropy(args(**wide), P, 1 << 40, None), "gradients need")
+    wide["reduction"] |= _lib.RF_REDUCE_MEAN
+    refused(L.rf_linear_cross_entropy(args(**wide), P, 1 << 40, None), "total")
+    refused(L.rf_linear_cross_entropy(args(**wide, total=P, dloss=P), P, 1 << 40, None), "exclude")
