@@ -360,9 +360,11 @@ __device__ __forceinline__ void LogitsJob<H, E, TILE, WP, WQ>::finish(const Logi
             m = fmaxf(fmaxf(fmaxf(m, acc[i][j][0]), acc[i][j][1]), fmaxf(acc[i][j][2], acc[i][j][3]));
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        // exp(z - m) = 2^(z log2(e) - m log2(e)), the product in one rounding with the
-        // difference; where nothing is here, exponentials of -inf are 0
-        const float base = m == -__builtin_inff() ? 0.0f : m * -LOG2E;
+        // the difference first: it is exact where it matters, and zero at the maximum, so that
+        // s is at least one and no loss below zero (2^(z log2(e) - m log2(e)) in one FMA carries
+        // the rounding of m log2(e), 2e-5 in the loss at logits of 400).  Where nothing is here,
+        // exponentials of -inf are 0
+        const float top = m == -__builtin_inff() ? 0.0f : m;
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < G::FP; i += 2) {
@@ -371,7 +373,7 @@ __device__ __forceinline__ void LogitsJob<H, E, TILE, WP, WQ>::finish(const Logi
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    e[k][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i + k][j][r], LOG2E, base));
+                    e[k][r] = __builtin_amdgcn_exp2f((acc[i + k][j][r] - top) * LOG2E);
                     s += e[k][r];
                 }
             if constexpr (__is_same(E, f16)) {

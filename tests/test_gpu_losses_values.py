@@ -8,7 +8,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_losses import BF16, F16, F32, make, product, rf
+from tests.test_gpu_losses import BF16, F16, F32, U, make, product, rf
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,57 @@ def test_f32_gradients_of_several_pieces():
     ref = rf().linear_cross_entropy_grad(hidden, weight, targets, reduction="mean")
     for x, y in zip(wide[1:], ref[1:]):
         assert x.dtype == F32 and torch.equal(x.to(F16), y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab", [64, 130, 1000])
+def test_confident_tokens_with_large_logits(vocab, dtype):
+    """The targets' logits are 50 to 500, all others 200, or 9 to 16, below them, true
+    losses zero or 1e-7 to 1e-1.  hidden is the identity and weight holds the logits in a
+    few bits, so that they are exact, and the gradient of weight is dz itself.
+
+    exp's argument d is rounded twice (log2(e) is, too): 3 |d| U, and exp2 within 2 ulps;
+    s is a sum of a one and at most 1000 terms in f32, its parts rounded in 10 + 16 sums
+    of a tile and the blocks': (d 3 + 4 + 26) U of what is added to the one, and U for each
+    of the sums that hold the one, 26; log and expm1 within 2 ulps each of their results.
+    dz is kept to 22 bits in f32."""
+    n = 64
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(61)
+    step = {F32: 2.0 ** -10, F16: 0.25, BF16: 2.0}[dtype]
+    top = torch.linspace(50.0, 500.0, n, device="cuda").div(step).round() * step
+    # 64 columns: a token each
+    far = torch.arange(n, device="cuda") % 2 == 0
+    gap = torch.where(far[:, None], 200.0, 9.0 + 7.0 * torch.rand(n, vocab, generator=gen, device="cuda"))
+    gap = gap.div(step).round() * step
+    z = top[:, None] - gap
+    targets = torch.randint(vocab, (n,), generator=gen, device="cuda")
+    at = torch.arange(n, device="cuda")
+    z[at, targets] = top
+    weight = z.t().contiguous().to(dtype)
+    assert torch.equal(weight.t().float(), z)
+    hidden = torch.eye(n, device="cuda").to(dtype)
+    z = z.double()
+    p = torch.exp(z - z.amax(1, keepdim=True))
+    p[at, targets] = 0.0
+    rest = p.sum(1)
+    loss = torch.log1p(rest)
+    d = (z.amax(1, keepdim=True) - z)
+    rel = (3 * d.clamp(max=200) + 30) * U
+    bound = 30 * U + (p * rel).sum(1) + 4 * U * loss
+    got = rf().linear_cross_entropy_grad(hidden, weight, targets, torch.ones(n, device="cuda"))
+    alone = rf().linear_cross_entropy(hidden, weight, targets)
+    for x in (got.loss, alone):
+        assert (x >= 0).all()
+        assert ((x.double() - loss).abs() <= bound).all()
+    dz = got.weight.double().t()
+    assert (dz[at, targets] <= 0).all()
+    half = {F32: 2.0 ** -22 + U, BF16: 2.0 ** -7, F16: 2.0 ** -10}[dtype]  # dz, and the result
+    true = -rest / (1 + rest)
+    tiny = 2.0 ** -24 if dtype == F16 else 0.0
+    assert ((dz[at, targets] - true).abs() <= bound + half * true.abs() + tiny).all()
+    if dtype == F32:
+        q = p / (1 + rest)[:, None]
+        off = q * (rel + 34 * U + half) + 2.0 ** -37  # dz is held down to 2^-38 of a dloss of one
+        off[at, targets] = 1.0
+        assert ((dz - q).abs() <= off).all()
