@@ -20,6 +20,7 @@
 //   k_dlogits  exp(z - m) to dz, in place (f32: to two f16 planes; where few tokens
 //              count to two planes of the tensors' type)
 //   GradJob    dhidden and dweight, two products of the same size
+//   k_level    between them, for tokens that weigh little beside others: hidden's rows
 // Loss alone ends with k_rows and writes no logits.  With gradients a piece of
 // tokens at a time holds at most PIECE bytes of exponentials; the pieces'
 // weight gradients are added in f32.  Three products, none computed twice.
@@ -59,12 +60,12 @@ struct Scalars {
 };
 
 // Of each piece of tokens: its products' shares, which depend on how many tokens count,
-// and bits of the largest row factor.
+// and bits of the largest row factor.  (Lifted: k_dlogits.)
 struct Piece {
     Share logits, dhidden, dweight;
     uint32_t dz_top;
     int32_t pairs;   // plane pairs of the gradients' products
-    uint32_t pad;
+    uint32_t uneven; // some token's dz was lifted
 };
 
 // The products of a piece, for k_select.
@@ -217,12 +218,13 @@ __device__ __forceinline__ void split8(const float (&v)[8], float scale, Raw<f16
 
 // Rows into the product's layout: 16 bits, columns padded with zeros to `pitch`.
 // With `order`: the rows that count, zeros up to a whole step behind them, and
-// zeros in the rows of `clear` that do not count.
+// zeros in the rows of `clear` that do not count.  `raised` (16 bits): the largest finite
+// magnitude of those that count, as k_top has it.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t cols, int64_t stride, int64_t pitch,
                                              const int32_t* __restrict__ order, const Scalars* sc, const uint32_t* top,
                                              uint16_t* __restrict__ hi, uint16_t* __restrict__ lo, void* __restrict__ clear,
-                                             int wide, int64_t rows)
+                                             int wide, uint32_t* raised, int64_t rows)
 {
     const int64_t r = blockIdx.x;
     int64_t from = r;
@@ -241,9 +243,19 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t c
     const T* const row = x + from * stride;
     float scale = 1.0f;
     if constexpr (sizeof(T) == 4) scale = scale_of(*top);
+    uint32_t best = 0;
     for (int64_t c = (int64_t)threadIdx.x * 8; c < pitch; c += 2048) {
         Raw<T> v{};
         if (!zero && c < cols) v = load8(row, c, cols);
+        if (sizeof(T) == 2 && raised) {
+            float w[8];
+            widen8(v, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t x = __float_as_uint(w[k]) & 0x7FFFFFFFu;
+                best = max(best, x < 0x7F800000u ? x : 0u);
+            }
+        }
         if constexpr (sizeof(T) == 4) {
             float w[8];
             widen8(v, w);
@@ -255,6 +267,9 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t c
             *(u32x4*)(hi + r * pitch + c) = v.a;
         }
     }
+    if (sizeof(T) == 4 || !raised) return;
+    for (int d = 1; d < WAVE; d *= 2) best = max(best, (uint32_t)__shfl_xor((int)best, d));
+    if (threadIdx.x % WAVE == 0) raise(raised, best);
 }
 
 // ------------------------------------------------------------- the logits ---
@@ -419,6 +434,8 @@ struct Rows {
     const float2* stats;
     const float *picked, *dloss;
     float *loss, *top, *factor, *at_target;  // [rows] each but loss
+    float* reach;        // [rows] row factors' magnitudes; NULL: bf16, which has the range
+    int32_t* lifts;      // [rows] powers of two that dz was lifted by
     const void* e;
     void* dz;
     uint16_t* dz_low;
@@ -455,7 +472,9 @@ __global__ __launch_bounds__(256) void k_rows(const Rows a)
         a.top[q] = m;
         a.factor[q] = dl * spread / s;
         a.at_target[q] = dl * (expm1f(below) + (spread - 1.0f) * expf(below));
-        const uint32_t mine = __float_as_uint(fmaxf(fabsf(dl * spread), fabsf(dl)));
+        const float reach = fmaxf(fabsf(dl * spread), fabsf(dl));
+        if (a.reach) a.reach[q] = reach;
+        const uint32_t mine = __float_as_uint(reach);
         if (mine < 0x7F800000u) most = max(most, mine);
     }
     if (!a.factor) return;
@@ -488,7 +507,19 @@ __global__ __launch_bounds__(SELECT) void k_total(const float* __restrict__ loss
 __device__ __forceinline__ float dz_scale(uint32_t top, bool wide)
 {
     const float t = __uint_as_float(top);
-    return t < 1e-30f ? 1.0f : (wide ? 1.0f : 16384.0f) / t;
+    return t < 0x1p-110f ? 1.0f : (wide ? 1.0f : 16384.0f) / t;
+}
+
+// In f16, which keeps 2^-38 of the largest, a token whose own factor is below a sixteenth
+// of it is lifted by a power of two to where the largest are: its dhidden keeps the bits of
+// any other's (dloss 1e-8 of another's: off by 1.5e-2 of its norm without it), whose
+// product takes the power away again; dweight's sums take it from the token's row of
+// hidden (k_level).  A sixteenth, so that the factors of a z-loss alone move nothing.  As
+// far as the scale is finite.
+__device__ __forceinline__ int lift_of(uint32_t top, float reach)
+{
+    const int d = min((int)(top >> 23) - (int)(__float_as_uint(reach) >> 23), (int)(top >> 23) - 17);
+    return d > 4 ? d : 0;
 }
 
 // dz of a token from its exponentials; zeros up to a whole step of
@@ -509,7 +540,15 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
         }
         return;
     }
-    const float scale = dz_scale(a.piece->dz_top, __is_same(P, bf16));
+    float scale = dz_scale(a.piece->dz_top, __is_same(P, bf16));
+    if (a.reach) {
+        const int lift = lift_of(a.piece->dz_top, a.reach[q]);
+        scale = ldexpf(scale, lift);
+        if (threadIdx.x == 0) {
+            a.lifts[q] = lift;
+            if (lift) raise(&a.piece->uneven, 1);
+        }
+    }
     const float m = a.top[q], f = a.factor[q] * scale;
     for (int b = threadIdx.x; b < a.blocks; b += 256) {
         const float top = a.stats[q * a.blocks + b].x;
@@ -551,6 +590,34 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
     }
 }
 
+// Where a token of the piece was lifted: hidden's packed rows once more, for dweight, each
+// divided by what its dz was multiplied by.  f16 rows are brought up to the top of the
+// range first, that less falls below it.
+template <typename T>
+__global__ __launch_bounds__(256) void k_level(const T* __restrict__ x, int64_t cols, int64_t stride, int64_t pitch,
+                                              const int32_t* __restrict__ order, int64_t first, int64_t most, const Scalars* sc,
+                                              const Piece* piece, const int32_t* __restrict__ lifts, uint16_t* __restrict__ hi,
+                                              uint16_t* __restrict__ lo)
+{
+    if (!piece->uneven) return;
+    const int64_t rows = min((int64_t)sc->count - first, most);
+    const float scale = scale_of(sc->hidden_top);
+    for (int64_t q = blockIdx.x; q < rows; q += gridDim.x) {
+        const T* const row = x + order[first + q] * stride;
+        const int lift = lifts[q];
+        for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += 2048) {  // (zeros stay behind them)
+            float v[8];
+            widen8(load8(row, c, cols), v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k] * scale, -lift);
+            Raw<f16> h, l;
+            split8(v, 1.0f, h, l);
+            *(u32x4*)(hi + q * pitch + c) = h.a;
+            if (sizeof(T) == 4) *(u32x4*)(lo + q * pitch + c) = l.a;
+        }
+    }
+}
+
 // ---------------------------------------------------------- the gradients ---
 struct Grad {
     Side p, q;
@@ -561,6 +628,7 @@ struct Grad {
     const Scalars* sc;
     const Piece* piece;
     const int32_t* order;          // dhidden: the output's row of packed token q; NULL: dweight
+    const int32_t* lifts;          // of the piece's tokens; NULL: none is lifted
     void* out;
     float* sums;                   // dweight, several pieces: f32 sums so far (may be out)
     int32_t begin, end;            // the first piece, the last one
@@ -572,6 +640,7 @@ __device__ __forceinline__ float unscale_of(const Grad& a, bool wide)
 {
     float u = 1.0f / dz_scale(a.piece->dz_top, wide);
     if (a.pairs > 1) u *= inverse(scale_of(a.order ? a.sc->weight_top : a.sc->hidden_top));
+    else if (!a.order && a.lifts && a.piece->uneven) u *= inverse(scale_of(a.sc->hidden_top));
     return u;
 }
 
@@ -580,7 +649,7 @@ __device__ __forceinline__ float unscale_of(const Grad& a, bool wide)
 struct Finish {
     void* out;
     float* sums;       // NULL: nothing before and nothing behind
-    const int32_t* order;
+    const int32_t *order, *lifts;
     int64_t cols;
     float unscale;
     bool add, keep;
@@ -588,13 +657,15 @@ struct Finish {
 
     __device__ __forceinline__ Finish(const Grad& a, bool wide)
         : out(a.out), sums(!a.order && !(a.begin && a.end) ? a.sums : nullptr), order(a.order ? a.order + a.first : nullptr),
-          cols(a.cols), unscale(unscale_of(a, wide)), add(sums && !a.begin), keep(sums && !a.end), dtype(a.dtype)
+          lifts(a.order && a.lifts && a.piece->uneven ? a.lifts : nullptr), cols(a.cols), unscale(unscale_of(a, wide)), add(sums && !a.begin), keep(sums && !a.end), dtype(a.dtype)
     {
     }
     // four of row q from p on, in f32 or element by element
     __device__ __forceinline__ void put4(int64_t q, int64_t p, f32x4 v) const
     {
         v *= unscale;
+        if (lifts)
+            for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], -lifts[q]);
         const int64_t left = cols - p, here = q * cols + p, at = (order ? order[q] : q) * cols + p;
         if (add) {
             if (left >= 4) v += __builtin_bit_cast(f32x4, *(const u32x4_at*)(sums + here));
@@ -648,9 +719,10 @@ template <typename H, Layout LQ, int TILE, int WP, int WQ> struct GradJob {
             const int64_t q = t.q0 + G::wq(wave) + 16 * j + lane % 16;
             if (f.plain()) {
                 uint16_t* const row = (uint16_t*)f.out + (f.order ? f.order[min(q, rows - 1)] : q) * f.cols;
+                const float unscale = f.lifts ? ldexpf(f.unscale, -f.lifts[min(q, rows - 1)]) : f.unscale;
 #pragma unroll
                 for (int i = 0; i < G::FP; i += 2) {
-                    const f32x4 x = acc[i][j] * f.unscale, y = acc[i + 1][j] * f.unscale;
+                    const f32x4 x = acc[i][j] * unscale, y = acc[i + 1][j] * unscale;
                     const u32x4 c = __is_same(H, bf16) ? chunk(narrow4<bf16>(x), narrow4<bf16>(y)) : chunk(narrow4<f16>(x), narrow4<f16>(y));
                     const int64_t from = p0 + 16 * i + chunk_of(lane);
                     if (q < rows && from < f.cols) put8<true, LQ == KDOWN>(row + from, Raw<uint16_t>{c}, f.cols - from);
@@ -706,11 +778,12 @@ int64_t parts_of(const Shape& s, int64_t tiles, int64_t steps)
 struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
     bool own_weight, f32, grad, few, wide;  // wide: gradients in f32
+    bool lifts;  // tokens' dz may be lifted
     int64_t bytes_of_weight;
     int32_t blocks, shift, pairs, cus;
     Shape logits, dhidden, dweight;
     // offsets in the workspace
-    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, hidden, weight, e, dz, low, sums, partial, bytes;
+    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, reach, lift, hidden, weight, e, dz, low, sums, partial, bytes;
 };
 
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
@@ -725,6 +798,8 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.grad = a.dweight != nullptr;
     p.wide = p.f32 || (a.reduction & RF_GRADS_F32);
     p.pairs = p.f32 ? 3 : 1;
+    // row factors of a reduction without a z-loss are all alike
+    p.lifts = p.grad && a.dtype != RF_BF16 && (reduction_of(a) == RF_REDUCE_NONE || a.z_loss > 0.0f);
     p.few = p.grad && !p.f32 && a.tokens <= HALF;
     p.pad = up(a.hidden, STEP);
     p.vpad = up(a.vocab, STEP);
@@ -764,6 +839,8 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.top = take(p.rows * 4);
         p.factor = take(p.rows * 4);
         p.at_target = take(p.rows * 4);
+        p.reach = take(p.rows * 4);
+        p.lift = take(p.rows * 4);
         p.e = take(held * p.vpad * (p.f32 ? 4 : 2));
         p.dz = p.f32 ? take(held * p.vpad * 4) : p.e;
         if (p.few) p.low = take(held * p.vpad * 2);
@@ -877,13 +954,14 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         if (s != RF_OK) return s;
     }
     s = launch<k_pack<T>>(all, 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride, p.pad, (const int32_t*)order,
-                          (const Scalars*)sc, (const uint32_t*)&sc->hidden_top, hidden, hidden + plane, a.dhidden, (int)p.wide, a.tokens);
+                          (const Scalars*)sc, (const uint32_t*)&sc->hidden_top, hidden, hidden + plane, a.dhidden, (int)p.wide,
+                          p.lifts && !p.f32 ? &sc->hidden_top : (uint32_t*)nullptr, a.tokens);
     if (s != RF_OK) return s;
     Side w{{a.weight, a.weight}, a.weight_stride * 2, a.vocab, a.vocab};
     if (p.own_weight) {
         uint16_t* const own = (uint16_t*)(ws + p.weight);
         s = launch<k_pack<T>>(a.vocab, 256, 0, st, (const T*)a.weight, a.hidden, a.weight_stride, p.pad, none, (const Scalars*)sc,
-                              (const uint32_t*)&sc->weight_top, own, own + a.vocab * p.pad, (void*)nullptr, 0, a.vocab);
+                              (const uint32_t*)&sc->weight_top, own, own + a.vocab * p.pad, (void*)nullptr, 0, (uint32_t*)nullptr, a.vocab);
         if (s != RF_OK) return s;
         w.base[0] = own;
         w.base[1] = own + (planes - 1) * a.vocab * p.pad;
@@ -938,6 +1016,10 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
             r.top = (float*)(ws + p.top);
             r.factor = (float*)(ws + p.factor);
             r.at_target = (float*)(ws + p.at_target);
+            if (p.lifts) {
+                r.reach = (float*)(ws + p.reach);
+                r.lifts = (int32_t*)(ws + p.lift);
+            }
         }
         r.e = l.e;
         r.dz = ws + p.dz;
@@ -963,10 +1045,19 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         g.rows = rows;
         g.steps = p.vpad / STEP;
         g.order = order;
+        g.lifts = r.lifts;
         g.out = a.dhidden;
         if (rows) {
             s = product<H, KALONG>(p, p.dhidden, (float*)(ws + p.partial), g, st);
             if (s != RF_OK) return s;
+        }
+        if constexpr (!__is_same(T, bf16)) {
+            if (p.lifts) {
+                s = launch<k_level<T>>(std::min<int64_t>(rows, 2048), 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride,
+                                       p.pad, (const int32_t*)order, first, rows, (const Scalars*)sc, (const Piece*)piece_info,
+                                       (const int32_t*)r.lifts, h, h + (planes - 1) * plane);
+                if (s != RF_OK) return s;
+            }
         }
         g.p = x;
         g.p.extent = p.pad;

@@ -5,10 +5,12 @@ bits; tolerances from the arithmetic, beside each test."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from tests.test_gpu_losses import BF16, F16, F32, U, make, product, rf
+from tests.test_gpu_losses import BF16, F16, F32, HALF_ULP, TINY, U, check, make, near, product, reference, rf
 
 pytestmark = pytest.mark.gpu
 
@@ -153,3 +155,112 @@ def test_confident_tokens_with_large_logits(vocab, dtype):
         off = q * (rel + 34 * U + half) + 2.0 ** -37  # dz is held down to 2^-38 of a dloss of one
         off[at, targets] = 1.0
         assert ((dz - q).abs() <= off).all()
+
+
+def spread(tokens, exponents, seed):
+    """dloss of either sign, a few powers of two apart."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    e = torch.tensor(exponents, device="cuda")[torch.randint(len(exponents), (tokens,), generator=gen, device="cuda")]
+    d = torch.ldexp(1.0 + torch.rand(tokens, generator=gen, device="cuda"), e)
+    return torch.where(torch.rand(tokens, generator=gen, device="cuda") < 0.5, d, -d)
+
+
+def check_rows(hidden, weight, targets, dloss, z_loss=0.0):
+    """dhidden row by row against that of a dloss of one, times the row's: as exact as where no
+    other token weighs more.  What is held beside a dloss of one is held down to 2^-38 of
+    it, or, where another weighs up to 2^5 of it, to 2^-33 (the bound's 2^-38 comes with the reference)."""
+    got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss, z_loss=z_loss)
+    loss, (dh, off), dw = reference(hidden, weight, targets, torch.sign(dloss), z_loss)
+    near(got.loss, loss, "loss")
+    most = (1 + 2 * z_loss * (loss[0].abs().max() + 100)).item()
+    off = off + 2.0 ** -33 * most * weight.double().abs().sum(0)
+    size = dloss.double().abs()[:, None]
+    value, off = dh * size, off * size
+    bound = HALF_ULP[got.hidden.dtype] * (value.abs() + off) * 1.01 + TINY[got.hidden.dtype] + off
+    assert ((got.hidden.double() - value).abs() <= bound).all()
+    return got
+
+
+@pytest.mark.parametrize("z_loss", [0.0, 1e-2])
+@pytest.mark.parametrize("exponents", [(0, -13, -27, -40), (60, 0, -60), (0, -3, -4, -5), (0, -100)])
+@pytest.mark.parametrize("size", [(96, 700, 128), (40, 5000, 65), (600, 300, 40)])
+def test_f32_tokens_that_weigh_little_keep_their_gradients(size, exponents, z_loss):
+    """A power of two for each token.  dweight's sums are right to what the heaviest tokens leave."""
+    hidden, weight, targets, _ = make(*size, F32, seed=63, masked=0.1)
+    dloss = spread(size[0], exponents, 64)
+    got = check_rows(hidden, weight, targets, dloss, z_loss)
+    _, _, dw = reference(hidden, weight, targets, dloss, z_loss)
+    near(got.weight, dw, "dweight")
+
+
+def test_f32_dweight_of_tokens_that_weigh_little():
+    """A token alone in its column of hidden: dweight's column is its own dz, which is held
+    to 22 bits however little it weighs, since hidden's row takes the power of two: ones,
+    held as 2^14, of which 2^-20 leaves 2^-6, 19 bits above what is lost, 2^-25."""
+    n, vocab = 64, 300
+    _, weight, targets, _ = make(n, vocab, n, F32, seed=65)
+    hidden = torch.eye(n, device="cuda")
+    e = -(torch.arange(n, device="cuda") % 5) * 5
+    dloss = torch.ldexp(torch.ones(n, device="cuda"), e)
+    got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    z = weight.double().t()
+    dz = torch.softmax(z, 1)
+    dz[torch.arange(n, device="cuda"), targets] -= 1
+    # of p: the split logits (3 * 2^-22 of at most 64 magnitudes' sum, here one), 16 ulps of exp and sums
+    rel = 2.0 ** -22 * 2 + (3 * 2.0 ** -22 + 3 * U) * z.abs().amax(1, keepdim=True) * 4 + (16 + 64 + 6 + 34) * U
+    off = dz.abs() * rel + (vocab / 64) * U * dz.abs()
+    assert ((got.weight.double().t() / dloss.double()[:, None] - dz).abs() <= off + 2.0 ** -37).all()
+
+
+@pytest.mark.parametrize("exponents", [(13, -15), (10, 6, 5, 4, -3)])
+def test_f16_tokens_that_weigh_little_keep_their_gradients(exponents):
+    """weight's rows have a common part, so that what is lost of many small dz shows."""
+    hidden, weight, targets, _ = make(300, 5000, 64, F16, seed=67, masked=0.1, logit=0.3)
+    weight = (weight.float() + 1.0).to(F16)
+    dloss = spread(300, exponents, 68)
+    got = check_rows(hidden, weight, targets, dloss)
+    _, _, dw = reference(hidden, weight, targets, dloss)
+    near(got.weight, dw, "dweight")
+
+
+def test_tokens_far_apart_in_several_pieces_and_few():
+    """Each piece has its own largest; f16's low parts of few tokens are lifted alike."""
+    hidden, weight, targets, _ = make(700, 1 << 20, 9, F32, seed=69, masked=0.1)
+    dloss = spread(700, (0, -30), 70)
+    dloss[:256] *= 2.0 ** -20
+    check_rows(hidden, weight, targets, dloss)
+    for tokens in (1, 7, 16):
+        hidden, weight, targets, _ = make(tokens, 900, 80, F16, seed=71)
+        check_rows(hidden, weight, targets, spread(tokens, (8, -4), 72))
+        check(hidden, weight, targets, spread(tokens, (8, -4), 72))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_zeros_and_values_that_are_not_finite_in_dloss(dtype):
+    """They change no other token's gradient of hidden."""
+    hidden, weight, targets, _ = make(50, 200, 64, dtype, seed=73)
+    dloss = spread(50, (0, -20) if dtype == F32 else (0, -8), 74)
+    ref = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    for value in (0.0, math.nan, math.inf):
+        bad = dloss.clone()
+        bad[7] = value
+        got = rf().linear_cross_entropy_grad(hidden, weight, targets, bad)
+        assert not got.hidden[7].any() if value == 0.0 else not got.hidden[7].isfinite().any()
+        keep = torch.arange(50, device="cuda") != 7
+        assert torch.equal(got.hidden[keep], ref.hidden[keep])
+
+
+def test_a_graph_replayed_with_other_weights_of_the_tokens():
+    hidden, weight, targets, dloss = make(130, 700, 64, F32, seed=75, masked=0.2)
+    rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    for turn, exponents in enumerate([(0, -30), (0,), (0, -7), (-90, 0)]):
+        dloss.copy_(spread(130, exponents, 80 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)):
+            assert torch.equal(x, y), turn
