@@ -25,8 +25,9 @@
 // tokens at a time holds at most PIECE bytes of exponentials; the pieces'
 // weight gradients are added in f32.  Three products, none computed twice.
 //
-// exp(z - m) is in [0, 1]: f16 rounds it by at most 2^-12 of its value (below
-// 2^-14 by 2^-25), a sixteenth of what bf16's rounding of dz adds.  At the target
+// exp(z - m) is in [0, 1]: f16 rounds it by at most 2^-11 of its value (below
+// 2^-14 by 2^-25, so that what is below 2^-25 of the largest of its block is lost), an
+// eighth of what bf16's rounding of dz adds, and as much as f16's.  At the target
 // dz comes from the f32 logit through expm1, since 1 - p cancels there.
 //
 // f32 tensors go to the matrix cores as two f16 planes each, high and low parts of
@@ -48,9 +49,10 @@ constexpr int64_t STATS = 256ll << 20;      // bytes of m and s held at once
 // Where so few 16-bit tokens count, dz goes to its products in two parts, high and low:
 // with few terms its rounding does not average out (bf16, 1 x 896 x 225: gradients off by
 // up to 2.8e-3 of their norm, so 1.7e-3, the rounding of the result; 16 tokens: 2.1e-3).
-// For all of 67 f16 tokens with 32000 x 4096 it would take 327 us in place of 261.
+// f16, 16 x 4000 x 96: off by 2.0e-4 where one part leaves 2.5e-4; beside the targets, where
+// the exponential is rounded to f16 as well, 1.4 and 1.7 of the result's rounding.  For all of 67 f16 tokens with 32000 x 4096 it would take 327 us in place of 261.
 constexpr int64_t FEW = 16;
-constexpr int64_t HALF = 128;               // tokens of a call that has a place for the low parts
+static_assert(FEW <= STEP, "the low parts are one step of tokens");
 
 // Written by the kernels, read by later ones.
 struct Scalars {
@@ -800,7 +802,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.pairs = p.f32 ? 3 : 1;
     // row factors of a reduction without a z-loss are all alike
     p.lifts = p.grad && a.dtype != RF_BF16 && (reduction_of(a) == RF_REDUCE_NONE || a.z_loss > 0.0f);
-    p.few = p.grad && !p.f32 && a.tokens <= HALF;
+    p.few = p.grad && !p.f32;
     p.pad = up(a.hidden, STEP);
     p.vpad = up(a.vocab, STEP);
     // weight as it is: whole steps of k, 16-byte rows
@@ -841,9 +843,12 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.at_target = take(p.rows * 4);
         p.reach = take(p.rows * 4);
         p.lift = take(p.rows * 4);
+        // Low parts of few tokens: one step of rows.  A tile of dhidden reads as many rows of
+        // them as of the high ones, up to `held`, for tokens that do not exist: those behind the
+        // step are the first of e, which lies next to it (both are multiples of 256 bytes).
+        if (p.few) p.low = take(STEP * p.vpad * 2);
         p.e = take(held * p.vpad * (p.f32 ? 4 : 2));
         p.dz = p.f32 ? take(held * p.vpad * 4) : p.e;
-        if (p.few) p.low = take(held * p.vpad * 2);
         if (p.pieces > 1 && !p.wide) p.sums = take(a.vocab * a.hidden * 4);
         p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, bytes, cus, true);
         p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, bytes, cus);
@@ -898,7 +903,7 @@ bool never_splits(const Shape& shape, const Plan& p, int64_t bytes, bool few, in
     if (tiles_q > 4) return false;
     for (int pairs = p.pairs; pairs <= (few ? 2 : p.pairs); ++pairs) {
         const Cost c = cost_of(shape.tile, pairs, 0, bytes);
-        for (int64_t q = 1; q <= tiles_q; ++q)
+        for (int64_t q = 1; q <= (pairs > p.pairs ? 1 : tiles_q); ++q)  // (two pairs: of at most FEW tokens)
             if (share_of((uint32_t)(shape.tiles_p * q), steps, shape.room, c).rest) return false;
     }
     return true;
