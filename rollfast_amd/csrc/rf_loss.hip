@@ -70,11 +70,13 @@ struct Piece {
     uint32_t uneven; // some token's dz was lifted
 };
 
-// The products of a piece, for k_select.
+// The products of a piece, for k_select.  The last three: no tile is split, and nothing is
+// launched that would settle one.
 struct Products {
     int64_t rows, vocab, hidden, logits_steps, dhidden_steps;
     int32_t pieces, pairs, grad, few, cus;  // few: dz may go in two parts
     int32_t logits_tile, dhidden_tile, dweight_tile;
+    int32_t logits_whole, dhidden_whole, dweight_whole;
 };
 
 // What dhidden's way through weight is counted as, whose rows it reads in pieces as wide as
@@ -89,17 +91,18 @@ __device__ __forceinline__ Piece piece_of(const Products& p, int64_t count, int6
     auto tiles = [](int64_t x, int64_t y, int tile) { return (uint32_t)(((x + tile - 1) / tile) * ((y + tile - 1) / tile)); };
     // each product reads weight, or writes a gradient as large
     const int64_t bytes = p.vocab * p.hidden * (p.pairs > 1 ? 4 : 2);
-    auto share = [&](int64_t x, int64_t y, int64_t n, int tile, int pairs, int64_t bytes) {
+    auto share = [&](int64_t x, int64_t y, int64_t n, int tile, int pairs, int64_t bytes, bool whole) {
+        if (whole) return Share{tiles(x, y, tile), 0, 1};
         return share_by_wave(tiles(x, y, tile), n, room_of(tile, p.cus), cost_of(tile, pairs, 0, bytes));
     };
     Piece out{};
-    out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile, p.pairs, bytes);
+    out.logits = share(p.vocab, rows, p.logits_steps, p.logits_tile, p.pairs, bytes, p.logits_whole);
     if (!p.grad) return out;
     out.pairs = p.few && count <= FEW ? 2 : p.pairs;
-    out.dhidden = share(p.hidden, rows, p.dhidden_steps, p.dhidden_tile, out.pairs, way_down(bytes, p.dhidden_tile));
+    out.dhidden = share(p.hidden, rows, p.dhidden_steps, p.dhidden_tile, out.pairs, way_down(bytes, p.dhidden_tile), p.dhidden_whole);
     // without tokens there is nothing to add, but what the pieces have summed is to be
     // written by the first and rounded by the last
-    if (steps) out.dweight = share(p.hidden, p.vocab, steps, p.dweight_tile, out.pairs, bytes);
+    if (steps) out.dweight = share(p.hidden, p.vocab, steps, p.dweight_tile, out.pairs, bytes, p.dweight_whole);
     else if (piece == 0 || piece + 1 == p.pieces) out.dweight = {tiles(p.hidden, p.vocab, p.dweight_tile), 0, 1};
     return out;
 }
@@ -781,9 +784,9 @@ struct Plan {
     int64_t pad, vpad, rows, pieces;  // hidden and vocab padded, tokens of a piece, pieces
     bool own_weight, f32, grad, few, wide;  // wide: gradients in f32
     bool lifts;  // tokens' dz may be lifted
-    int64_t bytes_of_weight;
     int32_t blocks, shift, pairs, cus;
     Shape logits, dhidden, dweight;
+    bool logits_whole, dhidden_whole, dweight_whole;  // never split: k_select is told, and nothing launched that settles
     // offsets in the workspace
     int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, reach, lift, hidden, weight, e, dz, low, sums, partial, bytes;
 };
@@ -791,6 +794,20 @@ struct Plan {
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
 
 int32_t reduction_of(const rf_cross_entropy& a) { return a.reduction & ~RF_GRADS_F32; }
+
+// Whether no number of tokens that count splits a tile, where that is soon found: a
+// launch with nothing to settle takes 4.5 us.
+bool never_splits(const Shape& shape, const Plan& p, int64_t bytes, bool few, int64_t tiles_q, int64_t steps)
+{
+    if (steps < 4) return true;  // (no part of fewer than two)
+    if (tiles_q > 4) return false;
+    for (int pairs = p.pairs; pairs <= (few ? 2 : p.pairs); ++pairs) {
+        const Cost c = cost_of(shape.tile, pairs, 0, bytes);
+        for (int64_t q = 1; q <= (pairs > p.pairs ? 1 : tiles_q); ++q)  // (two pairs: of at most FEW tokens)
+            if (share_of((uint32_t)(shape.tiles_p * q), steps, shape.room, c).rest) return false;
+    }
+    return true;
+}
 
 Plan plan_of(const rf_cross_entropy& a, int cus)
 {
@@ -821,7 +838,6 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
     p.logits = shape_of(a.vocab, p.rows, steps, p.pairs, bytes, cus);
     p.shift = p.logits.tile > 128 ? 7 : 6;
     p.blocks = (int32_t)((a.vocab + (1 << p.shift) - 1) >> p.shift);
-    p.bytes_of_weight = bytes;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t from = at;
@@ -852,6 +868,12 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         if (p.pieces > 1 && !p.wide) p.sums = take(a.vocab * a.hidden * 4);
         p.dhidden = shape_of(a.hidden, p.rows, p.vpad / STEP, p.pairs, bytes, cus, true);
         p.dweight = shape_of(a.hidden, a.vocab, held / STEP, p.pairs, bytes, cus);
+    }
+    auto down = [&](const Shape& s) { return (p.rows + s.tile - 1) / s.tile; };
+    p.logits_whole = never_splits(p.logits, p, bytes, false, down(p.logits), steps);
+    if (p.grad) {  // dhidden: the sums' steps are known, of dweight the tiles
+        p.dhidden_whole = never_splits(p.dhidden, p, way_down(bytes, p.dhidden.tile), p.few, down(p.dhidden), p.vpad / STEP);
+        p.dweight_whole = held / STEP < 4;
     }
     auto tiles = [](const Shape& s, int64_t rows) { return (int64_t)s.tiles_p * ((rows + s.tile - 1) / s.tile); };
     int64_t parts = parts_of(p.logits, tiles(p.logits, p.rows), steps);
@@ -895,26 +917,12 @@ template <typename J> rf_status multiply(const Shape& shape, int64_t tiles, cons
     return launch<k_settle<J>>((int64_t)std::min<int64_t>(tiles, shape.room) * J::G::WAVES, WAVE, 0, st, a);
 }
 
-// Whether no number of tokens that count splits a tile, where that is soon found: a
-// launch with nothing to settle takes 4.5 us.
-bool never_splits(const Shape& shape, const Plan& p, int64_t bytes, bool few, int64_t tiles_q, int64_t steps)
-{
-    if (steps < 4) return true;  // (no part of fewer than two)
-    if (tiles_q > 4) return false;
-    for (int pairs = p.pairs; pairs <= (few ? 2 : p.pairs); ++pairs) {
-        const Cost c = cost_of(shape.tile, pairs, 0, bytes);
-        for (int64_t q = 1; q <= (pairs > p.pairs ? 1 : tiles_q); ++q)  // (two pairs: of at most FEW tokens)
-            if (share_of((uint32_t)(shape.tiles_p * q), steps, shape.room, c).rest) return false;
-    }
-    return true;
-}
-
 int64_t tiles_of(const Shape& shape, int64_t rows) { return (int64_t)shape.tiles_p * ((rows + shape.tile - 1) / shape.tile); }
 
 template <typename H, typename E> rf_status logits(const Plan& p, const Logits& a, hipStream_t st)
 {
     const int64_t tiles = tiles_of(p.logits, a.rows);
-    const bool whole = never_splits(p.logits, p, p.bytes_of_weight, false, (a.rows + p.logits.tile - 1) / p.logits.tile, a.steps);
+    const bool whole = p.logits_whole;
     return p.logits.tile > 128  ? multiply<LogitsJob<H, E, 256, 2, 4>>(p.logits, tiles, a, st, whole)
            : p.logits.tile > 64 ? multiply<LogitsJob<H, E, 128, 2, 2>>(p.logits, tiles, a, st, whole)
                                 : multiply<LogitsJob<H, E, 64, 1, 4>>(p.logits, tiles, a, st, whole);
@@ -926,8 +934,7 @@ template <typename H, Layout LQ> rf_status product(const Plan& p, const Shape& s
     a.room = shape.room;
     a.partial = partial;
     const int64_t tiles = tiles_of(shape, a.rows);
-    // dhidden: the sums' steps are known, of dweight the tiles
-    const bool whole = LQ == KALONG ? never_splits(shape, p, way_down(p.bytes_of_weight, shape.tile), p.few, (a.rows + shape.tile - 1) / shape.tile, a.steps) : (a.piece_rows + STEP - 1) / STEP < 4;
+    const bool whole = LQ == KALONG ? p.dhidden_whole : p.dweight_whole;
     return shape.tile > 128  ? multiply<GradJob<H, LQ, 256, 2, 4>>(shape, tiles, a, st, whole)
            : shape.tile > 64 ? multiply<GradJob<H, LQ, 128, 2, 2>>(shape, tiles, a, st, whole)
                              : multiply<GradJob<H, LQ, 64, 2, 2>>(shape, tiles, a, st, whole);
@@ -942,7 +949,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
     uint16_t* const hidden = (uint16_t*)(ws + p.hidden);
     const int64_t all = up(a.tokens, STEP), plane = all * p.pad;
     const Products products{p.rows, a.vocab, a.hidden, p.pad / STEP, p.vpad / STEP, (int32_t)p.pieces, p.pairs, p.grad, p.few, p.cus,
-                            p.logits.tile, p.dhidden.tile, p.dweight.tile};
+                            p.logits.tile, p.dhidden.tile, p.dweight.tile, p.logits_whole, p.dhidden_whole, p.dweight_whole};
     rf_status s = a.target_bits == 64
         ? launch<k_select<int64_t>>(1, SELECT, 0, st, (const int64_t*)a.targets, a.tokens, a.ignore_index, a.vocab, a.loss, order,
                                     target, sc, (Piece*)(ws + p.piece), products)

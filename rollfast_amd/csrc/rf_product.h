@@ -334,8 +334,6 @@ template <typename H, Layout LP, Layout LQ, int TP, int TQ, int WP, int WQ, bool
 // take fragment i's, those of an odd one fragment i + 1's, so that the four lanes of
 // a row hold 64 bytes in order.  chunk_of() is the place of the first of them
 // behind fragment i's first column; quads() takes them apart again.
-typedef uint32_t u32x4_16 __attribute__((ext_vector_type(4), aligned(16)));
-
 __device__ __forceinline__ int chunk_of(int lane) { return (lane >> 4 & 1) * 16 + (lane >> 5) * 8; }
 
 __device__ __forceinline__ u32x4 chunk(u32x2 first, u32x2 second)
@@ -412,6 +410,7 @@ constexpr uint32_t PARTS_ROOM = 4, MOST_PARTS = 64;
 // small matrices took 9 to 21 % longer, with 650 for 780 some 5 % less, others 2 % more.)
 struct Cost {
     int32_t step, alone, ends, part, again;
+    uint32_t alone_in;  // `alone` holds up to this part of the room
     int64_t least;
 };
 
@@ -420,9 +419,9 @@ __host__ __device__ inline uint32_t room_of(int tile, int cus) { return (uint32_
 __host__ __device__ inline Cost cost_of(int tile, int pairs, int ends = 0, int64_t bytes = 0)
 {
     const int64_t least = bytes / 4900;  // at 4.9 TB/s
-    if (tile > 128) return {1600 * pairs, 1600 * pairs, ends ? ends : 6000, 110, 10000, least};
-    if (tile > 64) return {1050 * pairs, 630 * pairs, ends ? ends : 4000, 28, 14000, least};
-    return {780 * pairs, 400 * pairs, ends ? ends : 3000, 7, 6000, least};
+    if (tile > 128) return {1600 * pairs, 1600 * pairs, ends ? ends : 6000, 110, 10000, 2, least};
+    if (tile > 64) return {1050 * pairs, 630 * pairs, ends ? ends : 4000, 28, 14000, 2, least};
+    return {780 * pairs, 400 * pairs, ends ? ends : 3000, 7, 6000, 4, least};
 }
 
 // The last, incomplete round of `rest` tiles in n parts each; -1 where that is not done.
@@ -430,7 +429,7 @@ __host__ __device__ inline int64_t ns_of_rest(uint32_t rest, int64_t steps, uint
 {
     if (n > 1 && (n * rest > PARTS_ROOM * room || 2 * n > steps)) return -1;
     const uint32_t all = n * rest;
-    const int64_t ns = (all + room - 1) / room * ((steps + n - 1) / n * (all <= room / 4 || (all <= room / 2 && c.part > 7) ? c.alone : c.step) + c.ends);
+    const int64_t ns = (all + room - 1) / room * ((steps + n - 1) / n * (all <= room / c.alone_in ? c.alone : c.step) + c.ends);
     return (ns > c.least ? ns : c.least) + (n > 1 ? c.again + (int64_t)c.part * all : 0);
 }
 
