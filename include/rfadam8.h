@@ -645,7 +645,9 @@ RF_API rf_status rf_orthogonalize(const rf_orthogonal_matrix* matrices, int32_t 
  *   u = nesterov ? momentum m + rest g : m
  *   update = scale orthogonalised(u) + decay param
  * m is kept as rf_blockwise_quantize's dynamic signed codes and f32 scales, rows in
- * order, padding included, or as f32; u is formed before m is stored.  Matrices are
+ * order, padding included, or as f32; u is formed before m is stored.  Where grad is
+ * not finite update is NaN, and the blocks of codes it falls in (f32: the elements)
+ * keep their momentum.  Matrices are
  * dense; grad and update have one dtype.  steps, coefficients, eps, workspace and
  * limits as rf_orthogonalize's. */
 typedef struct rf_muon8_leaf {

@@ -7,6 +7,11 @@
 // scales, u in f32 to the place where the orthogonalisation's next X will lie (of
 // the same size, and free until then), and the sums of its squares; the
 // orthogonalisation (rf_schulz.hip) takes both up.
+//
+// A gradient that is not finite makes its matrix' update NaN, but does not get into the
+// momentum: a block of codes that it would (of an f32 momentum an element) stays as it
+// was.  A NaN's code would stand for about one, where its neighbours are a thousandth,
+// and every update would follow it for a hundred steps.
 #include <algorithm>
 
 #include "rf_device.h"
@@ -133,7 +138,12 @@ __global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* _
             }
             if (left > 0) {
                 put_u(a, from + c, left, u);
-                if (!a.codes) rfb::put8(a.momentum + from + c, rfb::narrow8<float>(m), left);
+                if (!a.codes) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < left && !__builtin_isfinite(m[k])) m[k] = a.momentum[from + c + k];
+                    rfb::put8(a.momentum + from + c, rfb::narrow8<float>(m), left);
+                }
             }
         }
         if (!a.codes) continue;
@@ -146,6 +156,7 @@ __global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* _
             __syncthreads();
             for (int w = 0; w < WAVES_PER_WG; ++w) top = max(top, tops[w]);
         }
+        if (top >= 0x7F800000u) continue;  // (the same for all that code this block)
         const float scale = scale_from_absmax_bits(top), rs = 1.0f / scale;
         const bool fast = block_is_fast(top, scale);
         for (int64_t c = mine ? first : bs; c < bs; c += WG * 8) {

@@ -214,7 +214,9 @@ def muon8(learning_rate, momentum: float = 0.95, *, nesterov: bool = True, weigh
     cols)), 'rms' 0.2 sqrt(max(rows, cols)), None 1.  m is stored as
     ``quantize_blocks`` stores it (dynamic signed codes, one float32 scale per
     ``block_size`` elements), below ``min_size`` elements in float32; u is formed
-    from m before that.  Every leaf is a matrix: give embeddings, vectors and the
+    from m before that.  A gradient that is not finite makes its matrix' update
+    NaN, and leaves the blocks (float32: the elements) that it falls in as they
+    were.  Every leaf is a matrix: give embeddings, vectors and the
     like to ``adamw8`` with ``multi_transform``.  ``learning_rate``: a number, or a
     function of the step count.  The momentum is updated in place: the returned
     state shares its tensors."""

@@ -1,0 +1,69 @@
+"""``muon8`` where gradients are not finite, and composed with the other
+transformations: clipping, accumulation, the guard, labels."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import oracle as orc
+from tests.test_gpu_muon8 import BF16, BOUND, F16, F32, exact, gaussian, low_rank, rf, step
+
+pytestmark = pytest.mark.gpu
+
+
+def moments(q):
+    return [x.clone() for x in ((q.values, q.scales) if isinstance(q, rf().QuantizedBlocks) else (q,))]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("block_size", [16, 100, 512, 2048, 5000])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_a_gradient_that_is_not_finite_does_not_get_into_the_momentum(value, block_size, dtype):
+    """The blocks that it falls in stay as they were, the others are this step's bit for
+    bit; the update is NaN, and the next one follows from finite gradients alone."""
+    tx = rf().muon8(0.02, block_size=block_size, min_size=0)
+    shape, at = (130, 97), [(0, 0), (77, 3), (77, 4), (129, 96)]
+    state = tx.init([gaussian(*shape, dtype)])
+    _, state = tx.update([low_rank(*shape, dtype, seed=1) * 1e-3], state)
+    old = moments(state.mu[0])
+    m = rf().dequantize_blocks(state.mu[0]).cpu().numpy()
+    bad = low_rank(*shape, dtype, seed=2) * 1e-3
+    g = bad.float().cpu().numpy()
+    for i, j in at:
+        bad[i, j] = value
+    updates, state = tx.update([bad], state)
+    assert updates[0].isnan().any()
+    codes, scales = orc.quantize(step(m, g, 0.95, True)[0], block_size)
+    hit = sorted({(i * shape[1] + j) // block_size for i, j in at})
+    keep = np.ones(len(scales), bool)
+    keep[hit] = False
+    got = [x.cpu().numpy().reshape(len(scales), -1) for x in moments(state.mu[0])]
+    was = [x.cpu().numpy().reshape(len(scales), -1) for x in old]
+    assert np.array_equal(got[0][keep], codes.reshape(len(scales), -1)[keep]) and np.array_equal(got[1][keep, 0], scales[keep])
+    assert np.array_equal(got[0][hit], was[0][hit]) and np.array_equal(got[1][hit], was[1][hit])
+    now = rf().dequantize_blocks(state.mu[0]).cpu().numpy()
+    assert np.isfinite(now).all()
+    good = low_rank(*shape, dtype, seed=3) * 1e-3
+    updates, state = tx.update([good], state)
+    ref = -0.02 * math.sqrt(shape[0] / shape[1]) * exact(torch.from_numpy(step(now, good.float().cpu().numpy(), 0.95, True)[1]).cuda())
+    assert (updates[0].double() - ref).norm().item() < BOUND[dtype] * ref.norm().item() * 1.2
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_an_f32_momentum_keeps_the_elements_that_would_not_be_finite(value):
+    tx = rf().muon8(0.02, min_size=100000)
+    shape = (45, 61)
+    state = tx.init([gaussian(*shape, F32)])
+    _, state = tx.update([low_rank(*shape, F32, seed=1)], state)
+    old = state.mu[0].clone()
+    bad = low_rank(*shape, F32, seed=2)
+    want = torch.from_numpy(step(old.cpu().numpy(), bad.cpu().numpy(), 0.95, True)[0]).cuda()
+    for i, j in ((0, 0), (20, 7), (44, 60)):
+        bad[i, j] = value
+        want[i, j] = old[i, j]
+    updates, state = tx.update([bad], state)
+    assert updates[0].isnan().any() and torch.equal(state.mu[0], want)
