@@ -60,6 +60,27 @@ def _inner_step(tx):
     return step
 
 
+def fuses(update) -> bool:
+    """Whether ``update._step`` runs on the kernels of adamw8 and its kind alone,
+    which take the clipping and the guard in.  With ``muon8`` anywhere inside a
+    composition does not: its parts are then called one after the other."""
+    from .multisteps import _MultiStepsUpdate
+    from .optim.adam8 import _Adamw8Update
+    from .transforms import _ApplyIfFiniteUpdate, _ClipUpdate
+
+    if isinstance(update, _ChainUpdate):
+        txs = update.transforms
+        clipped = len(txs) == 2 and isinstance(txs[0].update, _ClipUpdate)
+        return (len(txs) == 1 or clipped) and fuses(txs[-1].update)
+    if isinstance(update, (_MaskedUpdate, _ApplyIfFiniteUpdate)):
+        return fuses(update.inner.update)
+    if isinstance(update, _MultiStepsUpdate):
+        return fuses(update.ms._opt.update)
+    if isinstance(update, _MultiTransformUpdate):
+        return all(isinstance(tx.update, _Adamw8Update) for tx in update.transforms.values())
+    return hasattr(update, "_step")
+
+
 class _MaskedUpdate:
     """optax.masked(inner, mask).update: the inner transformation sees
     MaskedNode in place of the leaves whose mask is False; those leaves keep

@@ -38,6 +38,7 @@ import numpy as np
 
 from . import _lib, _tree
 from ._base import GradientTransformationExtraArgs, is_passthrough_leaf as _is_passthrough_leaf, safe_int32_increment
+from .combine import fuses
 
 
 class MultiStepsState(NamedTuple):
@@ -185,7 +186,7 @@ class _MultiStepsUpdate:
         emit = mini_step == k_steps - 1
         if emit:
             inner_upd = ms._opt.update
-            if hasattr(inner_upd, "_step"):
+            if hasattr(inner_upd, "_step") and (apply or fuses(inner_upd)):
                 out, inner_state = inner_upd._step(state.acc_grads, state.inner_opt_state, params, apply=apply,
                                                    **kwargs)
             elif apply:

@@ -67,3 +67,95 @@ def test_an_f32_momentum_keeps_the_elements_that_would_not_be_finite(value):
         want[i, j] = old[i, j]
     updates, state = tx.update([bad], state)
     assert updates[0].isnan().any() and torch.equal(state.mu[0], want)
+
+
+SPEC = {"embed": (300, 64), "norm": (64,), "up": (256, 64), "down": (64, 256)}
+LABELS = {"embed": "rest", "norm": "rest", "up": "matrix", "down": "matrix"}
+
+
+def tree(seed, dtype=BF16, scale=1e-2):
+    return {k: (low_rank(*s, dtype, seed=seed + i) if len(s) == 2 else gaussian(1, *s, dtype, seed=seed)[0]) * scale
+            for i, (k, s) in enumerate(SPEC.items())}
+
+
+def both():
+    return rf().multi_transform({"matrix": rf().muon8(0.02, weight_decay=0.1), "rest": rf().adamw8(1e-3)}, LABELS)
+
+
+def tensors(state):
+    """Every tensor of a state, copied."""
+    found = []
+
+    def walk(x):
+        if isinstance(x, torch.Tensor):
+            found.append(x.clone())
+        elif isinstance(x, rf().QuantizedBlocks):
+            found.extend(moments(x))
+        elif isinstance(x, dict):
+            for k in sorted(x):
+                walk(x[k])
+        elif isinstance(x, (list, tuple)):
+            for y in x:
+                walk(y)
+
+    walk(state)
+    return found
+
+
+def same(a, b):
+    assert len(a) == len(b) > 0 and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def same_tree(a, b):
+    assert a.keys() == b.keys() and all(torch.equal(a[k], b[k]) for k in a)
+
+
+MATRICES = ("up", "down")
+COMPOSITIONS = {
+    "muon8": (lambda: rf().muon8(0.02, weight_decay=0.1), MATRICES),
+    "clipped": (lambda: rf().chain(rf().clip_by_global_norm(0.5), rf().muon8(0.02, weight_decay=0.1)), MATRICES),
+    "labels": (both, tuple(SPEC)),
+    "clipped labels": (lambda: rf().chain(rf().clip_by_global_norm(0.5), both()), tuple(SPEC)),
+    "masked": (lambda: rf().masked(rf().muon8(0.02), {"up": True, "down": False}), MATRICES),
+    "chained twice": (lambda: rf().chain(rf().clip_by_global_norm(0.5), rf().clip_by_global_norm(0.1), both()), tuple(SPEC)),
+}
+
+
+def part(t, names):
+    return {k: t[k] for k in names}
+
+
+def test_clipped_before_muon8():
+    """The chain is the clipping and then the updates."""
+    params = part(tree(1), MATRICES)
+    tx, alone = COMPOSITIONS["clipped"][0](), rf().muon8(0.02, weight_decay=0.1)
+    clip = rf().clip_by_global_norm(0.5)
+    state, other, c = tx.init(params), alone.init(params), clip.init(params)
+    for turn in range(2):
+        grads = part(tree(10 + turn), MATRICES)
+        got, state = tx.update(grads, state, params)
+        clipped, c = clip.update(grads, c)
+        ref, other = alone.update(clipped, other, params)
+        same_tree(got, ref)
+    same(tensors(state), tensors(other))
+
+
+@pytest.mark.parametrize("name", COMPOSITIONS)
+def test_accumulated(name):
+    """MultiSteps of two: the inner update of the mean, zeros before it."""
+    make, names = COMPOSITIONS[name]
+    params = part(tree(1, F32), names)
+    tx, alone = rf().MultiSteps(make(), 2), make()
+    state, other = tx.init(params), alone.init(params)
+    for turn in range(4):
+        grads = part(tree(10 + turn, F32), names)
+        got, state = tx.update(grads, state, params)
+        if turn % 2 == 0:
+            assert not any(x.any() for x in got.values())
+            mean = grads
+            continue
+        # the running mean, each operation rounded
+        mean = {k: mean[k] + (grads[k] - mean[k]) * 0.5 for k in names}
+        ref, other = alone.update(mean, other, params)
+        same_tree(got, ref)
+        same(tensors(state.inner_opt_state), tensors(other))
