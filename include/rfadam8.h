@@ -369,6 +369,10 @@ typedef struct rf_clip_leaf {
 RF_API rf_status rf_clip_by_global_norm(const rf_clip_leaf* leaves, int32_t n_leaves, float max_norm,
                                         float* stats, void* stream);
 
+/* finite (device) = 1 where every element of every leaf is finite, else 0: that
+ * norm's pass alone, as RF_SKIP_NONFINITE tests it.  `out` is not used. */
+RF_API rf_status rf_all_finite(const rf_clip_leaf* leaves, int32_t n_leaves, int32_t* finite, void* stream);
+
 /* One leaf of the Magma pass of scale_by_adam(use_magma=True)
  * (optim/adam.py:127-131, :203-217; optim/magma.py:15-132). */
 typedef struct rf_magma_leaf {

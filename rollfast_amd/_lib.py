@@ -255,6 +255,7 @@ EXPORTS = (
     "rf_apply_updates",
     "rf_apply_updates_packed",
     "rf_clip_by_global_norm",
+    "rf_all_finite",
     "rf_magma_reduce",
     "rf_magma_scale",
     "rf_magma_apply_updates",
@@ -339,6 +340,7 @@ def lib() -> ctypes.CDLL:
     L.rf_muon8_update_workspace.argtypes = [ctypes.POINTER(Muon8Leaf), i32, ctypes.POINTER(i64)]
     L.rf_muon8_update.argtypes = [ctypes.POINTER(Muon8Leaf), i32, ctypes.c_float, ctypes.c_float, i32, i32, _p,
                                   ctypes.c_float, _p, i64, _p]
+    L.rf_all_finite.argtypes = [ctypes.POINTER(ClipLeaf), i32, _p, _p]
     L.rf_codebook.argtypes = [i32, _p]
     L.rf_host_table_codes.argtypes = [i32, u32, i64, _p]
     L.rf_host_search_index.argtypes = [i32, u32, i64, _p]

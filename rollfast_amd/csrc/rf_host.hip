@@ -3166,24 +3166,11 @@ rf_status sr_bf16_launch(const float* x, int64_t size, uint32_t key0, uint32_t k
     return RF_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-rf_status rf_sr_bf16(const float* x, int64_t size, uint32_t key0, uint32_t key1, const uint32_t* bits, uint16_t* out,
-                     void* stream)
-{
-    return sr_bf16_launch(x, size, key0, key1, bits, out, false, stream);
-}
-
-rf_status rf_sr_bf16_packed(const float* x, int64_t size, uint32_t key0, uint32_t key1, uint16_t* out, void* stream)
-{
-    return sr_bf16_launch(x, size, key0, key1, nullptr, out, true, stream);
-}
-
-rf_status rf_clip_by_global_norm(const rf_clip_leaf* leaves, int32_t n_leaves, float max_norm, float* stats,
-                                 void* stream)
-{
+// The leaves' norm pre-pass alone, with (scale, norm) in `stats` and the finite flag in
+// `finite`, and where `clip` the leaves scaled.
+rf_status norm_run(const rf_clip_leaf* leaves, int32_t n_leaves, float max_norm, bool clip, float* stats, int32_t* finite,
+                   void* stream, const char* what)
+try {
     if (n_leaves < 0 || (n_leaves > 0 && !leaves)) return fail(RF_ERR_INVALID, "bad leaf table");
     if (!(max_norm > 0.0f) || std::isinf(max_norm)) return fail(RF_ERR_INVALID, "max_norm must be positive.");
     if (n_leaves > 65535) return fail(RF_ERR_UNSUPPORTED, "more than 65535 leaves in one clip call");
@@ -3196,7 +3183,7 @@ rf_status rf_clip_by_global_norm(const rf_clip_leaf* leaves, int32_t n_leaves, f
         const rf_clip_leaf& L = leaves[i];
         if (L.size < 0) return fail(RF_ERR_INVALID, "negative size");
         if (!valid_dtype(L.dtype)) return fail(RF_ERR_UNSUPPORTED, "dtype must be f32, bf16 or f16");
-        if (L.size > 0 && (!L.grad || !L.out)) return fail(RF_ERR_INVALID, "null buffer");
+        if (L.size > 0 && (!L.grad || (clip && !L.out))) return fail(RF_ERR_INVALID, "null buffer");
         gl[i] = rf_adam8_leaf{};
         gl[i].grad = L.grad;
         gl[i].size = L.size;
@@ -3259,18 +3246,47 @@ rf_status rf_clip_by_global_norm(const rf_clip_leaf* leaves, int32_t n_leaves, f
         }
     }
     if (e == hipSuccess) {
-        hipLaunchKernelGGL(k_gnorm_finish, dim3(1), dim3(WG), 0, s, d_ls, nseg, max_norm, d_cp, stats, nullptr);
+        hipLaunchKernelGGL(k_gnorm_finish, dim3(1), dim3(WG), 0, s, d_ls, nseg, max_norm, d_cp, stats, finite);
         e = hipGetLastError();
     }
-    if (e == hipSuccess && maxsize > 0) {
+    if (e == hipSuccess && maxsize > 0 && clip) {
         const int gx = (int)std::max<int64_t>(1, std::min<int64_t>((maxsize / 8 + WG - 1) / WG,
                                                                    (int64_t)ds->num_cus * 4));
         hipLaunchKernelGGL(k_clip_scale, dim3(gx, n_leaves), dim3(WG), 0, s, d_cl, d_cp);
         e = hipGetLastError();
     }
     st = stg.finish(s);
-    if (e != hipSuccess) return fail(RF_ERR_HIP, std::string("rf_clip_by_global_norm: ") + hipGetErrorString(e));
+    if (e != hipSuccess) return fail(RF_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
     return st;
+} catch (const std::bad_alloc&) {
+    return fail(RF_ERR_HIP, "no memory for the leaf table");
+}
+
+}  // namespace
+
+extern "C" {
+
+rf_status rf_sr_bf16(const float* x, int64_t size, uint32_t key0, uint32_t key1, const uint32_t* bits, uint16_t* out,
+                     void* stream)
+{
+    return sr_bf16_launch(x, size, key0, key1, bits, out, false, stream);
+}
+
+rf_status rf_sr_bf16_packed(const float* x, int64_t size, uint32_t key0, uint32_t key1, uint16_t* out, void* stream)
+{
+    return sr_bf16_launch(x, size, key0, key1, nullptr, out, true, stream);
+}
+
+rf_status rf_clip_by_global_norm(const rf_clip_leaf* leaves, int32_t n_leaves, float max_norm, float* stats,
+                                 void* stream)
+{
+    return norm_run(leaves, n_leaves, max_norm, true, stats, nullptr, stream, "rf_clip_by_global_norm");
+}
+
+rf_status rf_all_finite(const rf_clip_leaf* leaves, int32_t n_leaves, int32_t* finite, void* stream)
+{
+    if (!finite) return fail(RF_ERR_INVALID, "null output");
+    return norm_run(leaves, n_leaves, 1.0f, false, nullptr, finite, stream, "rf_all_finite");
 }
 
 }  // extern "C"

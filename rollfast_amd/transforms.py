@@ -12,7 +12,8 @@ the fine-tune builders wrap around their chain (finetune/builders.py:
 1605-1609, ``GradientPolicy(nonfinite="skip", max_consecutive_nonfinite=1)``
 by default, finetune/config.py:226-233), for the optimizers of this package:
 the step's norm pre-pass tests every grad for Inf/NaN and the step units
-apply the reject branch on the device.
+apply the reject branch on the device; with ``muon8`` inside, that pass runs
+alone and the host decides.
 """
 
 from __future__ import annotations
@@ -114,6 +115,35 @@ def clip_by_global_norm(max_norm: float, *, axis_name=None, partition_axis_names
     return GradientTransformation(init_fn, _ClipUpdate(float(max_norm)))
 
 
+def _all_finite(updates) -> bool:
+    """Whether every element of every leaf is finite.  Waits for the device."""
+    import torch
+
+    rows, held, device = [], [], None
+    for leaf in _tree.leaves(updates, is_leaf=_is_passthrough_leaf):
+        if _is_passthrough_leaf(leaf):
+            continue
+        if not isinstance(leaf, torch.Tensor) or not leaf.is_cuda:
+            raise ValueError("updates must be torch tensors on a ROCm device")
+        device = leaf.device if device is None else device
+        if leaf.device != device:
+            raise ValueError("all leaves must live on the same device")
+        if leaf.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise NotImplementedError(f"dtype {leaf.dtype} is not supported (float32, bfloat16 or float16)")
+        held.append(leaf.contiguous())
+        row = _lib.ClipLeaf()
+        row.grad, row.size = held[-1].data_ptr(), int(leaf.numel())
+        row.dtype = {torch.bfloat16: _lib.RF_BF16, torch.float16: _lib.RF_F16}.get(leaf.dtype, _lib.RF_F32)
+        rows.append(row)
+    if not rows:
+        return True
+    with torch.cuda.device(device):
+        flag = torch.empty(1, dtype=torch.int32, device=device)
+        _lib.check(_lib.lib().rf_all_finite((_lib.ClipLeaf * len(rows))(*rows), len(rows), flag.data_ptr(),
+                                            _lib.stream_ptr()), "apply_if_finite")
+        return bool(flag.item())
+
+
 def _first_device(tree):
     """The device of some leaf of ``tree`` on a ROCm device, or None: the
     first found, without flattening the tree."""
@@ -152,6 +182,10 @@ class _ApplyIfFiniteUpdate:
     flag, so the host reads it back every step: the launch copies it to
     pinned host memory right after the norm pre-pass, and the call waits for
     that copy only, not for the step, which keeps running.
+
+    Around transformations that are not such a launch (``muon8``, alone or in a
+    composition) the pre-pass runs by itself, the call waits for its flag, and
+    a rejected step is not begun.
     """
 
     def __init__(self, inner, max_consecutive_errors: int):
@@ -162,18 +196,26 @@ class _ApplyIfFiniteUpdate:
     def _step(self, updates, state, params, *, apply: bool, **kwargs):
         import torch
 
+        from .combine import _inner_step, fuses
+
         notfinite_next = safe_int32_increment(int(np.asarray(state.notfinite_count)))
         may_reject = not notfinite_next > self.max_consecutive_errors
-        device = _first_device(updates)
-        flag = None
-        if device is not None:
-            if self._flag is None:
-                self._flag = torch.ones(1, dtype=torch.int32, pin_memory=True)
-            flag = self._flag
-            flag[0] = 1  # a run with no elements leaves it: vacuously finite
-        out, new_inner = self.inner.update._step(updates, state.inner_state, params, apply=apply,
-                                                 skip_nonfinite=may_reject, finite_host=flag, **kwargs)
-        isfinite = True if flag is None else bool(int(flag[0]))
+        if apply or fuses(self.inner.update):
+            device = _first_device(updates)
+            flag = None
+            if device is not None:
+                if self._flag is None:
+                    self._flag = torch.ones(1, dtype=torch.int32, pin_memory=True)
+                flag = self._flag
+                flag[0] = 1  # a run with no elements leaves it: vacuously finite
+            out, new_inner = _inner_step(self.inner)(updates, state.inner_state, params, apply=apply,
+                                                     skip_nonfinite=may_reject, finite_host=flag, **kwargs)
+            isfinite = True if flag is None else bool(int(flag[0]))
+        else:
+            isfinite = _all_finite(updates)
+            out = new_inner = None
+            if isfinite or not may_reject:
+                out, new_inner = self.inner.update(updates, state.inner_state, params)
         if isfinite or not may_reject:
             inner_state = new_inner
         else:
@@ -201,10 +243,13 @@ def apply_if_finite(inner: GradientTransformation, max_consecutive_errors: int) 
     finetune/builders.py:1605-1609).  ``inner`` is a transformation built by
     ``adamw8``, ``scale_by_adam8``, ``adamw`` or ``scale_by_adam``; the guarded
     step stays one launch (``adamw8_step`` / ``adamw_step`` accept the
-    wrapped transformation too)."""
-    if not hasattr(inner.update, "_step"):
-        raise NotImplementedError(
-            "apply_if_finite wraps the transformations built by adamw8, scale_by_adam8, adamw or scale_by_adam")
+    wrapped transformation too).  ``muon8`` and compositions with it are guarded
+    as well: all leaves are tested first, and a rejected step is not begun."""
+    from .optim.muon import _Muon8Update
+
+    if not hasattr(inner.update, "_step") and not isinstance(inner.update, _Muon8Update):
+        raise NotImplementedError("apply_if_finite wraps the transformations built by adamw8, scale_by_adam8, adamw, "
+                                  "scale_by_adam or muon8, and compositions of them")
 
     def init_fn(params):
         return ApplyIfFiniteState(

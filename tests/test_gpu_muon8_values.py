@@ -159,3 +159,81 @@ def test_accumulated(name):
         ref, other = alone.update(mean, other, params)
         same_tree(got, ref)
         same(tensors(state.inner_opt_state), tensors(other))
+
+
+@pytest.mark.parametrize("name", COMPOSITIONS)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_guarded(value, name):
+    """apply_if_finite: a step with a value that is not finite anywhere leaves all state
+    as it was and gives zeros; accepted steps are the unguarded ones."""
+    make, names = COMPOSITIONS[name]
+    params = part(tree(1), names)
+    tx, alone = rf().apply_if_finite(make(), 2), make()
+    state, other = tx.init(params), alone.init(params)
+    for turn, bad in enumerate([None, names[0], names[-1], None, None]):
+        grads = part(tree(10 + turn), names)
+        if bad is not None:
+            grads[bad].view(-1)[-1] = value
+        before = tensors(state.inner_state)
+        got, state = tx.update(grads, state, params)
+        assert bool(state.last_finite) == (bad is None)
+        if bad is not None:
+            assert all(x.dtype == grads[k].dtype and not x.any() for k, x in got.items())
+            same(before, tensors(state.inner_state))
+            continue
+        ref, other = alone.update(grads, other, params)
+        same_tree(got, ref)
+        same(tensors(state.inner_state), tensors(other))
+    assert int(state.total_notfinite) == 2 and int(state.notfinite_count) == 0
+    # more in a row than are allowed: the third goes through
+    for turn in range(3):
+        grads = part(tree(30 + turn), names)
+        grads["up"][0, 0] = value
+        got, state = tx.update(grads, state, params)
+        assert int(state.notfinite_count) == turn + 1
+        assert got["up"].isfinite().all() == (turn < 2)
+
+
+def test_guarded_inside_an_accumulation():
+    """As the builders of a fine-tuning step nest them."""
+    params = tree(1, F32)
+    tx = rf().MultiSteps(rf().apply_if_finite(rf().chain(rf().clip_by_global_norm(0.5), both()), 1), 2)
+    state = tx.init(params)
+    before = tensors(state.inner_opt_state)
+    for turn in range(2):
+        grads = tree(10 + turn, F32)
+        grads["norm"][3] = math.nan
+        got, state = tx.update(grads, state, params)
+        assert not any(x.any() for x in got.values())
+    same(before, tensors(state.inner_opt_state))
+    assert int(state.inner_opt_state.total_notfinite) == 1
+    # (the accumulator's reset is a product with zero, which leaves a NaN one: begun again)
+    alone, state = rf().chain(rf().clip_by_global_norm(0.5), both()), tx.init(params)
+    grads = tree(20, F32)
+    for _ in range(2):
+        got, state = tx.update(grads, state, params)
+    same_tree(got, alone.update(grads, alone.init(params), params)[0])
+
+
+def test_leaves_of_every_kind_are_tested():
+    """Empty ones, strided ones, every dtype, none, the last element of a large one."""
+    from rollfast_amd.transforms import _all_finite
+
+    x = gaussian(1000, 999, F32)
+    for t in ([], [None], [x[:0]], [x], [x.t(), None, x.to(BF16), x[:, 3:7].to(F16)], [x[3:], x[:0], x]):
+        assert _all_finite(t)
+    x[999, 998] = math.inf
+    assert not _all_finite([x.clone().zero_(), x]) and not _all_finite([x.t()]) and _all_finite([x[:, :998]])
+    assert not _all_finite([x.to(BF16)]) and not _all_finite([x.to(F16)])
+    big = torch.full((3,), 3e38, device="cuda")
+    assert _all_finite([big, big])
+
+
+def test_fused_steps_refuse_muon8():
+    params = tree(1)
+    for tx in (rf().apply_if_finite(both(), 1), both(), rf().MultiSteps(both(), 2), rf().muon8(0.1)):
+        p = params if tx.update.__class__.__name__ != "_Muon8Update" else part(params, MATRICES)
+        with pytest.raises((NotImplementedError, TypeError)):
+            state = tx.init(p)
+            for _ in range(2):
+                _, state = rf().adamw8_step(tx, p, {k: x.clone() for k, x in p.items()}, state, stochastic=False)

@@ -129,3 +129,27 @@ def test_python_refusals_on_the_device():
     other = small._replace(mu={"w": rf.quantize_blocks(x, quantizer="symmetric_int8")})
     with pytest.raises(ValueError, match="dynamic signed"):
         rf.muon8(0.1).update({"w": x}, other)
+
+
+def test_finite_test_refusals():
+    L = _lib.lib()
+    row = _lib.ClipLeaf()
+    row.grad, row.size, row.dtype = P, 8, _lib.RF_F32
+    refused(L.rf_all_finite((_lib.ClipLeaf * 1)(row), 1, None, None), "null output")
+    refused(L.rf_all_finite(None, 1, P, None), "bad leaf table")
+    refused(L.rf_all_finite((_lib.ClipLeaf * 1)(row), -1, P, None), "bad leaf table")
+    for over, text, code in (({"grad": None}, "null buffer", 1), ({"size": -1}, "negative size", 1), ({"dtype": 9}, "dtype", 3)):
+        bad = _lib.ClipLeaf.from_buffer_copy(row)
+        for k, v in over.items():
+            setattr(bad, k, v)
+        refused(L.rf_all_finite((_lib.ClipLeaf * 1)(bad), 1, P, None), text, code)
+
+
+def test_the_guard_takes_muon8_and_no_strangers():
+    tx = rf.apply_if_finite(rf.muon8(0.1), 1)
+    state = tx.init({"w": torch.zeros(4, 8)})
+    assert isinstance(state.inner_state, rf.Muon8State)
+    with pytest.raises(ValueError, match="ROCm device"):
+        tx.update({"w": torch.zeros(4, 8)}, state)
+    with pytest.raises(NotImplementedError, match="apply_if_finite wraps"):
+        rf.apply_if_finite(rf.clip_by_global_norm(1.0), 1)
