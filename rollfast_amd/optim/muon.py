@@ -74,10 +74,10 @@ def orthogonalize(matrices, *, steps: int = 5, coefficients=COEFFICIENTS, eps: f
         dtype = _rf_dtype(x.dtype, "matrix")
         y = torch.empty(x.shape, dtype=x.dtype, device=device)
         out.append(y)
+        if not x.numel():
+            continue
         pairs = [(x, y)] if x.dim() == 2 else list(zip(x.reshape(-1, *x.shape[-2:]), y.view(-1, *x.shape[-2:])))
         for g, o in pairs:
-            if not g.numel():
-                continue
             g, stride = _matrix_rows(g, "matrix")
             held.append(g)
             rows.append(_lib.OrthogonalMatrix(g.data_ptr(), o.data_ptr(), g.shape[0], g.shape[1], stride, o.shape[1], dtype,

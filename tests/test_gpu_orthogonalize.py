@@ -228,3 +228,11 @@ def test_one_matrix_of_each_tile(dtype):
     for r, c in ((200, 330), (390, 1300), (1000, 1100), (1700, 2600)):
         g = low_rank(r, c, dtype, seed=r, noise=0.2)
         assert off(rf().orthogonalize(g), exact(g)) < BOUND[dtype], (r, c)
+
+
+def test_stacks_without_elements():
+    """An empty stack, stacked matrices without rows or without columns, among others."""
+    g = gaussian(20, 30, F32)
+    shapes = [(0, 3, 4), (2, 0, 4), (2, 3, 0), (2, 0, 0, 5), (0, 4), (3, 0)]
+    got = rf().orthogonalize([torch.empty(s, device="cuda") for s in shapes] + [g])
+    assert [tuple(x.shape) for x in got[:-1]] == shapes and torch.equal(got[-1], rf().orthogonalize(g))
