@@ -1,11 +1,12 @@
 """Trains a small language model of gated feed-forward blocks, with a loss that
-holds no logits and 8-bit state for both of its optimizers.
+writes no logits and 8-bit state for both of its optimizers.
 
 The blocks' matrices are updated by ``muon8`` (orthogonalised momentum, the
 momentum in 8-bit blocks), the embedding, the head and the norms by ``adamw8``;
 ``multi_transform`` has them as one transformation.  The head and the loss are
 ``linear_cross_entropy``: the loss and the gradients of the head and of its input
-without a tensor of tokens by vocabulary.  Tokens of a sequence's prompt are
+in one pass, in which the exponentials of a piece of the tokens are all that is held
+by vocabulary.  Tokens of a sequence's prompt are
 ignored by the loss.
 
     python examples/train_language_model.py [--steps 50] [--save int8|input]

@@ -68,6 +68,7 @@ struct Piece {
     uint32_t dz_top;
     int32_t pairs;   // plane pairs of the gradients' products
     uint32_t uneven; // some token's dz was lifted
+    uint32_t hidden_top, pad;  // f16, then: bits of the largest finite magnitude of the piece's rows of hidden
 };
 
 // The products of a piece, for k_select.  The last three: no tile is split, and nothing is
@@ -223,13 +224,13 @@ __device__ __forceinline__ void split8(const float (&v)[8], float scale, Raw<f16
 
 // Rows into the product's layout: 16 bits, columns padded with zeros to `pitch`.
 // With `order`: the rows that count, zeros up to a whole step behind them, and
-// zeros in the rows of `clear` that do not count.  `raised` (16 bits): the largest finite
-// magnitude of those that count, as k_top has it.
+// zeros in the rows of `clear` that do not count.  `tops` (f16): bits of the largest
+// finite magnitude that each of a row's four waves has seen.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t cols, int64_t stride, int64_t pitch,
                                              const int32_t* __restrict__ order, const Scalars* sc, const uint32_t* top,
                                              uint16_t* __restrict__ hi, uint16_t* __restrict__ lo, void* __restrict__ clear,
-                                             int wide, uint32_t* raised, int64_t rows)
+                                             int wide, uint32_t* __restrict__ tops, int64_t rows)
 {
     const int64_t r = blockIdx.x;
     int64_t from = r;
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t c
     for (int64_t c = (int64_t)threadIdx.x * 8; c < pitch; c += 2048) {
         Raw<T> v{};
         if (!zero && c < cols) v = load8(row, c, cols);
-        if (sizeof(T) == 2 && raised) {
+        if (sizeof(T) == 2 && tops) {
             float w[8];
             widen8(v, w);
 #pragma unroll
@@ -272,9 +273,9 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ x, int64_t c
             *(u32x4*)(hi + r * pitch + c) = v.a;
         }
     }
-    if (sizeof(T) == 4 || !raised) return;
+    if (sizeof(T) == 4 || !tops) return;
     for (int d = 1; d < WAVE; d *= 2) best = max(best, (uint32_t)__shfl_xor((int)best, d));
-    if (threadIdx.x % WAVE == 0) raise(raised, best);
+    if (threadIdx.x % WAVE == 0) tops[r * 4 + threadIdx.x / WAVE] = best;
 }
 
 // ------------------------------------------------------------- the logits ---
@@ -601,12 +602,23 @@ template <typename P, typename E> __global__ __launch_bounds__(256) void k_dlogi
 template <typename T>
 __global__ __launch_bounds__(256) void k_level(const T* __restrict__ x, int64_t cols, int64_t stride, int64_t pitch,
                                               const int32_t* __restrict__ order, int64_t first, int64_t most, const Scalars* sc,
-                                              const Piece* piece, const int32_t* __restrict__ lifts, uint16_t* __restrict__ hi,
-                                              uint16_t* __restrict__ lo)
+                                              Piece* piece, const int32_t* __restrict__ lifts, const uint32_t* __restrict__ tops,
+                                              uint16_t* __restrict__ hi, uint16_t* __restrict__ lo)
 {
     if (!piece->uneven) return;
     const int64_t rows = min((int64_t)sc->count - first, most);
-    const float scale = scale_of(sc->hidden_top);
+    uint32_t top = sc->hidden_top;
+    if (sizeof(T) == 2) {  // every workgroup for itself: k_pack's waves have 12 ns each for an atomic
+        __shared__ uint32_t of_wave[4];
+        top = 0;
+        for (int64_t i = first * 4 + threadIdx.x; i < (first + rows) * 4; i += 256) top = max(top, tops[i]);
+        for (int d = 1; d < WAVE; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+        if (threadIdx.x % WAVE == 0) of_wave[threadIdx.x / WAVE] = top;
+        __syncthreads();
+        top = max(max(of_wave[0], of_wave[1]), max(of_wave[2], of_wave[3]));
+        if (blockIdx.x == 0 && threadIdx.x == 0) piece->hidden_top = top;
+    }
+    const float scale = scale_of(top);
     for (int64_t q = blockIdx.x; q < rows; q += gridDim.x) {
         const T* const row = x + order[first + q] * stride;
         const int lift = lifts[q];
@@ -645,7 +657,7 @@ __device__ __forceinline__ float unscale_of(const Grad& a, bool wide)
 {
     float u = 1.0f / dz_scale(a.piece->dz_top, wide);
     if (a.pairs > 1) u *= inverse(scale_of(a.order ? a.sc->weight_top : a.sc->hidden_top));
-    else if (!a.order && a.lifts && a.piece->uneven) u *= inverse(scale_of(a.sc->hidden_top));
+    else if (!a.order && a.lifts && a.piece->uneven) u *= inverse(scale_of(a.piece->hidden_top));
     return u;
 }
 
@@ -788,7 +800,7 @@ struct Plan {
     Shape logits, dhidden, dweight;
     bool logits_whole, dhidden_whole, dweight_whole;  // never split: k_select is told, and nothing launched that settles
     // offsets in the workspace
-    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, reach, lift, hidden, weight, e, dz, low, sums, partial, bytes;
+    int64_t scalars, piece, order, target, stats, picked, top, factor, at_target, reach, lift, tops, hidden, weight, e, dz, low, sums, partial, bytes;
 };
 
 bool known(int32_t dtype) { return dtype == RF_F32 || dtype == RF_BF16 || dtype == RF_F16; }
@@ -859,6 +871,7 @@ Plan plan_of(const rf_cross_entropy& a, int cus)
         p.at_target = take(p.rows * 4);
         p.reach = take(p.rows * 4);
         p.lift = take(p.rows * 4);
+        if (p.lifts && !p.f32) p.tops = take(up(a.tokens, STEP) * 16);
         // Low parts of few tokens: one step of rows.  A tile of dhidden reads as many rows of
         // them as of the high ones, up to `held`, for tokens that do not exist: those behind the
         // step are the first of e, which lies next to it (both are multiples of 256 bytes).
@@ -967,7 +980,7 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
     }
     s = launch<k_pack<T>>(all, 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride, p.pad, (const int32_t*)order,
                           (const Scalars*)sc, (const uint32_t*)&sc->hidden_top, hidden, hidden + plane, a.dhidden, (int)p.wide,
-                          p.lifts && !p.f32 ? &sc->hidden_top : (uint32_t*)nullptr, a.tokens);
+                          p.lifts && !p.f32 ? (uint32_t*)(ws + p.tops) : (uint32_t*)nullptr, a.tokens);
     if (s != RF_OK) return s;
     Side w{{a.weight, a.weight}, a.weight_stride * 2, a.vocab, a.vocab};
     if (p.own_weight) {
@@ -1065,9 +1078,9 @@ template <typename T, typename H> rf_status run(const rf_cross_entropy& a, const
         }
         if constexpr (!__is_same(T, bf16)) {
             if (p.lifts) {
-                s = launch<k_level<T>>(std::min<int64_t>(rows, 2048), 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride,
-                                       p.pad, (const int32_t*)order, first, rows, (const Scalars*)sc, (const Piece*)piece_info,
-                                       (const int32_t*)r.lifts, h, h + (planes - 1) * plane);
+                s = launch<k_level<T>>(std::min<int64_t>(rows, 1024), 256, 0, st, (const T*)a.hidden_rows, a.hidden, a.hidden_stride,
+                                       p.pad, (const int32_t*)order, first, rows, (const Scalars*)sc, piece_info,
+                                       (const int32_t*)r.lifts, (const uint32_t*)(ws + p.tops), h, h + (planes - 1) * plane);
                 if (s != RF_OK) return s;
             }
         }

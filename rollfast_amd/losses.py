@@ -4,11 +4,13 @@
 
     loss = lse - logit[target] + z_loss * lse ** 2,  lse = log(sum(exp(logits)))
 
-for every row of ``hidden``, without a tensor of all logits: each tile of the
-product is reduced to a maximum and a sum as it is computed.
+for every row of ``hidden``; no logit is written: each tile of the product is
+reduced to a maximum and a sum as it is computed.
 ``linear_cross_entropy_grad`` gives the gradients of ``hidden`` and ``weight`` as
-well, in the same pass: it holds the exponentials of a piece of the tokens in 16
-bits, at most 2 GiB at once, and computes no product twice.
+well, in the same pass, and computes no product twice.  For that it holds the
+exponentials of a piece of the tokens, at most 2 GiB at once: 16 bits each (up to
+that size all of them, as much as 16-bit logits), float32 tensors' 32 and as much
+again.
 ``rollfast_amd.autograd.linear_cross_entropy`` is differentiable.
 
 A token whose target is ``ignore_index`` has a loss of zero and no part in the
@@ -20,10 +22,20 @@ its own, since split numbers have no infinities of one sign.
 ``hidden`` and ``weight`` are float32, bfloat16 or float16 on a ROCm device, both
 of one dtype, which is the gradients' too; losses are float32.  Targets are int32
 or int64.  Any row stride is read in place.  Work is enqueued on the current
-stream.  16-bit tensors are multiplied as they are, float32 ones to 22 bits; sums
-are f32 in a fixed order: equal inputs give equal bits.  The gradient of a logit
-is rounded to the tensors' own dtype (float32: to 22 bits; 16-bit ones where at
-most 16 tokens count: to twice its bits) before it is multiplied.
+stream.
+
+Sums are f32 in a fixed order: equal inputs give equal bits.  (How they are split
+follows from how many tokens count, so a token's last bits may differ from batch to
+batch.)  16-bit tensors are multiplied as they are, float32 ones to 22 bits, of
+which those below 2^-39 of the largest magnitude in ``hidden``, or ``weight``, are
+lost.  The gradient of a logit is rounded to the tensors' own dtype (float32: to 22
+bits; 16-bit ones where at most 16 tokens count: to twice its bits) before it is
+multiplied.  In float16 and float32 it is held down to 2^-33 of its token's own
+``dloss`` at least, however much other tokens weigh; what a token adds to the
+weight's gradient is also lost below 2^-39 of what the heaviest one may add.  For
+16-bit tensors exponentials are rounded to float16: a probability below 2^-25 of
+the largest among its 64 or 128 neighbours in the vocabulary has no part in the
+gradients.
 """
 
 from __future__ import annotations
@@ -125,7 +137,9 @@ def linear_cross_entropy_grad(hidden, weight, targets, dloss=None, *, ignore_ind
                               reduction: str = "none") -> LossGrads:
     """The losses, and the gradients of ``sum(dloss * loss)`` with ``dloss``
     float32 of the targets' shape; or with a ``reduction`` in place of ``dloss``
-    the reduced loss and its gradients."""
+    the reduced loss and its gradients.  float16 gradients of a mean over many
+    tokens lie below float16's normal numbers: give a ``dloss`` with the scale of
+    the loss in it, or take ``autograd.linear_cross_entropy``."""
     if (dloss is None) == (reduction == "none"):
         raise ValueError("the gradient needs dloss, or a reduction in its place")
     return LossGrads(*_call(hidden, weight, targets, dloss, ignore_index, z_loss, reduction, True))

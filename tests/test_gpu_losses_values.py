@@ -305,3 +305,46 @@ def test_few_tokens_that_count_in_several_pieces(dtype):
     assert torch.equal(got.loss[rows], alone.loss) and torch.equal(got.hidden[rows], alone.hidden)
     assert not got.hidden[targets == -100].any()
     assert ((got.weight.double() - alone.weight.double()).norm() <= 2 * HALF_ULP[dtype] * alone.weight.double().norm()).item()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens", [6, 40, 300])
+def test_infinite_logits_of_16_bit_tensors(tokens, dtype):
+    """An entry of -inf is not there: losses and the other rows' gradients are those of
+    the table without it (sums may be in another order: twice the bounds), its own
+    gradient zero.  One of +inf makes its token's loss and gradients not finite, and no
+    other token's."""
+    hidden, weight, targets, dloss = make(tokens, 90, 8, dtype, seed=19)
+    hidden[:, 0] = hidden[:, 0].abs() + 0.125
+    weight[11] = 0.0
+    weight[11, 0] = -math.inf
+    targets[targets == 11] = 3
+    keep = torch.arange(90, device="cuda") != 11
+    less = weight[keep].contiguous()
+    moved = torch.where(targets > 11, targets - 1, targets)
+    loss, _, dw = reference(hidden, less, moved, dloss)
+    got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    for x in (got.loss, rf().linear_cross_entropy(hidden, weight, targets)):
+        near(x, (loss[0], 2 * loss[1]), "loss")
+    near(got.weight[keep], (dw[0], 2 * dw[1]), "dweight")
+    assert not got.weight[11].any()
+    hidden[2, 0] = -1.0  # its logit 11 is +inf
+    bad = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    other = torch.arange(tokens, device="cuda") != 2
+    assert torch.equal(bad.loss[other], got.loss[other])
+    assert not bad.loss[2].isfinite() and not bad.hidden[2].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_a_row_of_hidden_that_is_not_finite(dtype):
+    """A row of hidden with a NaN or an Inf: its loss is not finite, the others' as they were."""
+    hidden, weight, targets, dloss = make(20, 150, 16, dtype, seed=21)
+    ref = rf().linear_cross_entropy(hidden, weight, targets)
+    for value in (math.nan, math.inf):
+        bad = hidden.clone()
+        bad[5, 3] = value
+        got = rf().linear_cross_entropy_grad(bad, weight, targets, dloss)
+        other = torch.arange(20, device="cuda") != 5
+        assert torch.equal(got.loss[other], ref[other]) or dtype == F32
+        assert got.loss[other].isfinite().all() and got.hidden[other].isfinite().all()
+        assert not got.loss[5].isfinite() and not got.weight.isfinite().all()
