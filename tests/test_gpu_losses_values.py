@@ -348,3 +348,60 @@ def test_a_row_of_hidden_that_is_not_finite(dtype):
         assert torch.equal(got.loss[other], ref[other]) or dtype == F32
         assert got.loss[other].isfinite().all() and got.hidden[other].isfinite().all()
         assert not got.loss[5].isfinite() and not got.weight.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_forward_and_backward_in_one_graph(dtype):
+    """Captured together, replayed with other inputs and other work between, against eager
+    calls on leaves of their own."""
+    from rollfast_amd import autograd
+
+    def step(h, w, t, scale):
+        loss = autograd.linear_cross_entropy(h, w, t, z_loss=1e-3)
+        return (loss.detach(), *torch.autograd.grad(loss * scale, (h, w)))
+
+    hidden, weight, targets, _ = make(130, 700, 64, dtype, seed=95, masked=0.2)
+    scale = torch.full((), 2.0 ** 10, device="cuda")
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(h, w, targets, scale)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(h, w, targets, scale)
+    for turn in range(4):
+        h2, w2, t2, _ = make(130, 700, 64, dtype, seed=300 + turn, masked=0.1 * turn)
+        with torch.no_grad():
+            h.copy_(h2)
+            w.copy_(w2)
+            targets.copy_(t2)
+            scale.fill_(2.0 ** (10 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, step(h2.requires_grad_(), w2.requires_grad_(), t2, scale)):
+            assert torch.equal(x, y), turn
+
+
+def test_f16_tokens_far_apart_in_several_pieces():
+    """Pieces of 768 tokens: dhidden as from calls on their tokens alone, dweight their sum."""
+    hidden, weight, targets, _ = make(1100, 1 << 20, 8, F16, seed=97, masked=0.1)
+    dloss = spread(1100, (9, -9), 98)
+    got = rf().linear_cross_entropy_grad(hidden, weight, targets, dloss)
+    total = torch.zeros(weight.shape, dtype=torch.float64, device="cuda")
+    for part in (slice(0, 400), slice(400, 1100)):
+        one = rf().linear_cross_entropy_grad(hidden[part], weight, targets[part], dloss[part])
+        total += one.weight.double()
+        # four roundings of 2^-10 / sqrt(12) on either side, in rows of eight
+        assert rows_off(got.hidden[part], one.hidden.double()) < 2.0 ** -9
+    # of A, the sum of the terms' magnitudes: dz is rounded, 2^-11, on either side (at scales
+    # that differ), the parts and the whole are, and sums of up to 1100 terms; f16's own
+    # steps below 2^-14 are 2^-24, three times halved
+    rows = torch.nonzero(targets != -100)[:, 0]
+    h, d = hidden[rows].double().abs(), dloss[rows].double().abs()
+    z = torch.softmax(product(hidden[rows].double(), weight.double()), 1)
+    z[torch.arange(len(rows), device="cuda"), targets[rows]] += 1
+    a = torch.matmul((z * d[:, None]).t().contiguous(), h)
+    assert ((got.weight.double() - total).abs() <= (4 * 2.0 ** -11 + 2 * 1180 * U) * a + 2.0 ** -23).all()
