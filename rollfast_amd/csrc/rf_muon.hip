@@ -71,35 +71,39 @@ __device__ __forceinline__ void put_u(const Moment& a, int64_t e, int64_t left, 
 // A workgroup takes every PARTS-th block of a matrix; eight elements a lane, whole
 // blocks of up to 2048 in registers between the block's largest magnitude and its
 // codes, longer ones read twice.  Of blocks of 8, 16 .. 512 a wave takes as many as it has
-// lanes for.  Bound by memory: 202 million elements with bf16 gradients 383 us, 8 bytes an
-// element at 4.2 TB/s.  (Fewer workgroups, which would stage fewer tables of 22 KB: 376 us,
-// but 24 matrices of 2304 x 768 and 768 x 768 then take 71 us and not 67.)
-__global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* __restrict__ tables)
+// lanes for.  Bound by memory: 202 million elements with bf16 gradients 363 us, 8 bytes an
+// element at 4.5 TB/s, with seven workgroups a CU (four registers more, and six: 395).
+// (Fewer workgroups, which would stage fewer tables of 22 KB: 7 us less, but 24 matrices of
+// 2304 x 768 and 768 x 768 then take 4 more.)
+// CODES: of the matrices whose momentum is codes, else of those with an f32 one.  (In one
+// kernel, with what is done where values are not finite: 432 us.)
+template <bool CODES> __global__ __launch_bounds__(WG, 7) void k_momentum(const Moments t, const uint4* __restrict__ tables)
 {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[TABLE_BYTES];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[CODES ? TABLE_BYTES : 16];
     __shared__ uint32_t tops[WAVES_PER_WG];
     __shared__ double parts[WAVES_PER_WG];
     const Moment& a = t.item[blockIdx.x / rfs::PARTS];
+    if ((a.codes != nullptr) != CODES) return;
     const int part = blockIdx.x % rfs::PARTS, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
     const float* const book = (const float*)(lds + L_CBS);
-    const int64_t bs = a.codes ? a.block_size : 2048, blocks = (a.size + bs - 1) / bs;
-    const bool small = a.codes && bs >= 8 && bs <= WAVE * 8 && (bs & (bs - 1)) == 0;
+    const int64_t bs = CODES ? a.block_size : 2048, blocks = (a.size + bs - 1) / bs;
+    const bool small = CODES && bs >= 8 && bs <= WAVE * 8 && (bs & (bs - 1)) == 0;
     // what the workgroup takes at a time: a block, or as many small ones as it has lanes for
     const int64_t each = small ? WG * 8 / bs : 1, turns = (blocks + each - 1) / each;
-    if (part < turns && a.codes) stage_tables(lds, tables);
+    if (CODES && part < turns) stage_tables(lds, tables);
     double sum = 0;
     for (int64_t turn = part; turn < turns; turn += rfs::PARTS) {
         const int64_t b = small ? min(turn * each + tid * 8 / bs, blocks - 1) : turn;
         const bool mine = !small || turn * each + tid * 8 / bs < blocks;
         const int64_t from = b * bs;
-        const float old = a.codes ? a.scales[b] : 1.0f;
+        const float old = CODES ? a.scales[b] : 1.0f;
         float m[8];
         uint32_t top = 0;
         // momentum of the eight elements at c of the block
         auto moment = [&](int64_t c, float (&g)[8]) {
             const int64_t left = min(bs - c, a.size - from - c);
             load_grad(a, from + c, left, g);
-            if (a.codes) {
+            if constexpr (CODES) {
                 uint32_t w[2] = {};
                 const uint8_t* const p = a.codes + from + c;
                 if (bs - c >= 8) {
@@ -138,15 +142,15 @@ __global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* _
             }
             if (left > 0) {
                 put_u(a, from + c, left, u);
-                if (!a.codes) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (k < left && !__builtin_isfinite(m[k])) m[k] = a.momentum[from + c + k];
+                if (!CODES && top < 0x7F800000u) {
                     rfb::put8(a.momentum + from + c, rfb::narrow8<float>(m), left);
+                } else if (!CODES) {
+                    for (int k = 0; k < 8 && k < left; ++k)
+                        if (__builtin_isfinite(m[k])) a.momentum[from + c + k] = m[k];
                 }
             }
         }
-        if (!a.codes) continue;
+        if (!CODES) continue;
         if (small) {
             for (int d = 1; d < bs / 8; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
         } else {
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* _
             __syncthreads();
             for (int w = 0; w < WAVES_PER_WG; ++w) top = max(top, tops[w]);
         }
-        if (top >= 0x7F800000u) continue;  // (the same for all that code this block)
+        const bool kept = mine && top < 0x7F800000u;
         const float scale = scale_from_absmax_bits(top), rs = 1.0f / scale;
         const bool fast = block_is_fast(top, scale);
         for (int64_t c = mine ? first : bs; c < bs; c += WG * 8) {
@@ -171,7 +175,8 @@ __global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* _
                 w[k / 4] |= code << (8 * (k & 3));
             }
             uint8_t* const p = a.codes + from + c;
-            if (bs - c >= 8) {
+            if (!kept) {
+            } else if (bs - c >= 8) {
                 *(rfb::u32x2_at*)p = rfb::u32x2{w[0], w[1]};
             } else {
 #pragma unroll
@@ -180,7 +185,7 @@ __global__ __launch_bounds__(WG) void k_momentum(const Moments t, const uint4* _
             }
         }
         // (read at the block's start: before the barriers, or by this wave itself)
-        if (mine && (small ? first == 0 : tid == 0)) a.scales[b] = scale;
+        if (kept && (small ? first == 0 : tid == 0)) a.scales[b] = scale;
     }
     sum = wave_sum_f64(sum);
     if (lane == 0) parts[wave] = sum;
@@ -208,7 +213,9 @@ rf_status directions(void* context, const int64_t* which, int count, float* cons
         const rf_muon8_leaf& l = call.leaves[which[i]];
         t.item[i] = {l.grad, l.codes, l.scales, l.momentum, u[i], sums[i], l.rows * l.cols, l.block_size, l.dtype};
     }
-    k_momentum<<<count * rfs::PARTS, WG, 0, st>>>(t, call.tables);
+    const auto coded = [](const Moment& m) { return m.codes != nullptr; };
+    if (std::any_of(t.item, t.item + count, coded)) k_momentum<true><<<count * rfs::PARTS, WG, 0, st>>>(t, call.tables);
+    if (!std::all_of(t.item, t.item + count, coded)) k_momentum<false><<<count * rfs::PARTS, WG, 0, st>>>(t, call.tables);
     return RF_OK;
 }
 
