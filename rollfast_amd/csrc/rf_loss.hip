@@ -302,7 +302,7 @@ struct Even {
 };
 
 // Measured: 8192 x 50257 x 768 without exponentials 570 to 620 us (1.0 to 1.1 PFLOP/s),
-// with them 780 to 810, 824 MB written where the next tile's products could run; 16384 x 32000 x 4096
+// with them 780 to 820, 824 MB written where the next tile's products could run; 16384 x 32000 x 4096
 // 3170 us, 1.22 PFLOP/s.  A token alone is bound by weight's way from memory: 1 x 32000 x
 // 4096 41 us, where part of it lies in the last-level cache, else 90 for 33 tokens (2.9
 // TB/s: two steps of weight in flight a workgroup).
@@ -516,12 +516,12 @@ __device__ __forceinline__ float dz_scale(uint32_t top, bool wide)
     return t < 0x1p-110f ? 1.0f : (wide ? 1.0f : 16384.0f) / t;
 }
 
-// In f16, which keeps 2^-38 of the largest, a token whose own factor is below a sixteenth
-// of it is lifted by a power of two to where the largest are: its dhidden keeps the bits of
-// any other's (dloss 1e-8 of another's: off by 1.5e-2 of its norm without it), whose
-// product takes the power away again; dweight's sums take it from the token's row of
-// hidden (k_level).  A sixteenth, so that the factors of a z-loss alone move nothing.  As
-// far as the scale is finite.
+// In f16, which keeps 2^-38 of the largest, a token whose own factor has an exponent of 5
+// or more below its is lifted by a power of two to where the largest are: its dhidden keeps
+// the bits of any other's (dloss 1e-8 of another's: off by 1.5e-2 of its norm without it),
+// whose product takes the power away again; dweight's sums find it in the token's row of
+// hidden (k_level).  Five, so that the factors of a z-loss alone move nothing.  As far as
+// the scale is finite.
 __device__ __forceinline__ int lift_of(uint32_t top, float reach)
 {
     const int d = min((int)(top >> 23) - (int)(__float_as_uint(reach) >> 23), (int)(top >> 23) - 17);
